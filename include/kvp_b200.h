@@ -47,6 +47,8 @@ extern "C" {
 #define KVP_STATUS_BAD_BLOCK 1 /* a table / slot / pair block id outside [0, num_blocks); access skipped */
 #define KVP_STATUS_BAD_LEN 2   /* seq_len < 1 or ceil(seq_len / block_size) > max_blocks; sequence skipped */
 #define KVP_STATUS_TIMEOUT 4   /* a pipeline wait gave up after ~1 s; the kernel returned early */
+#define KVP_STATUS_BAD_POSITION 8 /* a position outside the rotation table; the token was skipped */
+#define KVP_STATUS_BAD_VALUE 16   /* a NaN or +inf logit or score; it counted as -inf */
 
 typedef enum kvp_dtype { KVP_DTYPE_F32 = 0, KVP_DTYPE_F16 = 1, KVP_DTYPE_BF16 = 2 } kvp_dtype;
 
@@ -204,6 +206,47 @@ typedef struct kvp_append_args {
 } kvp_append_args;
 KVP_API int kvp_append_scatter(const kvp_append_args* a, void* stream);
 
+/* Rotation and append: one layer's new rows on their way from the projections into the cache, in one pass.  For each
+ * token t: every query and key head is normed where weights are given (x * w / sqrt(mean(x^2) + eps), w in the input
+ * dtype), its first rot_dim elements are rotated by the token's position, the queries are written to q_out, the keys
+ * to their slot and, if k_out is not null, to k_out, and the values to their slot.  Without a cache (k_cache, v_cache
+ * and slots null; v unused) only q_out and k_out are written.
+ *   q [num_tokens][num_heads][head_dim], k and v [num_tokens][kv_heads][head_dim], in_dtype, a token's heads
+ *   contiguous; strides between tokens in elements (0: contiguous), so the columns of a fused QKV projection are
+ *   passed as they are.  q_out / k_out: out_dtype, likewise strided; they may be q / k themselves (same dtype and
+ *   stride), else they do not overlap the inputs.
+ *   table: fp32 [max_positions][rot_dim], the cosines of a position's rot_dim / 2 angles, then the sines.
+ *   interleaved 0: element i is paired with i + rot_dim / 2; 1: element 2i with 2i + 1.
+ *   positions: [num_tokens]; a negative one marks padding, whose rows are left as they were everywhere; one that is
+ *   not below max_positions skips the token and sets KVP_STATUS_BAD_POSITION.
+ *   slots: [num_tokens] as in kvp_append_scatter (negative: the token is not put into the cache, its q_out and k_out
+ *   are written; outside the pool: the same, and KVP_STATUS_BAD_BLOCK).  Slots must be distinct.
+ * head_dim a multiple of 16 up to 256, rot_dim a multiple of 16 up to head_dim; buffers 16-byte aligned, strides
+ * multiples of 16 bytes.  Arithmetic in fp32, one rounding at the end. */
+typedef struct kvp_rope_args {
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_stride, k_stride, v_stride; /* elements between tokens; 0: contiguous */
+    int32_t in_dtype, out_dtype;
+    void* q_out;
+    void* k_out;
+    int64_t q_out_stride, k_out_stride;
+    const float* table;
+    const int32_t* positions;
+    const void* q_norm; /* [head_dim] or null */
+    const void* k_norm;
+    float eps;
+    int32_t max_positions, rot_dim, interleaved;
+    void* k_cache; /* this layer's pools */
+    void* v_cache;
+    const int32_t* slots;
+    int32_t kv_dtype, num_tokens, num_heads, kv_heads, head_dim, block_size;
+    int64_t num_blocks;
+    int32_t* status;
+} kvp_rope_args;
+KVP_API int kvp_rope_append(const kvp_rope_args* a, void* stream);
+
 /* Copy-on-write: for each (src, dst) pair copies the whole block, every layer, K and V
  * (python/paged_model.py:92-95).  pairs: device int32 [n_pairs][2].  All pairs of one call run
  * concurrently, so no dst may equal another pair's src or dst. */
@@ -265,6 +308,31 @@ typedef struct kvp_swap_args {
 KVP_API int kvp_swap_out(const kvp_swap_args* a, void* stream);
 KVP_API int kvp_swap_in(const kvp_swap_args* a, void* stream);
 
+/* ======================================================================== beam selection
+ * For each request: the `select` best continuations (beam, token) by
+ *   value = scores[beam] + logits[beam][token] - log(sum over tokens of exp(logits[beam][.])),
+ * best first, ties to the lower beam, then the lower token.  logits [batch * beams][vocab] (row_stride elements between
+ * rows, 0: vocab; rows need no alignment beyond their type's), scores fp32 [batch][beams] (the running sums of
+ * log-probabilities; -inf: a beam not in use, as all but one are in a search's first step).  A logit of -inf is a banned
+ * token.  Continuations of value -inf are chosen only when the others run out, and are ordered like the rest.  NaN and
+ * +inf, in logits and scores, count as -inf and set KVP_STATUS_BAD_VALUE.  out_scores / out_parents / out_tokens:
+ * [batch][select].  beams and select at most 32, vocab at most 2^26.  The states follow their beams by
+ * kvp_mgr_reorder(), which moves no bytes.  The workspace (16-byte aligned) needs no initial value and keeps none. */
+typedef struct kvp_beam_args {
+    const void* logits;
+    int64_t row_stride;
+    const float* scores;
+    float* out_scores;
+    int32_t* out_parents;
+    int32_t* out_tokens;
+    int32_t logits_dtype, batch, beams, vocab, select;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t* status;
+} kvp_beam_args;
+KVP_API size_t kvp_beam_workspace_size(const kvp_beam_args* a);
+KVP_API int kvp_beam_select(const kvp_beam_args* a, void* stream);
+
 /* ======================================================================== host control plane
  * C view of kvp::KVManager (include/kvpage/kv_manager.h; reference include/kvpage/kv_manager.h:26-77).
  * Bool results come back as 1/0; a thrown std::logic_error becomes -KVP_ESTATE and std::invalid_argument
@@ -313,6 +381,12 @@ KVP_API int kvp_mgr_clear_cache(kvp_mgr* m);
  * append that found no block the batch stops there, that request's slot is -1 and later slots are -1. */
 KVP_API int kvp_mgr_append_batch(kvp_mgr* m, const int64_t* rids, int32_t n, int32_t* slots, int32_t* cow_pairs,
                                  int32_t* n_cow);
+/* Reordering of states: request rids[i] takes over the state that rids[parents[i]] had before the call (its tokens and
+ * its blocks, shared as after a fork), all at once; states that nobody takes over are released.  parents[i] in [0, n);
+ * the requests must be distinct.  Returns KVP_OK, KVP_EBOUNDS for a parent out of range or KVP_EINVAL for a request
+ * named twice (nothing changed), KVP_ESTATE for an unknown request.  Never needs a free block: the next append to a
+ * shared partial block copies it. */
+KVP_API int kvp_mgr_reorder(kvp_mgr* m, const int64_t* rids, const int32_t* parents, int32_t n);
 /* Dense table rows for a batch: row i = table of rids[i], padded with `pad` up to max_blocks; lens[i] =
  * tokens.  Returns KVP_EBOUNDS if a table is longer than max_blocks. */
 KVP_API int kvp_mgr_dense_tables(kvp_mgr* m, const int64_t* rids, int32_t n, int32_t max_blocks, int32_t pad,

@@ -48,6 +48,12 @@ public:
     // is shared, otherwise the same block.  false (state unchanged) when no block can be found.
     bool append_token(RequestId r);
     void free(RequestId r);
+    // Reordering of states (beam search): rids[i] takes over the tokens and blocks that rids[parents[i]] had, all at
+    // once; blocks are shared as after fork(), states that nobody takes over are released.  Needs no free block.
+    // Throws std::invalid_argument for a request named twice, std::out_of_range for a parent outside [0, n) and
+    // std::logic_error for an unknown request, in each case before anything changes.  Not part of the reference's
+    // interface.
+    void reorder(const std::vector<RequestId>& rids, const std::vector<int>& parents);
 
     bool contains(RequestId r) const { return requests_.count(r) != 0; }
     const BlockTable& table(RequestId r) const;
@@ -77,7 +83,7 @@ public:
     // When on, every mutating call validates and throws std::logic_error on a violation.  Default: on in
     // builds without NDEBUG.
     void set_check_each_op(bool on) { check_each_op_ = on; }
-    // Calls so far that created, changed or removed a block table (admissions, forks, appends, frees): a caller
+    // Calls so far that created, changed or removed a block table (admissions, forks, appends, frees, reorders): a caller
     // mirroring tables elsewhere (the decode-step runtime's staged rows) can tell whether any table changed since
     // it last looked.  Not part of the reference's interface.
     uint64_t table_changes() const { return table_changes_; }

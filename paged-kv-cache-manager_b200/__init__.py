@@ -22,6 +22,7 @@ LIB_PATH = os.path.join(_HERE, "libkvpage_b200.so")
 
 KVP_OK, KVP_EINVAL, KVP_ECUDA, KVP_EBOUNDS, KVP_ENOSPACE, KVP_ESTATE = 0, 1, 2, 3, 4, 5
 KVP_STATUS_BAD_BLOCK, KVP_STATUS_BAD_LEN, KVP_STATUS_TIMEOUT = 1, 2, 4
+KVP_STATUS_BAD_POSITION, KVP_STATUS_BAD_VALUE = 8, 16
 KVP_ATTN_WORKSPACE_CLEAN = 1
 KVP_ATTN_EARLY_START = 2
 KVP_ATTN_EARLY_LOAD = 4
@@ -62,6 +63,21 @@ class AppendArgs(C.Structure):
                 ("head_dim", _i32), ("block_size", _i32), ("num_blocks", _i64), ("status", _vp)]
 
 
+class RopeArgs(C.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_stride", _i64), ("k_stride", _i64), ("v_stride", _i64),
+                ("in_dtype", _i32), ("out_dtype", _i32), ("q_out", _vp), ("k_out", _vp), ("q_out_stride", _i64),
+                ("k_out_stride", _i64), ("table", _vp), ("positions", _vp), ("q_norm", _vp), ("k_norm", _vp),
+                ("eps", _f32), ("max_positions", _i32), ("rot_dim", _i32), ("interleaved", _i32), ("k_cache", _vp),
+                ("v_cache", _vp), ("slots", _vp), ("kv_dtype", _i32), ("num_tokens", _i32), ("num_heads", _i32),
+                ("kv_heads", _i32), ("head_dim", _i32), ("block_size", _i32), ("num_blocks", _i64), ("status", _vp)]
+
+
+class BeamArgs(C.Structure):
+    _fields_ = [("logits", _vp), ("row_stride", _i64), ("scores", _vp), ("out_scores", _vp), ("out_parents", _vp),
+                ("out_tokens", _vp), ("logits_dtype", _i32), ("batch", _i32), ("beams", _i32), ("vocab", _i32),
+                ("select", _i32), ("workspace", _vp), ("workspace_bytes", _sz), ("status", _vp)]
+
+
 class CowArgs(C.Structure):
     _fields_ = [("k_cache", _vp), ("v_cache", _vp), ("layer_stride", _i64), ("pairs", _vp), ("n_pairs", _i32),
                 ("kv_dtype", _i32), ("num_layers", _i32), ("kv_heads", _i32), ("head_dim", _i32),
@@ -100,6 +116,9 @@ _SIGNATURES = [
     ("kvp_attention_wait_test", C.c_int, [C.POINTER(AttnArgs), _vp, _i64, _i32]),
     ("kvp_paged_attention_host", C.c_int, [_i32] * 6 + [_vp] * 6 + [_i32]),
     ("kvp_append_scatter", C.c_int, [C.POINTER(AppendArgs), _vp]),
+    ("kvp_rope_append", C.c_int, [C.POINTER(RopeArgs), _vp]),
+    ("kvp_beam_workspace_size", _sz, [C.POINTER(BeamArgs)]),
+    ("kvp_beam_select", C.c_int, [C.POINTER(BeamArgs), _vp]),
     ("kvp_cow_copy", C.c_int, [C.POINTER(CowArgs), _vp]),
     ("kvp_migrate_blocks", C.c_int, [C.POINTER(MigrateArgs), _vp]),
     ("kvp_enable_peer_access", C.c_int, [_i32]),
@@ -134,6 +153,7 @@ _SIGNATURES = [
     ("kvp_mgr_shared_blocks_with_cached", C.c_int, [_vp, _i32, _i32, _i32]),
     ("kvp_mgr_clear_cache", C.c_int, [_vp]),
     ("kvp_mgr_append_batch", C.c_int, [_vp, _pi64, _i32, _pi32, _pi32, _pi32]),
+    ("kvp_mgr_reorder", C.c_int, [_vp, _pi64, _pi32, _i32]),
     ("kvp_mgr_dense_tables", C.c_int, [_vp, _pi64, _i32, _i32, _i32, _pi32, _pi32]),
     ("kvp_decoder_workspace_size", _sz, [C.POINTER(DecoderConfig)]),
     ("kvp_decoder_create", _vp, [C.POINTER(DecoderConfig), _vp]),
@@ -244,6 +264,20 @@ class KVManager:
 
     def free(self, r: int):
         _bool(self._L.kvp_mgr_free(self._h, r))
+
+    def reorder(self, rids: Sequence[int], parents: Sequence[int]):
+        """rids[i] takes over the state (tokens and blocks, shared as after a fork) that rids[parents[i]] has, all at
+        once; states that nobody takes over are released.  Moves no bytes and needs no free block: the next append
+        to a shared partial block copies it."""
+        import numpy as np
+        r = np.ascontiguousarray(np.asarray(rids, dtype=np.int64))
+        p = np.ascontiguousarray(np.asarray(parents, dtype=np.int32))
+        if r.ndim != 1 or r.shape != p.shape:
+            raise ValueError("one parent per request")
+        rc = self._L.kvp_mgr_reorder(self._h, r.ctypes.data_as(_pi64), p.ctypes.data_as(_pi32), len(r))
+        if rc == KVP_EBOUNDS:
+            raise ValueError(last_error())
+        _bool(-rc)
 
     def contains(self, r: int) -> bool:
         return bool(self._L.kvp_mgr_contains(self._h, r))
@@ -394,6 +428,17 @@ def _launch(device, fn, args, stream):
         _check(fn(C.byref(args), _stream_ptr(stream)))
 
 
+def _work_on(device, stream):
+    """Context in which an operator allocates and launches: `stream` (which must belong to the operands' device), or
+    the device's current stream.  What the caching allocator hands out inside belongs to the stream that uses it."""
+    import torch
+    if stream is None:
+        return torch.cuda.device(device)
+    if stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the operands on {device}")
+    return torch.cuda.stream(stream)
+
+
 def _stream_ptr(stream):
     import torch
     if stream is None:
@@ -508,6 +553,148 @@ def append_scatter(k_new, v_new, k_cache, v_cache, slots, *, status=None, stream
     dev = _same_device(("k_new", k_new), ("v_new", v_new), ("k_cache", k_cache), ("v_cache", v_cache),
                        ("slots", slots), ("status", status))
     _launch(dev, lib().kvp_append_scatter, a, stream)
+
+
+def rope_table(max_positions: int, rot_dim: int, *, base: float = 10000.0, inv_freq=None, scaling: float = 1.0,
+               device="cuda"):
+    """The rotation table of rope_append / qk_norm_rope: fp32 [max_positions][rot_dim], a position's rot_dim / 2
+    cosines, then its sines, times `scaling`.  Frequencies: base^(-2i / rot_dim), or `inv_freq` (rot_dim / 2 of
+    them).  The angles are computed in 64 bits: at position 100,000 a 32-bit angle is off by up to 0.004."""
+    import torch
+    if max_positions < 1 or rot_dim < 2 or rot_dim % 2:
+        raise ValueError("max_positions must be positive and rot_dim an even number")
+    if inv_freq is None:
+        inv_freq = float(base) ** -(torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
+    inv_freq = inv_freq.to(device=device, dtype=torch.float64)
+    if tuple(inv_freq.shape) != (rot_dim // 2,):
+        raise ValueError("inv_freq must hold rot_dim / 2 frequencies")
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * inv_freq
+    return (torch.cat([angle.cos(), angle.sin()], 1) * scaling).float().contiguous()
+
+
+def _heads_of(t, name, tokens, dim):
+    """Checks [tokens][heads][dim] with a token's heads contiguous; returns the stride between tokens."""
+    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != dim:
+        raise ValueError(f"{name} must be [tokens][heads][{dim}], got {tuple(t.shape)}")
+    st = t.stride()
+    if (dim > 1 and st[2] != 1) or (t.shape[1] > 1 and st[1] != dim):
+        raise ValueError(f"{name}: a token's heads must be contiguous")
+    return st[0] if tokens > 1 else t.shape[1] * dim
+
+
+def _device_vector(t, name, dtype, shape):
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
+    return t.data_ptr()
+
+
+def _rope(q, k, v, positions, table, k_cache, v_cache, slots, q_out, k_out, q_norm, k_norm, eps, interleaved, status,
+          stream):
+    import torch
+    dev = _same_device(("q", q), ("k", k), ("v", v), ("positions", positions), ("table", table), ("k_cache", k_cache),
+                       ("v_cache", v_cache), ("slots", slots), ("q_out", q_out), ("k_out", k_out), ("q_norm", q_norm),
+                       ("k_norm", k_norm), ("status", status))
+    n, nh, D = q.shape
+    a = RopeArgs()
+    a.q_stride, a.k_stride = _heads_of(q, "q", n, D), _heads_of(k, "k", n, D)
+    kvh = k.shape[1]
+    if k.dtype != q.dtype or (v is not None and (v.dtype != q.dtype or v.shape != k.shape)):
+        raise ValueError("q, k and v must share a dtype, k and v a shape")
+    a.q, a.k, a.in_dtype = q.data_ptr(), k.data_ptr(), _dtype_code(q)
+    if table.dim() != 2:
+        raise ValueError("table must be [max_positions][rot_dim]")
+    a.table = _device_vector(table, "table", torch.float32, table.shape)
+    a.max_positions, a.rot_dim = table.shape
+    a.positions = _device_vector(positions, "positions", torch.int32, (n,))
+    if q_norm is not None:
+        a.q_norm = _device_vector(q_norm, "q_norm", q.dtype, (D,))
+    if k_norm is not None:
+        a.k_norm = _device_vector(k_norm, "k_norm", q.dtype, (D,))
+    a.eps, a.interleaved = eps, 1 if interleaved else 0
+    a.num_tokens, a.num_heads, a.kv_heads, a.head_dim = n, nh, kvh, D
+    if k_cache is not None:
+        a.v, a.v_stride = v.data_ptr(), _heads_of(v, "v", n, D)
+        nb, B = k_cache.shape[:2]
+        if k_cache.shape != (nb, B, kvh, D) or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+            raise ValueError("k_cache and v_cache must be [num_blocks][block_size][kv_heads][head_dim] of one dtype")
+        a.k_cache, a.v_cache, a.kv_dtype = _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache"), _dtype_code(k_cache)
+        a.slots = _device_vector(slots, "slots", torch.int32, (n,))
+        a.block_size, a.num_blocks = B, nb
+    if status is not None:
+        a.status = _dev(status, "status")
+    with _work_on(dev, stream):
+        if q_out is None:
+            q_out = torch.empty((n, nh, D), dtype=q.dtype, device=dev)
+        elif q_out.shape != q.shape:
+            raise ValueError("q_out must have the shape of q")
+        a.q_out, a.out_dtype, a.q_out_stride = q_out.data_ptr(), _dtype_code(q_out), _heads_of(q_out, "q_out", n, D)
+        if k_out is not None or k_cache is None:
+            if k_out is None:
+                k_out = torch.empty((n, kvh, D), dtype=q_out.dtype, device=dev)
+            elif k_out.shape != k.shape or k_out.dtype != q_out.dtype:
+                raise ValueError("k_out must have the shape of k and the dtype of q_out")
+            a.k_out, a.k_out_stride = k_out.data_ptr(), _heads_of(k_out, "k_out", n, D)
+        _check(lib().kvp_rope_append(C.byref(a), _stream_ptr(stream)))
+    return q_out, k_out
+
+
+def rope_append(q, k, v, positions, table, k_cache, v_cache, slots, *, q_out=None, k_out=None, q_norm=None, k_norm=None,
+                eps: float = 1e-6, interleaved: bool = False, status=None, stream=None):
+    """kvp_rope_append: RMS norms of the query and key heads (where weights are given), the position rotation, and the
+    append of the keys and values to one layer's paged cache, in one pass.  q [n][num_heads][D], k / v [n][kv_heads][D]
+    (the columns of a fused projection are taken as they are: only a token's heads must be contiguous), positions and
+    slots int32 [n], table from rope_table(), k_cache / v_cache [num_blocks][B][kv_heads][D].  A negative position marks
+    a padded row, a negative slot a row that is not cached.  Returns the rotated queries (q_out, a new tensor unless
+    one is given; q itself is fine)."""
+    if v is None or k_cache is None or v_cache is None or slots is None:
+        raise ValueError("v, k_cache, v_cache and slots are needed; qk_norm_rope works without a cache")
+    return _rope(q, k, v, positions, table, k_cache, v_cache, slots, q_out, k_out, q_norm, k_norm, eps, interleaved,
+                 status, stream)[0]
+
+
+def qk_norm_rope(q, k, positions, table, *, q_out=None, k_out=None, q_norm=None, k_norm=None, eps: float = 1e-6,
+                 interleaved: bool = False, status=None, stream=None):
+    """The same pass without a cache: returns the normed and rotated (queries, keys), e.g. for a decode step whose
+    attention appends the keys itself (k_new of paged_attention and of the decoder)."""
+    return _rope(q, k, None, positions, table, None, None, None, q_out, k_out, q_norm, k_norm, eps, interleaved, status,
+                 stream)
+
+
+def beam_select(logits, scores, select: int, *, workspace=None, status=None, stream=None):
+    """kvp_beam_select: for each request the `select` best continuations over its beams and the vocabulary by running
+    score + log-probability, ties to the lower beam, then the lower token.  logits [batch * beams][vocab] (rows may be
+    strided), scores fp32 [batch][beams] (-inf: a beam not in use).  Returns (scores fp32, parents int32, tokens int32),
+    each [batch][select]; KVManager.reorder then moves the states.  workspace: kvp_beam_workspace_size() bytes of
+    uint8, allocated here unless given."""
+    import torch
+    dev = _same_device(("logits", logits), ("scores", scores), ("workspace", workspace), ("status", status))
+    if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.shape[0] * scores.shape[1]:
+        raise ValueError("logits must be [batch * beams][vocab] and scores [batch][beams]")
+    batch, beams = scores.shape
+    if logits.shape[1] > 1 and logits.stride(1) != 1:
+        raise ValueError("the logits of a row must be contiguous")
+    a = BeamArgs()
+    a.logits, a.logits_dtype, a.vocab = logits.data_ptr(), _dtype_code(logits), logits.shape[1]
+    a.row_stride = logits.stride(0) if logits.shape[0] > 1 else 0
+    if logits.shape[0] > 1 and a.row_stride < a.vocab:
+        raise ValueError("the rows of logits must not overlap")
+    a.scores = _device_vector(scores, "scores", torch.float32, scores.shape)
+    a.batch, a.beams, a.select = batch, beams, select
+    if status is not None:
+        a.status = _dev(status, "status")
+    with _work_on(dev, stream):
+        need = int(lib().kvp_beam_workspace_size(C.byref(a)))
+        if need == 0 and batch:
+            raise ValueError(last_error())
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = _dev(workspace, "workspace"), workspace.numel() * workspace.element_size()
+        out = torch.empty((batch, select), dtype=torch.float32, device=dev)
+        ints = torch.empty((2, batch, select), dtype=torch.int32, device=dev)
+        parents, tokens = ints[0], ints[1]
+        a.out_scores, a.out_parents, a.out_tokens = out.data_ptr(), parents.data_ptr(), tokens.data_ptr()
+        _check(lib().kvp_beam_select(C.byref(a), _stream_ptr(stream)))
+    return out, parents, tokens
 
 
 def cow_copy(k_cache, v_cache, pairs, *, status=None, stream=None):

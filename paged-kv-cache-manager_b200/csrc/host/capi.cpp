@@ -192,6 +192,22 @@ KVP_API int kvp_mgr_append_batch(kvp_mgr* m, const int64_t* rids, int32_t n, int
     });
 }
 
+KVP_API int kvp_mgr_reorder(kvp_mgr* m, const int64_t* rids, const int32_t* parents, int32_t n) {
+    if (!m || n < 0 || (n > 0 && (!rids || !parents))) {
+        kvpi::clear_error();
+        return kvpi::fail(KVP_EINVAL, "null argument or negative count");
+    }
+    const int rc = guarded([&] {
+        try {
+            m->m.reorder(std::vector<kvp::RequestId>(rids, rids + n), std::vector<int>(parents, parents + n));
+        } catch (const std::out_of_range& e) {  // a std::logic_error of its own kind
+            return -kvpi::fail(KVP_EBOUNDS, e.what());
+        }
+        return 0;
+    });
+    return rc < 0 ? -rc : rc;
+}
+
 KVP_API int kvp_mgr_dense_tables(kvp_mgr* m, const int64_t* rids, int32_t n, int32_t max_blocks, int32_t pad,
                                  int32_t* tables, int32_t* lens) {
     int rc = guarded([&] {

@@ -12,7 +12,9 @@
 #include "kvpage/kv_manager.h"
 
 #include <algorithm>
+#include <set>
 #include <stdexcept>
+#include <utility>
 
 namespace kvp {
 
@@ -251,6 +253,29 @@ void KVManager::free(RequestId r) {
     for (BlockId b : it->second.blocks) drop_ref(b);
     table_entries_ -= static_cast<int64_t>(it->second.blocks.size());
     requests_.erase(it);
+    ++table_changes_;
+    checkpoint();
+}
+
+void KVManager::reorder(const std::vector<RequestId>& rids, const std::vector<int>& parents) {
+    if (rids.size() != parents.size()) throw std::invalid_argument("KVManager: one parent per request");
+    const std::set<RequestId> named(rids.begin(), rids.end());
+    if (named.size() != rids.size()) throw std::invalid_argument("KVManager: a request is reordered twice");
+    for (RequestId r : rids) table(r);
+    for (int p : parents)
+        if (p < 0 || static_cast<size_t>(p) >= rids.size()) throw std::out_of_range("KVManager: parent out of range");
+    std::vector<BlockTable> taken;
+    taken.reserve(rids.size());
+    for (int p : parents) taken.push_back(table(rids[static_cast<size_t>(p)]));
+    // every new holder first, so no block that stays in use is released in between
+    for (const BlockTable& t : taken)
+        for (BlockId b : t.blocks) pool_.retain(b);
+    for (size_t i = 0; i < rids.size(); ++i) {
+        BlockTable& t = requests_.find(rids[i])->second;
+        for (BlockId b : t.blocks) drop_ref(b);
+        table_entries_ += static_cast<int64_t>(taken[i].blocks.size()) - static_cast<int64_t>(t.blocks.size());
+        t = std::move(taken[i]);
+    }
     ++table_changes_;
     checkpoint();
 }

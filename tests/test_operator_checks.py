@@ -1,0 +1,165 @@
+"""Argument checks of the serving operators (rotation with append, beam selection, reordering of states), which fail
+before anything touches the device, and the host control plane's reordering."""
+import ctypes as C
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PTR = 1 << 20  # a fake, aligned address: validation fails before any device access
+
+
+def _rope(kvb, **kw):
+    a = kvb.RopeArgs()
+    a.in_dtype = a.out_dtype = a.kv_dtype = kvb.BF16
+    a.num_tokens, a.num_heads, a.kv_heads, a.head_dim, a.rot_dim, a.block_size, a.num_blocks = 3, 8, 2, 64, 64, 16, 4
+    a.max_positions, a.eps = 100, 1e-6
+    a.q = a.k = a.v = a.q_out = a.table = a.positions = a.k_cache = a.v_cache = a.slots = PTR
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("bad", [dict(in_dtype=9), dict(out_dtype=3), dict(kv_dtype=0), dict(head_dim=40), dict(head_dim=272),
+                                 dict(rot_dim=8), dict(rot_dim=80), dict(rot_dim=24), dict(num_heads=0), dict(kv_heads=0),
+                                 dict(num_tokens=-1), dict(max_positions=0), dict(q=0), dict(k=0), dict(v=0), dict(q_out=0),
+                                 dict(table=0), dict(positions=0), dict(slots=0), dict(k_cache=0), dict(num_blocks=0),
+                                 dict(block_size=0), dict(q=PTR + 2), dict(k_cache=PTR + 8), dict(q_stride=100),
+                                 dict(k_stride=132), dict(v_stride=4), dict(q_out_stride=516), dict(k_out=PTR + 4),
+                                 dict(q_norm=PTR, eps=-1.0), dict(q_norm=PTR, eps=float("nan")), dict(q_norm=PTR + 2),
+                                 dict(k_cache=0, v_cache=0, slots=0), dict(num_heads=1 << 21)])
+def test_rope_refuses(kvb, bad):
+    assert kvb.lib().kvp_rope_append(C.byref(_rope(kvb, **bad)), None) == kvb.KVP_EINVAL and kvb.last_error()
+
+
+def test_rope_of_no_tokens_is_fine(kvb):
+    a = _rope(kvb, num_tokens=0, q=0, k=0, v=0)
+    assert kvb.lib().kvp_rope_append(C.byref(a), None) == kvb.KVP_OK
+    assert kvb.lib().kvp_rope_append(None, None) == kvb.KVP_EINVAL
+
+
+def _beam(kvb, **kw):
+    a = kvb.BeamArgs()
+    a.logits = a.scores = a.out_scores = a.out_parents = a.out_tokens = a.workspace = PTR
+    a.logits_dtype, a.batch, a.beams, a.vocab, a.select, a.workspace_bytes = kvb.BF16, 2, 4, 1000, 8, 1 << 20
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("bad", [dict(logits_dtype=5), dict(batch=-1), dict(beams=0), dict(beams=33), dict(select=0),
+                                 dict(select=33), dict(vocab=0), dict(vocab=(1 << 26) + 1), dict(vocab=1), dict(row_stride=999),
+                                 dict(logits=0), dict(scores=0), dict(out_tokens=0), dict(logits=PTR + 1),
+                                 dict(workspace=PTR + 8), dict(batch=1 << 23)])
+def test_beam_refuses(kvb, bad):
+    assert kvb.lib().kvp_beam_select(C.byref(_beam(kvb, **bad)), None) == kvb.KVP_EINVAL and kvb.last_error()
+
+
+def test_beam_workspace(kvb):
+    need = kvb.lib().kvp_beam_workspace_size(C.byref(_beam(kvb)))
+    assert 0 < need < 1 << 20
+    small = _beam(kvb, workspace_bytes=need - 1)
+    assert kvb.lib().kvp_beam_select(C.byref(small), None) == kvb.KVP_ENOSPACE
+    assert kvb.lib().kvp_beam_workspace_size(C.byref(_beam(kvb, select=40))) == 0 and kvb.last_error()
+    assert kvb.lib().kvp_beam_workspace_size(C.byref(_beam(kvb, batch=0))) == 0
+    assert kvb.lib().kvp_beam_select(C.byref(_beam(kvb, batch=0)), None) == kvb.KVP_OK
+    assert kvb.lib().kvp_beam_workspace_size(None) == 0 and kvb.lib().kvp_beam_select(None, None) == kvb.KVP_EINVAL
+
+
+def test_struct_layouts_match_the_header(kvb, tmp_path):
+    structs = {"kvp_rope_args": kvb.RopeArgs, "kvp_beam_args": kvb.BeamArgs}
+    if hasattr(kvb, "PrefixArgs"):
+        structs["kvp_prefix_args"] = kvb.PrefixArgs
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "kvp_b200.h"', "int main(void) {"]
+    for cname, py in structs.items():
+        lines.append(f'printf("{cname} sizeof %zu\\n", sizeof({cname}));')
+        lines += [f'printf("{cname} {f} %zu\\n", offsetof({cname}, {f}));' for f, _ in py._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join(lines + ["return 0;", "}"]))
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-std=c99", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    for ln in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines():
+        s, f, v = ln.split()
+        want = C.sizeof(structs[s]) if f == "sizeof" else getattr(structs[s], f).offset
+        assert int(v) == want, (s, f)
+
+
+# ------------------------------------------------------------------------------------------------ reordering of states
+class Plain:
+    """Block tables as plain lists: reordering is a permutation of their contents."""
+
+    def __init__(self, mgr, rids):
+        self.mgr, self.rids = mgr, rids
+        self.read()
+
+    def read(self):
+        self.tables = [self.mgr.block_table(r) for r in self.rids]
+        self.lens = [self.mgr.num_tokens(r) for r in self.rids]
+
+    def reorder(self, parents):
+        tables, lens = [self.tables[p] for p in parents], [self.lens[p] for p in parents]
+        self.mgr.reorder(self.rids, parents)
+        assert self.mgr.validate() == ""
+        self.read()
+        assert self.tables == tables and self.lens == lens
+
+
+def test_reorder_random_walk(kvb):
+    r = np.random.default_rng(3)
+    mgr = kvb.KVManager(200, 4)
+    rids = [10, 3, 77, 5]
+    assert mgr.admit(10, 9)
+    for x in rids[1:]:
+        assert mgr.fork(x, 10)
+    assert mgr.admit(1000, 30)  # a bystander
+    other = mgr.block_table(1000)
+    p = Plain(mgr, rids)
+    for step in range(120):
+        done, slots, pairs = mgr.append_batch(rids)
+        assert done == 4 and len(set(slots.tolist())) == 4
+        # no copy of a step reads what another one writes
+        assert not set(pairs[:, 1].tolist()) & set(pairs[:, 0].tolist())
+        p.read()
+        p.reorder(r.integers(0, 4, 4).tolist())
+        assert mgr.block_table(1000) == other
+    assert mgr.num_tokens(10) == 129
+    for x in rids + [1000]:
+        mgr.free(x)
+    assert mgr.free_blocks() == 200 and mgr.validate() == ""
+
+
+def test_reorder_of_different_lengths_and_a_full_pool(kvb):
+    """States of different lengths change hands; a pool without a free block is no obstacle."""
+    mgr = kvb.KVManager(6, 4)
+    assert mgr.admit(0, 15) and mgr.admit(1, 2) and mgr.admit(2, 1) and mgr.free_blocks() == 0
+    p = Plain(mgr, [0, 1, 2])
+    p.reorder([1, 0, 0])
+    assert mgr.free_blocks() == 1 and [mgr.num_tokens(r) for r in (0, 1, 2)] == [2, 15, 15]
+    p.reorder([2, 2, 2])
+    assert mgr.free_blocks() == 2 and mgr.stats()["blocks_saved"] == 8
+    p.reorder([0, 1, 2])
+    mgr.reorder([], [])
+    assert mgr.validate() == ""
+
+
+def test_reorder_keeps_cached_prefixes(kvb):
+    mgr = kvb.KVManager(20, 4)
+    assert mgr.admit(0, 9) and mgr.cache_prefix(5, 0, 8) and mgr.admit(1, 5)
+    mgr.reorder([0, 1], [1, 1])
+    assert mgr.cached_prefix_tokens(5) == 8 and mgr.validate() == ""
+    assert mgr.admit_with_cached_prefix(2, 5, 8, 12) and mgr.validate() == ""
+
+
+def test_reorder_refuses_and_changes_nothing(kvb):
+    mgr = kvb.KVManager(20, 4)
+    assert mgr.admit(0, 9) and mgr.admit(1, 5)
+    before = [mgr.block_table(r) for r in (0, 1)], mgr.stats()
+    for rids, parents, err in (([0, 1], [0, 2], ValueError), ([0, 1], [-1, 0], ValueError), ([0, 0], [0, 1], ValueError),
+                               ([0, 9], [0, 1], RuntimeError), ([0, 1], [0], ValueError)):
+        with pytest.raises(err):
+            mgr.reorder(rids, parents)
+    assert before == ([mgr.block_table(r) for r in (0, 1)], mgr.stats()) and mgr.validate() == ""
+    assert kvb.lib().kvp_mgr_reorder(None, None, None, 0) == kvb.KVP_EINVAL
+    assert kvb.lib().kvp_mgr_reorder(mgr.handle, None, None, -1) == kvb.KVP_EINVAL
