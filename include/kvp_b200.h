@@ -185,6 +185,41 @@ KVP_API int kvp_attention_wait_test(const kvp_attn_args* a, void* stream, int64_
 #define KVP_NOALLOC_SCRATCH_BYTES (32u << 20)
 KVP_API int kvp_paged_attention_noalloc(const kvp_attn_args* a, void* stream);
 
+/* ======================================================================== shared-prefix decode attention
+ * kvp_paged_attention for a batch in groups: the sequences of a group share their first prefix_blocks blocks (what
+ * KVManager::fork, admit_with_prefix and admit_with_cached_prefix produce), and the keys and values of those are read
+ * once for the group.  The result is that of kvp_paged_attention over the same tables and lengths, up to rounding.
+ *   group_starts [num_groups + 1]: group i holds sequences group_starts[i] .. group_starts[i + 1] - 1 of the batch;
+ *     the first entry is 0, the last num_seqs.
+ *   prefix_blocks [num_seqs]: leading blocks of each sequence that its group shares (equal within a group; 0 where
+ *     nothing is shared); they are completely filled, so prefix_blocks * block_size <= seq_len.  The first member's
+ *     table row gives the blocks.
+ * A sequence that breaks these rules, or whose length is invalid, gets zeros and sets KVP_STATUS_BAD_LEN.
+ * Types, head shapes and layouts as in kvp_paged_attention; at most 8192 sequences.  The sharing kernel takes head_dim
+ * 64 and 128, queries of the pools' 16-bit dtype (16-byte aligned) and block sizes that are multiples of 8; it rounds
+ * the probabilities to that dtype before the product with V (sums in fp32).  Other calls attend over every sequence's
+ * whole context.  The workspace (256-byte aligned) needs no initial value and keeps none; calls that overlap on the
+ * GPU need one each. */
+typedef struct kvp_prefix_args {
+    const void* q;
+    const void* k_cache; /* this layer's pools */
+    const void* v_cache;
+    const int32_t* block_tables;
+    const int32_t* seq_lens;
+    const int32_t* prefix_blocks;
+    const int32_t* group_starts;
+    void* out;
+    int32_t q_dtype, kv_dtype, out_dtype;
+    int32_t num_seqs, num_groups, num_heads, kv_heads, head_dim, block_size, max_blocks;
+    int64_t num_blocks; /* blocks in each pool; bounds every table entry */
+    float scale;        /* <= 0: 1/sqrt(head_dim) */
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t* status;
+} kvp_prefix_args;
+KVP_API size_t kvp_prefix_workspace_size(const kvp_prefix_args* a);
+KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stream);
+
 /* ======================================================================== KV-cache mutations
  * The device data plane of the reference's KVManager decisions (src/kv_manager.cpp:211-242), whose bytes
  * the reference moves only in Python (python/paged_model.py:54-55, 92-95, 113-117, 145-146). */

@@ -72,6 +72,14 @@ class RopeArgs(C.Structure):
                 ("kv_heads", _i32), ("head_dim", _i32), ("block_size", _i32), ("num_blocks", _i64), ("status", _vp)]
 
 
+class PrefixArgs(C.Structure):
+    _fields_ = [("q", _vp), ("k_cache", _vp), ("v_cache", _vp), ("block_tables", _vp), ("seq_lens", _vp),
+                ("prefix_blocks", _vp), ("group_starts", _vp), ("out", _vp), ("q_dtype", _i32), ("kv_dtype", _i32),
+                ("out_dtype", _i32), ("num_seqs", _i32), ("num_groups", _i32), ("num_heads", _i32), ("kv_heads", _i32),
+                ("head_dim", _i32), ("block_size", _i32), ("max_blocks", _i32), ("num_blocks", _i64), ("scale", _f32),
+                ("workspace", _vp), ("workspace_bytes", _sz), ("status", _vp)]
+
+
 class BeamArgs(C.Structure):
     _fields_ = [("logits", _vp), ("row_stride", _i64), ("scores", _vp), ("out_scores", _vp), ("out_parents", _vp),
                 ("out_tokens", _vp), ("logits_dtype", _i32), ("batch", _i32), ("beams", _i32), ("vocab", _i32),
@@ -117,6 +125,8 @@ _SIGNATURES = [
     ("kvp_paged_attention_host", C.c_int, [_i32] * 6 + [_vp] * 6 + [_i32]),
     ("kvp_append_scatter", C.c_int, [C.POINTER(AppendArgs), _vp]),
     ("kvp_rope_append", C.c_int, [C.POINTER(RopeArgs), _vp]),
+    ("kvp_prefix_workspace_size", _sz, [C.POINTER(PrefixArgs)]),
+    ("kvp_prefix_attention", C.c_int, [C.POINTER(PrefixArgs), _vp]),
     ("kvp_beam_workspace_size", _sz, [C.POINTER(BeamArgs)]),
     ("kvp_beam_select", C.c_int, [C.POINTER(BeamArgs), _vp]),
     ("kvp_cow_copy", C.c_int, [C.POINTER(CowArgs), _vp]),
@@ -658,6 +668,95 @@ def qk_norm_rope(q, k, positions, table, *, q_out=None, k_out=None, q_norm=None,
     attention appends the keys itself (k_new of paged_attention and of the decoder)."""
     return _rope(q, k, None, positions, table, None, None, None, q_out, k_out, q_norm, k_norm, eps, interleaved, status,
                  stream)
+
+
+def _prefix_shape(a, q, k_cache, block_tables, group_starts, num_heads, kv_heads):
+    nb, B, kvh, D = k_cache.shape
+    if q.dim() != 3 or q.shape[1] != num_heads or q.shape[2] != D or kvh != kv_heads:
+        raise ValueError("q must be [num_seqs][num_heads][head_dim] and the pools [num_blocks][block_size][kv_heads][head_dim]")
+    if block_tables.dim() != 2 or block_tables.shape[0] != q.shape[0] or group_starts.dim() != 1 or group_starts.shape[0] < 1:
+        raise ValueError("block_tables must be [num_seqs][max_blocks] and group_starts [num_groups + 1]")
+    a.q_dtype, a.kv_dtype = _dtype_code(q), _dtype_code(k_cache)
+    a.num_seqs, a.num_groups = q.shape[0], group_starts.shape[0] - 1
+    a.num_heads, a.kv_heads, a.head_dim, a.block_size = num_heads, kv_heads, D, B
+    a.max_blocks, a.num_blocks = block_tables.shape[1], nb
+
+
+def shared_prefix_workspace_bytes(q, k_cache, block_tables, group_starts, num_heads: int, kv_heads: int) -> int:
+    """Workspace of shared_prefix_attention for operands of these shapes (their contents do not matter)."""
+    import torch
+    a = PrefixArgs()
+    _prefix_shape(a, q, k_cache, block_tables, group_starts, num_heads, kv_heads)
+    with torch.cuda.device(q.device):
+        need = int(lib().kvp_prefix_workspace_size(C.byref(a)))
+    if need == 0 and last_error():
+        raise ValueError(last_error())
+    return need
+
+
+def shared_prefix_attention(q, k_cache, v_cache, block_tables, seq_lens, prefix_blocks, group_starts, num_heads: int,
+                            kv_heads: int, *, out=None, out_dtype=None, workspace=None, scale: float = 0.0, status=None,
+                            stream=None):
+    """kvp_prefix_attention: paged_attention for a batch in groups whose sequences share their first blocks, which are
+    read once for the group.  prefix_blocks int32 [num_seqs] (equal within a group), group_starts int32
+    [num_groups + 1]; shared_prefix_groups() finds both from the tables.  workspace: uint8, of
+    shared_prefix_workspace_bytes(), allocated here unless given."""
+    import torch
+    dev = _same_device(("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables),
+                       ("seq_lens", seq_lens), ("prefix_blocks", prefix_blocks), ("group_starts", group_starts),
+                       ("out", out), ("workspace", workspace), ("status", status))
+    a = PrefixArgs()
+    _prefix_shape(a, q, k_cache, block_tables, group_starts, num_heads, kv_heads)
+    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_cache and v_cache must share shape and dtype")
+    i32, n = torch.int32, q.shape[0]
+    a.q, a.k_cache, a.v_cache = _dev(q, "q"), _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache")
+    a.block_tables = _device_vector(block_tables, "block_tables", i32, block_tables.shape)
+    a.seq_lens = _device_vector(seq_lens, "seq_lens", i32, (n,))
+    a.prefix_blocks = _device_vector(prefix_blocks, "prefix_blocks", i32, (n,))
+    a.group_starts = _device_vector(group_starts, "group_starts", i32, group_starts.shape)
+    a.scale = scale
+    if status is not None:
+        a.status = _dev(status, "status")
+    with _work_on(dev, stream):
+        if out is None:
+            out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=dev)
+        elif out.shape != q.shape:
+            raise ValueError("out must have the shape of q")
+        a.out, a.out_dtype = _dev(out, "out"), _dtype_code(out)
+        if workspace is None:
+            need = int(lib().kvp_prefix_workspace_size(C.byref(a)))
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        if workspace is not None:
+            a.workspace, a.workspace_bytes = _dev(workspace, "workspace"), workspace.numel() * workspace.element_size()
+        _check(lib().kvp_prefix_attention(C.byref(a), _stream_ptr(stream)))
+    return out
+
+
+def shared_prefix_groups(tables, lens, block_size: int):
+    """The groups of shared_prefix_attention in a batch, from host tables [n][max_blocks] and lengths [n] (KVManager.
+    dense_tables): runs of neighbouring sequences whose tables start with the same blocks, and how many they all share.
+    Sequences that start in different blocks, or have no full block, stand alone with nothing shared.  Returns
+    (prefix_blocks int32 [n], group_starts int32 [num_groups + 1]) as numpy arrays."""
+    import numpy as np
+    t = np.asarray(tables)
+    full = np.asarray(lens, dtype=np.int64) // block_size
+    n = len(full)
+    if t.ndim != 2 or t.shape[0] != n or (n and int(full.max()) > t.shape[1]):
+        raise ValueError("tables must be [n][max_blocks] and hold every sequence's blocks")
+    prefix, starts, i = np.zeros(n, dtype=np.int32), [0], 0
+    while i < n:
+        j = i + 1
+        while j < n and full[i] > 0 and full[j] > 0 and t[j, 0] == t[i, 0]:
+            j += 1
+        if j > i + 1:
+            most = int(full[i:j].min())
+            same = (t[i:j, :most] == t[i, :most]).all(0)
+            prefix[i:j] = most if same.all() else int(same.argmin())
+        starts.append(j)
+        i = j
+    return prefix, np.asarray(starts, dtype=np.int32)
 
 
 def beam_select(logits, scores, select: int, *, workspace=None, status=None, stream=None):

@@ -32,19 +32,6 @@ size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 // Dynamic shared memory a CTA may use: the 227 KB opt-in limit less 1 KB for the static barriers.
 constexpr int kDynSmemCap = (227 << 10) - 1024;
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    });
-    return fn;
-}
-
 // Tensor map over one layer's pool.  per_head == 0: dims (head_dim, rows = num_blocks*B, kv_heads), box
 // (W, R, kvh_cta) -> smem [kvh][R][W].  per_head == 1: dims (head_dim, kv_heads, rows), box (W, 1, R).
 int encode_pool_map(CUtensorMap* map, const void* base, int kv_dtype, const kvp_attn_args& a, const AttnPlan& pl,
@@ -108,6 +95,19 @@ int pool_map_mode() {
 }
 
 }  // namespace
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
+}
 
 // Opts a kernel into the whole dynamic shared-memory budget, once per device.
 int allow_smem(const void* fn) {
@@ -331,8 +331,10 @@ extern "C" KVP_API size_t kvp_attention_workspace_size(const kvp_attn_args* a) {
 namespace {
 
 // kvp_paged_attention with every pipeline wait limited to `wait_limit` clock cycles; `stall` arms the first stage
-// of the CTAs in the grid's first row for a copy that is never issued (kvp_attention_wait_test only).
-int attention_call(const kvp_attn_args* a, void* stream, long long wait_limit, int stall) {
+// of the CTAs in the grid's first row for a copy that is never issued (kvp_attention_wait_test only).  With
+// `skip_blocks` the attention over the sequences' own parts (attention_own_parts).
+int attention_call(const kvp_attn_args* a, void* stream, long long wait_limit, int stall,
+                   const int32_t* skip_blocks = nullptr, float* lse = nullptr) {
     using namespace kvpi;
     clear_error();
     if (!a) return fail(KVP_EINVAL, "null arguments");
@@ -441,6 +443,9 @@ int attention_call(const kvp_attn_args* a, void* stream, long long wait_limit, i
     const float scale = a->scale > 0.f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
     prm.sl2 = scale * 1.4426950408889634f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    prm.skip_blocks = skip_blocks;
+    prm.lse = lse;
+    if (skip_blocks) return kvpd::launch_own_parts(*a, pl, prm, km, vm, s);
     const bool qres = a->q_dtype != a->kv_dtype;
     if (a->kv_dtype == KVP_DTYPE_F16)
         return qres ? kvpd::launch_f16_qres(*a, pl, prm, km, vm, s) : kvpd::launch_f16(*a, pl, prm, km, vm, s);
@@ -448,6 +453,10 @@ int attention_call(const kvp_attn_args* a, void* stream, long long wait_limit, i
 }
 
 }  // namespace
+
+int kvpi::attention_own_parts(const kvp_attn_args* a, const int32_t* skip_blocks, float* lse, cudaStream_t stream) {
+    return attention_call(a, stream, kvpd::kWaitLimitCycles, 0, skip_blocks, lse);
+}
 
 extern "C" KVP_API int kvp_paged_attention(const kvp_attn_args* a, void* stream) {
     return attention_call(a, stream, kvpd::kWaitLimitCycles, 0);

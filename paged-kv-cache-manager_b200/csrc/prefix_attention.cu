@@ -1,0 +1,882 @@
+// Decode attention over blocks that a group of sequences shares: every member's queries against the group's shared
+// keys and values, which are read once for the group instead of once per sequence.
+//
+// For one kv head, a group of m sequences with g query heads each has m * g query rows over the same keys, so what is a
+// matrix-vector product per sequence becomes a matrix product, S = Q K^T and O = P V, for the tensor cores:
+//   read  2 * P * head_dim * 2 bytes of K and V per kv head (P shared tokens),
+//   compute 4 * m * g * P * head_dim flops.
+// Up to about 128 rows the bytes take longer than the flops; beyond, the tensor cores and the exponentials bound it.
+//
+// Three launches.  prefix_kernel attends over the shared blocks and leaves partial results; the balanced decode kernel
+// (SFX) attends over each sequence's own blocks; join_kernel combines both and writes the output.
+//
+// prefix_kernel: one CTA per SM takes an even share of the step's units -- a unit is one tile of 128 keys for one (group,
+// kv head, pair of row tiles) -- regardless of where groups and heads begin and end.  A row tile is as many whole members
+// as fit 128 rows (tcgen05's M).  Two warpgroups of softmax, one per accumulator pair in TMEM, take turns with the tensor
+// cores: while one exponentiates its scores, the MMAs of the other run.
+//   two row tiles:  the warpgroups take one tile each and every key tile; K and V are read once for 256 rows.
+//   one row tile:   both warpgroups take the same rows, one the even, the other the odd key tiles, so that the wait for a
+//                   tile's exponentials is covered by the other tile; they leave two partial results.
+// Scores S and accumulators O live in TMEM (S0, S1 at columns 0 and 128, O0, O1 at 256 and 256 + head_dim); the
+// probabilities P overwrite S as 16-bit pairs and are the A operand of the second product straight from TMEM.  A thread
+// owns one row: the running maximum and sum need no exchange.  O is rescaled only when a row's maximum has grown by more
+// than 2^8 since its last rescaling (P then stays below 2^8, and the sum has the same scale, so nothing is lost).
+// P is rounded to the pools' 16-bit type: the products' rounding errors (half a step each, independent) average out over
+// the keys and stay below the rounding of a 16-bit output; the sum is taken over the unrounded values in fp32.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "attention_common.h"
+#include "kvp_device.cuh"
+
+namespace kvpd {
+
+constexpr int kKeys = 128;         // keys per tile
+constexpr int kRows = 128;         // rows per tile: M of the MMA
+constexpr int kPrefixThreads = 320;  // 8 softmax warps, the MMA warp, the loading warp
+constexpr int kTmemCols = 512;
+constexpr float kRescale = 8.0f;   // log2
+
+struct PrefixParams {
+    const int32_t* tables;
+    const int32_t* lens;
+    const int32_t* prefix_blocks;
+    const int32_t* group_starts;
+    int32_t* status;
+    int32_t* counters;         // the own parts' merge counters, cleared here
+    long long* unit_prefix;    // [num_groups + 1], written by CTA 0 for the joining kernel
+    float2* part_ml;           // partial rows: (maximum in log2 units, sum)
+    float* part_o;
+    const float* own_o;        // [num_seqs][num_heads][D] normalised
+    const float* own_lse;
+    void* out;
+    long long num_blocks;
+    long long wait_limit;
+    int num_counters;
+    int num_seqs, num_groups, nh, kvh, g, max_blocks, B, run, runs, oob_row;
+    int mt;                    // members per row tile
+    int slots;                 // ring slots
+    int bf16, out_dtype;
+    float sl2;
+};
+
+// ---------------------------------------------------------------- tcgen05
+__device__ __forceinline__ void tmem_alloc(uint32_t smem_dst) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "n"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t base) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(kTmemCols));
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D (TMEM) = or += A (shared memory) * B (shared memory)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+// D (TMEM) = or += A (TMEM) * B (shared memory)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+// 32 columns of this warp's 32 lanes, one row per thread.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand in the 128-byte swizzle: rows of 64 elements, 8-row atoms of 1024 bytes.
+//   along the rows (K-major: Q and K): atoms follow each other at 1024 bytes; a 16-element step is 32 bytes further.
+//   across them (MN-major: V, whose rows are the keys the product sums over): atoms of 8 keys at 1024 bytes (stride),
+//   64-dim columns at the column tile's size (leading); a 16-key step is 2048 bytes further.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading_bytes) {
+    return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | (static_cast<uint64_t>(leading_bytes >> 4) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16, fp32 accumulator, A and B both bf16 or both fp16; b_mn: B is MN-major.
+__device__ __forceinline__ uint32_t mma_desc(int bf16, int n, bool b_mn) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
+}
+
+// ---------------------------------------------------------------- units
+// Units of a group: kv heads x pairs of row tiles x key tiles.  A group with a bad range or a bad block count has none.
+struct Group {
+    int start, members, blocks, pairs, ktiles;
+    __device__ __forceinline__ long long units(int kvh) const { return static_cast<long long>(kvh) * pairs * ktiles; }
+};
+__device__ __forceinline__ Group load_group(const PrefixParams& p, int gi) {
+    Group r;
+    r.start = __ldg(p.group_starts + gi);
+    const int end = __ldg(p.group_starts + gi + 1);
+    r.members = 0;
+    r.blocks = 0;
+    if (r.start >= 0 && end > r.start && end <= p.num_seqs) {
+        r.members = end - r.start;
+        const int b = __ldg(p.prefix_blocks + r.start);
+        if (b > 0 && b <= p.max_blocks) r.blocks = b;
+    }
+    r.pairs = (r.members + 2 * p.mt - 1) / (2 * p.mt);
+    r.ktiles = static_cast<int>((static_cast<long long>(r.blocks) * p.B + kKeys - 1) / kKeys);
+    return r;
+}
+
+__device__ __forceinline__ long long floor_div(long long a, long long b, long long c) {  // a * b / c, a * b < 2^53
+    const long long n = a * b;
+    long long q = static_cast<long long>(static_cast<double>(n) / static_cast<double>(c));
+    if (q * c > n) --q;
+    else if ((q + 1) * c <= n) ++q;
+    return q;
+}
+// CTA c of G owns units [c T / G, (c + 1) T / G); the CTA that owns unit u.
+__device__ __forceinline__ long long first_unit(int c, long long T, int G) { return floor_div(c, T, G); }
+__device__ __forceinline__ int owner_of(long long u, long long T, int G) {
+    int c = static_cast<int>((static_cast<double>(u) + 0.5) * G / static_cast<double>(T));
+    c = min(max(c, 0), G - 1);
+    while (c > 0 && first_unit(c, T, G) > u) --c;
+    while (c + 1 < G && first_unit(c + 1, T, G) <= u) ++c;
+    return c;
+}
+
+// One stretch of a CTA's units: key tiles [k0, k0 + n) of (group, kv head, pair).
+struct Work {
+    int start, head, member0, k0, n, tokens;  // member0: the pair's first member, within the group
+    int rows0, rows1;                         // rows of the two row tiles; rows1 == 0: one row tile, key tiles in turn
+    long long part_row;
+};
+
+struct WorkList {
+    Group grp;
+    long long first, t, end;  // the group's first unit, the next unit, the CTA's last
+    int gi, cta;
+    __device__ __forceinline__ bool next(const PrefixParams& p, Work& w) {
+        if (t >= end) return false;
+        while (t >= first + grp.units(p.kvh)) {
+            first += grp.units(p.kvh);
+            grp = load_group(p, ++gi);
+        }
+        const long long rel = t - first;
+        const int triple = static_cast<int>(rel / grp.ktiles);
+        w.k0 = static_cast<int>(rel - static_cast<long long>(triple) * grp.ktiles);
+        w.n = static_cast<int>(min(static_cast<long long>(grp.ktiles - w.k0), end - t));
+        t += w.n;
+        w.start = grp.start;
+        w.head = triple / grp.pairs;
+        w.member0 = (triple - w.head * grp.pairs) * 2 * p.mt;
+        w.tokens = grp.blocks * p.B;
+        const int left = grp.members - w.member0;
+        w.rows0 = min(left, p.mt) * p.g;
+        w.rows1 = min(max(left - p.mt, 0), p.mt) * p.g;
+        // two partial rows per (member, head) row of the batch, 256 more per CTA: a stretch's rows are its own
+        w.part_row = 2LL * p.g * (static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(w.head) * grp.members + w.member0) +
+                     static_cast<long long>(cta) * 2 * kRows;
+        return true;
+    }
+};
+
+// Total units, and the group that holds unit `at` (its index and first unit; at < 0: none wanted).  CTA 0 leaves the
+// prefix sums for the joining kernel.
+__device__ __forceinline__ long long scan_groups(const PrefixParams& p, long long at, int* found_group, long long* found_first,
+                                                 long long* warp_sum) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long carry = 0;
+    for (int g0 = 0; g0 < p.num_groups; g0 += kPrefixThreads) {
+        const int gi = g0 + static_cast<int>(threadIdx.x);
+        long long u = 0;
+        if (gi < p.num_groups) {
+            const Group grp = load_group(p, gi);
+            u = grp.units(p.kvh);
+        }
+        long long x = u;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, off);
+            if (lane >= off) x += y;
+        }
+        if (lane == 31) warp_sum[warp] = x;
+        __syncthreads();
+        long long before = carry, all = 0;
+        for (int w = 0; w < kPrefixThreads / 32; ++w) {
+            const long long s = warp_sum[w];
+            if (w < warp) before += s;
+            all += s;
+        }
+        const long long mine = before + x - u;
+        if (at >= 0 && u > 0 && mine <= at && at < mine + u) {
+            *found_group = gi;
+            *found_first = mine;
+        }
+        if (at < 0 && blockIdx.x == 0 && gi < p.num_groups) p.unit_prefix[gi] = mine;
+        carry += all;
+        __syncthreads();
+    }
+    if (at < 0 && blockIdx.x == 0 && threadIdx.x == 0) p.unit_prefix[p.num_groups] = carry;
+    return carry;
+}
+
+// ---------------------------------------------------------------- the kernel
+struct PrefixShared {
+    uint64_t full[16], empty[16];  // ring slots
+    uint64_t q_full, q_free, s_full[2], p_full[2], o_full[2], drain;
+    uint32_t tmem;
+    int abort;
+    int found_group;
+    long long found_first;
+    long long warp_sum[kPrefixThreads / 32];
+};
+
+// Bounded wait that also ends once another role of the CTA gave up.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, const PrefixParams& p, PrefixShared& sh) {
+    const uint32_t b = smem_u32(bar);
+    if (mbar_try_wait(b, parity)) return true;
+    const long long t0 = clock64();
+    while (true) {
+        for (int i = 0; i < 32; ++i)
+            if (mbar_try_wait(b, parity)) return true;
+        if (*reinterpret_cast<volatile int*>(&sh.abort)) return false;
+        if (clock64() - t0 > p.wait_limit) {
+            report(p.status, KVP_STATUS_TIMEOUT);
+            *reinterpret_cast<volatile int*>(&sh.abort) = 1;
+            return false;
+        }
+    }
+}
+
+// The same for a whole warp, with one answer for all lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const PrefixParams& p, PrefixShared& sh) {
+    return __all_sync(0xffffffffu, wait_or_abort(bar, parity, p, sh));
+}
+
+// A place in the ring of tiles: its slot and the parity of the slot's current use.
+struct Cursor {
+    int slot;
+    uint32_t parity;
+    __device__ __forceinline__ Cursor next(int slots) const {
+        return slot + 1 == slots ? Cursor{0, parity ^ 1u} : Cursor{slot + 1, parity};
+    }
+};
+
+template <int D, class KV>
+__global__ void __launch_bounds__(kPrefixThreads, 1)
+    prefix_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                  const __grid_constant__ CUtensorMap vmap, const PrefixParams p) {
+    using Tr = F16Traits<KV>;
+    constexpr int NCH = D / 64;                      // 64-element columns of a head
+    constexpr uint32_t kCol = kKeys * 128;           // bytes of one such column of a tile
+    constexpr uint32_t kTile = NCH * kCol;           // one tile of Q, K or V
+    constexpr uint32_t kO = 256;                     // TMEM column of the first accumulator
+    __shared__ PrefixShared sh;
+    extern __shared__ uint8_t dyn[];
+    const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
+    const uint32_t ring = base + 2 * kTile;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // the next kernel may be scheduled as soon as this one's CTAs leave their SMs; it waits for all of them
+    griddep_launch_dependents();
+    for (int i = blockIdx.x * kPrefixThreads + threadIdx.x; i < p.num_counters; i += gridDim.x * kPrefixThreads) p.counters[i] = 0;
+    if (threadIdx.x == 0) {
+        sh.abort = 0;
+        for (int s = 0; s < p.slots; ++s) {
+            mbar_init(smem_u32(&sh.full[s]), 1);
+            mbar_init(smem_u32(&sh.empty[s]), 1);
+        }
+        mbar_init(smem_u32(&sh.q_full), 1);
+        mbar_init(smem_u32(&sh.q_free), 1);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(smem_u32(&sh.s_full[t]), 1);
+            mbar_init(smem_u32(&sh.p_full[t]), 4);
+            mbar_init(smem_u32(&sh.o_full[t]), 1);
+        }
+        mbar_init(smem_u32(&sh.drain), 1);
+        fence_barrier_init();
+    }
+    const long long T = scan_groups(p, -1, nullptr, nullptr, sh.warp_sum);
+    const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), T));
+    const int cta = blockIdx.x;
+    if (cta >= G) return;  // the whole CTA, before anything was allocated
+    WorkList list;
+    list.cta = cta;
+    list.t = first_unit(cta, T, G);
+    list.end = first_unit(cta + 1, T, G);
+    scan_groups(p, list.t, &sh.found_group, &sh.found_first, sh.warp_sum);
+    if (warp == 8) tmem_alloc(smem_u32(&sh.tmem));
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    list.gi = sh.found_group;
+    list.first = sh.found_first;
+    list.grp = load_group(p, list.gi);
+    const uint32_t tmem = sh.tmem;
+    Work w;
+
+    if (warp == 9) {
+        // ------------------------------------------------------------ loads
+        bool ok = true;
+        Cursor at{0, 0u};
+        int loaded = 0, queries = 0;  // tiles and query loads issued
+        if (lane == 0) {
+            prefetch_tensormap(&qmap);
+            prefetch_tensormap(&kmap);
+            prefetch_tensormap(&vmap);
+        }
+        while (ok && list.next(p, w)) {
+            // queries, once the previous stretch's products have read theirs
+            if (queries > 0) ok = warp_wait(&sh.q_free, (queries - 1) & 1, p, sh);
+            if (!ok) break;
+            ++queries;
+            if (lane == 0) {
+                const uint32_t bar = smem_u32(&sh.q_full);
+                const int tiles = w.rows1 ? 2 : 1;
+                mbar_arrive_expect_tx(bar, static_cast<uint32_t>(tiles * NCH * p.mt * p.g) * 128u);
+                for (int t = 0; t < tiles; ++t)
+                    for (int c = 0; c < NCH; ++c)
+                        tma_load_3d(base + t * kTile + c * kCol, &qmap, bar, c * 64, w.head * p.g, w.start + w.member0 + t * p.mt);
+            }
+            __syncwarp();
+            const int32_t* trow = p.tables + static_cast<long long>(w.start) * p.max_blocks;
+            const int ahead = w.rows1 ? 1 : 2;  // K runs ahead of V by as many tiles
+            const int run = lane / NCH, c = lane - run * NCH;  // this lane's copy of a tile
+            auto load = [&](const CUtensorMap* map, int kt) {
+                const int st = at.slot;
+                if (loaded >= p.slots && !warp_wait(&sh.empty[st], at.parity ^ 1u, p, sh)) return false;
+                const uint32_t bar = smem_u32(&sh.full[st]);
+                if (lane == 0) mbar_arrive_expect_tx(bar, kTile);
+                __syncwarp();
+                if (run < p.runs) {
+                    const int tok = kt * kKeys + run * p.run;
+                    int row = p.oob_row;  // zeros behind the shared tokens
+                    if (tok < w.tokens) {
+                        const int bi = tok / p.B;
+                        const int blk = __ldg(trow + bi);
+                        if (blk >= 0 && blk < p.num_blocks)
+                            row = blk * p.B + (tok - bi * p.B);
+                        else
+                            report(p.status, KVP_STATUS_BAD_BLOCK);
+                    }
+                    tma_load_3d(ring + st * kTile + c * kCol + static_cast<uint32_t>(run * p.run) * 128u, map, bar, c * 64, w.head, row);
+                }
+                at = at.next(p.slots);
+                ++loaded;
+                return true;
+            };
+            for (int i = 0; ok && i < min(ahead, w.n); ++i) ok = load(&kmap, w.k0 + i);
+            for (int j = 0; ok && j < w.n; ++j) {
+                ok = load(&vmap, w.k0 + j);
+                if (ok && j + ahead < w.n) ok = load(&kmap, w.k0 + j + ahead);
+            }
+        }
+        // Nothing may be in flight into this CTA's shared memory when it ends: all is consumed, unless a wait gave up.
+        if (!ok || *reinterpret_cast<volatile int*>(&sh.abort)) {
+            if (lane == 0) {
+                for (int s = 0; s < p.slots; ++s) {
+                    const int n = loaded > s ? (loaded - s - 1) / p.slots + 1 : 0;  // tiles loaded into slot s
+                    if (n > 0) mbar_wait(smem_u32(&sh.full[s]), static_cast<uint32_t>((n - 1) & 1), p.wait_limit);
+                }
+                if (queries > 0) mbar_wait(smem_u32(&sh.q_full), static_cast<uint32_t>((queries - 1) & 1), p.wait_limit);
+            }
+        }
+    } else if (warp == 8) {
+        // ------------------------------------------------------------ MMAs, one thread
+        if (lane == 0) {
+            const uint32_t qk_desc = mma_desc(p.bf16, kKeys, false);
+            const uint32_t pv_desc = mma_desc(p.bf16, D, true);
+            bool ok = true;
+            Cursor at{0, 0u};
+            int seg = 0;
+            uint32_t turn[2] = {0u, 0u};  // parity of the next P tile, per warpgroup
+            auto wait_tile = [&](Cursor c) { return wait_or_abort(&sh.full[c.slot], c.parity, p, sh); };
+            auto qk = [&](int t, int qt, Cursor c_) {
+                const uint32_t q = base + qt * kTile, k = ring + static_cast<uint32_t>(c_.slot) * kTile;
+#pragma unroll
+                for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+                        mma_ss(tmem + t * kKeys, smem_desc(q + c * kCol + s * 32, 16), smem_desc(k + c * kCol + s * 32, 16),
+                               qk_desc, c + s > 0);
+                tc_commit(smem_u32(&sh.s_full[t]));
+            };
+            while (ok && list.next(p, w)) {
+                const bool two = w.rows1 > 0;
+                const int ahead = two ? 1 : 2;
+                ok = wait_or_abort(&sh.q_full, seg & 1, p, sh);
+                // K tiles 0 .. ahead - 1, then V_j and K_{j + ahead} in turn
+                for (int i = 0; ok && i < min(ahead, w.n); ++i) {
+                    if (!(ok = wait_tile(at))) break;
+                    tc_fence_after();
+                    if (two) {
+                        qk(0, 0, at);
+                        qk(1, 1, at);
+                    } else {
+                        qk(i, 0, at);
+                    }
+                    tc_commit(smem_u32(&sh.empty[at.slot]));
+                    at = at.next(p.slots);
+                }
+                for (int j = 0; ok && j < w.n; ++j) {
+                    const bool more = j + ahead < w.n;
+                    const Cursor vn = at, kn = at.next(p.slots);
+                    if (!(ok = wait_tile(vn))) break;
+                    if (more && !(ok = wait_tile(kn))) break;
+                    for (int i = 0; i < (two ? 2 : 1); ++i) {
+                        const int t = two ? i : j & 1;
+                        if (!(ok = wait_or_abort(&sh.p_full[t], t ? turn[1] : turn[0], p, sh))) break;
+                        if (t) turn[1] ^= 1u; else turn[0] ^= 1u;
+                        tc_fence_after();
+                        const uint32_t v = ring + static_cast<uint32_t>(vn.slot) * kTile;
+                        const bool add = two ? j > 0 : j > 1;
+#pragma unroll
+                        for (int s = 0; s < kKeys / 16; ++s)
+                            mma_ts(tmem + kO + t * D, tmem + t * kKeys + s * 8, smem_desc(v + s * 2048, kCol), pv_desc, add || s > 0);
+                        if (more) qk(t, two ? t : 0, kn);
+                    }
+                    if (!ok) break;
+                    tc_commit(smem_u32(&sh.empty[vn.slot]));
+                    if (more) tc_commit(smem_u32(&sh.empty[kn.slot]));
+                    at = more ? kn.next(p.slots) : kn;
+                }
+                if (ok) {
+                    tc_commit(smem_u32(&sh.o_full[0]));
+                    tc_commit(smem_u32(&sh.o_full[1]));
+                    tc_commit(smem_u32(&sh.q_free));
+                }
+                ++seg;
+            }
+            // every MMA has to be done before the accumulators and the shared memory are given up
+            tc_commit(smem_u32(&sh.drain));
+            if (!mbar_wait(smem_u32(&sh.drain), 0, p.wait_limit)) report(p.status, KVP_STATUS_TIMEOUT);
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------ softmax: warpgroup t, one row per thread
+        const int t = warp >> 2;
+        const int row = threadIdx.x & 127;
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes per warp, in bits 16 and up
+        const uint32_t s_addr = tmem + lanes + t * kKeys, o_addr = tmem + lanes + kO + t * D;
+        bool ok = true;
+        int uses = 0, seg = 0;
+        while (ok && list.next(p, w)) {
+            const bool two = w.rows1 > 0;
+            const int rows = two && t ? w.rows1 : w.rows0;
+            const bool busy = (warp & 3) * 32 < rows;  // else this warp's lanes hold no row: it only keeps step
+            float m = -INFINITY, l = 0.f;              // maximum (scaled, log2) the accumulator refers to, sum
+            const int j0 = two ? 0 : t, dj = two ? 1 : 2;
+            for (int j = j0; j < w.n; j += dj) {
+                if (!(ok = warp_wait(&sh.s_full[t], uses & 1, p, sh))) break;
+                ++uses;
+                if (busy) {
+                    tc_fence_after();
+                    uint32_t s[4][32];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + i * 32, s[i]);
+                    tmem_wait_ld();
+                    const int valid = w.tokens - (w.k0 + j) * kKeys;
+                    if (valid < kKeys) {
+#pragma unroll
+                        for (int i = 0; i < kKeys; ++i)
+                            if (i >= valid) s[i >> 5][i & 31] = 0xff800000u;  // -inf
+                    }
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < kKeys; ++i) mx = fmaxf(mx, __uint_as_float(s[i >> 5][i & 31]));
+                    mx *= p.sl2;
+                    if (j == j0) {
+                        m = mx;  // the first product overwrites the accumulator
+                    } else if (__any_sync(0xffffffffu, mx > m + kRescale)) {
+                        const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+                        m = mn;
+                        l *= f;
+#pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(o_addr + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st32(o_addr + c, o);
+                        }
+                    }
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int e = h * 64 + 2 * i;
+                            const float a = fast_exp2(fmaf(__uint_as_float(s[e >> 5][e & 31]), p.sl2, -ref));
+                            const float b = fast_exp2(fmaf(__uint_as_float(s[(e + 1) >> 5][(e + 1) & 31]), p.sl2, -ref));
+                            sum[(2 * i) & 3] += a;
+                            sum[(2 * i + 1) & 3] += b;
+                            pk[i] = Tr::pack(a, b);
+                        }
+                        tmem_st32(s_addr + h * 32, pk);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_wait_st();
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[t]));
+            }
+            if (!ok) break;
+            if (!(ok = warp_wait(&sh.o_full[t], seg & 1, p, sh))) break;
+            ++seg;
+            if (busy) {
+                // Partial rows in [column / 4][row] order, so that a warp's rows lie side by side.
+                tc_fence_after();
+                const long long r0 = w.part_row + (t ? w.rows0 : 0);
+                float4* po = reinterpret_cast<float4*>(p.part_o + r0 * D);
+                if (row < rows) p.part_ml[r0 + row] = make_float2(m, l);
+                if (two || t < w.n) {
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(o_addr + c, o);
+                        tmem_wait_ld();
+                        if (row < rows) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                po[static_cast<long long>(c / 4 + i) * rows + row] =
+                                    make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                        }
+                    }
+                }
+                tc_fence_before();
+            }
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_free(tmem);
+    }
+}
+
+// ---------------------------------------------------------------- joining
+// One thread per (sequence, kv head, 4 columns, query head of the kv head): weighs the shared part's partial rows and
+// the own part by exp2 of their maxima and writes the output.
+__global__ void __launch_bounds__(256) join_kernel(const PrefixParams p, int D, int grid_ctas) {
+    const int c4n = D / 4;
+    const long long item = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    griddep_wait();
+    if (item >= static_cast<long long>(p.num_seqs) * p.nh * c4n) return;
+    const int j = static_cast<int>(item % p.g);
+    const long long rest = item / p.g;
+    const int c4 = static_cast<int>(rest % c4n);
+    const long long sh = rest / c4n;
+    const int h = static_cast<int>(sh % p.kvh), seq = static_cast<int>(sh / p.kvh);
+    const long long orow = static_cast<long long>(seq) * p.nh + h * p.g + j;
+    // the sequence's group: the last one that starts at or before it
+    int lo = 0, hi = p.num_groups - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (__ldg(p.group_starts + mid) <= seq) lo = mid; else hi = mid - 1;
+    }
+    const Group grp = load_group(p, lo);
+    const int len = __ldg(p.lens + seq), pb = __ldg(p.prefix_blocks + seq);
+    const long long nblk = (static_cast<long long>(len) + p.B - 1) / p.B;
+    const bool fine = len >= 1 && nblk <= p.max_blocks && pb >= 0 && static_cast<long long>(pb) * p.B <= len &&
+                      grp.start <= seq && seq < grp.start + grp.members && grp.blocks == pb;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float inv = 0.f;
+    if (!fine) {
+        if (c4 == 0 && h == 0 && j == 0) report(p.status, KVP_STATUS_BAD_LEN);
+    } else {
+        const float own = __ldcg(p.own_lse + orow);
+        float M = own, L = 0.f;
+        int c0 = 0, c1 = -1, rows = 0, parts = 1;
+        long long row0 = 0;
+        if (grp.ktiles > 0) {
+            const long long T = __ldcg(p.unit_prefix + p.num_groups);
+            const int G = static_cast<int>(min(static_cast<long long>(grid_ctas), T));
+            const int member = seq - grp.start, pair = member / (2 * p.mt);
+            const long long u0 = __ldcg(p.unit_prefix + lo) + (static_cast<long long>(h) * grp.pairs + pair) * grp.ktiles;
+            c0 = owner_of(u0, T, G);
+            c1 = owner_of(u0 + grp.ktiles - 1, T, G);
+            const int member0 = pair * 2 * p.mt, left = grp.members - member0;
+            const int rows0 = min(left, p.mt) * p.g;
+            row0 = 2LL * p.g * (static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(h) * grp.members + member0);
+            rows = rows0;
+            int r = (member - member0) * p.g + j;
+            if (left <= p.mt) {
+                parts = 2;  // even and odd key tiles
+            } else if (r >= rows0) {
+                r -= rows0;
+                row0 += rows0;
+                rows = (min(left, 2 * p.mt) - p.mt) * p.g;
+            }
+            row0 += static_cast<long long>(c0) * 2 * kRows;
+            // rows of a part: [column / 4][row]
+            for (int c = c0; c <= c1; ++c)
+                for (int k = 0; k < parts; ++k)
+                    M = fmaxf(M, __ldcg(&p.part_ml[row0 + static_cast<long long>(c - c0) * 2 * kRows + k * rows + r]).x);
+            for (int c = c0; c <= c1; ++c)
+                for (int k = 0; k < parts; ++k) {
+                    const long long b = row0 + static_cast<long long>(c - c0) * 2 * kRows + k * rows;
+                    const float2 ml = __ldcg(&p.part_ml[b + r]);
+                    if (ml.x == -INFINITY) continue;  // this half of a stretch had no key tile
+                    const float wgt = fast_exp2(ml.x - M);
+                    const float4 o = __ldcg(reinterpret_cast<const float4*>(p.part_o + b * D) + static_cast<long long>(c4) * rows + r);
+                    L += ml.y * wgt;
+                    acc.x += o.x * wgt;
+                    acc.y += o.y * wgt;
+                    acc.z += o.z * wgt;
+                    acc.w += o.w * wgt;
+                }
+        }
+        if (own != -INFINITY) {
+            const float wgt = fast_exp2(own - M);  // the own part is normalised: its sum is one
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(p.own_o + orow * D) + c4);
+            L += wgt;
+            acc.x += o.x * wgt;
+            acc.y += o.y * wgt;
+            acc.z += o.z * wgt;
+            acc.w += o.w * wgt;
+        }
+        inv = 1.f / L;
+    }
+    const size_t at = static_cast<size_t>(orow) * D + c4 * 4;
+    store_any(p.out, at + 0, p.out_dtype, acc.x * inv);
+    store_any(p.out, at + 1, p.out_dtype, acc.y * inv);
+    store_any(p.out, at + 2, p.out_dtype, acc.z * inv);
+    store_any(p.out, at + 3, p.out_dtype, acc.w * inv);
+}
+
+}  // namespace kvpd
+
+namespace kvpi {
+namespace {
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+// The decode attention over whole contexts with the same arguments.
+kvp_attn_args whole_contexts(const kvp_prefix_args& a) {
+    kvp_attn_args w;
+    std::memset(&w, 0, sizeof(w));
+    w.q = a.q;
+    w.q_dtype = a.q_dtype;
+    w.k_cache = a.k_cache;
+    w.v_cache = a.v_cache;
+    w.kv_dtype = a.kv_dtype;
+    w.num_blocks = a.num_blocks;
+    w.block_tables = a.block_tables;
+    w.seq_lens = a.seq_lens;
+    w.out = a.out;
+    w.out_dtype = a.out_dtype;
+    w.num_seqs = a.num_seqs;
+    w.num_heads = a.num_heads;
+    w.kv_heads = a.kv_heads;
+    w.head_dim = a.head_dim;
+    w.block_size = a.block_size;
+    w.max_blocks = a.max_blocks;
+    w.scale = a.scale;
+    w.workspace = a.workspace;
+    w.workspace_bytes = a.workspace_bytes;
+    w.status = a.status;
+    return w;
+}
+
+struct PrefixPlan {
+    bool shared = false;  // else the plain decode attention over every sequence's whole context
+    AttnPlan own;
+    size_t own_o = 0, own_lse = 0, units = 0, ml = 0, o = 0, bytes = 0;
+    int mt = 1, run = 8;
+};
+
+int gcd_of(int a, int b) { return b ? gcd_of(b, a % b) : a; }
+
+int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
+    if (!a) return fail(KVP_EINVAL, "null arguments");
+    if (!valid_dtype(a->q_dtype) || !valid_dtype(a->kv_dtype) || !valid_dtype(a->out_dtype))
+        return fail(KVP_EINVAL, "unsupported dtype");
+    if (a->num_seqs < 0 || a->num_groups < 0 || (a->num_seqs > 0 && a->num_groups < 1) || a->num_groups > a->num_seqs)
+        return fail(KVP_EINVAL, "bad num_seqs / num_groups");
+    if (a->num_seqs > kvpd::kMaxStreamSeqs) return fail(KVP_EINVAL, "at most 8192 sequences per call");
+    if (a->num_blocks < 1 || a->block_size < 1 || a->max_blocks < 1) return fail(KVP_EINVAL, "bad num_blocks / block_size / max_blocks");
+    kvp_attn_args w = whole_contexts(*a);
+    if (a->num_seqs == 0) return KVP_OK;
+    if (a->kv_dtype == KVP_DTYPE_F32) return KVP_OK;
+    // The shared kernel's tiles are 8-row atoms of 64 elements of one 16-bit type.
+    pl->run = gcd_of(a->block_size, kvpd::kKeys);
+    const int rc = plan_attention(w, true, &pl->own);
+    if (rc != KVP_OK) return rc;
+    pl->shared = (a->head_dim == 64 || a->head_dim == 128) && a->q_dtype == a->kv_dtype && pl->run >= 8 &&
+                 aligned16(a->q) && pl->own.streamk;
+    pl->bytes = pl->own.ws_bytes;
+    if (!pl->shared) return KVP_OK;
+    const size_t rows = static_cast<size_t>(a->num_seqs) * a->num_heads;
+    const size_t parts = 2 * rows + static_cast<size_t>(sm_count()) * 2 * kvpd::kRows;
+    pl->mt = kvpd::kRows / (a->num_heads / a->kv_heads);
+    pl->own_o = up256(pl->own.ws_bytes);
+    pl->own_lse = pl->own_o + up256(rows * a->head_dim * 4);
+    pl->units = pl->own_lse + up256(rows * 4);
+    pl->ml = pl->units + up256((static_cast<size_t>(a->num_groups) + 1) * 8);
+    pl->o = pl->ml + up256(parts * 8);
+    pl->bytes = pl->o + parts * a->head_dim * 4;
+    return KVP_OK;
+}
+
+int encode_3d(CUtensorMap* map, int dtype, const void* base, const cuuint64_t (&dims)[3], const cuuint64_t (&strides)[2],
+              const cuuint32_t (&box)[3]) {
+    auto fn = encode_fn();
+    if (!fn) return fail(KVP_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint32_t one[3] = {1, 1, 1};
+    const CUresult r = fn(map, dtype == KVP_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                          const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(KVP_ECUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(r));
+    return KVP_OK;
+}
+
+template <int D, class KV>
+int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, kvpd::PrefixParams p, cudaStream_t s) {
+    auto fn = &kvpd::prefix_kernel<D, KV>;
+    const int rc = allow_smem(reinterpret_cast<const void*>(fn));
+    if (rc != KVP_OK) return rc;
+    constexpr size_t tile = static_cast<size_t>(kvpd::kKeys) * D * 2;
+    p.slots = D == 128 ? 5 : 10;  // 160 KB of K and V in flight beside two query tiles
+    fn<<<sm_count(), kvpd::kPrefixThreads, 1024 + (2 + p.slots) * tile, s>>>(qm, km, vm, p);
+    return cuda_status(cudaGetLastError(), "shared prefix launch");
+}
+
+int launch_join(const kvpd::PrefixParams& p, int D, cudaStream_t s) {
+    const long long items = static_cast<long long>(p.num_seqs) * p.nh * (D / 4);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>((items + 255) / 256));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kvpd::join_kernel, p, D, sm_count()), "join launch");
+}
+
+}  // namespace
+}  // namespace kvpi
+
+extern "C" KVP_API size_t kvp_prefix_workspace_size(const kvp_prefix_args* a) {
+    kvpi::clear_error();
+    kvpi::PrefixPlan pl;
+    return kvpi::plan_prefix(a, &pl) == KVP_OK ? pl.bytes : 0;
+}
+
+extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stream) {
+    using namespace kvpi;
+    clear_error();
+    PrefixPlan pl;
+    int rc = plan_prefix(a, &pl);
+    if (rc != KVP_OK || a->num_seqs == 0) return rc;
+    if (!a->q || !a->k_cache || !a->v_cache || !a->block_tables || !a->seq_lens || !a->prefix_blocks || !a->group_starts || !a->out)
+        return fail(KVP_EINVAL, "null buffer");
+    if (pl.bytes > 0 && (!a->workspace || a->workspace_bytes < pl.bytes))
+        return fail(KVP_ENOSPACE, "workspace smaller than kvp_prefix_workspace_size()");
+    if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return fail(KVP_EINVAL, "workspace must be 256-byte aligned");
+    kvp_attn_args w = whole_contexts(*a);
+    if (!pl.shared) return kvp_paged_attention(&w, stream);
+    if (!aligned16(a->k_cache) || !aligned16(a->v_cache)) return fail(KVP_EINVAL, "K/V pools must be 16-byte aligned");
+    const long long rows = a->num_blocks * static_cast<long long>(a->block_size);
+    if (rows > 0x7fffffffLL) return fail(KVP_EINVAL, "num_blocks * block_size must stay below 2^31");
+    const int g = a->num_heads / a->kv_heads;
+    const cuuint64_t D = static_cast<cuuint64_t>(a->head_dim);
+    CUtensorMap qm, km, vm;
+    {
+        const cuuint64_t dims[3] = {D, static_cast<cuuint64_t>(a->num_heads), static_cast<cuuint64_t>(a->num_seqs)};
+        const cuuint64_t strides[2] = {D * 2, D * 2 * a->num_heads};
+        const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(g), static_cast<cuuint32_t>(pl.mt)};
+        rc = encode_3d(&qm, a->kv_dtype, a->q, dims, strides, box);
+        if (rc != KVP_OK) return rc;
+    }
+    {
+        const cuuint64_t dims[3] = {D, static_cast<cuuint64_t>(a->kv_heads), static_cast<cuuint64_t>(rows)};
+        const cuuint64_t strides[2] = {D * 2, D * 2 * a->kv_heads};
+        const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(pl.run)};
+        rc = encode_3d(&km, a->kv_dtype, a->k_cache, dims, strides, box);
+        if (rc != KVP_OK) return rc;
+        rc = encode_3d(&vm, a->kv_dtype, a->v_cache, dims, strides, box);
+        if (rc != KVP_OK) return rc;
+    }
+    char* ws = static_cast<char*>(a->workspace);
+    kvpd::PrefixParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.tables = a->block_tables;
+    p.lens = a->seq_lens;
+    p.prefix_blocks = a->prefix_blocks;
+    p.group_starts = a->group_starts;
+    p.status = a->status;
+    p.counters = reinterpret_cast<int32_t*>(ws + pl.own.ws_cnt_off);
+    p.num_counters = a->num_seqs * pl.own.groups;
+    p.unit_prefix = reinterpret_cast<long long*>(ws + pl.units);
+    p.part_ml = reinterpret_cast<float2*>(ws + pl.ml);
+    p.part_o = reinterpret_cast<float*>(ws + pl.o);
+    p.own_o = reinterpret_cast<float*>(ws + pl.own_o);
+    p.own_lse = reinterpret_cast<float*>(ws + pl.own_lse);
+    p.out = a->out;
+    p.num_blocks = a->num_blocks;
+    p.wait_limit = kvpd::kWaitLimitCycles;
+    p.num_seqs = a->num_seqs;
+    p.num_groups = a->num_groups;
+    p.nh = a->num_heads;
+    p.kvh = a->kv_heads;
+    p.g = g;
+    p.max_blocks = a->max_blocks;
+    p.B = a->block_size;
+    p.run = pl.run;
+    p.runs = kvpd::kKeys / pl.run;
+    p.oob_row = static_cast<int>(rows);
+    p.mt = pl.mt;
+    p.bf16 = a->kv_dtype == KVP_DTYPE_BF16;
+    p.out_dtype = a->out_dtype;
+    p.sl2 = (a->scale > 0.f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim))) * 1.4426950408889634f;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a->head_dim == 64)
+        rc = p.bf16 ? launch_prefix<64, __nv_bfloat16>(qm, km, vm, p, s) : launch_prefix<64, __half>(qm, km, vm, p, s);
+    else
+        rc = p.bf16 ? launch_prefix<128, __nv_bfloat16>(qm, km, vm, p, s) : launch_prefix<128, __half>(qm, km, vm, p, s);
+    if (rc != KVP_OK) return rc;
+    w.out = ws + pl.own_o;
+    w.out_dtype = KVP_DTYPE_F32;
+    w.flags = KVP_ATTN_WORKSPACE_CLEAN | KVP_ATTN_EARLY_LOAD;  // the counters were cleared by the kernel before
+    rc = attention_own_parts(&w, a->prefix_blocks, reinterpret_cast<float*>(ws + pl.own_lse), s);
+    if (rc != KVP_OK) return rc;
+    return launch_join(p, a->head_dim, s);
+}
