@@ -78,20 +78,22 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// D (TMEM) = or += A (shared memory) * B (shared memory)
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// D (TMEM) = or += A (shared memory) * B (shared memory); operands by the low and high words of their descriptors.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                       uint32_t idesc, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(static_cast<uint32_t>(add))
         : "memory");
 }
 // D (TMEM) = or += A (TMEM) * B (shared memory)
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(static_cast<uint32_t>(add))
         : "memory");
 }
 // 32 columns of this warp's 32 lanes, one row per thread.
@@ -117,21 +119,76 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// Waits for the loads so far; r: what the last one fills, so that no use of it is moved before the wait.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+    asm volatile(""
+                 : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two floats in a register pair, two operations at a time.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// One 32-byte sector of global memory.
+__device__ __forceinline__ void store_sector(float* p, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 
 // Shared-memory operand in the 128-byte swizzle: rows of 64 elements, 8-row atoms of 1024 bytes.
 //   along the rows (K-major: Q and K): atoms follow each other at 1024 bytes; a 16-element step is 32 bytes further.
 //   across them (MN-major: V, whose rows are the keys the product sums over): atoms of 8 keys at 1024 bytes (stride),
 //   64-dim columns at the column tile's size (leading); a 16-key step is 2048 bytes further.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t leading_bytes) {
-    return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | (static_cast<uint64_t>(leading_bytes >> 4) << 16) |
-           (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// The low word holds the address (in 16-byte units, so a step is an addition) and the leading distance, the high word
+// the stride, the version and the swizzle.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t leading_bytes) {
+    return ((addr & 0x3ffffu) >> 4) | ((leading_bytes >> 4) << 16);
 }
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 // kind::f16, fp32 accumulator, A and B both bf16 or both fp16; b_mn: B is MN-major.
 __device__ __forceinline__ uint32_t mma_desc(int bf16, int n, bool b_mn) {
     return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) |
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
+}
+
+// Scores of keys from `valid` on become -inf.
+__device__ __forceinline__ void mask_keys(uint32_t (&s)[32], int valid) {
+    if (valid >= 32) return;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (i >= valid) s[i] = 0xff800000u;
 }
 
 // ---------------------------------------------------------------- units
@@ -420,13 +477,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             int seg = 0;
             uint32_t turn[2] = {0u, 0u};  // parity of the next P tile, per warpgroup
             auto wait_tile = [&](Cursor c) { return wait_or_abort(&sh.full[c.slot], c.parity, p, sh); };
+            const uint32_t q_lo = desc_lo(base, 16), k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, kCol);
             auto qk = [&](int t, int qt, Cursor c_) {
-                const uint32_t q = base + qt * kTile, k = ring + static_cast<uint32_t>(c_.slot) * kTile;
+                const uint32_t q = q_lo + qt * (kTile >> 4), k = k_lo + static_cast<uint32_t>(c_.slot) * (kTile >> 4);
 #pragma unroll
                 for (int c = 0; c < NCH; ++c)
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
-                        mma_ss(tmem + t * kKeys, smem_desc(q + c * kCol + s * 32, 16), smem_desc(k + c * kCol + s * 32, 16),
+                        mma_ss(tmem + t * kKeys, q + ((c * kCol + s * 32) >> 4), kDescHi, k + ((c * kCol + s * 32) >> 4), kDescHi,
                                qk_desc, c + s > 0);
                 tc_commit(smem_u32(&sh.s_full[t]));
             };
@@ -457,11 +515,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
                         if (!(ok = wait_or_abort(&sh.p_full[t], t ? turn[1] : turn[0], p, sh))) break;
                         if (t) turn[1] ^= 1u; else turn[0] ^= 1u;
                         tc_fence_after();
-                        const uint32_t v = ring + static_cast<uint32_t>(vn.slot) * kTile;
+                        const uint32_t v = v_lo + static_cast<uint32_t>(vn.slot) * (kTile >> 4);
                         const bool add = two ? j > 0 : j > 1;
 #pragma unroll
                         for (int s = 0; s < kKeys / 16; ++s)
-                            mma_ts(tmem + kO + t * D, tmem + t * kKeys + s * 8, smem_desc(v + s * 2048, kCol), pv_desc, add || s > 0);
+                            mma_ts(tmem + kO + t * D, tmem + t * kKeys + s * 8, v + s * (2048 >> 4), kDescHi, pv_desc, add || s > 0);
                         if (more) qk(t, two ? t : 0, kn);
                     }
                     if (!ok) break;
@@ -500,20 +558,22 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
                 ++uses;
                 if (busy) {
                     tc_fence_after();
-                    uint32_t s[4][32];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + i * 32, s[i]);
-                    tmem_wait_ld();
                     const int valid = w.tokens - (w.k0 + j) * kKeys;
-                    if (valid < kKeys) {
+                    // First the maximum, then the exponentials, the scores read twice: a whole row of them beside the rest
+                    // does not fit the registers.  Each pass loads its next 32 columns while it works on these.
+                    uint32_t s[2][32];
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    tmem_ld32(s_addr, s[0]);
 #pragma unroll
-                        for (int i = 0; i < kKeys; ++i)
-                            if (i >= valid) s[i >> 5][i & 31] = 0xff800000u;  // -inf
+                    for (int h = 0; h < 4; ++h) {
+                        tmem_wait_ld(s[h & 1]);
+                        tmem_ld32(s_addr + ((h + 1) & 3) * 32, s[(h + 1) & 1]);
+                        mask_keys(s[h & 1], valid - h * 32);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2)
+                            top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[h & 1][e])), __uint_as_float(s[h & 1][e + 1]));
                     }
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < kKeys; ++i) mx = fmaxf(mx, __uint_as_float(s[i >> 5][i & 31]));
-                    mx *= p.sl2;
+                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.sl2;
                     if (j == j0) {
                         m = mx;  // the first product overwrites the accumulator
                     } else if (__any_sync(0xffffffffu, mx > m + kRescale)) {
@@ -524,29 +584,34 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
                         for (int c = 0; c < D; c += 32) {
                             uint32_t o[32];
                             tmem_ld32(o_addr + c, o);
-                            tmem_wait_ld();
+                            tmem_wait_ld(o);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
                             tmem_st32(o_addr + c, o);
                         }
                     }
                     const float ref = m == -INFINITY ? 0.f : m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const uint64_t scale2 = pack2(p.sl2, p.sl2), ref2 = pack2(-ref, -ref);
+                    uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t pk[32];
+                    for (int h = 0; h < 4; ++h) {
+                        // P's columns 16 h .. lie in score columns that are already in registers
+                        tmem_wait_ld(s[h & 1]);
+                        if (h < 3) tmem_ld32(s_addr + (h + 1) * 32, s[(h + 1) & 1]);
+                        mask_keys(s[h & 1], valid - h * 32);
+                        uint32_t pk[16];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int e = h * 64 + 2 * i;
-                            const float a = fast_exp2(fmaf(__uint_as_float(s[e >> 5][e & 31]), p.sl2, -ref));
-                            const float b = fast_exp2(fmaf(__uint_as_float(s[(e + 1) >> 5][(e + 1) & 31]), p.sl2, -ref));
-                            sum[(2 * i) & 3] += a;
-                            sum[(2 * i + 1) & 3] += b;
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 x = unpack2(fma2(pack2(__uint_as_float(s[h & 1][2 * i]), __uint_as_float(s[h & 1][2 * i + 1])),
+                                                          scale2, ref2));
+                            const float a = fast_exp2(x.x), b = fast_exp2(x.y);
+                            sum[i & 1] = add2(sum[i & 1], pack2(a, b));
                             pk[i] = Tr::pack(a, b);
                         }
-                        tmem_st32(s_addr + h * 32, pk);
+                        tmem_st16(s_addr + h * 16, pk);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    const float2 both = unpack2(add2(sum[0], sum[1]));
+                    l += both.x + both.y;
                     tmem_wait_st();
                     tc_fence_before();
                 }
@@ -557,23 +622,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             if (!(ok = warp_wait(&sh.o_full[t], seg & 1, p, sh))) break;
             ++seg;
             if (busy) {
-                // Partial rows in [column / 4][row] order, so that a warp's rows lie side by side.
                 tc_fence_after();
-                const long long r0 = w.part_row + (t ? w.rows0 : 0);
-                float4* po = reinterpret_cast<float4*>(p.part_o + r0 * D);
-                if (row < rows) p.part_ml[r0 + row] = make_float2(m, l);
+                const long long r0 = w.part_row + (t ? w.rows0 : 0) + row;
+                if (row < rows) p.part_ml[r0] = make_float2(m, l);
                 if (two || t < w.n) {
 #pragma unroll
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
                         tmem_ld32(o_addr + c, o);
-                        tmem_wait_ld();
+                        tmem_wait_ld(o);
                         if (row < rows) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                po[static_cast<long long>(c / 4 + i) * rows + row] =
-                                    make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                                __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                            for (int i = 0; i < 32; i += 8) store_sector(p.part_o + r0 * D + c + i, o + i);
                         }
                     }
                 }
@@ -591,93 +651,111 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 }
 
 // ---------------------------------------------------------------- joining
-// One thread per (sequence, kv head, 4 columns, query head of the kv head): weighs the shared part's partial rows and
-// the own part by exp2 of their maxima and writes the output.
-__global__ void __launch_bounds__(256) join_kernel(const PrefixParams p, int D, int grid_ctas) {
-    const int c4n = D / 4;
-    const long long item = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    griddep_wait();
-    if (item >= static_cast<long long>(p.num_seqs) * p.nh * c4n) return;
-    const int j = static_cast<int>(item % p.g);
-    const long long rest = item / p.g;
-    const int c4 = static_cast<int>(rest % c4n);
-    const long long sh = rest / c4n;
-    const int h = static_cast<int>(sh % p.kvh), seq = static_cast<int>(sh / p.kvh);
-    const long long orow = static_cast<long long>(seq) * p.nh + h * p.g + j;
-    // the sequence's group: the last one that starts at or before it
-    int lo = 0, hi = p.num_groups - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (__ldg(p.group_starts + mid) <= seq) lo = mid; else hi = mid - 1;
+// One warp per (sequence, query head): weighs the shared part's partial rows and the own part by exp2 of their maxima and
+// writes the output.  Bound by latency and L2: the lanes fetch up to 32 partials' maxima and sums at once, then whole rows,
+// four at a time.
+template <int D>
+__global__ void __launch_bounds__(128) join_kernel(const PrefixParams p, int grid_ctas) {
+    constexpr int PER = D / 32;  // output columns of a lane, side by side
+    const int lane = threadIdx.x & 31;
+    const long long orow = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    if (orow >= static_cast<long long>(p.num_seqs) * p.nh) return;
+    const int seq = static_cast<int>(orow / p.nh), head = static_cast<int>(orow - static_cast<long long>(seq) * p.nh);
+    const int h = head / p.g, j = head - h * p.g;
+    const int len = __ldg(p.lens + seq), pb = __ldg(p.prefix_blocks + seq);
+    // the sequence's group, the last one that starts at or before it: 32 candidates a step
+    int lo = 0, n = p.num_groups;
+    while (n > 1) {
+        const int step = (n + 31) >> 5;
+        const int at = lo + lane * step;
+        const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && __ldg(p.group_starts + at) <= seq);
+        const int k = below ? 31 - __clz(below) : 0;
+        lo += k * step;
+        n = min(step, n - k * step);
     }
     const Group grp = load_group(p, lo);
-    const int len = __ldg(p.lens + seq), pb = __ldg(p.prefix_blocks + seq);
     const long long nblk = (static_cast<long long>(len) + p.B - 1) / p.B;
     const bool fine = len >= 1 && nblk <= p.max_blocks && pb >= 0 && static_cast<long long>(pb) * p.B <= len &&
                       grp.start <= seq && seq < grp.start + grp.members && grp.blocks == pb;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float inv = 0.f;
-    if (!fine) {
-        if (c4 == 0 && h == 0 && j == 0) report(p.status, KVP_STATUS_BAD_LEN);
-    } else {
-        const float own = __ldcg(p.own_lse + orow);
-        float M = own, L = 0.f;
-        int c0 = 0, c1 = -1, rows = 0, parts = 1;
-        long long row0 = 0;
-        if (grp.ktiles > 0) {
-            const long long T = __ldcg(p.unit_prefix + p.num_groups);
-            const int G = static_cast<int>(min(static_cast<long long>(grid_ctas), T));
-            const int member = seq - grp.start, pair = member / (2 * p.mt);
-            const long long u0 = __ldcg(p.unit_prefix + lo) + (static_cast<long long>(h) * grp.pairs + pair) * grp.ktiles;
-            c0 = owner_of(u0, T, G);
-            c1 = owner_of(u0 + grp.ktiles - 1, T, G);
-            const int member0 = pair * 2 * p.mt, left = grp.members - member0;
-            const int rows0 = min(left, p.mt) * p.g;
-            row0 = 2LL * p.g * (static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(h) * grp.members + member0);
-            rows = rows0;
-            int r = (member - member0) * p.g + j;
-            if (left <= p.mt) {
-                parts = 2;  // even and odd key tiles
-            } else if (r >= rows0) {
-                r -= rows0;
-                row0 += rows0;
-                rows = (min(left, 2 * p.mt) - p.mt) * p.g;
-            }
-            row0 += static_cast<long long>(c0) * 2 * kRows;
-            // rows of a part: [column / 4][row]
-            for (int c = c0; c <= c1; ++c)
-                for (int k = 0; k < parts; ++k)
-                    M = fmaxf(M, __ldcg(&p.part_ml[row0 + static_cast<long long>(c - c0) * 2 * kRows + k * rows + r]).x);
-            for (int c = c0; c <= c1; ++c)
-                for (int k = 0; k < parts; ++k) {
-                    const long long b = row0 + static_cast<long long>(c - c0) * 2 * kRows + k * rows;
-                    const float2 ml = __ldcg(&p.part_ml[b + r]);
-                    if (ml.x == -INFINITY) continue;  // this half of a stretch had no key tile
-                    const float wgt = fast_exp2(ml.x - M);
-                    const float4 o = __ldcg(reinterpret_cast<const float4*>(p.part_o + b * D) + static_cast<long long>(c4) * rows + r);
-                    L += ml.y * wgt;
-                    acc.x += o.x * wgt;
-                    acc.y += o.y * wgt;
-                    acc.z += o.z * wgt;
-                    acc.w += o.w * wgt;
-                }
+    // this row's partials: `parts` for each CTA from c0 on, `rows` apart within a CTA, 256 between CTAs
+    int count = 0, parts = 1, rows = 0;
+    long long row0 = 0;
+    griddep_wait();
+    if (fine && grp.ktiles > 0) {
+        const long long T = __ldcg(p.unit_prefix + p.num_groups);
+        const int G = static_cast<int>(min(static_cast<long long>(grid_ctas), T));
+        const int member = seq - grp.start, pair = member / (2 * p.mt);
+        const long long u0 = __ldcg(p.unit_prefix + lo) + (static_cast<long long>(h) * grp.pairs + pair) * grp.ktiles;
+        const int c0 = owner_of(u0, T, G), c1 = owner_of(u0 + grp.ktiles - 1, T, G);
+        const int member0 = pair * 2 * p.mt, left = grp.members - member0;
+        row0 = 2LL * p.g * (static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(h) * grp.members + member0) +
+               static_cast<long long>(c0) * 2 * kRows + (member - member0) * p.g + j;  // two row tiles: one after the other
+        if (left <= p.mt) {  // one: the even and the odd key tiles'
+            parts = 2;
+            rows = left * p.g;
         }
-        if (own != -INFINITY) {
-            const float wgt = fast_exp2(own - M);  // the own part is normalised: its sum is one
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(p.own_o + orow * D) + c4);
-            L += wgt;
-            acc.x += o.x * wgt;
-            acc.y += o.y * wgt;
-            acc.z += o.z * wgt;
-            acc.w += o.w * wgt;
-        }
-        inv = 1.f / L;
+        count = (c1 - c0 + 1) * parts;
     }
-    const size_t at = static_cast<size_t>(orow) * D + c4 * 4;
-    store_any(p.out, at + 0, p.out_dtype, acc.x * inv);
-    store_any(p.out, at + 1, p.out_dtype, acc.y * inv);
-    store_any(p.out, at + 2, p.out_dtype, acc.z * inv);
-    store_any(p.out, at + 3, p.out_dtype, acc.w * inv);
+    float acc[PER];
+#pragma unroll
+    for (int q = 0; q < PER; ++q) acc[q] = 0.f;
+    float M = -INFINITY, L = 0.f;
+    if (fine) {
+        M = __ldcg(p.own_lse + orow);  // the own part is normalised: its sum is one
+        if (M != -INFINITY) {
+            L = 1.f;
+#pragma unroll
+            for (int q = 0; q < PER; q += 2) {
+                const float2 o = __ldcg(reinterpret_cast<const float2*>(p.own_o + orow * D + lane * PER + q));
+                acc[q] = o.x;
+                acc[q + 1] = o.y;
+            }
+        }
+    }
+    for (int k0 = 0; k0 < count; k0 += 32) {
+        const int k = k0 + lane;
+        const long long row = row0 + (parts == 2 ? static_cast<long long>(k >> 1) * 2 * kRows + (k & 1) * rows
+                                                 : static_cast<long long>(k) * 2 * kRows);
+        const float2 ml = k < count ? __ldcg(&p.part_ml[row]) : make_float2(-INFINITY, 0.f);
+        float top = ml.x;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float Mn = fmaxf(M, top);
+        const float old = M == -INFINITY ? 0.f : fast_exp2(M - Mn);
+        const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - Mn);  // 0: a half without a key tile, never written
+        float add = ml.y * w;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) add += __shfl_xor_sync(0xffffffffu, add, off);
+        L = L * old + add;
+#pragma unroll
+        for (int q = 0; q < PER; ++q) acc[q] *= old;
+        M = Mn;
+        const int left = min(32, count - k0);
+        for (int i0 = 0; i0 < left; i0 += 4) {
+            float o[4][PER], f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f[i] = __shfl_sync(0xffffffffu, w, (i0 + i) & 31);
+                const long long r = __shfl_sync(0xffffffffu, row, (i0 + i) & 31);
+                if (i0 + i >= left) f[i] = 0.f;
+#pragma unroll
+                for (int q = 0; q < PER; q += 2) {
+                    const float2 x = f[i] != 0.f ? __ldcg(reinterpret_cast<const float2*>(p.part_o + r * D + lane * PER + q))
+                                                 : make_float2(0.f, 0.f);
+                    o[i][q] = x.x;
+                    o[i][q + 1] = x.y;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int q = 0; q < PER; ++q) acc[q] += o[i][q] * f[i];
+        }
+    }
+    if (!fine && lane == 0 && head == 0) report(p.status, KVP_STATUS_BAD_LEN);
+    const float inv = fine ? 1.f / L : 0.f;
+#pragma unroll
+    for (int q = 0; q < PER; ++q) store_any(p.out, static_cast<size_t>(orow) * D + lane * PER + q, p.out_dtype, acc[q] * inv);
 }
 
 }  // namespace kvpd
@@ -778,17 +856,17 @@ int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMa
 }
 
 int launch_join(const kvpd::PrefixParams& p, int D, cudaStream_t s) {
-    const long long items = static_cast<long long>(p.num_seqs) * p.nh * (D / 4);
+    const long long rows = static_cast<long long>(p.num_seqs) * p.nh;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>((items + 255) / 256));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(static_cast<unsigned>((rows + 3) / 4));
+    cfg.blockDim = dim3(128);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, kvpd::join_kernel, p, D, sm_count()), "join launch");
+    return cuda_status(cudaLaunchKernelEx(&cfg, D == 64 ? kvpd::join_kernel<64> : kvpd::join_kernel<128>, p, sm_count()), "join launch");
 }
 
 }  // namespace
