@@ -196,6 +196,10 @@ def lib() -> C.CDLL:
     return _lib
 
 
+def _fn(name):
+    return getattr(_lib if _lib is not None else lib(), name)
+
+
 def exported_symbols() -> list:
     return [n for n, _, _ in _SIGNATURES]
 
@@ -397,12 +401,18 @@ class KVManager:
 
 
 # ============================================================================ device entry points
+_codes = {}  # torch dtype -> kvp_dtype
+
+
 def _dtype_code(t) -> int:
-    import torch
-    m = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if t.dtype not in m:
-        raise ValueError(f"unsupported dtype {t.dtype}")
-    return m[t.dtype]
+    code = _codes.get(t.dtype)
+    if code is None:
+        import torch
+        _codes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        code = _codes.get(t.dtype)
+        if code is None:
+            raise ValueError(f"unsupported dtype {t.dtype}")
+    return code
 
 
 def _dev(t, name):
@@ -436,17 +446,6 @@ def _launch(device, fn, args, stream):
     import torch
     with torch.cuda.device(device):
         _check(fn(C.byref(args), _stream_ptr(stream)))
-
-
-def _work_on(device, stream):
-    """Context in which an operator allocates and launches: `stream` (which must belong to the operands' device), or
-    the device's current stream.  What the caching allocator hands out inside belongs to the stream that uses it."""
-    import torch
-    if stream is None:
-        return torch.cuda.device(device)
-    if stream.device != device:
-        raise ValueError(f"the stream is on {stream.device}, the operands on {device}")
-    return torch.cuda.stream(stream)
 
 
 def _stream_ptr(stream):
@@ -582,18 +581,63 @@ def rope_table(max_positions: int, rot_dim: int, *, base: float = 10000.0, inv_f
     return (torch.cat([angle.cos(), angle.sin()], 1) * scaling).float().contiguous()
 
 
-def _heads_of(t, name, tokens, dim):
+def _gpu_of(q, name):
+    """Index of the operands' device."""
+    idx = q.get_device()
+    if idx < 0:
+        raise ValueError(f"{name} must be a CUDA tensor (the library has no CPU path)")
+    return idx
+
+
+def _elsewhere(idx, **named):
+    """Names the operand that is not on CUDA device `idx`."""
+    for name, t in named.items():
+        if t is not None and t.get_device() != idx:
+            where = t.device if t.is_cuda else "the host (the library has no CPU path)"
+            raise ValueError(f"{name} is on {where}, the other operands on cuda:{idx}")
+
+
+def _call_on(idx, stream, fn, a):
+    """Launches on `stream` or the current stream of device `idx`.  Cheap where the device is current, as it nearly
+    always is: a decode step makes several of these calls per layer."""
+    import torch
+    if stream is None:
+        ptr = torch._C._cuda_getCurrentRawStream(idx)
+        if torch._C._cuda_getDevice() == idx:
+            rc = fn(C.byref(a), ptr)
+            if rc:
+                _check(rc)
+            return
+    else:
+        ptr = stream.cuda_stream
+    with torch.cuda.device(idx):
+        _check(fn(C.byref(a), ptr))
+
+
+def _new_on(stream, like, shape, dtype):
+    """A tensor for an operator's results on the stream that fills it (the caching allocator's blocks belong to the
+    stream they were taken on)."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    import torch
+    if stream.device != like.device:
+        raise ValueError(f"the stream is on {stream.device}, the operands on {like.device}")
+    with torch.cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
+
+
+def _token_stride(t, name, shape):
     """Checks [tokens][heads][dim] with a token's heads contiguous; returns the stride between tokens."""
-    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != dim:
-        raise ValueError(f"{name} must be [tokens][heads][{dim}], got {tuple(t.shape)}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be of shape {tuple(shape)}, got {tuple(t.shape)}")
     st = t.stride()
-    if (dim > 1 and st[2] != 1) or (t.shape[1] > 1 and st[1] != dim):
+    if (st[2] != 1 and shape[2] > 1) or (st[1] != shape[2] and shape[1] > 1):
         raise ValueError(f"{name}: a token's heads must be contiguous")
-    return st[0] if tokens > 1 else t.shape[1] * dim
+    return st[0] if shape[0] > 1 else shape[1] * shape[2]
 
 
-def _device_vector(t, name, dtype, shape):
-    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+def _vector(t, name, dtype, shape):
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
     return t.data_ptr()
 
@@ -601,50 +645,59 @@ def _device_vector(t, name, dtype, shape):
 def _rope(q, k, v, positions, table, k_cache, v_cache, slots, q_out, k_out, q_norm, k_norm, eps, interleaved, status,
           stream):
     import torch
-    dev = _same_device(("q", q), ("k", k), ("v", v), ("positions", positions), ("table", table), ("k_cache", k_cache),
-                       ("v_cache", v_cache), ("slots", slots), ("q_out", q_out), ("k_out", k_out), ("q_norm", q_norm),
-                       ("k_norm", k_norm), ("status", status))
-    n, nh, D = q.shape
+    idx = _gpu_of(q, "q")
+    if (k.get_device() != idx or positions.get_device() != idx or table.get_device() != idx or
+            any(t is not None and t.get_device() != idx for t in (v, k_cache, v_cache, slots, q_out, k_out, q_norm, k_norm, status))):
+        _elsewhere(idx, k=k, v=v, positions=positions, table=table, k_cache=k_cache, v_cache=v_cache, slots=slots,
+                   q_out=q_out, k_out=k_out, q_norm=q_norm, k_norm=k_norm, status=status)
+    shape, kshape, dtype = q.shape, k.shape, q.dtype
+    if len(shape) != 3 or len(kshape) != 3 or kshape[0] != shape[0] or kshape[2] != shape[2]:
+        raise ValueError("q and k must be [tokens][heads][head_dim] of the same tokens and head_dim")
+    n, nh, D = shape
+    kvh = kshape[1]
+    if k.dtype is not dtype:
+        raise ValueError("q, k and v must share a dtype")
     a = RopeArgs()
-    a.q_stride, a.k_stride = _heads_of(q, "q", n, D), _heads_of(k, "k", n, D)
-    kvh = k.shape[1]
-    if k.dtype != q.dtype or (v is not None and (v.dtype != q.dtype or v.shape != k.shape)):
-        raise ValueError("q, k and v must share a dtype, k and v a shape")
-    a.q, a.k, a.in_dtype = q.data_ptr(), k.data_ptr(), _dtype_code(q)
+    a.q, a.q_stride, a.in_dtype = q.data_ptr(), _token_stride(q, "q", shape), _dtype_code(q)
+    a.k, a.k_stride = k.data_ptr(), _token_stride(k, "k", kshape)
     if table.dim() != 2:
         raise ValueError("table must be [max_positions][rot_dim]")
-    a.table = _device_vector(table, "table", torch.float32, table.shape)
-    a.max_positions, a.rot_dim = table.shape
-    a.positions = _device_vector(positions, "positions", torch.int32, (n,))
+    tshape = table.shape
+    a.table, a.max_positions, a.rot_dim = _vector(table, "table", torch.float32, tshape), tshape[0], tshape[1]
+    a.positions = _vector(positions, "positions", torch.int32, (n,))
     if q_norm is not None:
-        a.q_norm = _device_vector(q_norm, "q_norm", q.dtype, (D,))
+        a.q_norm = _vector(q_norm, "q_norm", dtype, (D,))
     if k_norm is not None:
-        a.k_norm = _device_vector(k_norm, "k_norm", q.dtype, (D,))
+        a.k_norm = _vector(k_norm, "k_norm", dtype, (D,))
     a.eps, a.interleaved = eps, 1 if interleaved else 0
     a.num_tokens, a.num_heads, a.kv_heads, a.head_dim = n, nh, kvh, D
     if k_cache is not None:
-        a.v, a.v_stride = v.data_ptr(), _heads_of(v, "v", n, D)
-        nb, B = k_cache.shape[:2]
-        if k_cache.shape != (nb, B, kvh, D) or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
-            raise ValueError("k_cache and v_cache must be [num_blocks][block_size][kv_heads][head_dim] of one dtype")
-        a.k_cache, a.v_cache, a.kv_dtype = _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache"), _dtype_code(k_cache)
-        a.slots = _device_vector(slots, "slots", torch.int32, (n,))
-        a.block_size, a.num_blocks = B, nb
+        if v.dtype is not dtype:
+            raise ValueError("q, k and v must share a dtype")
+        a.v, a.v_stride = v.data_ptr(), _token_stride(v, "v", kshape)
+        pool = k_cache.shape
+        if (len(pool) != 4 or pool[2] != kvh or pool[3] != D or v_cache.shape != pool or v_cache.dtype is not k_cache.dtype or
+                not k_cache.is_contiguous() or not v_cache.is_contiguous()):
+            raise ValueError("k_cache and v_cache must be contiguous [num_blocks][block_size][kv_heads][head_dim] of one dtype")
+        a.k_cache, a.v_cache, a.kv_dtype = k_cache.data_ptr(), v_cache.data_ptr(), _dtype_code(k_cache)
+        a.slots = _vector(slots, "slots", torch.int32, (n,))
+        a.num_blocks, a.block_size = pool[0], pool[1]
     if status is not None:
         a.status = _dev(status, "status")
-    with _work_on(dev, stream):
-        if q_out is None:
-            q_out = torch.empty((n, nh, D), dtype=q.dtype, device=dev)
-        elif q_out.shape != q.shape:
-            raise ValueError("q_out must have the shape of q")
-        a.q_out, a.out_dtype, a.q_out_stride = q_out.data_ptr(), _dtype_code(q_out), _heads_of(q_out, "q_out", n, D)
-        if k_out is not None or k_cache is None:
-            if k_out is None:
-                k_out = torch.empty((n, kvh, D), dtype=q_out.dtype, device=dev)
-            elif k_out.shape != k.shape or k_out.dtype != q_out.dtype:
-                raise ValueError("k_out must have the shape of k and the dtype of q_out")
-            a.k_out, a.k_out_stride = k_out.data_ptr(), _heads_of(k_out, "k_out", n, D)
-        _check(lib().kvp_rope_append(C.byref(a), _stream_ptr(stream)))
+    if q_out is None:
+        q_out = _new_on(stream, q, shape, dtype)
+        a.q_out, a.out_dtype = q_out.data_ptr(), a.in_dtype
+    else:
+        a.q_out, a.out_dtype, a.q_out_stride = q_out.data_ptr(), _dtype_code(q_out), _token_stride(q_out, "q_out", shape)
+    if k_out is None:
+        if k_cache is None:
+            k_out = _new_on(stream, q, kshape, q_out.dtype)
+            a.k_out = k_out.data_ptr()
+    else:
+        if k_out.dtype is not q_out.dtype:
+            raise ValueError("k_out must have the dtype of q_out")
+        a.k_out, a.k_out_stride = k_out.data_ptr(), _token_stride(k_out, "k_out", kshape)
+    _call_on(idx, stream, _fn("kvp_rope_append"), a)
     return q_out, k_out
 
 
@@ -671,15 +724,14 @@ def qk_norm_rope(q, k, positions, table, *, q_out=None, k_out=None, q_norm=None,
 
 
 def _prefix_shape(a, q, k_cache, block_tables, group_starts, num_heads, kv_heads):
-    nb, B, kvh, D = k_cache.shape
-    if q.dim() != 3 or q.shape[1] != num_heads or q.shape[2] != D or kvh != kv_heads:
+    qs, ks, ts, gs = q.shape, k_cache.shape, block_tables.shape, group_starts.shape
+    if len(qs) != 3 or len(ks) != 4 or qs[1] != num_heads or qs[2] != ks[3] or ks[2] != kv_heads:
         raise ValueError("q must be [num_seqs][num_heads][head_dim] and the pools [num_blocks][block_size][kv_heads][head_dim]")
-    if block_tables.dim() != 2 or block_tables.shape[0] != q.shape[0] or group_starts.dim() != 1 or group_starts.shape[0] < 1:
+    if len(ts) != 2 or ts[0] != qs[0] or len(gs) != 1 or gs[0] < 1:
         raise ValueError("block_tables must be [num_seqs][max_blocks] and group_starts [num_groups + 1]")
     a.q_dtype, a.kv_dtype = _dtype_code(q), _dtype_code(k_cache)
-    a.num_seqs, a.num_groups = q.shape[0], group_starts.shape[0] - 1
-    a.num_heads, a.kv_heads, a.head_dim, a.block_size = num_heads, kv_heads, D, B
-    a.max_blocks, a.num_blocks = block_tables.shape[1], nb
+    a.num_seqs, a.num_groups, a.num_heads, a.kv_heads, a.head_dim = qs[0], gs[0] - 1, num_heads, kv_heads, qs[2]
+    a.max_blocks, a.num_blocks, a.block_size = ts[1], ks[0], ks[1]
 
 
 def shared_prefix_workspace_bytes(q, k_cache, block_tables, group_starts, num_heads: int, kv_heads: int) -> int:
@@ -702,35 +754,36 @@ def shared_prefix_attention(q, k_cache, v_cache, block_tables, seq_lens, prefix_
     [num_groups + 1]; shared_prefix_groups() finds both from the tables.  workspace: uint8, of
     shared_prefix_workspace_bytes(), allocated here unless given."""
     import torch
-    dev = _same_device(("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables),
-                       ("seq_lens", seq_lens), ("prefix_blocks", prefix_blocks), ("group_starts", group_starts),
-                       ("out", out), ("workspace", workspace), ("status", status))
+    idx = _gpu_of(q, "q")
+    if any(t.get_device() != idx for t in (k_cache, v_cache, block_tables, seq_lens, prefix_blocks, group_starts)) or any(
+            t is not None and t.get_device() != idx for t in (out, workspace, status)):
+        _elsewhere(idx, k_cache=k_cache, v_cache=v_cache, block_tables=block_tables, seq_lens=seq_lens,
+                   prefix_blocks=prefix_blocks, group_starts=group_starts, out=out, workspace=workspace, status=status)
     a = PrefixArgs()
     _prefix_shape(a, q, k_cache, block_tables, group_starts, num_heads, kv_heads)
-    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+    if v_cache.shape != k_cache.shape or v_cache.dtype is not k_cache.dtype:
         raise ValueError("k_cache and v_cache must share shape and dtype")
-    i32, n = torch.int32, q.shape[0]
+    i32, n = torch.int32, (q.shape[0],)
     a.q, a.k_cache, a.v_cache = _dev(q, "q"), _dev(k_cache, "k_cache"), _dev(v_cache, "v_cache")
-    a.block_tables = _device_vector(block_tables, "block_tables", i32, block_tables.shape)
-    a.seq_lens = _device_vector(seq_lens, "seq_lens", i32, (n,))
-    a.prefix_blocks = _device_vector(prefix_blocks, "prefix_blocks", i32, (n,))
-    a.group_starts = _device_vector(group_starts, "group_starts", i32, group_starts.shape)
+    a.block_tables = _vector(block_tables, "block_tables", i32, block_tables.shape)
+    a.seq_lens, a.prefix_blocks = _vector(seq_lens, "seq_lens", i32, n), _vector(prefix_blocks, "prefix_blocks", i32, n)
+    a.group_starts = _vector(group_starts, "group_starts", i32, group_starts.shape)
     a.scale = scale
     if status is not None:
         a.status = _dev(status, "status")
-    with _work_on(dev, stream):
-        if out is None:
-            out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=dev)
-        elif out.shape != q.shape:
-            raise ValueError("out must have the shape of q")
-        a.out, a.out_dtype = _dev(out, "out"), _dtype_code(out)
-        if workspace is None:
+    if out is None:
+        out = _new_on(stream, q, q.shape, out_dtype or q.dtype)
+    elif out.shape != q.shape:
+        raise ValueError("out must have the shape of q")
+    a.out, a.out_dtype = _dev(out, "out"), _dtype_code(out)
+    if workspace is None:
+        with torch.cuda.device(idx):
             need = int(lib().kvp_prefix_workspace_size(C.byref(a)))
-            if need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        if workspace is not None:
-            a.workspace, a.workspace_bytes = _dev(workspace, "workspace"), workspace.numel() * workspace.element_size()
-        _check(lib().kvp_prefix_attention(C.byref(a), _stream_ptr(stream)))
+        if need:
+            workspace = _new_on(stream, q, (need,), torch.uint8)
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = _dev(workspace, "workspace"), workspace.numel() * workspace.element_size()
+    _call_on(idx, stream, _fn("kvp_prefix_attention"), a)
     return out
 
 
@@ -766,33 +819,35 @@ def beam_select(logits, scores, select: int, *, workspace=None, status=None, str
     each [batch][select]; KVManager.reorder then moves the states.  workspace: kvp_beam_workspace_size() bytes of
     uint8, allocated here unless given."""
     import torch
-    dev = _same_device(("logits", logits), ("scores", scores), ("workspace", workspace), ("status", status))
-    if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.shape[0] * scores.shape[1]:
+    idx = _gpu_of(logits, "logits")
+    _elsewhere(idx, scores=scores, workspace=workspace, status=status)
+    ls, ss, st = logits.shape, scores.shape, logits.stride()
+    if len(ss) != 2 or len(ls) != 2 or ls[0] != ss[0] * ss[1]:
         raise ValueError("logits must be [batch * beams][vocab] and scores [batch][beams]")
-    batch, beams = scores.shape
-    if logits.shape[1] > 1 and logits.stride(1) != 1:
+    batch, beams = ss
+    if ls[1] > 1 and st[1] != 1:
         raise ValueError("the logits of a row must be contiguous")
     a = BeamArgs()
-    a.logits, a.logits_dtype, a.vocab = logits.data_ptr(), _dtype_code(logits), logits.shape[1]
-    a.row_stride = logits.stride(0) if logits.shape[0] > 1 else 0
-    if logits.shape[0] > 1 and a.row_stride < a.vocab:
-        raise ValueError("the rows of logits must not overlap")
-    a.scores = _device_vector(scores, "scores", torch.float32, scores.shape)
+    a.logits, a.logits_dtype, a.vocab = logits.data_ptr(), _dtype_code(logits), ls[1]
+    if ls[0] > 1:
+        a.row_stride = st[0]
+        if st[0] < ls[1]:
+            raise ValueError("the rows of logits must not overlap")
+    a.scores = _vector(scores, "scores", torch.float32, ss)
     a.batch, a.beams, a.select = batch, beams, select
     if status is not None:
         a.status = _dev(status, "status")
-    with _work_on(dev, stream):
-        need = int(lib().kvp_beam_workspace_size(C.byref(a)))
+    if workspace is None:
+        with torch.cuda.device(idx):
+            need = int(lib().kvp_beam_workspace_size(C.byref(a)))
         if need == 0 and batch:
             raise ValueError(last_error())
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = _dev(workspace, "workspace"), workspace.numel() * workspace.element_size()
-        out = torch.empty((batch, select), dtype=torch.float32, device=dev)
-        ints = torch.empty((2, batch, select), dtype=torch.int32, device=dev)
-        parents, tokens = ints[0], ints[1]
-        a.out_scores, a.out_parents, a.out_tokens = out.data_ptr(), parents.data_ptr(), tokens.data_ptr()
-        _check(lib().kvp_beam_select(C.byref(a), _stream_ptr(stream)))
+        workspace = _new_on(stream, logits, (need,), torch.uint8)
+    a.workspace, a.workspace_bytes = _dev(workspace, "workspace"), workspace.numel() * workspace.element_size()
+    out = _new_on(stream, logits, (batch, select), torch.float32)
+    parents, tokens = _new_on(stream, logits, (2, batch, select), torch.int32)
+    a.out_scores, a.out_parents, a.out_tokens = out.data_ptr(), parents.data_ptr(), tokens.data_ptr()
+    _call_on(idx, stream, _fn("kvp_beam_select"), a)
     return out, parents, tokens
 
 
