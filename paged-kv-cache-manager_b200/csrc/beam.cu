@@ -2,16 +2,17 @@
 //     value = score[beam] + logit[beam][token] - log(sum over tokens of exp(logit[beam][.])),
 // ties to the lower beam, then the lower token.  One read of the logits, two launches.
 //
-// beam_scan_kernel (bound by HBM): a warp takes one segment of one row.  It keeps a running maximum and sum of
-// exponentials per lane, and the segment's best `select` logits as a list sorted over its 32 lanes; within a row the
-// order of the values is the order of the logits, so no logarithm is needed here.  The list starts from the lanes' own
-// maxima of the first 1024 logits (one sort), so that of the rest only what passes the list's last entry costs more than
-// one vote per 256 logits; it is inserted with a ballot and a shift.  Entries are 64-bit keys (ordered logit, ~token):
-// all different, so ties fall to the lower token however the segment is cut.
+// beam_scan_kernel (bound by HBM): a warp takes one segment of one row, 1024 logits a step, the next step's loads in flight
+// while it works on this one's.  It keeps a running maximum and sum of exponentials per lane, and the segment's best
+// `select` logits as a list sorted over its 32 lanes; within a row the order of the values is the order of the logits, so
+// no logarithm is needed here.  The list starts from the lanes' own maxima of the first step (one sort); of the rest only
+// what passes the list's last entry -- or that of another warp of the CTA, which works on the same row -- costs more than
+// one vote per step, and is inserted with a ballot and a shift.  Entries are 64-bit keys (ordered logit, ~token): all
+// different, so ties fall to the lower token however the row is cut.
 //
-// beam_pick_kernel (bound by latency): one CTA per request joins the segments' sums in 64 bits, turns the lists' heads
-// into values in 64 bits -- continuations of different beams are ordered by their values, not by a 32-bit rounding --
-// and takes the best head `select` times, first within each warp's lists, then over the warps.
+// beam_pick_kernel (bound by latency): one CTA per request joins each beam's segments -- their sums in 64 bits, their lists
+// by bitonic merges -- and takes the best head of the beams' lists `select` times, comparing values in 64 bits:
+// continuations of different beams are ordered by their values, not by a 32-bit rounding.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -22,10 +23,10 @@
 
 namespace kvpd {
 
-constexpr int kBeamMost = 32;        // beams and selected continuations per request: a warp's lanes
-constexpr int kBeamLists = 256;      // lists per request: one per thread of the picking CTA
-constexpr int kBeamEntries = 5400;   // and their entries: 42 KB of its shared memory
-constexpr int kBeamStep = 1024;      // logits a warp takes at once
+constexpr int kBeamMost = 32;    // beams and selected continuations per request: a warp's lanes
+constexpr int kBeamSegs = 64;    // segments of a row
+constexpr int kBeamStep = 1024;  // logits a warp takes at once, 32 per lane
+constexpr int kBeamWarps = 4;    // warps per CTA of the scan, all on one row
 constexpr int kBeamTokenBits = 26;
 
 struct BeamParams {
@@ -67,31 +68,76 @@ __device__ __forceinline__ unsigned long long warp_sort_desc(unsigned long long 
     return v;
 }
 
-template <class T>
-struct BeamVec {  // 16-bit logits: 8 per 16-byte vector
-    static constexpr int N = 8;
-    uint4 u;
-    __device__ __forceinline__ void load(const T* p) { u = __ldcs(reinterpret_cast<const uint4*>(p)); }
-    __device__ __forceinline__ void get(float (&x)[N]) const {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Two lists sorted over the lanes, largest first, become the 32 largest of both.
+__device__ __forceinline__ unsigned long long warp_merge_desc(unsigned long long a, unsigned long long b, int lane) {
+    const unsigned long long r = __shfl_xor_sync(0xffffffffu, b, 31);
+    unsigned long long v = a > r ? a : r;  // a bitonic sequence of the 32 largest
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = F16Traits<T>::unpack_lo(w[i]);
-            x[2 * i + 1] = F16Traits<T>::unpack_hi(w[i]);
+    for (int j = 16; j > 0; j >>= 1) {
+        const unsigned long long w = __shfl_xor_sync(0xffffffffu, v, j);
+        v = (lane & j) == 0 ? (v > w ? v : w) : (v < w ? v : w);
+    }
+    return v;
+}
+
+// One step of a row, 32 logits per lane: element e of a lane is token at + ((e / N) * 32 + lane) * N + e % N - shift.
+// Vec: 16-byte loads, where all rows of a request lie alike against 16-byte boundaries.  Else single loads of
+// neighbouring tokens by neighbouring lanes: with an odd vocabulary the rows start at different offsets, and vectors would
+// group the sums of two equal rows differently, so that their tie fell to a rounding.
+template <class T, bool Vec>
+struct BeamStep {
+    static constexpr int N = 1;
+    T u[32];
+    __device__ __forceinline__ void load(const T* p, int lane) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) u[j] = __ldcs(p + j * 32 + lane);
+    }
+    __device__ __forceinline__ void get(float (&x)[32]) const {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = one(u + j);
+    }
+    static __device__ __forceinline__ float one(const T* p) {
+        if constexpr (sizeof(T) == 4) return *p;
+        else return F16Traits<T>::to_float(*p);
+    }
+};
+template <class T>
+struct BeamStep<T, true> {  // 16-bit logits: 8 per vector
+    static constexpr int N = 8;
+    uint4 u[4];
+    __device__ __forceinline__ void load(const T* p, int lane) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = __ldcs(reinterpret_cast<const uint4*>(p) + j * 32 + lane);
+    }
+    __device__ __forceinline__ void get(float (&x)[32]) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[j * 8 + 2 * i] = F16Traits<T>::unpack_lo(w[i]);
+                x[j * 8 + 2 * i + 1] = F16Traits<T>::unpack_hi(w[i]);
+            }
         }
     }
     static __device__ __forceinline__ float one(const T* p) { return F16Traits<T>::to_float(*p); }
 };
 template <>
-struct BeamVec<float> {
+struct BeamStep<float, true> {
     static constexpr int N = 4;
-    float4 u;
-    __device__ __forceinline__ void load(const float* p) { u = __ldcs(reinterpret_cast<const float4*>(p)); }
-    __device__ __forceinline__ void get(float (&x)[N]) const {
-        x[0] = u.x;
-        x[1] = u.y;
-        x[2] = u.z;
-        x[3] = u.w;
+    float4 u[8];
+    __device__ __forceinline__ void load(const float* p, int lane) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = __ldcs(reinterpret_cast<const float4*>(p) + j * 32 + lane);
+    }
+    __device__ __forceinline__ void get(float (&x)[32]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[4 * j] = u[j].x;
+            x[4 * j + 1] = u[j].y;
+            x[4 * j + 2] = u[j].z;
+            x[4 * j + 3] = u[j].w;
+        }
     }
     static __device__ __forceinline__ float one(const float* p) { return *p; }
 };
@@ -99,16 +145,39 @@ struct BeamVec<float> {
 // A beam takes part when its score is finite; -inf is a beam that is not in use.
 __device__ __forceinline__ bool beam_live(float score) { return score > -INFINITY && score < INFINITY; }
 
-template <class T>
-__global__ void __launch_bounds__(128) beam_scan_kernel(const BeamParams p) {
-    constexpr int N = BeamVec<T>::N;
-    constexpr int NV = kBeamStep / (32 * N);
+__device__ __forceinline__ float max32(const float (&x)[32]) {
+    float t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = fmaxf(x[i], x[i + 4]);
+#pragma unroll
+    for (int i = 8; i < 32; i += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], x[i + k]), x[i + 4 + k]);
+    return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+}
+// Sum of exp(x - ref): the difference is taken first, so that the large terms, whose difference is small, are exact to
+// the exponential's own error.
+__device__ __forceinline__ float expsum32(const float (&x)[32], float ref) {
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t[i & 3] += __expf(x[i] - ref);
+    return (t[0] + t[1]) + (t[2] + t[3]);
+}
+
+template <class T, bool Vec>
+__global__ void __launch_bounds__(kBeamWarps * 32) beam_scan_kernel(const BeamParams p) {
+    using Step = BeamStep<T, Vec>;
+    constexpr int N = Step::N;
+    __shared__ unsigned long long floor_key;  // no entry below it is among the row's best `select`
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const long long item = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (item >= static_cast<long long>(p.batch) * p.beams * p.segs) return;
-    const long long row = item / p.segs;
-    const int seg = static_cast<int>(item - row * p.segs);
+    const int groups = (p.segs + kBeamWarps - 1) / kBeamWarps;  // CTAs per row
+    const long long row = blockIdx.x / groups;
+    const int seg = static_cast<int>(blockIdx.x - row * groups) * kBeamWarps + (threadIdx.x >> 5);
+    const long long item = row * p.segs + seg;
+    if (threadIdx.x == 0) floor_key = 0ull;
+    __syncthreads();
+    if (seg >= p.segs) return;
     unsigned long long* out = p.keys + item * p.select;
     const float score = __ldg(p.scores + row);
     if (!beam_live(score)) {
@@ -120,97 +189,94 @@ __global__ void __launch_bounds__(128) beam_scan_kernel(const BeamParams p) {
     }
     const T* base = static_cast<const T*>(p.logits) + row * p.row_stride;
     // vectors start at 16-byte boundaries: token = place - shift
-    const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15u) / sizeof(T));
+    const int shift = Vec ? static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15u) / sizeof(T)) : 0;
     const int end = p.vocab + shift;
     const int first = seg * p.seg_steps * kBeamStep;
     const int last = min(end, first + p.seg_steps * kBeamStep);
+    auto inside = [&](int at) { return at >= shift && at + kBeamStep <= end; };
     float m = -INFINITY, sum = 0.f;
-    unsigned long long best = 0ull, least = 0ull;  // the list (one entry per lane), its entry select - 1
-    bool bad = false, seeded = false;
+    unsigned long long best = 0ull, least = 0ull;  // the list (one entry per lane); what an entry has to exceed
+    bool bad = false;
+    Step raw;
+    if (first < last && inside(first)) raw.load(base + (first - shift), lane);
     for (int at = first; at < last; at += kBeamStep) {
-        BeamVec<T> raw[NV];
-        const bool inside = at >= shift && at + kBeamStep <= end;  // the whole warp's step
-        if (inside) {
+        float x[32];
+        unsigned live = 0xffffffffu;
+        const int place = at + lane * N - shift;  // token of this lane's first element
+        if (inside(at)) {
+            raw.get(x);
+        } else {  // a row's first or last step
 #pragma unroll
-            for (int j = 0; j < NV; ++j) raw[j].load(base + (at + (j * 32 + lane) * N - shift));
-        }
-        unsigned long long mine = 0ull;  // seeding: this lane's best of the step
-#pragma unroll 1
-        for (int pass = seeded ? 1 : 0; pass < 2; ++pass) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                float x[N];
-                const int place = at + (j * 32 + lane) * N;
-                unsigned live = (1u << N) - 1u;
-                if (inside) {
-                    raw[j].get(x);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const int tok = place + i - shift;
-                        const bool in = tok >= 0 && tok < p.vocab;
-                        x[i] = in ? BeamVec<T>::one(base + tok) : -INFINITY;
-                        if (!in) live &= ~(1u << i);
-                    }
-                }
-                float vm = x[0];
-#pragma unroll
-                for (int i = 1; i < N; ++i) vm = fmaxf(vm, x[i]);
-                // NaN and +inf count as -inf.  A sum shows both: fmaxf drops a NaN, but the sum keeps it.
-                float chk = 0.f;
-#pragma unroll
-                for (int i = 0; i < N; ++i) chk += x[i];
-                if (!(chk < INFINITY) || !(vm < INFINITY)) {
-                    vm = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        if (!(x[i] < INFINITY)) {
-                            x[i] = -INFINITY;
-                            bad = true;
-                        }
-                        vm = fmaxf(vm, x[i]);
-                    }
-                }
-                if (pass == 0) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const unsigned long long key = (live >> i) & 1u ? beam_key(x[i], place + i - shift) : 0ull;
-                        mine = key > mine ? key : mine;
-                    }
-                    continue;
-                }
-                const float mn = fmaxf(m, vm);
-                if (mn > -INFINITY) {
-                    sum *= __expf(m - mn);
-                    m = mn;
-#pragma unroll
-                    for (int i = 0; i < N; ++i) sum += __expf(x[i] - mn);
-                }
-                const uint32_t least_hi = static_cast<uint32_t>(least >> 32);
-                if (!__any_sync(0xffffffffu, ordered32(vm + 0.f) >= least_hi)) continue;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const unsigned long long key = (live >> i) & 1u ? beam_key(x[i], place + i - shift) : 0ull;
-                    // entries of the seed come by again: the list never holds a key twice
-                    unsigned who = __ballot_sync(0xffffffffu, key > least && key != mine);
-                    while (who) {
-                        const int src = __ffs(who) - 1;
-                        who &= who - 1;
-                        const unsigned long long add = __shfl_sync(0xffffffffu, key, src);
-                        if (add <= least) continue;
-                        const int rank = __popc(__ballot_sync(0xffffffffu, best > add));
-                        const unsigned long long up = __shfl_up_sync(0xffffffffu, best, 1);
-                        best = lane < rank ? best : lane == rank ? add : up;
-                        least = __shfl_sync(0xffffffffu, best, p.select - 1);
-                    }
-                }
-            }
-            if (pass == 0) {
-                best = warp_sort_desc(mine, lane);
-                least = __shfl_sync(0xffffffffu, best, p.select - 1);
-                seeded = true;
+            for (int e = 0; e < 32; ++e) {
+                const int tok = place + (e / N) * 32 * N + e % N;
+                const bool in = tok >= 0 && tok < p.vocab;
+                x[e] = in ? Step::one(base + tok) : -INFINITY;
+                if (!in) live &= ~(1u << e);
             }
         }
+        if (at + kBeamStep < last && inside(at + kBeamStep)) raw.load(base + (at + kBeamStep - shift), lane);
+        float top = max32(x);
+        float mn = fmaxf(m, top);
+        float add = expsum32(x, mn > -INFINITY ? mn : 0.f);
+        if (!(add <= 32.f)) {  // NaN or +inf among them, which count as -inf (each term is at most 1)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if (!(x[e] < INFINITY)) x[e] = -INFINITY;
+            bad = true;
+            top = max32(x);
+            mn = fmaxf(m, top);
+            add = expsum32(x, mn > -INFINITY ? mn : 0.f);
+        }
+        if (mn > -INFINITY) {
+            sum = sum * __expf(m - mn) + add;
+            m = mn;
+        }
+        unsigned done = 0u;  // elements that the seed holds already
+        if (at == first) {
+            int arg = 31;
+#pragma unroll
+            for (int e = 31; e >= 0; --e)
+                if (x[e] == top && ((live >> e) & 1u)) arg = e;
+            const bool any = (live >> arg) & 1u;
+            best = warp_sort_desc(any ? beam_key(top, place + (arg / N) * 32 * N + arg % N) : 0ull, lane);
+            done = 1u << arg;
+            least = __shfl_sync(0xffffffffu, best, p.select - 1);
+        }
+        const unsigned long long known = *reinterpret_cast<volatile unsigned long long*>(&floor_key);
+        least = known > least ? known : least;
+        const float lv = least ? unordered32(static_cast<uint32_t>(least >> 32)) : -INFINITY;
+        if (!__any_sync(0xffffffffu, top >= lv)) continue;
+        const int ltok = least ? static_cast<int>(~static_cast<uint32_t>(least)) : 0x7fffffff;
+        unsigned pass = 0u;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            const int tok = place + (e / N) * 32 * N + e % N;
+            if (x[e] > lv || (x[e] == lv && tok < ltok)) pass |= 1u << e;
+        }
+        pass &= live & ~done;
+        bool grown = at == first;
+        while (__any_sync(0xffffffffu, pass != 0u)) {
+            const int e = __ffs(pass) - 1;  // -1: nothing left in this lane
+            float v = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v = e == i ? x[i] : v;
+            const unsigned long long key = pass ? beam_key(v, place + (e / N) * 32 * N + e % N) : 0ull;
+            pass &= pass - 1u;
+            unsigned who = __ballot_sync(0xffffffffu, key > least);
+            while (who) {
+                const int src = __ffs(who) - 1;
+                who &= who - 1u;
+                const unsigned long long in = __shfl_sync(0xffffffffu, key, src);
+                if (in <= least) continue;
+                const int rank = __popc(__ballot_sync(0xffffffffu, best > in));
+                const unsigned long long up = __shfl_up_sync(0xffffffffu, best, 1);
+                best = lane < rank ? best : lane == rank ? in : up;
+                const unsigned long long own = __shfl_sync(0xffffffffu, best, p.select - 1);
+                least = own > least ? own : least;
+                grown = true;
+            }
+        }
+        if (grown && lane == 0 && least > known) atomicMax(&floor_key, least);
     }
     float top = m;
 #pragma unroll
@@ -232,79 +298,77 @@ __device__ __forceinline__ int best_lane(uint32_t hi, uint32_t lo, uint32_t plac
     return __ffs(__ballot_sync(0xffffffffu, in && place == w)) - 1;
 }
 
-struct BeamEntry {
-    uint32_t hi, lo, place;  // ordered 64-bit value (0, 0: none), beam << 26 | token
-};
-
-__global__ void __launch_bounds__(kBeamLists) beam_pick_kernel(const BeamParams p) {
-    extern __shared__ unsigned long long keys[];  // [lists][select]
+__global__ void __launch_bounds__(256) beam_pick_kernel(const BeamParams p) {
+    __shared__ unsigned long long keys[kBeamMost][kBeamMost];  // [beam][entry]
     __shared__ double lse[kBeamMost];
-    __shared__ BeamEntry won[kBeamLists / 32][kBeamMost];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int lists = p.beams * p.segs, warps = (lists + 31) >> 5;
-    const long long list0 = static_cast<long long>(blockIdx.x) * lists;
+    const long long row0 = static_cast<long long>(blockIdx.x) * p.beams;
     griddep_wait();
-    for (int i = threadIdx.x; i < lists * p.select; i += blockDim.x) keys[i] = __ldcg(p.keys + list0 * p.select + i);
-    // log-sum-exp of each beam, a warp per beam
-    for (int b = warp; b < p.beams; b += blockDim.x >> 5) {
+    for (int b = warp; b < p.beams; b += 8) {
+        const long long item0 = (row0 + b) * p.segs;
+        // the beam's lists become one
+        unsigned long long best = 0ull;
+        for (int s0 = 0; s0 < p.segs; s0 += 8) {
+            unsigned long long k[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                k[i] = s0 + i < p.segs && lane < p.select ? __ldcg(p.keys + (item0 + s0 + i) * p.select + lane) : 0ull;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (s0 + i < p.segs) best = warp_merge_desc(best, k[i], lane);
+        }
+        keys[b][lane] = best;
+        // and its sums of exponentials
+        float2 ml[kBeamSegs / 32];
         float top = -INFINITY;
-        for (int s = lane; s < p.segs; s += 32) top = fmaxf(top, __ldcg(p.seg_ml + list0 + b * p.segs + s).x);
+#pragma unroll
+        for (int i = 0; i < kBeamSegs / 32; ++i) {
+            const int s = i * 32 + lane;
+            ml[i] = s < p.segs ? __ldcg(p.seg_ml + item0 + s) : make_float2(-INFINITY, 0.f);
+            top = fmaxf(top, ml[i].x);
+        }
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         double total = 0.0;
-        if (top > -INFINITY)
-            for (int s = lane; s < p.segs; s += 32) {
-                const float2 ml = __ldcg(p.seg_ml + list0 + b * p.segs + s);
-                if (ml.x > -INFINITY) total += static_cast<double>(ml.y) * exp(static_cast<double>(ml.x) - top);
-            }
+#pragma unroll
+        for (int i = 0; i < kBeamSegs / 32; ++i)
+            if (ml[i].x > -INFINITY) total += static_cast<double>(ml[i].y) * exp(static_cast<double>(ml[i].x) - top);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
         if (lane == 0) lse[b] = top > -INFINITY ? top + log(total) : -static_cast<double>(INFINITY);
     }
     __syncthreads();
-    // each lane's list, its head as a value in 64 bits
-    BeamEntry e{0u, 0u, 0xffffffffu};
+    if (warp != 0) return;
+    // one lane per beam, its best continuation left as a value in 64 bits
+    uint32_t hi = 0u, lo = 0u, place = 0xffffffffu;  // ordered value (0, 0: none), beam << 26 | token
     int next = 0;
-    const int list = threadIdx.x, beam = list / p.segs;
+    const float score = lane < p.beams ? __ldg(p.scores + row0 + lane) : -INFINITY;
+    const double beam_lse = lane < p.beams ? lse[lane] : 0.0;
     auto head = [&] {
-        e = BeamEntry{0u, 0u, 0xffffffffu};
-        if (list >= lists || next >= p.select) return;
-        const unsigned long long key = keys[list * p.select + next];
+        hi = lo = 0u;
+        place = 0xffffffffu;
+        const unsigned long long key = lane < p.beams && next < p.select ? keys[lane][next] : 0ull;
         if (!key) return;
         const float x = unordered32(static_cast<uint32_t>(key >> 32));
-        const float score = __ldg(p.scores + static_cast<long long>(blockIdx.x) * p.beams + beam);
-        const double v = x > -INFINITY && beam_live(score) ? score + (x - lse[beam]) : -static_cast<double>(INFINITY);
+        const double v = x > -INFINITY && beam_live(score) ? score + (x - beam_lse) : -static_cast<double>(INFINITY);
         const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v + 0.0));
         const unsigned long long o = b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
-        e = BeamEntry{static_cast<uint32_t>(o >> 32), static_cast<uint32_t>(o),
-                      (static_cast<uint32_t>(beam) << kBeamTokenBits) | ~static_cast<uint32_t>(key)};
+        hi = static_cast<uint32_t>(o >> 32);
+        lo = static_cast<uint32_t>(o);
+        place = (static_cast<uint32_t>(lane) << kBeamTokenBits) | ~static_cast<uint32_t>(key);
     };
-    if (warp < warps) {
-        head();
-        for (int r = 0; r < p.select; ++r) {
-            const int w = best_lane(e.hi, e.lo, e.place);
-            if (lane == w) {
-                won[warp][r] = e;
-                ++next;
-                head();
-            }
-        }
-    }
-    __syncthreads();
-    if (warp != 0) return;
-    next = 0;
-    e = lane < warps ? won[lane][0] : BeamEntry{0u, 0u, 0xffffffffu};
+    head();
     for (int r = 0; r < p.select; ++r) {
-        const int w = best_lane(e.hi, e.lo, e.place);
+        const int w = best_lane(hi, lo, place);
         if (lane == w) {
-            const unsigned long long o = (static_cast<unsigned long long>(e.hi) << 32) | e.lo;
+            const unsigned long long o = (static_cast<unsigned long long>(hi) << 32) | lo;
             const unsigned long long b = o ^ ((o >> 63) ? 0x8000000000000000ull : ~0ull);
             const long long at = static_cast<long long>(blockIdx.x) * p.select + r;
             p.out_scores[at] = static_cast<float>(__longlong_as_double(static_cast<long long>(b)));
-            p.out_parents[at] = static_cast<int32_t>(e.place >> kBeamTokenBits);
-            p.out_tokens[at] = static_cast<int32_t>(e.place & ((1u << kBeamTokenBits) - 1u));
+            p.out_parents[at] = lane;
+            p.out_tokens[at] = static_cast<int32_t>(place & ((1u << kBeamTokenBits) - 1u));
             ++next;
-            e = next < p.select && lane < warps ? won[lane][next] : BeamEntry{0u, 0u, 0xffffffffu};
+            head();
         }
     }
 }
@@ -314,15 +378,13 @@ __global__ void __launch_bounds__(kBeamLists) beam_pick_kernel(const BeamParams 
 namespace kvpi {
 namespace {
 
-// Segments of a row: enough warps to fill the GPU about twice (32 resident warps an SM cover the memory latency with
-// four 16-byte loads a lane each), none shorter than one step, and no more lists per request than the picking CTA has
-// threads and shared memory for.
+// Segments of a row: about 24 warps for each processor -- what the scan's registers let reside -- in fours, since a CTA's
+// warps share what they have found; none shorter than one step.
 void plan_beam(const kvp_beam_args& a, int* segs, int* steps) {
     const long long rows = static_cast<long long>(a.batch) * a.beams;
     const long long total = (static_cast<long long>(a.vocab) + 7 + kvpd::kBeamStep - 1) / kvpd::kBeamStep;
-    const long long want = std::max<long long>(1, static_cast<long long>(sm_count()) * 64 / std::max<long long>(rows, 1));
-    const long long most = std::min(kvpd::kBeamLists / a.beams, kvpd::kBeamEntries / (a.beams * a.select));
-    const long long n = std::min(std::min(want, most), total);
+    const long long want = (static_cast<long long>(sm_count()) * 24 / std::max<long long>(rows, 1) + 3) / 4 * 4;
+    const long long n = std::max<long long>(1, std::min(std::min<long long>(want, kvpd::kBeamSegs), total));
     *steps = static_cast<int>((total + n - 1) / n);
     *segs = static_cast<int>((total + *steps - 1) / *steps);
 }
@@ -382,20 +444,20 @@ extern "C" KVP_API int kvp_beam_select(const kvp_beam_args* a, void* stream) {
     p.vocab = a->vocab;
     p.select = a->select;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const unsigned grid = static_cast<unsigned>((items + 3) / 4);
-    if (a->logits_dtype == KVP_DTYPE_F32)
-        kvpd::beam_scan_kernel<float><<<grid, 128, 0, s>>>(p);
-    else if (a->logits_dtype == KVP_DTYPE_F16)
-        kvpd::beam_scan_kernel<__half><<<grid, 128, 0, s>>>(p);
-    else
-        kvpd::beam_scan_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
+    const unsigned grid = static_cast<unsigned>(static_cast<size_t>(a->batch) * a->beams *
+                                                ((p.segs + kvpd::kBeamWarps - 1) / kvpd::kBeamWarps));
+    const bool vec = a->beams == 1 || (p.row_stride * dtype_bytes(a->logits_dtype)) % 16 == 0;
+    auto scan = a->logits_dtype == KVP_DTYPE_F32   ? (vec ? kvpd::beam_scan_kernel<float, true> : kvpd::beam_scan_kernel<float, false>)
+                : a->logits_dtype == KVP_DTYPE_F16 ? (vec ? kvpd::beam_scan_kernel<__half, true> : kvpd::beam_scan_kernel<__half, false>)
+                                                   : (vec ? kvpd::beam_scan_kernel<__nv_bfloat16, true>
+                                                          : kvpd::beam_scan_kernel<__nv_bfloat16, false>);
+    scan<<<grid, kvpd::kBeamWarps * 32, 0, s>>>(p);
     rc = cuda_status(cudaGetLastError(), "beam scan launch");
     if (rc != KVP_OK) return rc;
     // the second kernel's launch overlaps the first one's run; it waits for it before its first read
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a->batch));
-    cfg.blockDim = dim3(kvpd::kBeamLists);
-    cfg.dynamicSmemBytes = static_cast<size_t>(a->beams) * p.segs * a->select * 8;
+    cfg.blockDim = dim3(256);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
