@@ -27,6 +27,7 @@ constexpr int kBeamMost = 32;    // beams and selected continuations per request
 constexpr int kBeamSegs = 64;    // segments of a row
 constexpr int kBeamStep = 1024;  // logits a warp takes at once, 32 per lane
 constexpr int kBeamWarps = 4;    // warps per CTA of the scan, all on one row
+constexpr int kPickWarps = 16;
 constexpr int kBeamTokenBits = 26;
 
 struct BeamParams {
@@ -155,17 +156,36 @@ __device__ __forceinline__ float max32(const float (&x)[32]) {
         for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], x[i + k]), x[i + 4 + k]);
     return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
 }
-// Sum of exp(x - ref): the difference is taken first, so that the large terms, whose difference is small, are exact to
-// the exponential's own error.
+// Sum of exp(x - ref), two at a time: the difference is taken first, so that the large terms, whose difference is small,
+// are exact to the exponential's own error.
 __device__ __forceinline__ float expsum32(const float (&x)[32], float ref) {
-    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint64_t back = pack2(-ref, -ref), log2e = pack2(1.4426950408889634f, 1.4426950408889634f);
+    uint64_t t[2] = {0ull, 0ull};
 #pragma unroll
-    for (int i = 0; i < 32; ++i) t[i & 3] += __expf(x[i] - ref);
-    return (t[0] + t[1]) + (t[2] + t[3]);
+    for (int i = 0; i < 16; ++i) {
+        const float2 d = unpack2(mul2(add2(pack2(x[2 * i], x[2 * i + 1]), back), log2e));
+        t[i & 1] = add2(t[i & 1], pack2(fast_exp2(d.x), fast_exp2(d.y)));
+    }
+    const float2 r = unpack2(add2(t[0], t[1]));
+    return r.x + r.y;
+}
+__device__ __forceinline__ float exp_of(float d) { return fast_exp2(d * 1.4426950408889634f); }
+
+// Element e of a lane's 32, e different from lane to lane: a tree of selections instead of an array in memory.
+__device__ __forceinline__ float pick32(const float (&x)[32], int e) {
+    float t[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[i] = e & 16 ? x[i + 16] : x[i];
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < w) t[i] = e & w ? t[i + w] : t[i];
+    return t[0];
 }
 
 template <class T, bool Vec>
-__global__ void __launch_bounds__(kBeamWarps * 32) beam_scan_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(kBeamWarps * 32, 5) beam_scan_kernel(const BeamParams p) {
     using Step = BeamStep<T, Vec>;
     constexpr int N = Step::N;
     __shared__ unsigned long long floor_key;  // no entry below it is among the row's best `select`
@@ -228,7 +248,7 @@ __global__ void __launch_bounds__(kBeamWarps * 32) beam_scan_kernel(const BeamPa
             add = expsum32(x, mn > -INFINITY ? mn : 0.f);
         }
         if (mn > -INFINITY) {
-            sum = sum * __expf(m - mn) + add;
+            sum = sum * exp_of(m - mn) + add;
             m = mn;
         }
         unsigned done = 0u;  // elements that the seed holds already
@@ -245,22 +265,25 @@ __global__ void __launch_bounds__(kBeamWarps * 32) beam_scan_kernel(const BeamPa
         const unsigned long long known = *reinterpret_cast<volatile unsigned long long*>(&floor_key);
         least = known > least ? known : least;
         const float lv = least ? unordered32(static_cast<uint32_t>(least >> 32)) : -INFINITY;
-        if (!__any_sync(0xffffffffu, top >= lv)) continue;
+        // A value equal to the last entry's counts only before that entry's token, which lies ahead only where another warp
+        // set the floor.
         const int ltok = least ? static_cast<int>(~static_cast<uint32_t>(least)) : 0x7fffffff;
+        const bool ties = at - shift < ltok;
+        if (!__any_sync(0xffffffffu, top > lv || (ties && top == lv))) continue;
         unsigned pass = 0u;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            const int tok = place + (e / N) * 32 * N + e % N;
-            if (x[e] > lv || (x[e] == lv && tok < ltok)) pass |= 1u << e;
+        for (int e = 0; e < 32; ++e)
+            if (x[e] > lv) pass |= 1u << e;
+        if (ties) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if (x[e] == lv && place + (e / N) * 32 * N + e % N < ltok) pass |= 1u << e;
         }
         pass &= live & ~done;
         bool grown = at == first;
         while (__any_sync(0xffffffffu, pass != 0u)) {
             const int e = __ffs(pass) - 1;  // -1: nothing left in this lane
-            float v = 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v = e == i ? x[i] : v;
-            const unsigned long long key = pass ? beam_key(v, place + (e / N) * 32 * N + e % N) : 0ull;
+            const unsigned long long key = pass ? beam_key(pick32(x, e), place + (e / N) * 32 * N + e % N) : 0ull;
             pass &= pass - 1u;
             unsigned who = __ballot_sync(0xffffffffu, key > least);
             while (who) {
@@ -281,7 +304,7 @@ __global__ void __launch_bounds__(kBeamWarps * 32) beam_scan_kernel(const BeamPa
     float top = m;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    float total = top > -INFINITY ? sum * __expf(m - top) : 0.f;
+    float total = top > -INFINITY ? sum * exp_of(m - top) : 0.f;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
     if (lane == 0) p.seg_ml[item] = make_float2(top, total);
@@ -298,46 +321,62 @@ __device__ __forceinline__ int best_lane(uint32_t hi, uint32_t lo, uint32_t plac
     return __ffs(__ballot_sync(0xffffffffu, in && place == w)) - 1;
 }
 
-__global__ void __launch_bounds__(256) beam_pick_kernel(const BeamParams p) {
-    __shared__ unsigned long long keys[kBeamMost][kBeamMost];  // [beam][entry]
+__global__ void __launch_bounds__(kPickWarps * 32) beam_pick_kernel(const BeamParams p) {
+    __shared__ unsigned long long part[kPickWarps][32];
+    __shared__ unsigned long long keys[kBeamMost][32];  // [beam][entry]
     __shared__ double lse[kBeamMost];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row0 = static_cast<long long>(blockIdx.x) * p.beams;
+    const int per = max(1, kPickWarps / p.beams);  // warps that share a beam's lists
+    auto fold = [&](unsigned long long best, unsigned long long k) {  // only a list whose head gets in
+        return __shfl_sync(0xffffffffu, k, 0) > __shfl_sync(0xffffffffu, best, p.select - 1) ? warp_merge_desc(best, k, lane) : best;
+    };
     griddep_wait();
-    for (int b = warp; b < p.beams; b += 8) {
-        const long long item0 = (row0 + b) * p.segs;
-        // the beam's lists become one
-        unsigned long long best = 0ull;
-        for (int s0 = 0; s0 < p.segs; s0 += 8) {
-            unsigned long long k[8];
+    for (int b0 = 0; b0 < p.beams; b0 += kPickWarps) {
+        const int b = b0 + warp / per, sub = warp % per;
+        const bool mine = b < p.beams && warp < per * p.beams;
+        if (mine) {
+            const long long item0 = (row0 + b) * p.segs;
+            unsigned long long best = 0ull;
+            for (int s0 = sub; s0 < p.segs; s0 += 4 * per) {
+                unsigned long long k[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                k[i] = s0 + i < p.segs && lane < p.select ? __ldcg(p.keys + (item0 + s0 + i) * p.select + lane) : 0ull;
+                for (int i = 0; i < 4; ++i) {
+                    const int seg = s0 + i * per;
+                    k[i] = seg < p.segs && lane < p.select ? __ldcg(p.keys + (item0 + seg) * p.select + lane) : 0ull;
+                }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (s0 + i < p.segs) best = warp_merge_desc(best, k[i], lane);
+                for (int i = 0; i < 4; ++i) best = fold(best, k[i]);
+            }
+            part[warp][lane] = best;
+            if (sub == 0) {  // the beam's sums of exponentials, in 64 bits
+                float2 ml[kBeamSegs / 32];
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kBeamSegs / 32; ++i) {
+                    const int s = i * 32 + lane;
+                    ml[i] = s < p.segs ? __ldcg(p.seg_ml + item0 + s) : make_float2(-INFINITY, 0.f);
+                    top = fmaxf(top, ml[i].x);
+                }
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                double total = 0.0;
+#pragma unroll
+                for (int i = 0; i < kBeamSegs / 32; ++i)
+                    if (ml[i].x > -INFINITY) total += static_cast<double>(ml[i].y) * exp(static_cast<double>(ml[i].x) - top);
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+                if (lane == 0) lse[b] = top > -INFINITY ? top + log(total) : -static_cast<double>(INFINITY);
+            }
         }
-        keys[b][lane] = best;
-        // and its sums of exponentials
-        float2 ml[kBeamSegs / 32];
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kBeamSegs / 32; ++i) {
-            const int s = i * 32 + lane;
-            ml[i] = s < p.segs ? __ldcg(p.seg_ml + item0 + s) : make_float2(-INFINITY, 0.f);
-            top = fmaxf(top, ml[i].x);
+        __syncthreads();
+        if (mine && sub == 0) {
+            unsigned long long best = part[warp][lane];
+            for (int i = 1; i < per; ++i) best = fold(best, part[warp + i][lane]);
+            keys[b][lane] = best;
         }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        double total = 0.0;
-#pragma unroll
-        for (int i = 0; i < kBeamSegs / 32; ++i)
-            if (ml[i].x > -INFINITY) total += static_cast<double>(ml[i].y) * exp(static_cast<double>(ml[i].x) - top);
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-        if (lane == 0) lse[b] = top > -INFINITY ? top + log(total) : -static_cast<double>(INFINITY);
+        __syncthreads();
     }
-    __syncthreads();
     if (warp != 0) return;
     // one lane per beam, its best continuation left as a value in 64 bits
     uint32_t hi = 0u, lo = 0u, place = 0xffffffffu;  // ordered value (0, 0: none), beam << 26 | token
@@ -378,12 +417,12 @@ __global__ void __launch_bounds__(256) beam_pick_kernel(const BeamParams p) {
 namespace kvpi {
 namespace {
 
-// Segments of a row: about 24 warps for each processor -- what the scan's registers let reside -- in fours, since a CTA's
+// Segments of a row: about 20 warps for each processor -- what the scan's registers let reside -- in fours, since a CTA's
 // warps share what they have found; none shorter than one step.
 void plan_beam(const kvp_beam_args& a, int* segs, int* steps) {
     const long long rows = static_cast<long long>(a.batch) * a.beams;
     const long long total = (static_cast<long long>(a.vocab) + 7 + kvpd::kBeamStep - 1) / kvpd::kBeamStep;
-    const long long want = (static_cast<long long>(sm_count()) * 24 / std::max<long long>(rows, 1) + 3) / 4 * 4;
+    const long long want = (static_cast<long long>(sm_count()) * 20 / std::max<long long>(rows, 1) + 3) / 4 * 4;
     const long long n = std::max<long long>(1, std::min(std::min<long long>(want, kvpd::kBeamSegs), total));
     *steps = static_cast<int>((total + n - 1) / n);
     *segs = static_cast<int>((total + *steps - 1) / *steps);
@@ -457,7 +496,7 @@ extern "C" KVP_API int kvp_beam_select(const kvp_beam_args* a, void* stream) {
     // the second kernel's launch overlaps the first one's run; it waits for it before its first read
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a->batch));
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(kvpd::kPickWarps * 32);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

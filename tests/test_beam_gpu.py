@@ -10,7 +10,7 @@ exponential is off by at most 2 + 1.16 |d| ulps of 2^-23 for an argument d <= 0 
 weighted by its value e^d: at most 3 ulps of the largest term for any d; an addition adds half an ulp, and a lane adds at
 most 32 times the steps of its segment plus a rescaling, the warp five more.  So the sum's relative error, which is
 the logarithm's absolute one, is at most (16 + 64 steps) 2^-24.  A segment has as many steps of 1024 tokens as the row's
-steps over the segments it is cut into, at most 64, for about 24 warps on each of 148 processors."""
+steps over the segments it is cut into, at most 64, for about 20 warps on each of 148 processors."""
 import math
 
 import numpy as np
@@ -21,7 +21,7 @@ pytestmark = pytest.mark.gpu
 
 def _steps(batch, beams, vocab, select):
     total = -(-(vocab + 7) // 1024)
-    segments = min((148 * 24 // (batch * beams) + 3) // 4 * 4, 64, total)
+    segments = min((148 * 20 // (batch * beams) + 3) // 4 * 4, 64, total)
     return -(-total // max(1, segments))
 
 
