@@ -2,7 +2,7 @@
 //     value = score[beam] + logit[beam][token] - log(sum over tokens of exp(logit[beam][.])),
 // ties to the lower beam, then the lower token.  One read of the logits, two launches.
 //
-// beam_scan_kernel (bound by HBM): a warp takes one segment of one row, 1024 logits a step, the next step's loads in flight
+// beam_scan_kernel (bound by HBM): a warp takes one segment of one row, 512 logits a step, the next step's loads in flight
 // while it works on this one's.  It keeps a running maximum and sum of exponentials per lane, and the segment's best
 // `select` logits as a list sorted over its 32 lanes; within a row the order of the values is the order of the logits, so
 // no logarithm is needed here.  The list starts from the lanes' own maxima of the first step (one sort); of the rest only
@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kvp_device.cuh"
 #include "kvp_internal.h"
@@ -24,9 +25,11 @@
 namespace kvpd {
 
 constexpr int kBeamMost = 32;    // beams and selected continuations per request: a warp's lanes
-constexpr int kBeamSegs = 64;    // segments of a row
-constexpr int kBeamStep = 1024;  // logits a warp takes at once, 32 per lane
+constexpr int kBeamSegs = 32;    // segments of a row
+constexpr int kBeamLane = 16;    // logits a lane takes at once
+constexpr int kBeamStep = 32 * kBeamLane;
 constexpr int kBeamWarps = 4;    // warps per CTA of the scan, all on one row
+constexpr int kBeamShows = 6;    // times a CTA's warps compare their lists
 constexpr int kPickWarps = 16;
 constexpr int kBeamTokenBits = 26;
 
@@ -81,21 +84,21 @@ __device__ __forceinline__ unsigned long long warp_merge_desc(unsigned long long
     return v;
 }
 
-// One step of a row, 32 logits per lane: element e of a lane is token at + ((e / N) * 32 + lane) * N + e % N - shift.
+// One step of a row, 16 logits per lane: element e of a lane is token at + ((e / N) * 32 + lane) * N + e % N - shift.
 // Vec: 16-byte loads, where all rows of a request lie alike against 16-byte boundaries.  Else single loads of
 // neighbouring tokens by neighbouring lanes: with an odd vocabulary the rows start at different offsets, and vectors would
 // group the sums of two equal rows differently, so that their tie fell to a rounding.
 template <class T, bool Vec>
 struct BeamStep {
     static constexpr int N = 1;
-    T u[32];
+    T u[kBeamLane];
     __device__ __forceinline__ void load(const T* p, int lane) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) u[j] = __ldcs(p + j * 32 + lane);
+        for (int j = 0; j < kBeamLane; ++j) u[j] = __ldcs(p + j * 32 + lane);
     }
-    __device__ __forceinline__ void get(float (&x)[32]) const {
+    __device__ __forceinline__ void get(float (&x)[kBeamLane]) const {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] = one(u + j);
+        for (int j = 0; j < kBeamLane; ++j) x[j] = one(u + j);
     }
     static __device__ __forceinline__ float one(const T* p) {
         if constexpr (sizeof(T) == 4) return *p;
@@ -105,14 +108,14 @@ struct BeamStep {
 template <class T>
 struct BeamStep<T, true> {  // 16-bit logits: 8 per vector
     static constexpr int N = 8;
-    uint4 u[4];
+    uint4 u[kBeamLane / 8];
     __device__ __forceinline__ void load(const T* p, int lane) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = __ldcs(reinterpret_cast<const uint4*>(p) + j * 32 + lane);
+        for (int j = 0; j < kBeamLane / 8; ++j) u[j] = __ldcs(reinterpret_cast<const uint4*>(p) + j * 32 + lane);
     }
-    __device__ __forceinline__ void get(float (&x)[32]) const {
+    __device__ __forceinline__ void get(float (&x)[kBeamLane]) const {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kBeamLane / 8; ++j) {
             const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -126,14 +129,14 @@ struct BeamStep<T, true> {  // 16-bit logits: 8 per vector
 template <>
 struct BeamStep<float, true> {
     static constexpr int N = 4;
-    float4 u[8];
+    float4 u[kBeamLane / 4];
     __device__ __forceinline__ void load(const float* p, int lane) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = __ldcs(reinterpret_cast<const float4*>(p) + j * 32 + lane);
+        for (int j = 0; j < kBeamLane / 4; ++j) u[j] = __ldcs(reinterpret_cast<const float4*>(p) + j * 32 + lane);
     }
-    __device__ __forceinline__ void get(float (&x)[32]) const {
+    __device__ __forceinline__ void get(float (&x)[kBeamLane]) const {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < kBeamLane / 4; ++j) {
             x[4 * j] = u[j].x;
             x[4 * j + 1] = u[j].y;
             x[4 * j + 2] = u[j].z;
@@ -146,23 +149,24 @@ struct BeamStep<float, true> {
 // A beam takes part when its score is finite; -inf is a beam that is not in use.
 __device__ __forceinline__ bool beam_live(float score) { return score > -INFINITY && score < INFINITY; }
 
-__device__ __forceinline__ float max32(const float (&x)[32]) {
-    float t[4];
+// Maxima of each group of eight, and of all.
+__device__ __forceinline__ float max_of(const float (&x)[kBeamLane], float (&group)[kBeamLane / 8]) {
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = fmaxf(x[i], x[i + 4]);
-#pragma unroll
-    for (int i = 8; i < 32; i += 8)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) t[k] = fmaxf(fmaxf(t[k], x[i + k]), x[i + 4 + k]);
-    return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+    for (int g = 0; g < kBeamLane / 8; ++g) {
+        const float a = fmaxf(fmaxf(x[8 * g], x[8 * g + 1]), x[8 * g + 2]), b = fmaxf(fmaxf(x[8 * g + 3], x[8 * g + 4]), x[8 * g + 5]);
+        group[g] = fmaxf(fmaxf(a, b), fmaxf(x[8 * g + 6], x[8 * g + 7]));
+        top = fmaxf(top, group[g]);
+    }
+    return top;
 }
 // Sum of exp(x - ref), two at a time: the difference is taken first, so that the large terms, whose difference is small,
 // are exact to the exponential's own error.
-__device__ __forceinline__ float expsum32(const float (&x)[32], float ref) {
+__device__ __forceinline__ float expsum(const float (&x)[kBeamLane], float ref) {
     const uint64_t back = pack2(-ref, -ref), log2e = pack2(1.4426950408889634f, 1.4426950408889634f);
     uint64_t t[2] = {0ull, 0ull};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < kBeamLane / 2; ++i) {
         const float2 d = unpack2(mul2(add2(pack2(x[2 * i], x[2 * i + 1]), back), log2e));
         t[i & 1] = add2(t[i & 1], pack2(fast_exp2(d.x), fast_exp2(d.y)));
     }
@@ -171,29 +175,38 @@ __device__ __forceinline__ float expsum32(const float (&x)[32], float ref) {
 }
 __device__ __forceinline__ float exp_of(float d) { return fast_exp2(d * 1.4426950408889634f); }
 
-// Element e of a lane's 32, e different from lane to lane: a tree of selections instead of an array in memory.
-__device__ __forceinline__ float pick32(const float (&x)[32], int e) {
-    float t[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t[i] = e & 16 ? x[i + 16] : x[i];
-#pragma unroll
-    for (int w = 8; w > 0; w >>= 1)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < w) t[i] = e & w ? t[i + w] : t[i];
-    return t[0];
+// Named barrier 1 + k, with a constant number: a number from a register would claim all sixteen for each CTA, and four
+// CTAs an SM would be the most.
+__device__ __forceinline__ void barrier_of(int k, bool only_arrive, int threads) {
+    auto at = [&](auto id) {
+        if (only_arrive)
+            asm volatile("bar.arrive %0, %1;" ::"n"(decltype(id)::value), "r"(threads) : "memory");
+        else
+            asm volatile("bar.sync %0, %1;" ::"n"(decltype(id)::value), "r"(threads) : "memory");
+    };
+    switch (k) {
+        case 0: at(std::integral_constant<int, 1>{}); break;
+        case 1: at(std::integral_constant<int, 2>{}); break;
+        case 2: at(std::integral_constant<int, 3>{}); break;
+        case 3: at(std::integral_constant<int, 4>{}); break;
+        case 4: at(std::integral_constant<int, 5>{}); break;
+        default: at(std::integral_constant<int, 6>{}); break;
+    }
 }
 
 template <class T, bool Vec>
-__global__ void __launch_bounds__(kBeamWarps * 32, 5) beam_scan_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const BeamParams p) {
     using Step = BeamStep<T, Vec>;
     constexpr int N = Step::N;
     __shared__ unsigned long long floor_key;  // no entry below it is among the row's best `select`
+    __shared__ unsigned long long shown[kBeamShows][kBeamWarps][32];
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int groups = (p.segs + kBeamWarps - 1) / kBeamWarps;  // CTAs per row
     const long long row = blockIdx.x / groups;
-    const int seg = static_cast<int>(blockIdx.x - row * groups) * kBeamWarps + (threadIdx.x >> 5);
+    const int warp = threadIdx.x >> 5;
+    const int seg = static_cast<int>(blockIdx.x - row * groups) * kBeamWarps + warp;
+    const int partners = min(kBeamWarps, p.segs - (seg - warp));  // warps of this CTA that have a segment
     const long long item = row * p.segs + seg;
     if (threadIdx.x == 0) floor_key = 0ull;
     __syncthreads();
@@ -217,17 +230,35 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 5) beam_scan_kernel(const Bea
     float m = -INFINITY, sum = 0.f;
     unsigned long long best = 0ull, least = 0ull;  // the list (one entry per lane); what an entry has to exceed
     bool bad = false;
+    // After steps 1, 2, 4, ... the warps show their lists; the first one joins them and raises the floor for all.  Each such
+    // moment has its own barrier and its own place, so the other warps only arrive and go on.  Every warp of the CTA that has
+    // a segment takes part in all of them.
+    int show = 0, shows = 0;
+    if (partners > 1)
+        while (shows < kBeamShows && (1 << shows) < p.seg_steps) ++shows;
+    auto compare = [&] {
+        shown[show][warp][lane] = best;
+        __threadfence_block();
+        __syncwarp();
+        barrier_of(show, warp > 0, partners * 32);
+        if (warp == 0) {
+            unsigned long long all = best;
+            for (int i = 1; i < partners; ++i) all = warp_merge_desc(all, shown[show][i][lane], lane);
+            if (lane == p.select - 1) *reinterpret_cast<volatile unsigned long long*>(&floor_key) = all;
+        }
+        ++show;
+    };
     Step raw;
     if (first < last && inside(first)) raw.load(base + (first - shift), lane);
     for (int at = first; at < last; at += kBeamStep) {
-        float x[32];
-        unsigned live = 0xffffffffu;
+        float x[kBeamLane];
+        unsigned live = (1u << kBeamLane) - 1u;
         const int place = at + lane * N - shift;  // token of this lane's first element
         if (inside(at)) {
             raw.get(x);
         } else {  // a row's first or last step
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
+            for (int e = 0; e < kBeamLane; ++e) {
                 const int tok = place + (e / N) * 32 * N + e % N;
                 const bool in = tok >= 0 && tok < p.vocab;
                 x[e] = in ? Step::one(base + tok) : -INFINITY;
@@ -235,17 +266,18 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 5) beam_scan_kernel(const Bea
             }
         }
         if (at + kBeamStep < last && inside(at + kBeamStep)) raw.load(base + (at + kBeamStep - shift), lane);
-        float top = max32(x);
+        float group[kBeamLane / 8];
+        float top = max_of(x, group);
         float mn = fmaxf(m, top);
-        float add = expsum32(x, mn > -INFINITY ? mn : 0.f);
-        if (!(add <= 32.f)) {  // NaN or +inf among them, which count as -inf (each term is at most 1)
+        float add = expsum(x, mn > -INFINITY ? mn : 0.f);
+        if (!(add <= static_cast<float>(kBeamLane))) {  // NaN or +inf among them, which count as -inf (each term is at most 1)
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < kBeamLane; ++e)
                 if (!(x[e] < INFINITY)) x[e] = -INFINITY;
             bad = true;
-            top = max32(x);
+            top = max_of(x, group);
             mn = fmaxf(m, top);
-            add = expsum32(x, mn > -INFINITY ? mn : 0.f);
+            add = expsum(x, mn > -INFINITY ? mn : 0.f);
         }
         if (mn > -INFINITY) {
             sum = sum * exp_of(m - mn) + add;
@@ -253,9 +285,9 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 5) beam_scan_kernel(const Bea
         }
         unsigned done = 0u;  // elements that the seed holds already
         if (at == first) {
-            int arg = 31;
+            int arg = kBeamLane - 1;
 #pragma unroll
-            for (int e = 31; e >= 0; --e)
+            for (int e = kBeamLane - 1; e >= 0; --e)
                 if (x[e] == top && ((live >> e) & 1u)) arg = e;
             const bool any = (live >> arg) & 1u;
             best = warp_sort_desc(any ? beam_key(top, place + (arg / N) * 32 * N + arg % N) : 0ull, lane);
@@ -264,43 +296,47 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 5) beam_scan_kernel(const Bea
         }
         const unsigned long long known = *reinterpret_cast<volatile unsigned long long*>(&floor_key);
         least = known > least ? known : least;
-        const float lv = least ? unordered32(static_cast<uint32_t>(least >> 32)) : -INFINITY;
         // A value equal to the last entry's counts only before that entry's token, which lies ahead only where another warp
         // set the floor.
+        float lv = least ? unordered32(static_cast<uint32_t>(least >> 32)) : -INFINITY;
         const int ltok = least ? static_cast<int>(~static_cast<uint32_t>(least)) : 0x7fffffff;
         const bool ties = at - shift < ltok;
-        if (!__any_sync(0xffffffffu, top > lv || (ties && top == lv))) continue;
-        unsigned pass = 0u;
+        if (__any_sync(0xffffffffu, top > lv || (ties && top == lv))) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-            if (x[e] > lv) pass |= 1u << e;
-        if (ties) {
+            for (int g = 0; g < kBeamLane / 8; ++g) {
+                if (!__any_sync(0xffffffffu, group[g] > lv || (ties && group[g] == lv))) continue;
+                unsigned pass = 0u;
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-                if (x[e] == lv && place + (e / N) * 32 * N + e % N < ltok) pass |= 1u << e;
-        }
-        pass &= live & ~done;
-        bool grown = at == first;
-        while (__any_sync(0xffffffffu, pass != 0u)) {
-            const int e = __ffs(pass) - 1;  // -1: nothing left in this lane
-            const unsigned long long key = pass ? beam_key(pick32(x, e), place + (e / N) * 32 * N + e % N) : 0ull;
-            pass &= pass - 1u;
-            unsigned who = __ballot_sync(0xffffffffu, key > least);
-            while (who) {
-                const int src = __ffs(who) - 1;
-                who &= who - 1u;
-                const unsigned long long in = __shfl_sync(0xffffffffu, key, src);
-                if (in <= least) continue;
-                const int rank = __popc(__ballot_sync(0xffffffffu, best > in));
-                const unsigned long long up = __shfl_up_sync(0xffffffffu, best, 1);
-                best = lane < rank ? best : lane == rank ? in : up;
-                const unsigned long long own = __shfl_sync(0xffffffffu, best, p.select - 1);
-                least = own > least ? own : least;
-                grown = true;
+                for (int e = 0; e < 8; ++e)
+                    if (x[8 * g + e] > lv || (ties && x[8 * g + e] == lv)) pass |= 1u << e;
+                pass &= (live & ~done) >> (8 * g);
+                while (__any_sync(0xffffffffu, pass != 0u)) {
+                    const int e = __ffs(pass) - 1;  // -1: nothing left in this lane
+                    float t[4], v;  // element e: a tree of selections instead of an array in memory
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) t[i] = e & 4 ? x[8 * g + i + 4] : x[8 * g + i];
+                    v = e & 2 ? (e & 1 ? t[3] : t[2]) : (e & 1 ? t[1] : t[0]);
+                    const int el = 8 * g + e;
+                    const unsigned long long key = pass ? beam_key(v, place + (el / N) * 32 * N + el % N) : 0ull;
+                    pass &= pass - 1u;
+                    unsigned who = __ballot_sync(0xffffffffu, key > least);
+                    while (who) {
+                        const int src = __ffs(who) - 1;
+                        who &= who - 1u;
+                        const unsigned long long in = __shfl_sync(0xffffffffu, key, src);
+                        if (in <= least) continue;
+                        const int rank = __popc(__ballot_sync(0xffffffffu, best > in));
+                        const unsigned long long up = __shfl_up_sync(0xffffffffu, best, 1);
+                        best = lane < rank ? best : lane == rank ? in : up;
+                        const unsigned long long own = __shfl_sync(0xffffffffu, best, p.select - 1);
+                        least = own > least ? own : least;
+                    }
+                }
             }
         }
-        if (grown && lane == 0 && least > known) atomicMax(&floor_key, least);
+        if (show < shows && (at - first) / kBeamStep + 1 == 1 << show) compare();
     }
+    while (show < shows) compare();  // a short or empty last segment: its partners wait for as many
     float top = m;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
@@ -417,12 +453,12 @@ __global__ void __launch_bounds__(kPickWarps * 32) beam_pick_kernel(const BeamPa
 namespace kvpi {
 namespace {
 
-// Segments of a row: about 20 warps for each processor -- what the scan's registers let reside -- in fours, since a CTA's
+// Segments of a row: about 28 warps for each processor -- what the scan's registers let reside -- in fours, since a CTA's
 // warps share what they have found; none shorter than one step.
 void plan_beam(const kvp_beam_args& a, int* segs, int* steps) {
     const long long rows = static_cast<long long>(a.batch) * a.beams;
     const long long total = (static_cast<long long>(a.vocab) + 7 + kvpd::kBeamStep - 1) / kvpd::kBeamStep;
-    const long long want = (static_cast<long long>(sm_count()) * 20 / std::max<long long>(rows, 1) + 3) / 4 * 4;
+    const long long want = (static_cast<long long>(sm_count()) * 28 / std::max<long long>(rows, 1) + 3) / 4 * 4;
     const long long n = std::max<long long>(1, std::min(std::min<long long>(want, kvpd::kBeamSegs), total));
     *steps = static_cast<int>((total + n - 1) / n);
     *segs = static_cast<int>((total + *steps - 1) / *steps);

@@ -8,9 +8,9 @@ lower token.
 Bound of a score: its last rounding is half an ulp, 2^-24 relative.  The sum of exponentials is taken in fp32: each
 exponential is off by at most 2 + 1.16 |d| ulps of 2^-23 for an argument d <= 0 (the documented error of the intrinsic),
 weighted by its value e^d: at most 3 ulps of the largest term for any d; an addition adds half an ulp, and a lane adds at
-most 32 times the steps of its segment plus a rescaling, the warp five more.  So the sum's relative error, which is
-the logarithm's absolute one, is at most (16 + 64 steps) 2^-24.  A segment has as many steps of 1024 tokens as the row's
-steps over the segments it is cut into, at most 64, for about 20 warps on each of 148 processors."""
+most 16 times the steps of its segment plus a rescaling, the warp five more.  So the sum's relative error, which is
+the logarithm's absolute one, is at most (16 + 34 steps) 2^-24.  A segment has as many steps of 512 tokens as the row's
+steps over the segments it is cut into, at most 32, for about 28 warps on each of 148 processors."""
 import math
 
 import numpy as np
@@ -20,13 +20,13 @@ pytestmark = pytest.mark.gpu
 
 
 def _steps(batch, beams, vocab, select):
-    total = -(-(vocab + 7) // 1024)
-    segments = min((148 * 20 // (batch * beams) + 3) // 4 * 4, 64, total)
+    total = -(-(vocab + 7) // 512)
+    segments = min((148 * 28 // (batch * beams) + 3) // 4 * 4, 32, total)
     return -(-total // max(1, segments))
 
 
 def _bound(steps, values):
-    return (16 + 64 * steps) * 2.0 ** -24 + np.abs(np.where(np.isfinite(values), values, 0)) * 2.0 ** -24
+    return (16 + 34 * steps) * 2.0 ** -24 + np.abs(np.where(np.isfinite(values), values, 0)) * 2.0 ** -24
 
 
 def _definition(logits, scores, select):
