@@ -2,8 +2,8 @@
 //     value = score[beam] + logit[beam][token] - log(sum over tokens of exp(logit[beam][.])),
 // ties to the lower beam, then the lower token.  One read of the logits, two launches.
 //
-// beam_scan_kernel (bound by HBM): a warp takes one segment of one row, 512 logits a step, the next step's loads in flight
-// while it works on this one's.  It keeps a running maximum and sum of exponentials per lane, and the segment's best
+// beam_scan_kernel (bound by HBM): a warp takes its share of one row, 512 logits a step, three steps in
+// flight.  It keeps a running maximum and sum of exponentials per lane, and its best
 // `select` logits as a list sorted over its 32 lanes; within a row the order of the values is the order of the logits, so
 // no logarithm is needed here.  The list starts from the lanes' own maxima of the first step (one sort); of the rest only
 // what passes the list's last entry -- or that of another warp of the CTA, which works on the same row -- costs more than
@@ -28,6 +28,7 @@ constexpr int kBeamMost = 32;    // beams and selected continuations per request
 constexpr int kBeamSegs = 32;    // segments of a row
 constexpr int kBeamLane = 16;    // logits a lane takes at once
 constexpr int kBeamStep = 32 * kBeamLane;
+constexpr int kBeamRing = 3;     // steps of a warp in flight
 constexpr int kBeamWarps = 4;    // warps per CTA of the scan, all on one row
 constexpr int kBeamShows = 6;    // times a CTA's warps compare their lists
 constexpr int kPickWarps = 16;
@@ -44,7 +45,7 @@ struct BeamParams {
     int32_t* status;
     long long row_stride;       // elements
     int batch, beams, vocab, select, segs;
-    int seg_steps;              // kBeamStep logits each
+    int seg_steps;              // most steps of a warp
 };
 
 __device__ __forceinline__ uint32_t ordered32(float x) {
@@ -106,44 +107,45 @@ struct BeamStep {
     }
 };
 template <class T>
-struct BeamStep<T, true> {  // 16-bit logits: 8 per vector
-    static constexpr int N = 8;
-    uint4 u[kBeamLane / 8];
-    __device__ __forceinline__ void load(const T* p, int lane) {
+struct BeamStep<T, true> {
+    static constexpr int N = 16 / sizeof(T);       // logits of a vector
+    static constexpr int kVecs = kBeamLane / N;    // vectors of a lane
+    static __device__ __forceinline__ float one(const T* p) { return BeamStep<T, false>::one(p); }
+};
+// A warp's steps on their way, each lane's vectors in places of its own: copied asynchronously, so that three steps are in
+// flight without registers, and read back by the lane that asked for them.
+template <class T>
+struct BeamRing {
+    using Step = BeamStep<T, true>;
+    uint32_t at;  // this lane's first place
+    __device__ __forceinline__ void load(int slot, const T* p, int lane) const {
 #pragma unroll
-        for (int j = 0; j < kBeamLane / 8; ++j) u[j] = __ldcs(reinterpret_cast<const uint4*>(p) + j * 32 + lane);
+        for (int j = 0; j < Step::kVecs; ++j)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + static_cast<uint32_t>(slot * Step::kVecs + j) * 512u),
+                         "l"(p + (j * 32 + lane) * Step::N)
+                         : "memory");
     }
-    __device__ __forceinline__ void get(float (&x)[kBeamLane]) const {
+    static __device__ __forceinline__ void close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kBeamRing - 1) : "memory"); }
+    __device__ __forceinline__ void get(int slot, float (&x)[kBeamLane]) const {
 #pragma unroll
-        for (int j = 0; j < kBeamLane / 8; ++j) {
-            const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+        for (int j = 0; j < Step::kVecs; ++j) {
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(at + static_cast<uint32_t>(slot * Step::kVecs + j) * 512u)
+                         : "memory");
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[j * 8 + 2 * i] = F16Traits<T>::unpack_lo(w[i]);
-                x[j * 8 + 2 * i + 1] = F16Traits<T>::unpack_hi(w[i]);
+                if constexpr (sizeof(T) == 4) {
+                    x[4 * j + i] = __uint_as_float(w[i]);
+                } else {
+                    x[8 * j + 2 * i] = F16Traits<T>::unpack_lo(w[i]);
+                    x[8 * j + 2 * i + 1] = F16Traits<T>::unpack_hi(w[i]);
+                }
             }
         }
     }
-    static __device__ __forceinline__ float one(const T* p) { return F16Traits<T>::to_float(*p); }
-};
-template <>
-struct BeamStep<float, true> {
-    static constexpr int N = 4;
-    float4 u[kBeamLane / 4];
-    __device__ __forceinline__ void load(const float* p, int lane) {
-#pragma unroll
-        for (int j = 0; j < kBeamLane / 4; ++j) u[j] = __ldcs(reinterpret_cast<const float4*>(p) + j * 32 + lane);
-    }
-    __device__ __forceinline__ void get(float (&x)[kBeamLane]) const {
-#pragma unroll
-        for (int j = 0; j < kBeamLane / 4; ++j) {
-            x[4 * j] = u[j].x;
-            x[4 * j + 1] = u[j].y;
-            x[4 * j + 2] = u[j].z;
-            x[4 * j + 3] = u[j].w;
-        }
-    }
-    static __device__ __forceinline__ float one(const float* p) { return *p; }
 };
 
 // A beam takes part when its score is finite; -inf is a beam that is not in use.
@@ -200,6 +202,9 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
     constexpr int N = Step::N;
     __shared__ unsigned long long floor_key;  // no entry below it is among the row's best `select`
     __shared__ unsigned long long shown[kBeamShows][kBeamWarps][32];
+    __shared__ __align__(16) uint8_t steps[Vec ? kBeamWarps * kBeamRing * kBeamStep * sizeof(T) : 16];
+    BeamRing<T> ring;
+    ring.at = smem_u32(steps) + (threadIdx.x >> 5) * (kBeamRing * kBeamStep * sizeof(T)) + (threadIdx.x & 31) * 16;
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int groups = (p.segs + kBeamWarps - 1) / kBeamWarps;  // CTAs per row
@@ -221,18 +226,63 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
         return;
     }
     const T* base = static_cast<const T*>(p.logits) + row * p.row_stride;
-    // vectors start at 16-byte boundaries: token = place - shift
+    // Steps start at 16-byte boundaries: token = place - shift.  A row's warps take its steps in turn, so that at any time
+    // they read one stretch of memory.
     const int shift = Vec ? static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15u) / sizeof(T)) : 0;
-    const int end = p.vocab + shift;
-    const int first = seg * p.seg_steps * kBeamStep;
-    const int last = min(end, first + p.seg_steps * kBeamStep);
-    auto inside = [&](int at) { return at >= shift && at + kBeamStep <= end; };
+    const int end = p.vocab + shift, first = seg * kBeamStep, ahead = p.segs * kBeamStep;
+    const int n = first < end ? (end - first - 1) / ahead + 1 : 0;  // steps of this warp
+    // those that lie inside the row from end to end
+    const int f0 = first < shift ? 1 : 0, f1 = n > 0 && first + (n - 1) * ahead + kBeamStep > end ? n - 1 : n;
+    auto at_edge = [&](int place, float (&x)[kBeamLane]) {  // a row's first or last step; the elements that exist
+        unsigned live = 0u;
+#pragma unroll
+        for (int e = 0; e < kBeamLane; ++e) {
+            const int tok = place + (e / N) * 32 * N + e % N;
+            const bool in = tok >= 0 && tok < p.vocab;
+            x[e] = in ? Step::one(base + tok) : -INFINITY;
+            if (in) live |= 1u << e;
+        }
+        return live;
+    };
+    bool bad = false;
+    auto ban = [&](float (&x)[kBeamLane]) {  // NaN and +inf count as -inf
+#pragma unroll
+        for (int e = 0; e < kBeamLane; ++e)
+            if (!(x[e] < INFINITY)) {
+                x[e] = -INFINITY;
+                bad = true;
+            }
+    };
+    constexpr unsigned kAll = (1u << kBeamLane) - 1u;
+    const T* next = base + (first - shift);  // the step to ask for next
+    int asked = 0, slot = 0;
+    Step raw;
+    auto ask = [&](int to) {
+        if (asked >= f0 && asked < f1) {
+            if constexpr (Vec) ring.load(to, next, lane);
+            else raw.load(next, lane);
+        }
+        if constexpr (Vec) ring.close();
+        next += ahead;
+        ++asked;
+    };
+#pragma unroll
+    for (int k = 0; k < (Vec ? kBeamRing : 1); ++k) ask(k);
     float m = -INFINITY, sum = 0.f;
     unsigned long long best = 0ull, least = 0ull;  // the list (one entry per lane); what an entry has to exceed
-    bool bad = false;
+    // The same as a value and a token.  An equal value counts only before that token, which lies ahead only where another
+    // warp set the floor.
+    float lv = -INFINITY;
+    int ltok = 0x7fffffff;
+    auto refresh = [&] {
+        if (least) {
+            lv = unordered32(static_cast<uint32_t>(least >> 32));
+            ltok = static_cast<int>(~static_cast<uint32_t>(least));
+        }
+    };
     // After steps 1, 2, 4, ... the warps show their lists; the first one joins them and raises the floor for all.  Each such
     // moment has its own barrier and its own place, so the other warps only arrive and go on.  Every warp of the CTA that has
-    // a segment takes part in all of them.
+    // a share takes part in all of them.
     int show = 0, shows = 0;
     if (partners > 1)
         while (shows < kBeamShows && (1 << shows) < p.seg_steps) ++shows;
@@ -248,33 +298,50 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
         }
         ++show;
     };
-    Step raw;
-    if (first < last && inside(first)) raw.load(base + (first - shift), lane);
-    for (int at = first; at < last; at += kBeamStep) {
-        float x[kBeamLane];
-        unsigned live = (1u << kBeamLane) - 1u;
-        const int place = at + lane * N - shift;  // token of this lane's first element
-        if (inside(at)) {
-            raw.get(x);
-        } else {  // a row's first or last step
-#pragma unroll
-            for (int e = 0; e < kBeamLane; ++e) {
-                const int tok = place + (e / N) * 32 * N + e % N;
-                const bool in = tok >= 0 && tok < p.vocab;
-                x[e] = in ? Step::one(base + tok) : -INFINITY;
-                if (!in) live &= ~(1u << e);
-            }
+    // The list starts from each lane's best of the first step.
+    unsigned done = 0u;  // elements of the first step that it holds already
+    if (n > 0) {
+        float x[kBeamLane], group[kBeamLane / 8];
+        unsigned live = kAll;
+        const int place = first + lane * N - shift;
+        if constexpr (Vec) ring.wait();
+        if (f0 > 0 || f1 == 0) {
+            live = at_edge(place, x);
+        } else {
+            if constexpr (Vec) ring.get(0, x);
+            else raw.get(x);
         }
-        if (at + kBeamStep < last && inside(at + kBeamStep)) raw.load(base + (at + kBeamStep - shift), lane);
-        float group[kBeamLane / 8];
+        ban(x);
+        const float top = max_of(x, group);
+        int arg = kBeamLane - 1;
+#pragma unroll
+        for (int e = kBeamLane - 1; e >= 0; --e)
+            if (x[e] == top && ((live >> e) & 1u)) arg = e;
+        best = warp_sort_desc((live >> arg) & 1u ? beam_key(top, place + (arg / N) * 32 * N + arg % N) : 0ull, lane);
+        done = 1u << arg;
+        least = __shfl_sync(0xffffffffu, best, p.select - 1);
+        refresh();
+    }
+    for (int i = 0; i < n; ++i) {
+        float x[kBeamLane], group[kBeamLane / 8];
+        unsigned live = kAll;
+        const int at = first + i * ahead - shift, place = at + lane * N;  // tokens: the step's and this lane's first
+        if constexpr (Vec) ring.wait();
+        if (i >= f0 && i < f1) {
+            if constexpr (Vec) ring.get(slot, x);
+            else raw.get(x);
+        } else {
+            live = at_edge(place, x);
+        }
+        ask(slot);
+        slot = slot + 1 == kBeamRing ? 0 : slot + 1;
         float top = max_of(x, group);
         float mn = fmaxf(m, top);
         float add = expsum(x, mn > -INFINITY ? mn : 0.f);
-        if (!(add <= static_cast<float>(kBeamLane))) {  // NaN or +inf among them, which count as -inf (each term is at most 1)
-#pragma unroll
-            for (int e = 0; e < kBeamLane; ++e)
-                if (!(x[e] < INFINITY)) x[e] = -INFINITY;
-            bad = true;
+        // A NaN or a +inf among them shows here: each term is at most 1 else.  (Asked of the whole warp, so that what is rare
+        // is branched over and not predicated.)
+        if (__any_sync(0xffffffffu, !(add <= static_cast<float>(kBeamLane)))) {
+            ban(x);
             top = max_of(x, group);
             mn = fmaxf(m, top);
             add = expsum(x, mn > -INFINITY ? mn : 0.f);
@@ -283,24 +350,12 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
             sum = sum * exp_of(m - mn) + add;
             m = mn;
         }
-        unsigned done = 0u;  // elements that the seed holds already
-        if (at == first) {
-            int arg = kBeamLane - 1;
-#pragma unroll
-            for (int e = kBeamLane - 1; e >= 0; --e)
-                if (x[e] == top && ((live >> e) & 1u)) arg = e;
-            const bool any = (live >> arg) & 1u;
-            best = warp_sort_desc(any ? beam_key(top, place + (arg / N) * 32 * N + arg % N) : 0ull, lane);
-            done = 1u << arg;
-            least = __shfl_sync(0xffffffffu, best, p.select - 1);
-        }
         const unsigned long long known = *reinterpret_cast<volatile unsigned long long*>(&floor_key);
-        least = known > least ? known : least;
-        // A value equal to the last entry's counts only before that entry's token, which lies ahead only where another warp
-        // set the floor.
-        float lv = least ? unordered32(static_cast<uint32_t>(least >> 32)) : -INFINITY;
-        const int ltok = least ? static_cast<int>(~static_cast<uint32_t>(least)) : 0x7fffffff;
-        const bool ties = at - shift < ltok;
+        if (__any_sync(0xffffffffu, known > least)) {
+            least = known;
+            refresh();
+        }
+        const bool ties = at < ltok;
         if (__any_sync(0xffffffffu, top > lv || (ties && top == lv))) {
 #pragma unroll
             for (int g = 0; g < kBeamLane / 8; ++g) {
@@ -308,13 +363,18 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
                 unsigned pass = 0u;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (x[8 * g + e] > lv || (ties && x[8 * g + e] == lv)) pass |= 1u << e;
+                    if (x[8 * g + e] > lv) pass |= 1u << e;
+                if (ties) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (x[8 * g + e] == lv) pass |= 1u << e;
+                }
                 pass &= (live & ~done) >> (8 * g);
                 while (__any_sync(0xffffffffu, pass != 0u)) {
                     const int e = __ffs(pass) - 1;  // -1: nothing left in this lane
                     float t[4], v;  // element e: a tree of selections instead of an array in memory
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) t[i] = e & 4 ? x[8 * g + i + 4] : x[8 * g + i];
+                    for (int k = 0; k < 4; ++k) t[k] = e & 4 ? x[8 * g + k + 4] : x[8 * g + k];
                     v = e & 2 ? (e & 1 ? t[3] : t[2]) : (e & 1 ? t[1] : t[0]);
                     const int el = 8 * g + e;
                     const unsigned long long key = pass ? beam_key(v, place + (el / N) * 32 * N + el % N) : 0ull;
@@ -332,11 +392,13 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
                         least = own > least ? own : least;
                     }
                 }
+                refresh();
             }
         }
-        if (show < shows && (at - first) / kBeamStep + 1 == 1 << show) compare();
+        done = 0u;
+        if (show < shows && i + 1 == 1 << show) compare();
     }
-    while (show < shows) compare();  // a short or empty last segment: its partners wait for as many
+    while (show < shows) compare();  // a warp with fewer steps: its partners wait for as many
     float top = m;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
@@ -348,19 +410,10 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
     if (bad) report(p.status, KVP_STATUS_BAD_VALUE);
 }
 
-// The best of the warp's heads: (value as two ordered halves, then the lower place); the lane that holds it.
-__device__ __forceinline__ int best_lane(uint32_t hi, uint32_t lo, uint32_t place) {
-    const uint32_t h = __reduce_max_sync(0xffffffffu, hi);
-    const uint32_t l = __reduce_max_sync(0xffffffffu, hi == h ? lo : 0u);
-    const bool in = hi == h && lo == l;
-    const uint32_t w = __reduce_min_sync(0xffffffffu, in ? place : 0xffffffffu);
-    return __ffs(__ballot_sync(0xffffffffu, in && place == w)) - 1;
-}
-
 __global__ void __launch_bounds__(kPickWarps * 32) beam_pick_kernel(const BeamParams p) {
     __shared__ unsigned long long part[kPickWarps][32];
-    __shared__ unsigned long long keys[kBeamMost][32];  // [beam][entry]
-    __shared__ double lse[kBeamMost];
+    __shared__ unsigned long long value[kBeamMost][32];  // [beam][entry]
+    __shared__ int token[kBeamMost][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row0 = static_cast<long long>(blockIdx.x) * p.beams;
     const int per = max(1, kPickWarps / p.beams);  // warps that share a beam's lists
@@ -371,6 +424,8 @@ __global__ void __launch_bounds__(kPickWarps * 32) beam_pick_kernel(const BeamPa
     for (int b0 = 0; b0 < p.beams; b0 += kPickWarps) {
         const int b = b0 + warp / per, sub = warp % per;
         const bool mine = b < p.beams && warp < per * p.beams;
+        const float score = mine ? __ldg(p.scores + row0 + b) : 0.f;
+        double lse = 0.0;
         if (mine) {
             const long long item0 = (row0 + b) * p.segs;
             unsigned long long best = 0ull;
@@ -402,46 +457,42 @@ __global__ void __launch_bounds__(kPickWarps * 32) beam_pick_kernel(const BeamPa
                     if (ml[i].x > -INFINITY) total += static_cast<double>(ml[i].y) * exp(static_cast<double>(ml[i].x) - top);
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-                if (lane == 0) lse[b] = top > -INFINITY ? top + log(total) : -static_cast<double>(INFINITY);
+                lse = top > -INFINITY ? top + log(total) : -static_cast<double>(INFINITY);
             }
         }
         __syncthreads();
         if (mine && sub == 0) {
             unsigned long long best = part[warp][lane];
             for (int i = 1; i < per; ++i) best = fold(best, part[warp + i][lane]);
-            keys[b][lane] = best;
+            // each entry as an ordered value in 64 bits (0: none) and its place
+            const float x = unordered32(static_cast<uint32_t>(best >> 32));
+            const double v = x > -INFINITY && beam_live(score) ? score + (x - lse) : -static_cast<double>(INFINITY);
+            const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(v + 0.0));
+            value[b][lane] = best && lane < p.select ? bits ^ ((bits >> 63) ? ~0ull : 0x8000000000000000ull) : 0ull;
+            token[b][lane] = static_cast<int>(~static_cast<uint32_t>(best));
         }
         __syncthreads();
     }
     if (warp != 0) return;
-    // one lane per beam, its best continuation left as a value in 64 bits
-    uint32_t hi = 0u, lo = 0u, place = 0xffffffffu;  // ordered value (0, 0: none), beam << 26 | token
-    int next = 0;
-    const float score = lane < p.beams ? __ldg(p.scores + row0 + lane) : -INFINITY;
-    const double beam_lse = lane < p.beams ? lse[lane] : 0.0;
+    // one lane per beam, its best continuation left; the best of these `select` times
+    int next = 0, tok = 0;
+    unsigned long long val = 0ull;
     auto head = [&] {
-        hi = lo = 0u;
-        place = 0xffffffffu;
-        const unsigned long long key = lane < p.beams && next < p.select ? keys[lane][next] : 0ull;
-        if (!key) return;
-        const float x = unordered32(static_cast<uint32_t>(key >> 32));
-        const double v = x > -INFINITY && beam_live(score) ? score + (x - beam_lse) : -static_cast<double>(INFINITY);
-        const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v + 0.0));
-        const unsigned long long o = b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
-        hi = static_cast<uint32_t>(o >> 32);
-        lo = static_cast<uint32_t>(o);
-        place = (static_cast<uint32_t>(lane) << kBeamTokenBits) | ~static_cast<uint32_t>(key);
+        val = lane < p.beams && next < 32 ? value[lane][next] : 0ull;
+        tok = lane < p.beams && next < 32 ? token[lane][next] : 0;
     };
     head();
     for (int r = 0; r < p.select; ++r) {
-        const int w = best_lane(hi, lo, place);
-        if (lane == w) {
-            const unsigned long long o = (static_cast<unsigned long long>(hi) << 32) | lo;
-            const unsigned long long b = o ^ ((o >> 63) ? 0x8000000000000000ull : ~0ull);
+        // the largest value, by its halves; of equal ones the lowest beam, which is the lowest lane
+        const uint32_t hi = static_cast<uint32_t>(val >> 32), lo = static_cast<uint32_t>(val);
+        const uint32_t h = __reduce_max_sync(0xffffffffu, hi);
+        const uint32_t l = __reduce_max_sync(0xffffffffu, hi == h ? lo : 0u);
+        if (lane == __ffs(__ballot_sync(0xffffffffu, hi == h && lo == l)) - 1) {
+            const unsigned long long b = val ^ ((val >> 63) ? 0x8000000000000000ull : ~0ull);
             const long long at = static_cast<long long>(blockIdx.x) * p.select + r;
             p.out_scores[at] = static_cast<float>(__longlong_as_double(static_cast<long long>(b)));
             p.out_parents[at] = lane;
-            p.out_tokens[at] = static_cast<int32_t>(place & ((1u << kBeamTokenBits) - 1u));
+            p.out_tokens[at] = tok;
             ++next;
             head();
         }
