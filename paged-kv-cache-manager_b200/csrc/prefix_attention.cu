@@ -20,7 +20,7 @@
 // Scores S and accumulators O live in TMEM (S0, S1 at columns 0 and 128, O0, O1 at 256 and 256 + head_dim); the
 // probabilities P overwrite S as 16-bit pairs and are the A operand of the second product straight from TMEM.  A thread
 // owns one row: the running maximum and sum need no exchange.  O is rescaled only when a row's maximum has grown by more
-// than 2^8 since its last rescaling (P then stays below 2^8, and the sum has the same scale, so nothing is lost).
+// than 2^14 (fp16) or 2^40 (bf16) since its last rescaling: P, O and the sum have one scale, so nothing is lost.
 // P is rounded to the pools' 16-bit type: the products' rounding errors (half a step each, independent) average out over
 // the keys and stay below the rounding of a 16-bit output; the sum is taken over the unrounded values in fp32.
 #include <cuda.h>
@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "attention_common.h"
 #include "kvp_device.cuh"
@@ -39,7 +40,6 @@ constexpr int kKeys = 128;         // keys per tile
 constexpr int kRows = 128;         // rows per tile: M of the MMA
 constexpr int kPrefixThreads = 320;  // 8 softmax warps, the MMA warp, the loading warp
 constexpr int kTmemCols = 512;
-constexpr float kRescale = 8.0f;   // log2
 
 struct PrefixParams {
     const int32_t* tables;
@@ -57,7 +57,7 @@ struct PrefixParams {
     long long num_blocks;
     long long wait_limit;
     int num_counters;
-    int num_seqs, num_groups, nh, kvh, g, max_blocks, B, run, runs, oob_row;
+    int num_seqs, num_groups, nh, kvh, g, max_blocks, B, Bshift, run, runs, oob_row;
     int mt;                    // members per row tile
     int slots;                 // ring slots
     int bf16, out_dtype;
@@ -108,7 +108,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
         "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
@@ -117,14 +117,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
         "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 // Waits for the loads so far; r: what the last one fills, so that no use of it is moved before the wait.
@@ -137,13 +129,6 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
                    "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// One 32-byte sector of global memory.
-__device__ __forceinline__ void store_sector(float* p, const uint32_t* v) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-}
 
 // Shared-memory operand in the 128-byte swizzle: rows of 64 elements, 8-row atoms of 1024 bytes.
 //   along the rows (K-major: Q and K): atoms follow each other at 1024 bytes; a 16-element step is 32 bytes further.
@@ -167,6 +152,46 @@ __device__ __forceinline__ void mask_keys(uint32_t (&s)[32], int valid) {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
         if (i >= valid) s[i] = 0xff800000u;
+}
+
+// A row's largest score.
+__device__ __forceinline__ float row_max(uint32_t addr, uint32_t (&s)[2][32], int valid) {
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    tmem_ld32(addr, s[0]);
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+        tmem_wait_ld(s[h & 1]);
+        if (h < 3) tmem_ld32(addr + (h + 1) * 32, s[(h + 1) & 1]);
+        mask_keys(s[h & 1], valid - h * 32);
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+            top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[h & 1][e])), __uint_as_float(s[h & 1][e + 1]));
+    }
+    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+__device__ __forceinline__ float exp2_unit(float x) {  // free to be moved, unlike fast_exp2
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^x of a pair on the FMA pipe: x = n + f with n the nearest whole number (added as the exponent) and f in
+// [-1/2, 1/2], 2^f by the polynomial of degree 4 with the smallest largest relative error there (2.7e-6, found by the
+// Remez exchange), far below the rounding of P.  One pair in four goes this way: the special-function unit, at 16 results
+// a clock, would otherwise take as long as both matrix products of a tile.  What lies below 2^-126 stays there (the
+// exponent must not wrap), which no sum of this kernel notices.
+__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
+    const float2 v = unpack2(x);
+    const uint64_t y = pack2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+    const uint64_t t = add2(y, pack2(12582912.f, 12582912.f));  // 1.5 * 2^23: n in the low bits
+    const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), y);
+    uint64_t q = pack2(0.00957010221f, 0.00957010221f);
+    q = fma2(q, f, pack2(0.0559178591f, 0.0559178591f));
+    q = fma2(q, f, pack2(0.240247443f, 0.240247443f));
+    q = fma2(q, f, pack2(0.693121791f, 0.693121791f));
+    q = fma2(q, f, pack2(0.999999285f, 0.999999285f));
+    const float2 qv = unpack2(q), tv = unpack2(t);
+    return pack2(__uint_as_float(__float_as_uint(qv.x) + (__float_as_uint(tv.x) << 23)),
+                 __uint_as_float(__float_as_uint(qv.y) + (__float_as_uint(tv.y) << 23)));
 }
 
 // ---------------------------------------------------------------- units
@@ -244,19 +269,15 @@ struct WorkList {
     }
 };
 
-// Total units, and the group that holds unit `at` (its index and first unit; at < 0: none wanted).  CTA 0 leaves the
-// prefix sums for the joining kernel.
-__device__ __forceinline__ long long scan_groups(const PrefixParams& p, long long at, int* found_group, long long* found_first,
-                                                 long long* warp_sum) {
+// Where a CTA's units begin: the total, the group that holds the CTA's first unit and that group's first unit.  CTA 0 leaves
+// the prefix sums for the joining kernel.  One pass over the groups while there is a thread for each, else a second one.
+struct Start {
+    long long total, first;
+    int group;
+};
+__device__ __forceinline__ Start find_start(const PrefixParams& p, long long* warp_sum, Start* found) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long carry = 0;
-    for (int g0 = 0; g0 < p.num_groups; g0 += kPrefixThreads) {
-        const int gi = g0 + static_cast<int>(threadIdx.x);
-        long long u = 0;
-        if (gi < p.num_groups) {
-            const Group grp = load_group(p, gi);
-            u = grp.units(p.kvh);
-        }
+    auto scan = [&](long long u, long long carry, long long* mine) {  // all of a chunk; *mine: what lies before this thread
         long long x = u;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -266,22 +287,39 @@ __device__ __forceinline__ long long scan_groups(const PrefixParams& p, long lon
         if (lane == 31) warp_sum[warp] = x;
         __syncthreads();
         long long before = carry, all = 0;
+#pragma unroll
         for (int w = 0; w < kPrefixThreads / 32; ++w) {
             const long long s = warp_sum[w];
             if (w < warp) before += s;
             all += s;
         }
-        const long long mine = before + x - u;
-        if (at >= 0 && u > 0 && mine <= at && at < mine + u) {
-            *found_group = gi;
-            *found_first = mine;
-        }
-        if (at < 0 && blockIdx.x == 0 && gi < p.num_groups) p.unit_prefix[gi] = mine;
-        carry += all;
+        *mine = before + x - u;
         __syncthreads();
+        return all;
+    };
+    auto units_of = [&](int gi) { return gi < p.num_groups ? load_group(p, gi).units(p.kvh) : 0ll; };
+    long long total = 0, u = 0, mine = 0;
+    for (int g0 = 0; g0 < p.num_groups; g0 += kPrefixThreads) {
+        const int gi = g0 + static_cast<int>(threadIdx.x);
+        u = units_of(gi);
+        total += scan(u, total, &mine);
+        if (blockIdx.x == 0 && gi < p.num_groups) p.unit_prefix[gi] = mine;
     }
-    if (at < 0 && blockIdx.x == 0 && threadIdx.x == 0) p.unit_prefix[p.num_groups] = carry;
-    return carry;
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.unit_prefix[p.num_groups] = total;
+    const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+    if (static_cast<int>(blockIdx.x) >= G) return Start{total, 0, 0};
+    const long long at = first_unit(blockIdx.x, total, G);
+    long long carry = 0;
+    for (int g0 = 0; g0 < p.num_groups; g0 += kPrefixThreads) {
+        const int gi = g0 + static_cast<int>(threadIdx.x);
+        if (p.num_groups > kPrefixThreads) {
+            u = units_of(gi);
+            carry += scan(u, carry, &mine);
+        }
+        if (u > 0 && mine <= at && at < mine + u) *found = Start{total, mine, gi};
+    }
+    __syncthreads();
+    return *found;
 }
 
 // ---------------------------------------------------------------- the kernel
@@ -290,8 +328,7 @@ struct PrefixShared {
     uint64_t q_full, q_free, s_full[2], p_full[2], o_full[2], drain;
     uint32_t tmem;
     int abort;
-    int found_group;
-    long long found_first;
+    Start found;
     long long warp_sum[kPrefixThreads / 32];
 };
 
@@ -335,10 +372,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     constexpr uint32_t kCol = kKeys * 128;           // bytes of one such column of a tile
     constexpr uint32_t kTile = NCH * kCol;           // one tile of Q, K or V
     constexpr uint32_t kO = 256;                     // TMEM column of the first accumulator
+    // How far (log2) a score may exceed the maximum that P, O and the sum refer to: P has to stay below the type's
+    // largest value, O and the sum below fp32's; nothing is lost up to there.
+    constexpr float kFar = std::is_same<KV, __half>::value ? 14.f : 40.f;
     __shared__ PrefixShared sh;
     extern __shared__ uint8_t dyn[];
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
-    const uint32_t ring = base + 2 * kTile;
+    const uint32_t ring = base + 2 * kTile, stage = ring + p.slots * kTile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // the next kernel may be scheduled as soon as this one's CTAs leave their SMs; it waits for all of them
@@ -360,21 +400,27 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         mbar_init(smem_u32(&sh.drain), 1);
         fence_barrier_init();
     }
-    const long long T = scan_groups(p, -1, nullptr, nullptr, sh.warp_sum);
-    const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), T));
-    const int cta = blockIdx.x;
-    if (cta >= G) return;  // the whole CTA, before anything was allocated
-    WorkList list;
-    list.cta = cta;
-    list.t = first_unit(cta, T, G);
-    list.end = first_unit(cta + 1, T, G);
-    scan_groups(p, list.t, &sh.found_group, &sh.found_first, sh.warp_sum);
-    if (warp == 8) tmem_alloc(smem_u32(&sh.tmem));
+    if (warp == 9 && lane == 0) {
+        prefetch_tensormap(&qmap);
+        prefetch_tensormap(&kmap);
+        prefetch_tensormap(&vmap);
+    }
+    if (warp == 8) tmem_alloc(smem_u32(&sh.tmem));  // while the others wait for the groups
+    const Start from = find_start(p, sh.warp_sum, &sh.found);
+    const int cta = blockIdx.x, G = static_cast<int>(min(static_cast<long long>(gridDim.x), from.total));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    list.gi = sh.found_group;
-    list.first = sh.found_first;
+    if (cta >= G) {  // more CTAs than units
+        if (warp == 8) tmem_free(sh.tmem);
+        return;
+    }
+    WorkList list;
+    list.cta = cta;
+    list.t = first_unit(cta, from.total, G);
+    list.end = first_unit(cta + 1, from.total, G);
+    list.gi = from.group;
+    list.first = from.first;
     list.grp = load_group(p, list.gi);
     const uint32_t tmem = sh.tmem;
     Work w;
@@ -384,11 +430,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         bool ok = true;
         Cursor at{0, 0u};
         int loaded = 0, queries = 0;  // tiles and query loads issued
-        if (lane == 0) {
-            prefetch_tensormap(&qmap);
-            prefetch_tensormap(&kmap);
-            prefetch_tensormap(&vmap);
-        }
         while (ok && list.next(p, w)) {
             // queries, once the previous stretch's products have read theirs
             if (queries > 0) ok = warp_wait(&sh.q_free, (queries - 1) & 1, p, sh);
@@ -406,33 +447,39 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             const int32_t* trow = p.tables + static_cast<long long>(w.start) * p.max_blocks;
             const int ahead = w.rows1 ? 1 : 2;  // K runs ahead of V by as many tiles
             const int run = lane / NCH, c = lane - run * NCH;  // this lane's copy of a tile
-            auto load = [&](const CUtensorMap* map, int kt) {
+            // The pool row of this lane's run of a tile.  Rows of the next four tiles are kept, so that the table's latency
+            // is long past when a tile's copies are issued: looked up one by one it held the loads to 1750 clocks a tile.
+            auto row_of = [&](int kt) {
+                const int tok = kt * kKeys + run * p.run;
+                if (run >= p.runs || tok >= w.tokens || kt >= w.k0 + w.n) return p.oob_row;  // zeros behind the shared tokens
+                const int bi = p.Bshift >= 0 ? tok >> p.Bshift : tok / p.B;
+                const int blk = __ldg(trow + bi);
+                if (blk >= 0 && blk < p.num_blocks) return blk * p.B + (tok - bi * p.B);
+                report(p.status, KVP_STATUS_BAD_BLOCK);
+                return p.oob_row;
+            };
+            auto load = [&](const CUtensorMap* map, int row) {
                 const int st = at.slot;
                 if (loaded >= p.slots && !warp_wait(&sh.empty[st], at.parity ^ 1u, p, sh)) return false;
                 const uint32_t bar = smem_u32(&sh.full[st]);
                 if (lane == 0) mbar_arrive_expect_tx(bar, kTile);
                 __syncwarp();
-                if (run < p.runs) {
-                    const int tok = kt * kKeys + run * p.run;
-                    int row = p.oob_row;  // zeros behind the shared tokens
-                    if (tok < w.tokens) {
-                        const int bi = tok / p.B;
-                        const int blk = __ldg(trow + bi);
-                        if (blk >= 0 && blk < p.num_blocks)
-                            row = blk * p.B + (tok - bi * p.B);
-                        else
-                            report(p.status, KVP_STATUS_BAD_BLOCK);
-                    }
+                if (run < p.runs)
                     tma_load_3d(ring + st * kTile + c * kCol + static_cast<uint32_t>(run * p.run) * 128u, map, bar, c * 64, w.head, row);
-                }
                 at = at.next(p.slots);
                 ++loaded;
                 return true;
             };
-            for (int i = 0; ok && i < min(ahead, w.n); ++i) ok = load(&kmap, w.k0 + i);
+            int r0 = row_of(w.k0), r1 = row_of(w.k0 + 1), r2 = row_of(w.k0 + 2), r3 = row_of(w.k0 + 3);
+            ok = load(&kmap, r0);
+            if (ok && ahead == 2 && w.n > 1) ok = load(&kmap, r1);
             for (int j = 0; ok && j < w.n; ++j) {
-                ok = load(&vmap, w.k0 + j);
-                if (ok && j + ahead < w.n) ok = load(&kmap, w.k0 + j + ahead);
+                ok = load(&vmap, r0);
+                if (ok && j + ahead < w.n) ok = load(&kmap, ahead == 1 ? r1 : r2);
+                r0 = r1;
+                r1 = r2;
+                r2 = r3;
+                r3 = row_of(w.k0 + j + 4);
             }
         }
         // Nothing may be in flight into this CTA's shared memory when it ends: all is consumed, unless a wait gave up.
@@ -537,59 +584,59 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
                 if (busy) {
                     tc_fence_after();
                     const int valid = w.tokens - (w.k0 + j) * kKeys;
-                    // First the maximum, then the exponentials, the scores read twice: a whole row of them beside the rest
-                    // does not fit the registers.  Each pass loads its next 32 columns while it works on these.
-                    uint32_t s[2][32];
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    tmem_ld32(s_addr, s[0]);
+                    // The exponentials of a tile refer to the maximum so far, so one pass over the scores does; its own maximum
+                    // comes out of the same pass.  Only a first tile has to look for it beforehand, and a tile that exceeds
+                    // it too far is done again, with O and the sum rescaled.  P stays in registers until that is known: it
+                    // overwrites the scores.
+                    uint32_t s[2][32], pk[64];
+                    if (j == j0) m = row_max(s_addr, s, valid) * p.sl2;
+                    float2 both;
+                    while (true) {
+                        const float ref = m == -INFINITY ? 0.f : m;
+                        const uint64_t scale2 = pack2(p.sl2, p.sl2), ref2 = pack2(-ref, -ref);
+                        uint64_t sum[2] = {0ull, 0ull};
+                        float top[2] = {-INFINITY, -INFINITY};
+                        tmem_ld32(s_addr, s[0]);
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        tmem_wait_ld(s[h & 1]);
-                        tmem_ld32(s_addr + ((h + 1) & 3) * 32, s[(h + 1) & 1]);
-                        mask_keys(s[h & 1], valid - h * 32);
+                        for (int h = 0; h < 4; ++h) {
+                            tmem_wait_ld(s[h & 1]);
+                            if (h < 3) tmem_ld32(s_addr + (h + 1) * 32, s[(h + 1) & 1]);
+                            mask_keys(s[h & 1], valid - h * 32);
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2)
-                            top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[h & 1][e])), __uint_as_float(s[h & 1][e + 1]));
-                    }
-                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.sl2;
-                    if (j == j0) {
-                        m = mx;  // the first product overwrites the accumulator
-                    } else if (__any_sync(0xffffffffu, mx > m + kRescale)) {
+                            for (int i = 0; i < 16; ++i) {
+                                const float s0 = __uint_as_float(s[h & 1][2 * i]), s1 = __uint_as_float(s[h & 1][2 * i + 1]);
+                                top[i & 1] = fmaxf(fmaxf(top[i & 1], s0), s1);
+                                const uint64_t x = fma2(pack2(s0, s1), scale2, ref2);
+                                uint64_t e;
+                                if (i % 4 == 3) {
+                                    e = exp2_poly2(x);
+                                } else {
+                                    const float2 v = unpack2(x);
+                                    e = pack2(exp2_unit(v.x), exp2_unit(v.y));
+                                }
+                                sum[i & 1] = add2(sum[i & 1], e);
+                                const float2 v = unpack2(e);
+                                pk[h * 16 + i] = Tr::pack(v.x, v.y);
+                            }
+                        }
+                        both = unpack2(add2(sum[0], sum[1]));
+                        const float mx = fmaxf(top[0], top[1]) * p.sl2;
+                        if (!__any_sync(0xffffffffu, mx > m + kFar)) break;
                         const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
                         m = mn;
                         l *= f;
 #pragma unroll
                         for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(o_addr + c, o);
-                            tmem_wait_ld(o);
+                            tmem_ld32(o_addr + c, s[0]);
+                            tmem_wait_ld(s[0]);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st32(o_addr + c, o);
+                            for (int i = 0; i < 32; ++i) s[0][i] = __float_as_uint(__uint_as_float(s[0][i]) * f);
+                            tmem_st32(o_addr + c, s[0]);
                         }
                     }
-                    const float ref = m == -INFINITY ? 0.f : m;
-                    const uint64_t scale2 = pack2(p.sl2, p.sl2), ref2 = pack2(-ref, -ref);
-                    uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        // P's columns 16 h .. lie in score columns that are already in registers
-                        tmem_wait_ld(s[h & 1]);
-                        if (h < 3) tmem_ld32(s_addr + (h + 1) * 32, s[(h + 1) & 1]);
-                        mask_keys(s[h & 1], valid - h * 32);
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float2 x = unpack2(fma2(pack2(__uint_as_float(s[h & 1][2 * i]), __uint_as_float(s[h & 1][2 * i + 1])),
-                                                          scale2, ref2));
-                            const float a = fast_exp2(x.x), b = fast_exp2(x.y);
-                            sum[i & 1] = add2(sum[i & 1], pack2(a, b));
-                            pk[i] = Tr::pack(a, b);
-                        }
-                        tmem_st16(s_addr + h * 16, pk);
-                    }
-                    const float2 both = unpack2(add2(sum[0], sum[1]));
                     l += both.x + both.y;
+                    tmem_st32(s_addr, pk);
+                    tmem_st32(s_addr + 32, pk + 32);
                     tmem_wait_st();
                     tc_fence_before();
                 }
@@ -601,18 +648,36 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             ++seg;
             if (busy) {
                 tc_fence_after();
-                const long long r0 = w.part_row + (t ? w.rows0 : 0) + row;
-                if (row < rows) p.part_ml[r0] = make_float2(m, l);
+                const long long r0 = w.part_row + (t ? w.rows0 : 0);
+                if (row < rows) p.part_ml[r0 + row] = make_float2(m, l);
                 if (two || t < w.n) {
+                    // 32 columns at a time through shared memory (16-byte places, swizzled), so that a store covers whole
+                    // 128-byte lines of four rows instead of a piece of 32 rows: 5800 clocks for a tile without it.
+                    const uint32_t mine = stage + warp * 4096u;
+                    const int first_row = (warp & 3) * 32;
 #pragma unroll
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
                         tmem_ld32(o_addr + c, o);
                         tmem_wait_ld(o);
-                        if (row < rows) {
 #pragma unroll
-                            for (int i = 0; i < 32; i += 8) store_sector(p.part_o + r0 * D + c + i, o + i);
+                        for (int i = 0; i < 8; ++i)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + lane * 128u + ((i ^ (lane & 7)) << 4)),
+                                         "r"(o[4 * i]), "r"(o[4 * i + 1]), "r"(o[4 * i + 2]), "r"(o[4 * i + 3])
+                                         : "memory");
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int r = i * 4 + (lane >> 3), c4 = lane & 7;
+                            float4 v;
+                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                         : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                                         : "r"(mine + r * 128u + ((c4 ^ (r & 7)) << 4))
+                                         : "memory");
+                            if (first_row + r < rows)
+                                *reinterpret_cast<float4*>(p.part_o + (r0 + first_row + r) * D + c + c4 * 4) = v;
                         }
+                        __syncwarp();
                     }
                 }
                 tc_fence_before();
@@ -828,8 +893,9 @@ int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMa
     const int rc = allow_smem(reinterpret_cast<const void*>(fn));
     if (rc != KVP_OK) return rc;
     constexpr size_t tile = static_cast<size_t>(kvpd::kKeys) * D * 2;
-    p.slots = D == 128 ? 5 : 10;  // 160 KB of K and V in flight beside two query tiles
-    fn<<<sm_count(), kvpd::kPrefixThreads, 1024 + (2 + p.slots) * tile, s>>>(qm, km, vm, p);
+    // 128 or 144 KB of K and V in flight beside two query tiles and the 32 KB that outputs pass through
+    p.slots = D == 128 ? 4 : 9;
+    fn<<<sm_count(), kvpd::kPrefixThreads, 1024 + (2 + p.slots) * tile + 32768, s>>>(qm, km, vm, p);
     return cuda_status(cudaGetLastError(), "shared prefix launch");
 }
 
@@ -916,6 +982,9 @@ extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stre
     p.g = g;
     p.max_blocks = a->max_blocks;
     p.B = a->block_size;
+    p.Bshift = -1;
+    if ((a->block_size & (a->block_size - 1)) == 0)
+        for (p.Bshift = 0; (1 << p.Bshift) < a->block_size;) ++p.Bshift;
     p.run = pl.run;
     p.runs = kvpd::kKeys / pl.run;
     p.oob_row = static_cast<int>(rows);
