@@ -38,7 +38,7 @@ namespace kvpd {
 
 constexpr int kKeys = 128;         // keys per tile
 constexpr int kRows = 128;         // rows per tile: M of the MMA
-constexpr int kPrefixThreads = 320;  // 8 softmax warps, the MMA warp, the loading warp
+constexpr int kPrefixThreads = 352;  // 8 softmax warps, the MMA warp, the warps that load K (and Q) and V
 constexpr int kTmemCols = 512;
 
 struct PrefixParams {
@@ -59,7 +59,6 @@ struct PrefixParams {
     int num_counters;
     int num_seqs, num_groups, nh, kvh, g, max_blocks, B, Bshift, run, runs, oob_row;
     int mt;                    // members per row tile
-    int slots;                 // ring slots
     int bf16, out_dtype;
     float sl2;
 };
@@ -108,7 +107,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
         "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
@@ -117,6 +116,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
         "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 // Waits for the loads so far; r: what the last one fills, so that no use of it is moved before the wait.
@@ -129,6 +136,13 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
                    "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One 32-byte sector of global memory.
+__device__ __forceinline__ void store_sector(float* p, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 
 // Shared-memory operand in the 128-byte swizzle: rows of 64 elements, 8-row atoms of 1024 bytes.
 //   along the rows (K-major: Q and K): atoms follow each other at 1024 bytes; a 16-element step is 32 bytes further.
@@ -155,17 +169,16 @@ __device__ __forceinline__ void mask_keys(uint32_t (&s)[32], int valid) {
 }
 
 // A row's largest score.
-__device__ __forceinline__ float row_max(uint32_t addr, uint32_t (&s)[2][32], int valid) {
+__device__ __forceinline__ float row_max(uint32_t addr, uint32_t (&s)[32], int valid) {
     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    tmem_ld32(addr, s[0]);
-#pragma unroll
+#pragma unroll 1
     for (int h = 0; h < 4; ++h) {
-        tmem_wait_ld(s[h & 1]);
-        if (h < 3) tmem_ld32(addr + (h + 1) * 32, s[(h + 1) & 1]);
-        mask_keys(s[h & 1], valid - h * 32);
+        tmem_ld32(addr + h * 32, s);
+        tmem_wait_ld(s);
+        mask_keys(s, valid - h * 32);
 #pragma unroll
         for (int e = 0; e < 32; e += 2)
-            top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[h & 1][e])), __uint_as_float(s[h & 1][e + 1]));
+            top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
     }
     return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
@@ -324,7 +337,7 @@ __device__ __forceinline__ Start find_start(const PrefixParams& p, long long* wa
 
 // ---------------------------------------------------------------- the kernel
 struct PrefixShared {
-    uint64_t full[16], empty[16];  // ring slots
+    uint64_t full[2][8], empty[2][8];  // the rings' slots: K, V
     uint64_t q_full, q_free, s_full[2], p_full[2], o_full[2], drain;
     uint32_t tmem;
     int abort;
@@ -378,7 +391,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     __shared__ PrefixShared sh;
     extern __shared__ uint8_t dyn[];
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
-    const uint32_t ring = base + 2 * kTile, stage = ring + p.slots * kTile;
+    // Slots of K and of V beside two query tiles: 160 KB in all.
+    constexpr int kSlotsK = D == 128 ? 2 : 5, kSlotsV = D == 128 ? 3 : 5;
+    const uint32_t ring_k = base + 2 * kTile, ring_v = ring_k + kSlotsK * kTile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // the next kernel may be scheduled as soon as this one's CTAs leave their SMs; it waits for all of them
@@ -386,9 +401,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     for (int i = blockIdx.x * kPrefixThreads + threadIdx.x; i < p.num_counters; i += gridDim.x * kPrefixThreads) p.counters[i] = 0;
     if (threadIdx.x == 0) {
         sh.abort = 0;
-        for (int s = 0; s < p.slots; ++s) {
-            mbar_init(smem_u32(&sh.full[s]), 1);
-            mbar_init(smem_u32(&sh.empty[s]), 1);
+        for (int s = 0; s < 8; ++s) {
+            mbar_init(smem_u32(&sh.full[0][s]), 1);
+            mbar_init(smem_u32(&sh.empty[0][s]), 1);
+            mbar_init(smem_u32(&sh.full[1][s]), 1);
+            mbar_init(smem_u32(&sh.empty[1][s]), 1);
         }
         mbar_init(smem_u32(&sh.q_full), 1);
         mbar_init(smem_u32(&sh.q_free), 1);
@@ -400,7 +417,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         mbar_init(smem_u32(&sh.drain), 1);
         fence_barrier_init();
     }
-    if (warp == 9 && lane == 0) {
+    if (warp == 10 && lane == 0) {
         prefetch_tensormap(&qmap);
         prefetch_tensormap(&kmap);
         prefetch_tensormap(&vmap);
@@ -425,30 +442,21 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const uint32_t tmem = sh.tmem;
     Work w;
 
-    if (warp == 9) {
-        // ------------------------------------------------------------ loads
+    if (warp >= 9) {
+        // ------------------------------------------------------------ loads: K and the queries, and V
+        // Each lane issues one copy (a run of tokens within a block, 64 dims); the copies of a warp's lanes are issued one
+        // after the other, at about 60 clocks each, which is why K and V have a warp each.
+        const int v = warp - 9, slots = v ? kSlotsV : kSlotsK;
+        const uint32_t ring = v ? ring_v : ring_k;
+        const CUtensorMap* map = v ? &vmap : &kmap;
         bool ok = true;
         Cursor at{0, 0u};
         int loaded = 0, queries = 0;  // tiles and query loads issued
         while (ok && list.next(p, w)) {
-            // queries, once the previous stretch's products have read theirs
-            if (queries > 0) ok = warp_wait(&sh.q_free, (queries - 1) & 1, p, sh);
-            if (!ok) break;
-            ++queries;
-            if (lane == 0) {
-                const uint32_t bar = smem_u32(&sh.q_full);
-                const int tiles = w.rows1 ? 2 : 1;
-                mbar_arrive_expect_tx(bar, static_cast<uint32_t>(tiles * NCH * p.mt * p.g) * 128u);
-                for (int t = 0; t < tiles; ++t)
-                    for (int c = 0; c < NCH; ++c)
-                        tma_load_3d(base + t * kTile + c * kCol, &qmap, bar, c * 64, w.head * p.g, w.start + w.member0 + t * p.mt);
-            }
-            __syncwarp();
             const int32_t* trow = p.tables + static_cast<long long>(w.start) * p.max_blocks;
-            const int ahead = w.rows1 ? 1 : 2;  // K runs ahead of V by as many tiles
-            const int run = lane / NCH, c = lane - run * NCH;  // this lane's copy of a tile
-            // The pool row of this lane's run of a tile.  Rows of the next four tiles are kept, so that the table's latency
-            // is long past when a tile's copies are issued: looked up one by one it held the loads to 1750 clocks a tile.
+            const int run = lane / NCH, c = lane - run * NCH;
+            // The pool row of this lane's run of a tile, looked up a tile ahead, so that the table's latency is past when it is
+            // needed.
             auto row_of = [&](int kt) {
                 const int tok = kt * kKeys + run * p.run;
                 if (run >= p.runs || tok >= w.tokens || kt >= w.k0 + w.n) return p.oob_row;  // zeros behind the shared tokens
@@ -458,53 +466,58 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
                 report(p.status, KVP_STATUS_BAD_BLOCK);
                 return p.oob_row;
             };
-            auto load = [&](const CUtensorMap* map, int row) {
-                const int st = at.slot;
-                if (loaded >= p.slots && !warp_wait(&sh.empty[st], at.parity ^ 1u, p, sh)) return false;
-                const uint32_t bar = smem_u32(&sh.full[st]);
+            int row = row_of(w.k0);
+            if (v == 0) {  // queries, once the previous stretch's products have read theirs
+                if (queries > 0) ok = warp_wait(&sh.q_free, (queries - 1) & 1, p, sh);
+                if (!ok) break;
+                ++queries;
+                if (lane == 0) {
+                    const uint32_t bar = smem_u32(&sh.q_full);
+                    const int tiles = w.rows1 ? 2 : 1;
+                    mbar_arrive_expect_tx(bar, static_cast<uint32_t>(tiles * NCH * p.mt * p.g) * 128u);
+                    for (int t = 0; t < tiles; ++t)
+                        for (int k = 0; k < NCH; ++k)
+                            tma_load_3d(base + t * kTile + k * kCol, &qmap, bar, k * 64, w.head * p.g, w.start + w.member0 + t * p.mt);
+                }
+                __syncwarp();
+            }
+            for (int j = 0; ok && j < w.n; ++j) {
+                const int next_row = row_of(w.k0 + j + 1);
+                if (loaded >= slots && !(ok = warp_wait(&sh.empty[v][at.slot], at.parity ^ 1u, p, sh))) break;
+                const uint32_t bar = smem_u32(&sh.full[v][at.slot]);
                 if (lane == 0) mbar_arrive_expect_tx(bar, kTile);
                 __syncwarp();
                 if (run < p.runs)
-                    tma_load_3d(ring + st * kTile + c * kCol + static_cast<uint32_t>(run * p.run) * 128u, map, bar, c * 64, w.head, row);
-                at = at.next(p.slots);
+                    tma_load_3d(ring + at.slot * kTile + c * kCol + static_cast<uint32_t>(run * p.run) * 128u, map, bar, c * 64,
+                                w.head, row);
+                row = next_row;
+                at = at.next(slots);
                 ++loaded;
-                return true;
-            };
-            int r0 = row_of(w.k0), r1 = row_of(w.k0 + 1), r2 = row_of(w.k0 + 2), r3 = row_of(w.k0 + 3);
-            ok = load(&kmap, r0);
-            if (ok && ahead == 2 && w.n > 1) ok = load(&kmap, r1);
-            for (int j = 0; ok && j < w.n; ++j) {
-                ok = load(&vmap, r0);
-                if (ok && j + ahead < w.n) ok = load(&kmap, ahead == 1 ? r1 : r2);
-                r0 = r1;
-                r1 = r2;
-                r2 = r3;
-                r3 = row_of(w.k0 + j + 4);
             }
         }
         // Nothing may be in flight into this CTA's shared memory when it ends: all is consumed, unless a wait gave up.
-        if (!ok || *reinterpret_cast<volatile int*>(&sh.abort)) {
-            if (lane == 0) {
-                for (int s = 0; s < p.slots; ++s) {
-                    const int n = loaded > s ? (loaded - s - 1) / p.slots + 1 : 0;  // tiles loaded into slot s
-                    if (n > 0) mbar_wait(smem_u32(&sh.full[s]), static_cast<uint32_t>((n - 1) & 1), p.wait_limit);
-                }
-                if (queries > 0) mbar_wait(smem_u32(&sh.q_full), static_cast<uint32_t>((queries - 1) & 1), p.wait_limit);
+        if ((!ok || *reinterpret_cast<volatile int*>(&sh.abort)) && lane == 0) {
+            for (int s = 0; s < slots; ++s) {
+                const int n = loaded > s ? (loaded - s - 1) / slots + 1 : 0;  // tiles loaded into slot s
+                if (n > 0) mbar_wait(smem_u32(&sh.full[v][s]), static_cast<uint32_t>((n - 1) & 1), p.wait_limit);
             }
+            if (queries > 0) mbar_wait(smem_u32(&sh.q_full), static_cast<uint32_t>((queries - 1) & 1), p.wait_limit);
         }
+        __syncwarp();
     } else if (warp == 8) {
         // ------------------------------------------------------------ MMAs, one thread
+        // One thread for both warpgroups keeps their products one after the other, and with them the turns of the
+        // warpgroups: issued by two threads the products of both ran side by side, both softmaxes waited for them and then
+        // ran at the same time, 4950 clocks for a pair of tiles.
         if (lane == 0) {
             const uint32_t qk_desc = mma_desc(p.bf16, kKeys, false);
             const uint32_t pv_desc = mma_desc(p.bf16, D, true);
             bool ok = true;
-            Cursor at{0, 0u};
-            int seg = 0;
-            uint32_t turn[2] = {0u, 0u};  // parity of the next P tile, per warpgroup
-            auto wait_tile = [&](Cursor c) { return wait_or_abort(&sh.full[c.slot], c.parity, p, sh); };
-            const uint32_t q_lo = desc_lo(base, 16), k_lo = desc_lo(ring, 16), v_lo = desc_lo(ring, kCol);
-            auto qk = [&](int t, int qt, Cursor c_) {
-                const uint32_t q = q_lo + qt * (kTile >> 4), k = k_lo + static_cast<uint32_t>(c_.slot) * (kTile >> 4);
+            Cursor kat{0, 0u}, vat{0, 0u};
+            uint32_t seg = 0, turn0 = 0, turn1 = 0;  // parities of the next queries and of the next P tile of each warpgroup
+            const uint32_t q_lo = desc_lo(base, 16), k_lo = desc_lo(ring_k, 16), v_lo = desc_lo(ring_v, kCol);
+            auto qk = [&](int t, int qt, int slot) {
+                const uint32_t q = q_lo + qt * (kTile >> 4), k = k_lo + static_cast<uint32_t>(slot) * (kTile >> 4);
 #pragma unroll
                 for (int c = 0; c < NCH; ++c)
 #pragma unroll
@@ -513,44 +526,42 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
                                qk_desc, c + s > 0);
                 tc_commit(smem_u32(&sh.s_full[t]));
             };
+            auto wait_k = [&] { return wait_or_abort(&sh.full[0][kat.slot], kat.parity, p, sh); };
+            auto done_k = [&] {
+                tc_commit(smem_u32(&sh.empty[0][kat.slot]));
+                kat = kat.next(kSlotsK);
+            };
             while (ok && list.next(p, w)) {
                 const bool two = w.rows1 > 0;
                 const int ahead = two ? 1 : 2;
                 ok = wait_or_abort(&sh.q_full, seg & 1, p, sh);
-                // K tiles 0 .. ahead - 1, then V_j and K_{j + ahead} in turn
                 for (int i = 0; ok && i < min(ahead, w.n); ++i) {
-                    if (!(ok = wait_tile(at))) break;
+                    if (!(ok = wait_k())) break;
                     tc_fence_after();
-                    if (two) {
-                        qk(0, 0, at);
-                        qk(1, 1, at);
-                    } else {
-                        qk(i, 0, at);
-                    }
-                    tc_commit(smem_u32(&sh.empty[at.slot]));
-                    at = at.next(p.slots);
+                    for (int t = two ? 0 : i; t <= (two ? 1 : i); ++t) qk(t, two ? t : 0, kat.slot);
+                    done_k();
                 }
                 for (int j = 0; ok && j < w.n; ++j) {
                     const bool more = j + ahead < w.n;
-                    const Cursor vn = at, kn = at.next(p.slots);
-                    if (!(ok = wait_tile(vn))) break;
-                    if (more && !(ok = wait_tile(kn))) break;
-                    for (int i = 0; i < (two ? 2 : 1); ++i) {
-                        const int t = two ? i : j & 1;
-                        if (!(ok = wait_or_abort(&sh.p_full[t], t ? turn[1] : turn[0], p, sh))) break;
-                        if (t) turn[1] ^= 1u; else turn[0] ^= 1u;
+                    if (!(ok = wait_or_abort(&sh.full[1][vat.slot], vat.parity, p, sh))) break;
+                    for (int t = two ? 0 : j & 1; t <= (two ? 1 : j & 1); ++t) {
+                        if (!(ok = wait_or_abort(&sh.p_full[t], (t ? turn1 : turn0) & 1, p, sh))) break;
+                        if (t) ++turn1; else ++turn0;
                         tc_fence_after();
-                        const uint32_t v = v_lo + static_cast<uint32_t>(vn.slot) * (kTile >> 4);
-                        const bool add = two ? j > 0 : j > 1;
+                        const uint32_t v = v_lo + static_cast<uint32_t>(vat.slot) * (kTile >> 4);
+                        const bool add = j >= ahead;
 #pragma unroll
                         for (int s = 0; s < kKeys / 16; ++s)
                             mma_ts(tmem + kO + t * D, tmem + t * kKeys + s * 8, v + s * (2048 >> 4), kDescHi, pv_desc, add || s > 0);
-                        if (more) qk(t, two ? t : 0, kn);
+                        if (more) {
+                            if (!(ok = wait_k())) break;
+                            qk(t, two ? t : 0, kat.slot);
+                        }
                     }
                     if (!ok) break;
-                    tc_commit(smem_u32(&sh.empty[vn.slot]));
-                    if (more) tc_commit(smem_u32(&sh.empty[kn.slot]));
-                    at = more ? kn.next(p.slots) : kn;
+                    tc_commit(smem_u32(&sh.empty[1][vat.slot]));
+                    vat = vat.next(kSlotsV);
+                    if (more) done_k();
                 }
                 if (ok) {
                     tc_commit(smem_u32(&sh.o_full[0]));
@@ -584,59 +595,53 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
                 if (busy) {
                     tc_fence_after();
                     const int valid = w.tokens - (w.k0 + j) * kKeys;
-                    // The exponentials of a tile refer to the maximum so far, so one pass over the scores does; its own maximum
-                    // comes out of the same pass.  Only a first tile has to look for it beforehand, and a tile that exceeds
-                    // it too far is done again, with O and the sum rescaled.  P stays in registers until that is known: it
-                    // overwrites the scores.
-                    uint32_t s[2][32], pk[64];
-                    if (j == j0) m = row_max(s_addr, s, valid) * p.sl2;
-                    float2 both;
-                    while (true) {
-                        const float ref = m == -INFINITY ? 0.f : m;
-                        const uint64_t scale2 = pack2(p.sl2, p.sl2), ref2 = pack2(-ref, -ref);
-                        uint64_t sum[2] = {0ull, 0ull};
-                        float top[2] = {-INFINITY, -INFINITY};
-                        tmem_ld32(s_addr, s[0]);
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) {
-                            tmem_wait_ld(s[h & 1]);
-                            if (h < 3) tmem_ld32(s_addr + (h + 1) * 32, s[(h + 1) & 1]);
-                            mask_keys(s[h & 1], valid - h * 32);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const float s0 = __uint_as_float(s[h & 1][2 * i]), s1 = __uint_as_float(s[h & 1][2 * i + 1]);
-                                top[i & 1] = fmaxf(fmaxf(top[i & 1], s0), s1);
-                                const uint64_t x = fma2(pack2(s0, s1), scale2, ref2);
-                                uint64_t e;
-                                if (i % 4 == 3) {
-                                    e = exp2_poly2(x);
-                                } else {
-                                    const float2 v = unpack2(x);
-                                    e = pack2(exp2_unit(v.x), exp2_unit(v.y));
-                                }
-                                sum[i & 1] = add2(sum[i & 1], e);
-                                const float2 v = unpack2(e);
-                                pk[h * 16 + i] = Tr::pack(v.x, v.y);
-                            }
-                        }
-                        both = unpack2(add2(sum[0], sum[1]));
-                        const float mx = fmaxf(top[0], top[1]) * p.sl2;
-                        if (!__any_sync(0xffffffffu, mx > m + kFar)) break;
+                    // The row's maximum, then the exponentials, the scores read twice and 32 at a time: loops, not one long
+                    // stretch of code, whose way through the instruction caches cost a launch 10 us.
+                    uint32_t s[32];
+                    const float mx = row_max(s_addr, s, valid) * p.sl2;
+                    if (j == j0) {
+                        m = mx;  // the first product overwrites the accumulator
+                    } else if (__any_sync(0xffffffffu, mx > m + kFar)) {
                         const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
                         m = mn;
                         l *= f;
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D; c += 32) {
-                            tmem_ld32(o_addr + c, s[0]);
-                            tmem_wait_ld(s[0]);
+                            tmem_ld32(o_addr + c, s);
+                            tmem_wait_ld(s);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) s[0][i] = __float_as_uint(__uint_as_float(s[0][i]) * f);
-                            tmem_st32(o_addr + c, s[0]);
+                            for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * f);
+                            tmem_st32(o_addr + c, s);
                         }
                     }
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    const uint64_t scale2 = pack2(p.sl2, p.sl2), ref2 = pack2(-ref, -ref);
+                    uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll 1
+                    for (int h = 0; h < 4; ++h) {
+                        // P's columns 16 h .. lie in score columns that have been read
+                        tmem_ld32(s_addr + h * 32, s);
+                        tmem_wait_ld(s);
+                        mask_keys(s, valid - h * 32);
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const uint64_t x = fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, ref2);
+                            uint64_t e;
+                            if (i % 4 == 3) {
+                                e = exp2_poly2(x);
+                            } else {
+                                const float2 v = unpack2(x);
+                                e = pack2(exp2_unit(v.x), exp2_unit(v.y));
+                            }
+                            sum[i & 1] = add2(sum[i & 1], e);
+                            const float2 v = unpack2(e);
+                            pk[i] = Tr::pack(v.x, v.y);
+                        }
+                        tmem_st16(s_addr + h * 16, pk);
+                    }
+                    const float2 both = unpack2(add2(sum[0], sum[1]));
                     l += both.x + both.y;
-                    tmem_st32(s_addr, pk);
-                    tmem_st32(s_addr + 32, pk + 32);
                     tmem_wait_st();
                     tc_fence_before();
                 }
@@ -648,36 +653,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             ++seg;
             if (busy) {
                 tc_fence_after();
-                const long long r0 = w.part_row + (t ? w.rows0 : 0);
-                if (row < rows) p.part_ml[r0 + row] = make_float2(m, l);
+                const long long r0 = w.part_row + (t ? w.rows0 : 0) + row;
+                if (row < rows) p.part_ml[r0] = make_float2(m, l);
                 if (two || t < w.n) {
-                    // 32 columns at a time through shared memory (16-byte places, swizzled), so that a store covers whole
-                    // 128-byte lines of four rows instead of a piece of 32 rows: 5800 clocks for a tile without it.
-                    const uint32_t mine = stage + warp * 4096u;
-                    const int first_row = (warp & 3) * 32;
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
                         tmem_ld32(o_addr + c, o);
                         tmem_wait_ld(o);
+                        if (row < rows) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + lane * 128u + ((i ^ (lane & 7)) << 4)),
-                                         "r"(o[4 * i]), "r"(o[4 * i + 1]), "r"(o[4 * i + 2]), "r"(o[4 * i + 3])
-                                         : "memory");
-                        __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int r = i * 4 + (lane >> 3), c4 = lane & 7;
-                            float4 v;
-                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                         : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                                         : "r"(mine + r * 128u + ((c4 ^ (r & 7)) << 4))
-                                         : "memory");
-                            if (first_row + r < rows)
-                                *reinterpret_cast<float4*>(p.part_o + (r0 + first_row + r) * D + c + c4 * 4) = v;
+                            for (int i = 0; i < 32; i += 8) store_sector(p.part_o + r0 * D + c + i, o + i);
                         }
-                        __syncwarp();
                     }
                 }
                 tc_fence_before();
@@ -893,9 +880,7 @@ int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMa
     const int rc = allow_smem(reinterpret_cast<const void*>(fn));
     if (rc != KVP_OK) return rc;
     constexpr size_t tile = static_cast<size_t>(kvpd::kKeys) * D * 2;
-    // 128 or 144 KB of K and V in flight beside two query tiles and the 32 KB that outputs pass through
-    p.slots = D == 128 ? 4 : 9;
-    fn<<<sm_count(), kvpd::kPrefixThreads, 1024 + (2 + p.slots) * tile + 32768, s>>>(qm, km, vm, p);
+    fn<<<sm_count(), kvpd::kPrefixThreads, 1024 + (2 + (D == 128 ? 5 : 10)) * tile, s>>>(qm, km, vm, p);
     return cuda_status(cudaGetLastError(), "shared prefix launch");
 }
 
