@@ -168,17 +168,21 @@ __device__ __forceinline__ void mask_keys(uint32_t (&s)[32], int valid) {
         if (i >= valid) s[i] = 0xff800000u;
 }
 
-// A row's largest score.
-__device__ __forceinline__ float row_max(uint32_t addr, uint32_t (&s)[32], int valid) {
+// A row's largest score; its first 32 scores are on their way to s[0] again when it returns.
+__device__ __forceinline__ float row_max(uint32_t addr, uint32_t (&s)[2][32], int valid) {
     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    tmem_ld32(addr, s[0]);
 #pragma unroll 1
-    for (int h = 0; h < 4; ++h) {
-        tmem_ld32(addr + h * 32, s);
-        tmem_wait_ld(s);
-        mask_keys(s, valid - h * 32);
+    for (int h = 0; h < 4; h += 2) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 2)
-            top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
+        for (int b = 0; b < 2; ++b) {
+            tmem_wait_ld(s[b]);
+            tmem_ld32(addr + ((h + b + 1) & 3) * 32, s[b ^ 1]);
+            mask_keys(s[b], valid - (h + b) * 32);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+                top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[b][e])), __uint_as_float(s[b][e + 1]));
+        }
     }
     return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
@@ -338,7 +342,7 @@ __device__ __forceinline__ Start find_start(const PrefixParams& p, long long* wa
 // ---------------------------------------------------------------- the kernel
 struct PrefixShared {
     uint64_t full[2][8], empty[2][8];  // the rings' slots: K, V
-    uint64_t q_full, q_free, s_full[2], p_full[2], o_full[2], drain;
+    uint64_t q_full, q_free, s_full[2], p_full[2][2], o_full[2], drain;  // p_full: P's first and second 64 keys
     uint32_t tmem;
     int abort;
     Start found;
@@ -411,7 +415,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         mbar_init(smem_u32(&sh.q_free), 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(smem_u32(&sh.s_full[t]), 1);
-            mbar_init(smem_u32(&sh.p_full[t]), 4);
+            mbar_init(smem_u32(&sh.p_full[t][0]), 4);
+            mbar_init(smem_u32(&sh.p_full[t][1]), 4);
             mbar_init(smem_u32(&sh.o_full[t]), 1);
         }
         mbar_init(smem_u32(&sh.drain), 1);
@@ -545,14 +550,20 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
                     const bool more = j + ahead < w.n;
                     if (!(ok = wait_or_abort(&sh.full[1][vat.slot], vat.parity, p, sh))) break;
                     for (int t = two ? 0 : j & 1; t <= (two ? 1 : j & 1); ++t) {
-                        if (!(ok = wait_or_abort(&sh.p_full[t], (t ? turn1 : turn0) & 1, p, sh))) break;
+                        const uint32_t turn = (t ? turn1 : turn0) & 1;
                         if (t) ++turn1; else ++turn0;
-                        tc_fence_after();
                         const uint32_t v = v_lo + static_cast<uint32_t>(vat.slot) * (kTile >> 4);
                         const bool add = j >= ahead;
 #pragma unroll
-                        for (int s = 0; s < kKeys / 16; ++s)
-                            mma_ts(tmem + kO + t * D, tmem + t * kKeys + s * 8, v + s * (2048 >> 4), kDescHi, pv_desc, add || s > 0);
+                        for (int half = 0; half < 2; ++half) {  // the first half runs while the second's P is computed
+                            if (ok) ok = wait_or_abort(&sh.p_full[t][half], turn, p, sh);
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int s = half * 4; s < half * 4 + 4; ++s)
+                                mma_ts(tmem + kO + t * D, tmem + t * kKeys + s * 8, v + s * (2048 >> 4), kDescHi, pv_desc, add || s > 0);
+                        }
+                        if (!ok) break;
                         if (more) {
                             if (!(ok = wait_k())) break;
                             qk(t, two ? t : 0, kat.slot);
@@ -597,7 +608,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
                     const int valid = w.tokens - (w.k0 + j) * kKeys;
                     // The row's maximum, then the exponentials, the scores read twice and 32 at a time: loops, not one long
                     // stretch of code, whose way through the instruction caches cost a launch 10 us.
-                    uint32_t s[32];
+                    uint32_t s[2][32];
                     const float mx = row_max(s_addr, s, valid) * p.sl2;
                     if (j == j0) {
                         m = mx;  // the first product overwrites the accumulator
@@ -607,46 +618,54 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
                         l *= f;
 #pragma unroll 1
                         for (int c = 0; c < D; c += 32) {
-                            tmem_ld32(o_addr + c, s);
-                            tmem_wait_ld(s);
+                            tmem_ld32(o_addr + c, s[1]);
+                            tmem_wait_ld(s[1]);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * f);
-                            tmem_st32(o_addr + c, s);
+                            for (int i = 0; i < 32; ++i) s[1][i] = __float_as_uint(__uint_as_float(s[1][i]) * f);
+                            tmem_st32(o_addr + c, s[1]);
                         }
                     }
                     const float ref = m == -INFINITY ? 0.f : m;
                     const uint64_t scale2 = pack2(p.sl2, p.sl2), ref2 = pack2(-ref, -ref);
                     uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll 1
-                    for (int h = 0; h < 4; ++h) {
-                        // P's columns 16 h .. lie in score columns that have been read
-                        tmem_ld32(s_addr + h * 32, s);
-                        tmem_wait_ld(s);
-                        mask_keys(s, valid - h * 32);
-                        uint32_t pk[16];
+                    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const uint64_t x = fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, ref2);
-                            uint64_t e;
-                            if (i % 4 == 3) {
-                                e = exp2_poly2(x);
-                            } else {
-                                const float2 v = unpack2(x);
-                                e = pack2(exp2_unit(v.x), exp2_unit(v.y));
+                        for (int b = 0; b < 2; ++b) {
+                            // P's columns 16 h .. lie in score columns that are in registers
+                            const int h = half * 2 + b;
+                            tmem_wait_ld(s[b]);
+                            if (h < 3) tmem_ld32(s_addr + (h + 1) * 32, s[b ^ 1]);
+                            mask_keys(s[b], valid - h * 32);
+                            uint32_t pk[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const uint64_t x = fma2(pack2(__uint_as_float(s[b][2 * i]), __uint_as_float(s[b][2 * i + 1])), scale2, ref2);
+                                uint64_t e;
+                                if (i % 4 == 3) {
+                                    e = exp2_poly2(x);
+                                } else {
+                                    const float2 v = unpack2(x);
+                                    e = pack2(exp2_unit(v.x), exp2_unit(v.y));
+                                }
+                                sum[i & 1] = add2(sum[i & 1], e);
+                                const float2 v = unpack2(e);
+                                pk[i] = Tr::pack(v.x, v.y);
                             }
-                            sum[i & 1] = add2(sum[i & 1], e);
-                            const float2 v = unpack2(e);
-                            pk[i] = Tr::pack(v.x, v.y);
+                            tmem_st16(s_addr + h * 16, pk);
                         }
-                        tmem_st16(s_addr + h * 16, pk);
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[t][half]));
                     }
                     const float2 both = unpack2(add2(sum[0], sum[1]));
                     l += both.x + both.y;
-                    tmem_wait_st();
-                    tc_fence_before();
+                } else if (lane == 0) {
+                    mbar_arrive(smem_u32(&sh.p_full[t][0]));
+                    mbar_arrive(smem_u32(&sh.p_full[t][1]));
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[t]));
             }
             if (!ok) break;
             if (!(ok = warp_wait(&sh.o_full[t], seg & 1, p, sh))) break;
