@@ -331,10 +331,8 @@ extern "C" KVP_API size_t kvp_attention_workspace_size(const kvp_attn_args* a) {
 namespace {
 
 // kvp_paged_attention with every pipeline wait limited to `wait_limit` clock cycles; `stall` arms the first stage
-// of the CTAs in the grid's first row for a copy that is never issued (kvp_attention_wait_test only).  With
-// `skip_blocks` the attention over the sequences' own parts (attention_own_parts).
-int attention_call(const kvp_attn_args* a, void* stream, long long wait_limit, int stall,
-                   const int32_t* skip_blocks = nullptr, float* lse = nullptr) {
+// of the CTAs in the grid's first row for a copy that is never issued (kvp_attention_wait_test only).
+int attention_call(const kvp_attn_args* a, void* stream, long long wait_limit, int stall) {
     using namespace kvpi;
     clear_error();
     if (!a) return fail(KVP_EINVAL, "null arguments");
@@ -443,9 +441,6 @@ int attention_call(const kvp_attn_args* a, void* stream, long long wait_limit, i
     const float scale = a->scale > 0.f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
     prm.sl2 = scale * 1.4426950408889634f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    prm.skip_blocks = skip_blocks;
-    prm.lse = lse;
-    if (skip_blocks) return kvpd::launch_own_parts(*a, pl, prm, km, vm, s);
     const bool qres = a->q_dtype != a->kv_dtype;
     if (a->kv_dtype == KVP_DTYPE_F16)
         return qres ? kvpd::launch_f16_qres(*a, pl, prm, km, vm, s) : kvpd::launch_f16(*a, pl, prm, km, vm, s);
@@ -453,10 +448,6 @@ int attention_call(const kvp_attn_args* a, void* stream, long long wait_limit, i
 }
 
 }  // namespace
-
-int kvpi::attention_own_parts(const kvp_attn_args* a, const int32_t* skip_blocks, float* lse, cudaStream_t stream) {
-    return attention_call(a, stream, kvpd::kWaitLimitCycles, 0, skip_blocks, lse);
-}
 
 extern "C" KVP_API int kvp_paged_attention(const kvp_attn_args* a, void* stream) {
     return attention_call(a, stream, kvpd::kWaitLimitCycles, 0);

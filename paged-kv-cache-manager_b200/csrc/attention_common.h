@@ -12,11 +12,8 @@
 namespace kvpi {
 // Opts a kernel into the whole dynamic shared-memory budget, once per device.
 int allow_smem(const void* fn);
+// The driver's tensor-map encoder, or null.
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
-// The attention over each sequence's own part: its context behind skip_blocks[s] blocks, into a->out (normalised) and
-// lse (log2 of the softmax sum of each [num_seqs][num_heads] row, -inf where there is nothing).  a: the balanced
-// schedule (a workspace, split_tiles 0), the shapes of launch_own_parts().
-int attention_own_parts(const kvp_attn_args* a, const int32_t* skip_blocks, float* lse, cudaStream_t stream);
 }  // namespace kvpi
 
 namespace kvpd {
@@ -73,10 +70,6 @@ struct AttnParams {
     // 32-bit signed difference (bounded wait, KVP_STATUS_TIMEOUT).
     const int32_t* inputs_ready;
     const int32_t* inputs_epoch;
-    // Sequences in groups that share leading blocks (the SFX kernels, else null): blocks of each sequence that are
-    // attended over elsewhere, and the log2 of each (sequence, head) row's softmax sum, written beside `out`.
-    const int32_t* skip_blocks;
-    float* lse;
 };
 
 // Per-CTA pipeline state in shared memory: `abort` is raised by a consumer warp whose wait gave up, so the
@@ -96,8 +89,5 @@ KVPD_DECLARE_VARIANT(f16_qres)
 KVPD_DECLARE_VARIANT(bf16)
 KVPD_DECLARE_VARIANT(bf16_qres)
 #undef KVPD_DECLARE_VARIANT
-// The own parts of sequences in groups (attention_inst_own.cu): head_dim 64 or 128, queries of the pools' dtype.
-int launch_own_parts(const kvp_attn_args& a, const kvpi::AttnPlan& pl, const AttnParams& prm, const CUtensorMap& km,
-                     const CUtensorMap& vm, cudaStream_t s);
 
 }  // namespace kvpd

@@ -52,23 +52,6 @@ __device__ __forceinline__ int tiles_of_len(const AttnParams& p, int len) {
     return (len + 15) >> 4;
 }
 
-// The context a kernel attends over for sequence `seq`: all of it, or (SFX: the own part of a sequence whose leading
-// blocks another kernel attends over for a whole group) what lies behind its first skip_blocks blocks -- possibly
-// nothing.  A sequence with an invalid length or skip count has none.
-template <bool SFX>
-__device__ __forceinline__ int own_len(const AttnParams& p, int seq) {
-    const int len = __ldg(p.lens + seq);
-    if constexpr (!SFX) {
-        return len;
-    } else {
-        const long long skip = static_cast<long long>(__ldg(p.skip_blocks + seq)) * p.B;
-        if (tiles_of_len(p, len) == 0 || skip < 0 || skip > len) return 0;
-        return static_cast<int>(len - skip);
-    }
-}
-// Log2 of a (sequence, head) row's softmax sum, beside its normalised output (SFX).
-__device__ __forceinline__ void store_lse(const AttnParams& p, size_t row, float m, float l) { p.lse[row] = m + log2f(l); }
-
 template <int D>
 struct Geo {
     static constexpr int W = (D % 64 == 0) ? 64 : 32;  // elements per smem row
@@ -79,12 +62,11 @@ struct Geo {
 };
 
 // ---------------------------------------------------------------- producer: one tile into one stage
-// All 32 lanes call this (the table cache is a warp-wide register array); lane 0 issues the copies.  row_blocks:
-// entries of the table row that may be read.
+// All 32 lanes call this (the table cache is a warp-wide register array); lane 0 issues the copies.
 template <int D>
 __device__ __forceinline__ void produce_tile(const AttnParams& p, const CUtensorMap* km, const CUtensorMap* vm,
                                              uint32_t kst, uint32_t vst, uint32_t fb, int tb, int len,
-                                             const int32_t* trow, int row_blocks, int kvh0, int lane, int& cache_lo,
+                                             const int32_t* trow, int kvh0, int lane, int& cache_lo,
                                              int32_t& cached) {
     using G_ = Geo<D>;
     const int nr = min(p.nruns, (len - tb + p.R - 1) / p.R);
@@ -94,7 +76,7 @@ __device__ __forceinline__ void produce_tile(const AttnParams& p, const CUtensor
         const int bi = blk_of(p, tok);
         if (bi < cache_lo || bi >= cache_lo + 32) {
             cache_lo = bi;
-            cached = (bi + lane < row_blocks) ? __ldg(trow + bi + lane) : 0;
+            cached = (bi + lane < p.max_blocks) ? __ldg(trow + bi + lane) : 0;
         }
         const int32_t blk = __shfl_sync(0xffffffffu, cached, bi - cache_lo);
         int row = blk * p.B + (tok - bi * p.B);
@@ -158,15 +140,15 @@ __device__ __forceinline__ void append_new_token(const AttnParams& p, int seq, i
 template <int D>
 __device__ __forceinline__ bool produce_batch(const AttnParams& p, const CUtensorMap* km, const CUtensorMap* vm,
                                               uint32_t smem_base, uint64_t* full_bar, uint64_t* empty_bar, int st0,
-                                              int r0, int tile, int nb, int len, const int32_t* trow, int row_blocks,
-                                              int kvh0, int lane, int& cache_lo, int32_t& cached, unsigned& issued) {
+                                              int r0, int tile, int nb, int len, const int32_t* trow, int kvh0,
+                                              int lane, int& cache_lo, int32_t& cached, unsigned& issued) {
     using G_ = Geo<D>;
     const int S = p.stages;
     const int bi_first = blk_of(p, tile * 16);
     const int bi_last = blk_of(p, min((tile + nb) * 16, len) - 1);
     if (bi_first < cache_lo || bi_last >= cache_lo + 32) {
         cache_lo = bi_first;
-        cached = (bi_first + lane < row_blocks) ? __ldg(trow + bi_first + lane) : 0;
+        cached = (bi_first + lane < p.max_blocks) ? __ldg(trow + bi_first + lane) : 0;
     }
     const bool act = lane < nb;
     const int tok = (tile + (act ? lane : 0)) * 16;
@@ -472,7 +454,6 @@ struct Consumer {
     }
 
     // Segment epilogue: the final normalised output (`single`) or a partial row `part_row` (nh heads).
-    template <bool SFX>
     __device__ __forceinline__ void finish(const AttnParams& p, int lane, int seq, int kvh_global, bool single,
                                            size_t part_row) {
         const int gid = lane >> 2, c4 = lane & 3;
@@ -495,9 +476,6 @@ struct Consumer {
                 if (single) {
                     const float inv = 1.f / l_run[nt][e];
                     const size_t ob = (static_cast<size_t>(seq) * p.nh + hq) * D;
-                    if constexpr (SFX) {
-                        if (gid == 0) store_lse(p, static_cast<size_t>(seq) * p.nh + hq, m_run[nt][e], l_run[nt][e]);
-                    }
 #pragma unroll
                     for (int mt = 0; mt < KS; ++mt) {
                         store_any(p.out, ob + mt * 16 + gid, p.out_dtype, o[nt][mt][e] * inv);
@@ -684,10 +662,10 @@ __device__ __forceinline__ void init_barriers(const AttnParams& p, uint64_t* ful
 // copy it issued that no consumer waited for, so the CTA never exits with a bulk copy in flight into its
 // shared memory.  What it issued is known from registers: every tile before the counter (okst, okr) after its
 // last fully issued batch, plus the lanes `fmask` of the batch at (fst0, fr0) that failed; query loads: jq.
-template <int D, bool SFX>
+template <int D>
 __device__ __forceinline__ void merge_rows(const AttnParams& p, size_t row0, size_t stride, int n, size_t out_off,
                                            int lane);
-template <int D, int IT, int U, bool SFX>
+template <int D, int IT, int U>
 __device__ __forceinline__ void merge_group(const AttnParams& p, int seq, int c0, int nseg, int hq0, int heads,
                                             int tid, int nthreads);
 
@@ -730,7 +708,7 @@ __device__ __forceinline__ void drain_copies(const AttnParams& p, uint64_t* full
     __syncwarp();
 }
 
-template <int D, int NT, class KV, bool QLO, bool SFX, class Segs>
+template <int D, int NT, class KV, bool QLO, class Segs>
 __device__ __forceinline__ void cta_body(const AttnParams& p, const CUtensorMap* km, const CUtensorMap* vm, Segs segs,
                                          uint8_t* dyn, uint32_t smem_base, uint64_t* full_bar, uint64_t* empty_bar,
                                          uint64_t* qfull, uint64_t* qempty, int grp, int* pend, bool waited,
@@ -766,12 +744,6 @@ __device__ __forceinline__ void cta_body(const AttnParams& p, const CUtensorMap*
         while (segs.next(sg)) {
             const int len = sg.len;
             const int32_t* trow = p.tables + static_cast<size_t>(sg.seq) * p.max_blocks;
-            int row_blocks = p.max_blocks;  // entries of the row that may be read
-            if constexpr (SFX) {
-                const int skip = __ldg(p.skip_blocks + sg.seq);
-                trow += skip;
-                row_blocks -= skip;
-            }
             int cache_lo = -(1 << 30);
             int32_t cached = 0;
             // One run per tile: issue in batches of up to 8 tiles (one per lane); else one tile at a time.
@@ -784,7 +756,7 @@ __device__ __forceinline__ void cta_body(const AttnParams& p, const CUtensorMap*
                         if (nb_max > 1) {
                             unsigned issued = 0;
                             ok = produce_batch<D>(p, km, vm, smem_base, full_bar, empty_bar, pst, pr, tile, nb, len, trow,
-                                                  row_blocks, kvh0, lane, cache_lo, cached, issued);
+                                                  kvh0, lane, cache_lo, cached, issued);
                             if (!ok) {
                                 fst0 = pst;
                                 fr0 = pr;
@@ -800,7 +772,7 @@ __device__ __forceinline__ void cta_body(const AttnParams& p, const CUtensorMap*
                             } else {
                                 const uint32_t kst = smem_base + static_cast<uint32_t>(st) * p.stage_bytes;
                                 produce_tile<D>(p, km, vm, kst, kst + p.stage_half, smem_u32(&full_bar[st]), tile * 16,
-                                                len, trow, row_blocks, kvh0, lane, cache_lo, cached);
+                                                len, trow, kvh0, lane, cache_lo, cached);
                                 sent_all = true;
                             }
                         }
@@ -946,7 +918,7 @@ __device__ __forceinline__ void cta_body(const AttnParams& p, const CUtensorMap*
             named_barrier(1 + head, p.wph * 32);  // the area is rewritten by the next segment
         }
         if (write_wait) griddep_wait();
-        if (sub == 0 && ok) cs.template finish<SFX>(p, lane, sg.seq, kvh_global, sg.single, sg.part_row);
+        if (sub == 0 && ok) cs.finish(p, lane, sg.seq, kvh_global, sg.single, sg.part_row);
         // Stream-K, sequence split across CTAs: each head's writer warp counts its partial rows as done with
         // one releasing add (the warp barrier orders its lanes' rows before it); a sequence is complete when
         // every writer warp of every CTA holding part of it has added (nseg * kvh_cta).  The add's old value
@@ -994,12 +966,12 @@ __device__ __forceinline__ void cta_body(const AttnParams& p, const CUtensorMap*
             if constexpr (MS::per_warp) {
                 for (int jj = warp; jj < p.kvh_cta * p.g; jj += NC) {
                     const int hq = kvh0 * p.g + jj;
-                    merge_rows<D, SFX>(p, static_cast<size_t>(c0 + seq) * p.nh + hq, static_cast<size_t>(p.nh), nseg,
+                    merge_rows<D>(p, static_cast<size_t>(c0 + seq) * p.nh + hq, static_cast<size_t>(p.nh), nseg,
                                   (static_cast<size_t>(seq) * p.nh + hq) * D, lane);
                 }
             } else {
                 // all consumer threads merge the group's query heads, a 4-float column each
-                merge_group<D, MS::IT, MS::U, SFX>(p, seq, c0, nseg, kvh0 * p.g, p.kvh_cta * p.g, threadIdx.x, NC * 32);
+                merge_group<D, MS::IT, MS::U>(p, seq, c0, nseg, kvh0 * p.g, p.kvh_cta * p.g, threadIdx.x, NC * 32);
             }
         }
     }
@@ -1047,7 +1019,7 @@ __global__ void __launch_bounds__((kMaxConsumerWarps + 1) * 32, 1)
     segs.seg.c0 = 0;
     segs.seg.nseg = 0;
     segs.done = false;
-    cta_body<D, NT, KV, QLO, false>(p, &kmap, &vmap, segs, dyn_smem + base_off, smem_u32(dyn_smem) + base_off, full_bar,
+    cta_body<D, NT, KV, QLO>(p, &kmap, &vmap, segs, dyn_smem + base_off, smem_u32(dyn_smem) + base_off, full_bar,
                         empty_bar, qfull, qempty, grp, nullptr, true, &ps);
 }
 
@@ -1056,7 +1028,6 @@ __global__ void __launch_bounds__((kMaxConsumerWarps + 1) * 32, 1)
 // Unit prefix sums P[0..ns] of all sequences into shared memory (a valid sequence counts seq_units start-cost
 // units plus its tiles, an invalid length counts nothing), and R[s] =
 // the tokens in sequence s's last tile, so segment starts need no global load of the length.
-template <bool SFX>
 __device__ __forceinline__ void build_prefix(const AttnParams& p, int32_t* P, uint8_t* R, int32_t* warp_tot) {
     const int ns = p.num_seqs, nthr = blockDim.x, tid = threadIdx.x;
     const int warp = tid >> 5, lane = tid & 31, nwarps = (nthr + 31) >> 5;
@@ -1064,7 +1035,7 @@ __device__ __forceinline__ void build_prefix(const AttnParams& p, int32_t* P, ui
     const int b = min(tid * per, ns), e = min(b + per, ns);
     int local = 0;
     for (int i = b; i < e; ++i) {
-        const int n = tiles_of_len(p, own_len<SFX>(p, i));
+        const int n = tiles_of_len(p, __ldg(p.lens + i));
         local += n ? n + p.seq_units : 0;
     }
     int x = local;
@@ -1087,7 +1058,7 @@ __device__ __forceinline__ void build_prefix(const AttnParams& p, int32_t* P, ui
     __syncthreads();
     int run = (warp > 0 ? warp_tot[warp - 1] : 0) + (x - local);
     for (int i = b; i < e; ++i) {
-        const int len = own_len<SFX>(p, i);
+        const int len = __ldg(p.lens + i);
         P[i] = run;
         const int n = tiles_of_len(p, len);
         run += n ? n + p.seq_units : 0;
@@ -1107,7 +1078,7 @@ __device__ __forceinline__ int seq_of_tile(const int32_t* P, int ns, long long t
     return lo;
 }
 
-template <int D, int NT, class KV, bool QLO, bool SFX>
+template <int D, int NT, class KV, bool QLO>
 __global__ void __launch_bounds__((kMaxConsumerWarps + 1) * 32, 1)
     paged_decode_streamk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                 const AttnParams p) {
@@ -1126,7 +1097,7 @@ __global__ void __launch_bounds__((kMaxConsumerWarps + 1) * 32, 1)
     const uint32_t base_off = ((smem_u32(dyn_smem) + 1023u) & ~1023u) - smem_u32(dyn_smem);
     int32_t* P = reinterpret_cast<int32_t*>(dyn_smem + base_off + p.pre_off);
     uint8_t* R = reinterpret_cast<uint8_t*>(P + p.num_seqs + 1);
-    build_prefix<SFX>(p, P, R, warp_tot);
+    build_prefix(p, P, R, warp_tot);
     const int ns = p.num_seqs;
     const long long T = P[ns];
     // With fewer tiles than CTAs only the first T CTAs work, so every working CTA owns >= 1 tile.
@@ -1160,11 +1131,6 @@ __global__ void __launch_bounds__((kMaxConsumerWarps + 1) * 32, 1)
             const int heads = p.kvh_cta * p.g;
             for (int s = 0; s < ns; ++s) {
                 if (P[s + 1] != P[s]) continue;
-                if constexpr (SFX) {  // nothing of its own (or invalid, which the joining kernel reports)
-                    for (int i = threadIdx.x; i < heads; i += blockDim.x)
-                        p.lse[static_cast<size_t>(s) * p.nh + grp * heads + i] = -INFINITY;
-                    continue;
-                }
                 if (threadIdx.x == 0 && grp == 0) report(p.status, KVP_STATUS_BAD_LEN);
                 for (int i = threadIdx.x; i < heads * D; i += blockDim.x)
                     store_any(p.out, (static_cast<size_t>(s) * p.nh + grp * heads + i / D) * D + i % D, p.out_dtype, 0.f);
@@ -1172,7 +1138,7 @@ __global__ void __launch_bounds__((kMaxConsumerWarps + 1) * 32, 1)
         }
     }
     if (c >= Ge) return;
-    cta_body<D, NT, KV, QLO, SFX>(p, &kmap, &vmap, segs, dyn_smem + base_off, smem_u32(dyn_smem) + base_off, full_bar,
+    cta_body<D, NT, KV, QLO>(p, &kmap, &vmap, segs, dyn_smem + base_off, smem_u32(dyn_smem) + base_off, full_bar,
                         empty_bar, qfull, qempty, grp, pend, waited, &ps);
 }
 
@@ -1181,7 +1147,7 @@ __global__ void __launch_bounds__((kMaxConsumerWarps + 1) * 32, 1)
 // Lane k holds partial k's (m, l) (one L2 round trip), the weights stay in registers and the output loop's
 // loads are independent of each other.  Partials written by other CTAs of the same launch are read through
 // L2 (ld.global.cg).
-template <int D, bool SFX>
+template <int D>
 __device__ __forceinline__ void merge_rows(const AttnParams& p, size_t row0, size_t stride, int n, size_t out_off,
                                            int lane) {
     constexpr int PER = (D + 31) / 32;
@@ -1218,9 +1184,6 @@ __device__ __forceinline__ void merge_rows(const AttnParams& p, size_t row0, siz
         }
     }
     const float invL = 1.f / L;
-    if constexpr (SFX) {
-        if (lane == 0) store_lse(p, out_off / D, M, L);
-    }
 #pragma unroll
     for (int q = 0; q < PER; ++q) {
         const int d = q * 32 + lane;
@@ -1234,7 +1197,7 @@ __device__ __forceinline__ void merge_rows(const AttnParams& p, size_t row0, siz
 // combined (a running max with rescaling), so a merge costs about one L2 round trip per U partials and IT items
 // instead of a dependent chain per head.  Partials
 // written by other CTAs of the same launch are read through L2 (ld.global.cg).
-template <int D, int IT, int U, bool SFX>
+template <int D, int IT, int U>
 __device__ __forceinline__ void merge_group(const AttnParams& p, int seq, int c0, int nseg, int hq0, int heads,
                                             int tid, int nthreads) {
     constexpr int C4 = D / 4;
@@ -1293,9 +1256,6 @@ __device__ __forceinline__ void merge_group(const AttnParams& p, int seq, int c0
             if (!on[t]) continue;
             const float inv = 1.f / Lsum[t];
             const size_t out = (row0[t] - static_cast<size_t>(c0) * p.nh) * D + static_cast<size_t>(col[t]) * 4;
-            if constexpr (SFX) {
-                if (col[t] == 0) store_lse(p, row0[t] - static_cast<size_t>(c0) * p.nh, M[t], Lsum[t]);
-            }
             store_any(p.out, out + 0, p.out_dtype, acc[t].x * inv);
             store_any(p.out, out + 1, p.out_dtype, acc[t].y * inv);
             store_any(p.out, out + 2, p.out_dtype, acc[t].z * inv);
@@ -1314,7 +1274,7 @@ __global__ void __launch_bounds__(128) merge_splits_kernel(const AttnParams p) {
     const int ntiles = tiles_of_len(p, p.lens[seq]);
     const int nsplit = (ntiles + p.split_tiles - 1) / p.split_tiles;
     if (nsplit <= 1) return;
-    merge_rows<D, false>(p, static_cast<size_t>(seq) * p.max_splits * p.nh + hq, static_cast<size_t>(p.nh), nsplit,
+    merge_rows<D>(p, static_cast<size_t>(seq) * p.max_splits * p.nh + hq, static_cast<size_t>(p.nh), nsplit,
                   (static_cast<size_t>(seq) * p.nh + hq) * D, lane);
 }
 
@@ -1323,7 +1283,7 @@ __global__ void __launch_bounds__(128) merge_splits_kernel(const AttnParams p) {
 template <int D, int NT, class KV, bool QLO>
 struct Kernels {
     static const void* decode() { return reinterpret_cast<const void*>(&paged_decode_kernel<D, NT, KV, QLO>); }
-    static const void* streamk() { return reinterpret_cast<const void*>(&paged_decode_streamk_kernel<D, NT, KV, QLO, false>); }
+    static const void* streamk() { return reinterpret_cast<const void*>(&paged_decode_streamk_kernel<D, NT, KV, QLO>); }
 };
 
 template <class KV, bool QLO, int D>
@@ -1376,10 +1336,10 @@ int launch_typed(const kvp_attn_args& a, const kvpi::AttnPlan& pl, const AttnPar
             attr[0].val.programmaticStreamSerializationAllowed = 1;
             cfg.attrs = attr;
             cfg.numAttrs = 1;
-            cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_streamk_kernel<D, NT, KV, QLO, false>, km, vm, prm);
+            cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_streamk_kernel<D, NT, KV, QLO>, km, vm, prm);
             if (e != cudaSuccess) return kvpi::cuda_status(e, "attention kernel launch");
         } else {
-            paged_decode_streamk_kernel<D, NT, KV, QLO, false><<<grid, block, pl.smem, stream>>>(km, vm, prm);
+            paged_decode_streamk_kernel<D, NT, KV, QLO><<<grid, block, pl.smem, stream>>>(km, vm, prm);
         }
     } else {
         dim3 grid(static_cast<unsigned>(a.num_seqs * pl.groups), static_cast<unsigned>(pl.max_splits));
@@ -1409,27 +1369,6 @@ int launch_d(const kvp_attn_args& a, const kvpi::AttnPlan& pl, const AttnParams&
         case 256: return launch_nt<256, KV, QLO>(a, pl, prm, km, vm, s);
         default: return kvpi::fail(KVP_EINVAL, "unsupported head_dim");
     }
-}
-
-// The own parts of sequences in groups (SFX): the balanced schedule only, queries of the pools' dtype, always with an
-// early load -- the kernel before it, the groups' shared part, writes neither the tables nor the pools.
-template <int D, int NT, class KV>
-int launch_own(const kvpi::AttnPlan& pl, const AttnParams& prm, const CUtensorMap& km, const CUtensorMap& vm,
-               cudaStream_t stream) {
-    auto fn = &paged_decode_streamk_kernel<D, NT, KV, false, true>;
-    const int rc = kvpi::allow_smem(reinterpret_cast<const void*>(fn));
-    if (rc != KVP_OK) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(pl.G), static_cast<unsigned>(pl.groups));
-    cfg.blockDim = dim3(static_cast<unsigned>((pl.kvh_cta * pl.wph + 1) * 32));
-    cfg.dynamicSmemBytes = pl.smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return kvpi::cuda_status(cudaLaunchKernelEx(&cfg, fn, km, vm, prm), "attention kernel launch");
 }
 
 // Defines the entry points of one variant (used once per instantiation translation unit).

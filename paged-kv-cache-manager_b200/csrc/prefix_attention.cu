@@ -7,8 +7,8 @@
 //   compute 4 * m * g * P * head_dim flops.
 // Up to about 128 rows the bytes take longer than the flops; beyond, the tensor cores and the exponentials bound it.
 //
-// Three launches.  prefix_kernel attends over the shared blocks and leaves partial results; the balanced decode kernel
-// (SFX) attends over each sequence's own blocks; join_kernel combines both and writes the output.
+// Two launches.  prefix_kernel attends over the shared blocks and leaves partial results; own_kernel attends over each
+// sequence's own blocks, combines both and writes the output.
 //
 // prefix_kernel: one CTA per SM takes an even share of the step's units -- a unit is one tile of 128 keys for one (group,
 // kv head, pair of row tiles) -- regardless of where groups and heads begin and end.  A row tile is as many whole members
@@ -47,16 +47,15 @@ struct PrefixParams {
     const int32_t* prefix_blocks;
     const int32_t* group_starts;
     int32_t* status;
-    int32_t* counters;         // the own parts' merge counters, cleared here
-    long long* unit_prefix;    // [num_groups + 1], written by CTA 0 for the joining kernel
+    int2* spans;               // first and last CTA of each (group, kv head, pair), at its first row's (member, kv head)
     float2* part_ml;           // partial rows: (maximum in log2 units, sum)
     float* part_o;
-    const float* own_o;        // [num_seqs][num_heads][D] normalised
-    const float* own_lse;
+    const void* q;
+    const void* k_cache;
+    const void* v_cache;
     void* out;
     long long num_blocks;
     long long wait_limit;
-    int num_counters;
     int num_seqs, num_groups, nh, kvh, g, max_blocks, B, Bshift, run, runs, oob_row;
     int mt;                    // members per row tile
     int bf16, out_dtype;
@@ -240,20 +239,14 @@ __device__ __forceinline__ long long floor_div(long long a, long long b, long lo
     else if ((q + 1) * c <= n) ++q;
     return q;
 }
-// CTA c of G owns units [c T / G, (c + 1) T / G); the CTA that owns unit u.
+// CTA c of G owns units [c T / G, (c + 1) T / G).
 __device__ __forceinline__ long long first_unit(int c, long long T, int G) { return floor_div(c, T, G); }
-__device__ __forceinline__ int owner_of(long long u, long long T, int G) {
-    int c = static_cast<int>((static_cast<double>(u) + 0.5) * G / static_cast<double>(T));
-    c = min(max(c, 0), G - 1);
-    while (c > 0 && first_unit(c, T, G) > u) --c;
-    while (c + 1 < G && first_unit(c + 1, T, G) <= u) ++c;
-    return c;
-}
 
 // One stretch of a CTA's units: key tiles [k0, k0 + n) of (group, kv head, pair).
 struct Work {
-    int start, head, member0, k0, n, tokens;  // member0: the pair's first member, within the group
+    int start, head, member0, k0, n, ktiles, tokens;  // member0: the pair's first member, within the group
     int rows0, rows1;                         // rows of the two row tiles; rows1 == 0: one row tile, key tiles in turn
+    long long pair_at;   // the pair's place among all (member, kv head) rows of the batch
     long long part_row;
 };
 
@@ -275,19 +268,19 @@ struct WorkList {
         w.start = grp.start;
         w.head = triple / grp.pairs;
         w.member0 = (triple - w.head * grp.pairs) * 2 * p.mt;
+        w.ktiles = grp.ktiles;
         w.tokens = grp.blocks * p.B;
         const int left = grp.members - w.member0;
         w.rows0 = min(left, p.mt) * p.g;
         w.rows1 = min(max(left - p.mt, 0), p.mt) * p.g;
         // two partial rows per (member, head) row of the batch, 256 more per CTA: a stretch's rows are its own
-        w.part_row = 2LL * p.g * (static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(w.head) * grp.members + w.member0) +
-                     static_cast<long long>(cta) * 2 * kRows;
+        w.pair_at = static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(w.head) * grp.members + w.member0;
+        w.part_row = 2LL * p.g * w.pair_at + static_cast<long long>(cta) * 2 * kRows;
         return true;
     }
 };
 
-// Where a CTA's units begin: the total, the group that holds the CTA's first unit and that group's first unit.  CTA 0 leaves
-// the prefix sums for the joining kernel.  One pass over the groups while there is a thread for each, else a second one.
+// Where a CTA's units begin: the total, the group that holds the CTA's first unit and that group's first unit.  One pass over the groups while there is a thread for each, else a second one.
 struct Start {
     long long total, first;
     int group;
@@ -320,9 +313,7 @@ __device__ __forceinline__ Start find_start(const PrefixParams& p, long long* wa
         const int gi = g0 + static_cast<int>(threadIdx.x);
         u = units_of(gi);
         total += scan(u, total, &mine);
-        if (blockIdx.x == 0 && gi < p.num_groups) p.unit_prefix[gi] = mine;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.unit_prefix[p.num_groups] = total;
     const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
     if (static_cast<int>(blockIdx.x) >= G) return Start{total, 0, 0};
     const long long at = first_unit(blockIdx.x, total, G);
@@ -402,7 +393,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 
     // the next kernel may be scheduled as soon as this one's CTAs leave their SMs; it waits for all of them
     griddep_launch_dependents();
-    for (int i = blockIdx.x * kPrefixThreads + threadIdx.x; i < p.num_counters; i += gridDim.x * kPrefixThreads) p.counters[i] = 0;
     if (threadIdx.x == 0) {
         sh.abort = 0;
         for (int s = 0; s < 8; ++s) {
@@ -670,6 +660,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             if (!ok) break;
             if (!(ok = warp_wait(&sh.o_full[t], seg & 1, p, sh))) break;
             ++seg;
+            if (threadIdx.x == 0) {
+                if (w.k0 == 0) p.spans[w.pair_at].x = cta;
+                if (w.k0 + w.n == w.ktiles) p.spans[w.pair_at].y = cta;
+            }
             if (busy) {
                 tc_fence_after();
                 const long long r0 = w.part_row + (t ? w.rows0 : 0) + row;
@@ -699,112 +693,319 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     }
 }
 
-// ---------------------------------------------------------------- joining
-// One warp per (sequence, query head): weighs the shared part's partial rows and the own part by exp2 of their maxima and
-// writes the output.  Bound by latency and L2: the lanes fetch up to 32 partials' maxima and sums at once, then whole rows,
-// four at a time.
-template <int D>
-__global__ void __launch_bounds__(128) join_kernel(const PrefixParams p, int grid_ctas) {
-    constexpr int PER = D / 32;  // output columns of a lane, side by side
-    const int lane = threadIdx.x & 31;
-    const long long orow = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (orow >= static_cast<long long>(p.num_seqs) * p.nh) return;
-    const int seq = static_cast<int>(orow / p.nh), head = static_cast<int>(orow - static_cast<long long>(seq) * p.nh);
-    const int h = head / p.g, j = head - h * p.g;
+// ---------------------------------------------------------------- own parts
+// One CTA of four warps per (sequence, kv head) -- or, where those are few, a cluster of up to eight CTAs -- attends over
+// the sequence's own blocks, 16 tokens a warp at a time, combines the warps' results with the shared part's partial rows
+// and writes the output.  Bound by HBM, and by latency where the own parts are short, which most of them are: a warp takes K
+// and V from global memory straight into the registers of its matrix instructions, without a pipeline to fill and drain.
+//   S^T[tokens x heads] = K Q^T:  a lane holds 8 neighbouring dims of a token's K (one 16-byte load); the sum over dims does
+//                                 not care for their order, so these are the dims of two steps, for K and Q alike.
+//   O^T[dims x heads] += V^T P^T: a lane holds 8 neighbouring dims of four tokens' V and pairs up two tokens' halves; the
+//                                 rows of the instruction are dims in an order of their own.  P^T by an 8 x 8 transposition.
+// The heads are the 8 columns of the instruction (NT times, for more than 8): as its 16 rows they took twice the
+// instructions and accumulators, and twice the time at head_dim 128.
+constexpr int kOwnWarps = 4;  // as many as a Fold takes at once
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// This CTA's shared address as seen in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+// Four partial results (maximum, sum; four columns of the output) at a time, folded into what there is.  One with the maximum
+// -inf is nothing, and its columns may never have been written.
+struct Fold {
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    __device__ __forceinline__ void add(const float2 (&ml)[4], const float4 (&x)[4]) {
+        const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m);
+        if (mn == -INFINITY) return;
+        const float f = fast_exp2(m - mn);
+        m = mn;
+        l *= f;
+        o.x *= f;
+        o.y *= f;
+        o.z *= f;
+        o.w *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool some = ml[i].x != -INFINITY;
+            const float w = fast_exp2(ml[i].x - mn);
+            l += ml[i].y * w;
+            o.x += some ? x[i].x * w : 0.f;
+            o.y += some ? x[i].y * w : 0.f;
+            o.z += some ? x[i].z * w : 0.f;
+            o.w += some ? x[i].w * w : 0.f;
+        }
+    }
+};
+
+// NT: groups of 8 query heads per kv head.
+template <int D, class KV, int NT>
+__global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 3) own_kernel(const PrefixParams p) {
+    using Tr = F16Traits<KV>;
+    constexpr int NI = D / 32;   // 16-byte pieces of a row that a lane of four holds
+    constexpr int NH = D / 64;   // and that a lane of eight holds
+    constexpr int ROWS = 8 * NT;
+    __shared__ float2 sm_ml[kOwnWarps][ROWS];
+    __shared__ __align__(16) float sm_o[kOwnWarps][ROWS][D];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c4 = lane & 3;
+    const int ctas = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
+    const int item = static_cast<int>(blockIdx.x) / ctas;
+    const int seq = item / p.kvh, h = item - seq * p.kvh;
     const int len = __ldg(p.lens + seq), pb = __ldg(p.prefix_blocks + seq);
-    // the sequence's group, the last one that starts at or before it: 32 candidates a step
-    int lo = 0, n = p.num_groups;
-    while (n > 1) {
+    const long long nblk = (static_cast<long long>(len) + p.B - 1) / p.B;
+    bool fine = len >= 1 && nblk <= p.max_blocks && pb >= 0 && static_cast<long long>(pb) * p.B <= len;
+    const int own = fine ? len - pb * p.B : 0;
+    const int32_t* trow = p.tables + static_cast<long long>(seq) * p.max_blocks + (fine ? pb : 0);
+    const int tiles = (own + 15) >> 4, stride = ctas * kOwnWarps;
+
+    // queries of head 8 nt + gid
+    uint4 qr[NT][NI];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int j = 8 * nt + gid;
+        const uint4* src = reinterpret_cast<const uint4*>(
+            static_cast<const KV*>(p.q) + (static_cast<long long>(seq) * p.nh + h * p.g + min(j, p.g - 1)) * D + c4 * 8);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) qr[nt][i] = j < p.g ? __ldg(src + i * 4) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    // the pool row of token `lane % 16` of a tile; -1: none (behind the context, or a block outside the pool)
+    auto row_of = [&](int tile) {
+        const int tok = tile * 16 + (lane & 15);
+        if (tok >= own) return -1;
+        const int bi = p.Bshift >= 0 ? tok >> p.Bshift : tok / p.B;
+        const int blk = __ldg(trow + bi);
+        if (blk >= 0 && blk < p.num_blocks) return blk * p.B + (tok - bi * p.B);
+        report(p.status, KVP_STATUS_BAD_BLOCK);
+        return -1;
+    };
+    float o[NT][D / 16][4];
+    float m[NT][2], l[NT][2];  // of heads 8 nt + 2 c4, + 1
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+    }
+    uint4 kr[2][NI], vr[4][NH];
+    auto load_k = [&](int row) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int x = __shfl_sync(0xffffffffu, row, gid + 8 * r);
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const KV*>(p.k_cache) +
+                                                              (static_cast<long long>(max(x, 0)) * p.kvh + h) * D + c4 * 8);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) kr[r][i] = x >= 0 ? __ldg(src + i * 4) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    };
+    auto load_v = [&](int row) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int x = __shfl_sync(0xffffffffu, row, 2 * c4 + (r & 1) + (r >> 1) * 8);
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const KV*>(p.v_cache) +
+                                                              (static_cast<long long>(max(x, 0)) * p.kvh + h) * D + gid * 8);
+#pragma unroll
+            for (int i = 0; i < NH; ++i) vr[r][i] = x >= 0 ? __ldg(src + i * 8) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    };
+    // The next tile's K is on its way as soon as this one's scores are there, its V as soon as this one's is used.
+    const int first_tile = rank * kOwnWarps + warp;
+    {
+        const int row = row_of(first_tile);
+        load_k(row);
+        load_v(row);
+    }
+    int row = row_of(first_tile + stride);
+    // meanwhile: the sequence's group, the last one that starts at or before it, 32 candidates a step
+    int lo = 0;
+    for (int n = p.num_groups; n > 1;) {
         const int step = (n + 31) >> 5;
-        const int at = lo + lane * step;
-        const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && __ldg(p.group_starts + at) <= seq);
+        const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && __ldg(p.group_starts + lo + lane * step) <= seq);
         const int k = below ? 31 - __clz(below) : 0;
         lo += k * step;
         n = min(step, n - k * step);
     }
     const Group grp = load_group(p, lo);
-    const long long nblk = (static_cast<long long>(len) + p.B - 1) / p.B;
-    const bool fine = len >= 1 && nblk <= p.max_blocks && pb >= 0 && static_cast<long long>(pb) * p.B <= len &&
-                      grp.start <= seq && seq < grp.start + grp.members && grp.blocks == pb;
-    // this row's partials: `parts` for each CTA from c0 on, `rows` apart within a CTA, 256 between CTAs
+    fine = fine && grp.start <= seq && seq < grp.start + grp.members && grp.blocks == pb;
+    // and the shared part's partial rows of head 0: `parts` for each CTA from the first on, `rows` apart within a CTA, 256
+    // between CTAs
+    griddep_wait();
     int count = 0, parts = 1, rows = 0;
     long long row0 = 0;
-    griddep_wait();
     if (fine && grp.ktiles > 0) {
-        const long long T = __ldcg(p.unit_prefix + p.num_groups);
-        const int G = static_cast<int>(min(static_cast<long long>(grid_ctas), T));
-        const int member = seq - grp.start, pair = member / (2 * p.mt);
-        const long long u0 = __ldcg(p.unit_prefix + lo) + (static_cast<long long>(h) * grp.pairs + pair) * grp.ktiles;
-        const int c0 = owner_of(u0, T, G), c1 = owner_of(u0 + grp.ktiles - 1, T, G);
-        const int member0 = pair * 2 * p.mt, left = grp.members - member0;
-        row0 = 2LL * p.g * (static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(h) * grp.members + member0) +
-               static_cast<long long>(c0) * 2 * kRows + (member - member0) * p.g + j;  // two row tiles: one after the other
+        const int member = seq - grp.start, member0 = member / (2 * p.mt) * 2 * p.mt, left = grp.members - member0;
+        const long long pair_at = static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(h) * grp.members + member0;
+        const int2 span = __ldcg(p.spans + pair_at);
+        row0 = 2LL * p.g * pair_at + static_cast<long long>(span.x) * 2 * kRows + (member - member0) * p.g;  // two row tiles: one after the other
         if (left <= p.mt) {  // one: the even and the odd key tiles'
             parts = 2;
             rows = left * p.g;
         }
-        count = (c1 - c0 + 1) * parts;
+        count = (span.y - span.x + 1) * parts;
     }
-    float acc[PER];
+    for (int tile = first_tile; tile < tiles; tile += stride) {
+        const bool in0 = tile * 16 + gid < own, in1 = tile * 16 + gid + 8 < own;
+        uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
-    for (int q = 0; q < PER; ++q) acc[q] = 0.f;
-    float M = -INFINITY, L = 0.f;
-    if (fine) {
-        M = __ldcg(p.own_lse + orow);  // the own part is normalised: its sum is one
-        if (M != -INFINITY) {
-            L = 1.f;
+        for (int nt = 0; nt < NT; ++nt) {
+            // scores of tokens gid, gid + 8 for heads 2 c4, 2 c4 + 1
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int q = 0; q < PER; q += 2) {
-                const float2 o = __ldcg(reinterpret_cast<const float2*>(p.own_o + orow * D + lane * PER + q));
-                acc[q] = o.x;
-                acc[q + 1] = o.y;
+            for (int i = 0; i < NI; ++i) {
+                const uint32_t a0[4] = {kr[0][i].x, kr[1][i].x, kr[0][i].y, kr[1][i].y};
+                mma16816<KV>(s, a0, qr[nt][i].x, qr[nt][i].y);
+                const uint32_t a1[4] = {kr[0][i].z, kr[1][i].z, kr[0][i].w, kr[1][i].w};
+                mma16816<KV>(s, a1, qr[nt][i].z, qr[nt][i].w);
             }
-        }
-    }
-    for (int k0 = 0; k0 < count; k0 += 32) {
-        const int k = k0 + lane;
-        const long long row = row0 + (parts == 2 ? static_cast<long long>(k >> 1) * 2 * kRows + (k & 1) * rows
-                                                 : static_cast<long long>(k) * 2 * kRows);
-        const float2 ml = k < count ? __ldcg(&p.part_ml[row]) : make_float2(-INFINITY, 0.f);
-        float top = ml.x;
+            if (nt == NT - 1) load_k(row);
+            // softmax over the tokens of the tile, which eight lanes share
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const float Mn = fmaxf(M, top);
-        const float old = M == -INFINITY ? 0.f : fast_exp2(M - Mn);
-        const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - Mn);  // 0: a half without a key tile, never written
-        float add = ml.y * w;
+            for (int e = 0; e < 2; ++e) {
+                s[e] = in0 ? s[e] * p.sl2 : -INFINITY;
+                s[2 + e] = in1 ? s[2 + e] * p.sl2 : -INFINITY;
+                float mx = fmaxf(s[e], s[2 + e]);
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) add += __shfl_xor_sync(0xffffffffu, add, off);
-        L = L * old + add;
+                for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                const float mn = fmaxf(m[nt][e], mx), ref = mn == -INFINITY ? 0.f : mn, f = fast_exp2(m[nt][e] - ref);
+                m[nt][e] = mn;
+                s[e] = fast_exp2(s[e] - ref);
+                s[2 + e] = fast_exp2(s[2 + e] - ref);
+                l[nt][e] = l[nt][e] * f + (s[e] + s[2 + e]);
 #pragma unroll
-        for (int q = 0; q < PER; ++q) acc[q] *= old;
-        M = Mn;
-        const int left = min(32, count - k0);
-        for (int i0 = 0; i0 < left; i0 += 4) {
-            float o[4][PER], f[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f[i] = __shfl_sync(0xffffffffu, w, (i0 + i) & 31);
-                const long long r = __shfl_sync(0xffffffffu, row, (i0 + i) & 31);
-                if (i0 + i >= left) f[i] = 0.f;
-#pragma unroll
-                for (int q = 0; q < PER; q += 2) {
-                    const float2 x = f[i] != 0.f ? __ldcg(reinterpret_cast<const float2*>(p.part_o + r * D + lane * PER + q))
-                                                 : make_float2(0.f, 0.f);
-                    o[i][q] = x.x;
-                    o[i][q + 1] = x.y;
+                for (int i = 0; i < D / 16; ++i) {
+                    o[nt][i][e] *= f;
+                    o[nt][i][2 + e] *= f;
                 }
             }
+            // P as a 16-bit part and a 16-bit rest: the memory leaves time for both, and the result keeps close to fp32
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int q = 0; q < PER; ++q) acc[q] += o[i][q] * f[i];
+            for (int r = 0; r < 2; ++r) {
+                const uint32_t hi = Tr::pack(s[2 * r], s[2 * r + 1]);
+                ph[nt][r] = movmatrix_trans(hi);
+                pl[nt][r] = movmatrix_trans(Tr::pack(s[2 * r] - Tr::unpack_lo(hi), s[2 * r + 1] - Tr::unpack_hi(hi)));
+            }
         }
-    }
-    if (!fine && lane == 0 && head == 0) report(p.status, KVP_STATUS_BAD_LEN);
-    const float inv = fine ? 1.f / L : 0.f;
 #pragma unroll
-    for (int q = 0; q < PER; ++q) store_any(p.out, static_cast<size_t>(orow) * D + lane * PER + q, p.out_dtype, acc[q] * inv);
+        for (int i = 0; i < NH; ++i) {
+            const uint32_t w[4][4] = {{vr[0][i].x, vr[0][i].y, vr[0][i].z, vr[0][i].w},
+                                      {vr[1][i].x, vr[1][i].y, vr[1][i].z, vr[1][i].w},
+                                      {vr[2][i].x, vr[2][i].y, vr[2][i].z, vr[2][i].w},
+                                      {vr[3][i].x, vr[3][i].y, vr[3][i].z, vr[3][i].w}};
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {  // rows r and r + 8 are dims 64 i + 8 r + 2 t and the one behind it
+                const uint32_t a[4] = {__byte_perm(w[0][t], w[1][t], 0x5410u), __byte_perm(w[0][t], w[1][t], 0x7632u),
+                                       __byte_perm(w[2][t], w[3][t], 0x5410u), __byte_perm(w[2][t], w[3][t], 0x7632u)};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma16816<KV>(o[nt][i * 4 + t], a, ph[nt][0], ph[nt][1]);
+                    mma16816<KV>(o[nt][i * 4 + t], a, pl[nt][0], pl[nt][1]);
+                }
+            }
+        }
+        load_v(row);
+        row = row_of(tile + 2 * stride);
+    }
+    // Each thread's outputs, four columns of a query head, are known by now: its first partial rows start on their way before
+    // the warps meet.
+    const int outs = p.g * (D / 4), at0 = rank * kOwnWarps * 32 + static_cast<int>(threadIdx.x);
+    float2 pml[4];
+    float4 px[4];
+    auto part = [&](int at, int k0) {
+        const int j = at / (D / 4), col = (at - j * (D / 4)) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = k0 + i;
+            const long long r = row0 + j + (parts == 2 ? static_cast<long long>(k >> 1) * 2 * kRows + (k & 1) * rows
+                                                       : static_cast<long long>(k) * 2 * kRows);
+            pml[i] = k < count ? __ldcg(&p.part_ml[r]) : make_float2(-INFINITY, 0.f);
+            px[i] = k < count ? __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    if (at0 < outs) part(at0, 0);
+    // this warp's heads into shared memory: a lane holds dims 64 i + 8 gid .. + 7 of heads 2 c4, 2 c4 + 1
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float sum = l[nt][e];
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            const int j = 8 * nt + 2 * c4 + e;
+            if (gid == 0) sm_ml[warp][j] = make_float2(m[nt][e], sum);
+#pragma unroll
+            for (int i = 0; i < NH; ++i)
+#pragma unroll
+                for (int t = 0; t < 4; t += 2)
+                    *reinterpret_cast<float4*>(&sm_o[warp][j][64 * i + 8 * gid + 2 * t]) =
+                        make_float4(o[nt][i * 4 + t][e], o[nt][i * 4 + t][2 + e], o[nt][i * 4 + t + 1][e], o[nt][i * 4 + t + 1][2 + e]);
+        }
+    if (ctas > 1) cluster_sync();
+    else __syncthreads();
+    for (int at = at0; at < outs; at += ctas * kOwnWarps * 32) {
+        const int j = at / (D / 4), col = (at - j * (D / 4)) * 4;
+        if (at != at0) part(at, 0);
+        Fold all;
+        for (int c = 0; c < ctas; ++c) {
+            float2 ml[4];
+            float4 x[4];
+#pragma unroll
+            for (int w = 0; w < kOwnWarps; ++w) {
+                if (ctas == 1) {
+                    ml[w] = sm_ml[w][j];
+                    x[w] = *reinterpret_cast<const float4*>(&sm_o[w][j][col]);
+                } else {
+                    ml[w] = ld_cluster2(map_rank(smem_u32(&sm_ml[w][j]), c));
+                    x[w] = ld_cluster4(map_rank(smem_u32(&sm_o[w][j][col]), c));
+                }
+            }
+            all.add(ml, x);
+        }
+        all.add(pml, px);
+        for (int k0 = 4; k0 < count; k0 += 4) {
+            part(at, k0);
+            all.add(pml, px);
+        }
+        if (!fine && at == 0 && h == 0) report(p.status, KVP_STATUS_BAD_LEN);
+        const float inv = fine ? 1.f / all.l : 0.f;
+        const float y[4] = {fine ? all.o.x * inv : 0.f, fine ? all.o.y * inv : 0.f, fine ? all.o.z * inv : 0.f, fine ? all.o.w * inv : 0.f};
+        const size_t out = (static_cast<size_t>(seq) * p.nh + h * p.g + j) * D + col;
+        if (p.out_dtype == KVP_DTYPE_F32)
+            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + out) = make_float4(y[0], y[1], y[2], y[3]);
+        else
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + out) =
+                p.out_dtype == KVP_DTYPE_F16 ? make_uint2(F16Traits<__half>::pack(y[0], y[1]), F16Traits<__half>::pack(y[2], y[3]))
+                                             : make_uint2(F16Traits<__nv_bfloat16>::pack(y[0], y[1]), F16Traits<__nv_bfloat16>::pack(y[2], y[3]));
+    }
+    if (ctas > 1) cluster_sync();  // others may still read this CTA's shared memory
 }
 
 }  // namespace kvpd
@@ -843,8 +1044,7 @@ kvp_attn_args whole_contexts(const kvp_prefix_args& a) {
 
 struct PrefixPlan {
     bool shared = false;  // else the plain decode attention over every sequence's whole context
-    AttnPlan own;
-    size_t own_o = 0, own_lse = 0, units = 0, ml = 0, o = 0, bytes = 0;
+    size_t ml = 0, o = 0, bytes = 0;
     int mt = 1, run = 8;
 };
 
@@ -856,28 +1056,26 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
         return fail(KVP_EINVAL, "unsupported dtype");
     if (a->num_seqs < 0 || a->num_groups < 0 || (a->num_seqs > 0 && a->num_groups < 1) || a->num_groups > a->num_seqs)
         return fail(KVP_EINVAL, "bad num_seqs / num_groups");
-    if (a->num_seqs > kvpd::kMaxStreamSeqs) return fail(KVP_EINVAL, "at most 8192 sequences per call");
     if (a->num_blocks < 1 || a->block_size < 1 || a->max_blocks < 1) return fail(KVP_EINVAL, "bad num_blocks / block_size / max_blocks");
     kvp_attn_args w = whole_contexts(*a);
     if (a->num_seqs == 0) return KVP_OK;
     if (a->kv_dtype == KVP_DTYPE_F32) return KVP_OK;
     // The shared kernel's tiles are 8-row atoms of 64 elements of one 16-bit type.
     pl->run = gcd_of(a->block_size, kvpd::kKeys);
-    const int rc = plan_attention(w, true, &pl->own);
+    AttnPlan whole;
+    const int rc = plan_attention(w, true, &whole);
     if (rc != KVP_OK) return rc;
-    pl->shared = (a->head_dim == 64 || a->head_dim == 128) && a->q_dtype == a->kv_dtype && pl->run >= 8 &&
-                 aligned16(a->q) && pl->own.streamk;
-    pl->bytes = pl->own.ws_bytes;
+    pl->shared = (a->head_dim == 64 || a->head_dim == 128) && a->q_dtype == a->kv_dtype && pl->run >= 8 && aligned16(a->q) &&
+                 aligned16(a->out) && static_cast<long long>(a->num_seqs) * a->kv_heads <= (1LL << 27);
+    pl->bytes = whole.ws_bytes;
     if (!pl->shared) return KVP_OK;
     const size_t rows = static_cast<size_t>(a->num_seqs) * a->num_heads;
     const size_t parts = 2 * rows + static_cast<size_t>(sm_count()) * 2 * kvpd::kRows;
     pl->mt = kvpd::kRows / (a->num_heads / a->kv_heads);
-    pl->own_o = up256(pl->own.ws_bytes);
-    pl->own_lse = pl->own_o + up256(rows * a->head_dim * 4);
-    pl->units = pl->own_lse + up256(rows * 4);
-    pl->ml = pl->units + up256((static_cast<size_t>(a->num_groups) + 1) * 8);
+    pl->ml = up256(static_cast<size_t>(a->num_seqs) * a->kv_heads * 8);
     pl->o = pl->ml + up256(parts * 8);
-    pl->bytes = pl->o + parts * a->head_dim * 4;
+    // (the larger of both: where q or out are not aligned the other path runs in the same workspace)
+    pl->bytes = std::max(pl->bytes, pl->o + parts * a->head_dim * 4);
     return KVP_OK;
 }
 
@@ -903,18 +1101,33 @@ int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMa
     return cuda_status(cudaGetLastError(), "shared prefix launch");
 }
 
-int launch_join(const kvpd::PrefixParams& p, int D, cudaStream_t s) {
-    const long long rows = static_cast<long long>(p.num_seqs) * p.nh;
+template <int D, class KV>
+int launch_own(const kvpd::PrefixParams& p, cudaStream_t s) {
+    auto fn = p.g > 8 ? &kvpd::own_kernel<D, KV, 2> : &kvpd::own_kernel<D, KV, 1>;
+    // Few (sequence, kv head) pairs: clusters share one, so that a long own part does not hang on four warps.
+    const long long items = static_cast<long long>(p.num_seqs) * p.kvh, room = static_cast<long long>(sm_count()) * 3;
+    unsigned ctas = 1;
+    while (ctas < 8 && items * ctas * 2 <= room) ctas *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>((rows + 3) / 4));
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(static_cast<unsigned>(items) * ctas);
+    cfg.blockDim = dim3(kvpd::kOwnWarps * 32);
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, D == 64 ? kvpd::join_kernel<64> : kvpd::join_kernel<128>, p, sm_count()), "join launch");
+    cfg.numAttrs = 2;
+    return cuda_status(cudaLaunchKernelEx(&cfg, fn, p), "own part launch");
+}
+
+template <int D, class KV>
+int launch_both(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const kvpd::PrefixParams& p, cudaStream_t s) {
+    const int rc = launch_prefix<D, KV>(qm, km, vm, p, s);
+    return rc != KVP_OK ? rc : launch_own<D, KV>(p, s);
 }
 
 }  // namespace
@@ -937,8 +1150,10 @@ extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stre
     if (pl.bytes > 0 && (!a->workspace || a->workspace_bytes < pl.bytes))
         return fail(KVP_ENOSPACE, "workspace smaller than kvp_prefix_workspace_size()");
     if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return fail(KVP_EINVAL, "workspace must be 256-byte aligned");
-    kvp_attn_args w = whole_contexts(*a);
-    if (!pl.shared) return kvp_paged_attention(&w, stream);
+    if (!pl.shared) {
+        const kvp_attn_args w = whole_contexts(*a);
+        return kvp_paged_attention(&w, stream);
+    }
     if (!aligned16(a->k_cache) || !aligned16(a->v_cache)) return fail(KVP_EINVAL, "K/V pools must be 16-byte aligned");
     const long long rows = a->num_blocks * static_cast<long long>(a->block_size);
     if (rows > 0x7fffffffLL) return fail(KVP_EINVAL, "num_blocks * block_size must stay below 2^31");
@@ -969,13 +1184,12 @@ extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stre
     p.prefix_blocks = a->prefix_blocks;
     p.group_starts = a->group_starts;
     p.status = a->status;
-    p.counters = reinterpret_cast<int32_t*>(ws + pl.own.ws_cnt_off);
-    p.num_counters = a->num_seqs * pl.own.groups;
-    p.unit_prefix = reinterpret_cast<long long*>(ws + pl.units);
+    p.spans = reinterpret_cast<int2*>(ws);
     p.part_ml = reinterpret_cast<float2*>(ws + pl.ml);
     p.part_o = reinterpret_cast<float*>(ws + pl.o);
-    p.own_o = reinterpret_cast<float*>(ws + pl.own_o);
-    p.own_lse = reinterpret_cast<float*>(ws + pl.own_lse);
+    p.q = a->q;
+    p.k_cache = a->k_cache;
+    p.v_cache = a->v_cache;
     p.out = a->out;
     p.num_blocks = a->num_blocks;
     p.wait_limit = kvpd::kWaitLimitCycles;
@@ -998,14 +1212,8 @@ extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stre
     p.sl2 = (a->scale > 0.f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim))) * 1.4426950408889634f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->head_dim == 64)
-        rc = p.bf16 ? launch_prefix<64, __nv_bfloat16>(qm, km, vm, p, s) : launch_prefix<64, __half>(qm, km, vm, p, s);
+        rc = p.bf16 ? launch_both<64, __nv_bfloat16>(qm, km, vm, p, s) : launch_both<64, __half>(qm, km, vm, p, s);
     else
-        rc = p.bf16 ? launch_prefix<128, __nv_bfloat16>(qm, km, vm, p, s) : launch_prefix<128, __half>(qm, km, vm, p, s);
-    if (rc != KVP_OK) return rc;
-    w.out = ws + pl.own_o;
-    w.out_dtype = KVP_DTYPE_F32;
-    w.flags = KVP_ATTN_WORKSPACE_CLEAN | KVP_ATTN_EARLY_LOAD;  // the counters were cleared by the kernel before
-    rc = attention_own_parts(&w, a->prefix_blocks, reinterpret_cast<float*>(ws + pl.own_lse), s);
-    if (rc != KVP_OK) return rc;
-    return launch_join(p, a->head_dim, s);
+        rc = p.bf16 ? launch_both<128, __nv_bfloat16>(qm, km, vm, p, s) : launch_both<128, __half>(qm, km, vm, p, s);
+    return rc;
 }
