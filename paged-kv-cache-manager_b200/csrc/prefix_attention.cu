@@ -391,8 +391,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const uint32_t ring_k = base + 2 * kTile, ring_v = ring_k + kSlotsK * kTile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // the next kernel may be scheduled as soon as this one's CTAs leave their SMs; it waits for all of them
-    griddep_launch_dependents();
     if (threadIdx.x == 0) {
         sh.abort = 0;
         for (int s = 0; s < 8; ++s) {
@@ -417,7 +415,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         prefetch_tensormap(&kmap);
         prefetch_tensormap(&vmap);
     }
-    if (warp == 8) tmem_alloc(smem_u32(&sh.tmem));  // while the others wait for the groups
+    // Nothing is read or written before the kernels ahead are done, and no tensor memory is held while waiting for them.
+    // The kernels behind start only once every CTA here has its own: one of them that takes tensor memory while it waits
+    // for this kernel could otherwise keep it from ever getting any.
+    griddep_wait();
+    if (warp == 8) {
+        tmem_alloc(smem_u32(&sh.tmem));
+        griddep_launch_dependents();
+    }
     const Start from = find_start(p, sh.warp_sum, &sh.found);
     const int cta = blockIdx.x, G = static_cast<int>(min(static_cast<long long>(gridDim.x), from.total));
     tc_fence_before();
@@ -776,6 +781,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 3) own_kernel(co
     constexpr int ROWS = 8 * NT;
     __shared__ float2 sm_ml[kOwnWarps][ROWS];
     __shared__ __align__(16) float sm_o[kOwnWarps][ROWS][D];
+    griddep_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c4 = lane & 3;
     const int ctas = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
     const int item = static_cast<int>(blockIdx.x) / ctas;
@@ -1097,8 +1103,18 @@ int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMa
     const int rc = allow_smem(reinterpret_cast<const void*>(fn));
     if (rc != KVP_OK) return rc;
     constexpr size_t tile = static_cast<size_t>(kvpd::kKeys) * D * 2;
-    fn<<<sm_count(), kvpd::kPrefixThreads, 1024 + (2 + (D == 128 ? 5 : 10)) * tile, s>>>(qm, km, vm, p);
-    return cuda_status(cudaGetLastError(), "shared prefix launch");
+    // Its start -- barriers, tensor memory -- may overlap the kernel before it.
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(sm_count()));
+    cfg.blockDim = dim3(kvpd::kPrefixThreads);
+    cfg.dynamicSmemBytes = 1024 + (2 + (D == 128 ? 5 : 10)) * tile;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, fn, qm, km, vm, p), "shared prefix launch");
 }
 
 template <int D, class KV>
