@@ -195,11 +195,12 @@ KVP_API int kvp_paged_attention_noalloc(const kvp_attn_args* a, void* stream);
  *     nothing is shared); they are completely filled, so prefix_blocks * block_size <= seq_len.  The first member's
  *     table row gives the blocks.
  * A sequence that breaks these rules, or whose length is invalid, gets zeros and sets KVP_STATUS_BAD_LEN.
- * Types, head shapes and layouts as in kvp_paged_attention; at most 8192 sequences.  The sharing kernel takes head_dim
- * 64 and 128, queries of the pools' 16-bit dtype (16-byte aligned) and block sizes that are multiples of 8; it rounds
- * the probabilities to that dtype before the product with V (sums in fp32).  Other calls attend over every sequence's
- * whole context.  The workspace (256-byte aligned) needs no initial value and keeps none; calls that overlap on the
- * GPU need one each. */
+ * Types, head shapes and layouts as in kvp_paged_attention.  Sharing takes head_dim 64 and 128, queries of the pools'
+ * 16-bit dtype, block sizes that are multiples of 8, q and out on 16-byte boundaries, num_seqs * kv_heads <= 2^27 and
+ * max_blocks * block_size < 2^31; over the shared keys it rounds the probabilities to the pools' dtype before the
+ * product with V (sums in fp32).  Every other call attends over each sequence's whole context, as
+ * kvp_paged_attention does.  The workspace (256-byte aligned) needs no initial value and keeps none; calls that overlap
+ * on the GPU need one each. */
 typedef struct kvp_prefix_args {
     const void* q;
     const void* k_cache; /* this layer's pools */

@@ -1072,7 +1072,8 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
     const int rc = plan_attention(w, true, &whole);
     if (rc != KVP_OK) return rc;
     pl->shared = (a->head_dim == 64 || a->head_dim == 128) && a->q_dtype == a->kv_dtype && pl->run >= 8 && aligned16(a->q) &&
-                 aligned16(a->out) && static_cast<long long>(a->num_seqs) * a->kv_heads <= (1LL << 27);
+                 aligned16(a->out) && static_cast<long long>(a->num_seqs) * a->kv_heads <= (1LL << 27) &&
+                 static_cast<long long>(a->max_blocks) * a->block_size <= 0x7fffffffLL;  // tokens of a table row, 32 bits below
     pl->bytes = whole.ws_bytes;
     if (!pl->shared) return KVP_OK;
     const size_t rows = static_cast<size_t>(a->num_seqs) * a->num_heads;
@@ -1171,8 +1172,8 @@ extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stre
         return kvp_paged_attention(&w, stream);
     }
     if (!aligned16(a->k_cache) || !aligned16(a->v_cache)) return fail(KVP_EINVAL, "K/V pools must be 16-byte aligned");
-    const long long rows = a->num_blocks * static_cast<long long>(a->block_size);
-    if (rows > 0x7fffffffLL) return fail(KVP_EINVAL, "num_blocks * block_size must stay below 2^31");
+    if (a->num_blocks > 0x7fffffffLL / a->block_size) return fail(KVP_EINVAL, "num_blocks * block_size must stay below 2^31");
+    const long long rows = a->num_blocks * a->block_size;
     const int g = a->num_heads / a->kv_heads;
     const cuuint64_t D = static_cast<cuuint64_t>(a->head_dim);
     CUtensorMap qm, km, vm;

@@ -68,6 +68,57 @@ def test_beam_workspace(kvb):
     assert kvb.lib().kvp_beam_workspace_size(None) == 0 and kvb.lib().kvp_beam_select(None, None) == kvb.KVP_EINVAL
 
 
+def _prefix(kvb, **kw):
+    a = kvb.PrefixArgs()
+    a.q = a.k_cache = a.v_cache = a.block_tables = a.seq_lens = a.prefix_blocks = a.group_starts = a.out = a.workspace = PTR
+    a.q_dtype = a.kv_dtype = a.out_dtype = kvb.BF16
+    a.num_seqs, a.num_groups, a.num_heads, a.kv_heads, a.head_dim, a.block_size, a.max_blocks = 6, 2, 8, 2, 64, 16, 10
+    a.num_blocks, a.workspace_bytes = 40, 1 << 30
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("bad", [dict(q_dtype=7), dict(kv_dtype=-1), dict(out_dtype=3), dict(num_seqs=-1), dict(num_groups=-1),
+                                 dict(num_groups=0), dict(num_groups=7), dict(num_blocks=0), dict(num_blocks=-5),
+                                 dict(block_size=0), dict(max_blocks=0), dict(head_dim=48), dict(head_dim=0), dict(num_heads=7),
+                                 dict(num_heads=0), dict(kv_heads=0), dict(num_heads=34), dict(q=0), dict(out=0),
+                                 dict(k_cache=0), dict(v_cache=0), dict(block_tables=0), dict(seq_lens=0),
+                                 dict(prefix_blocks=0), dict(group_starts=0), dict(k_cache=PTR + 8), dict(v_cache=PTR + 2),
+                                 dict(workspace=PTR + 16), dict(num_blocks=1 << 27), dict(num_blocks=(1 << 60) + 1)])
+def test_prefix_refuses(kvb, bad):
+    assert kvb.lib().kvp_prefix_attention(C.byref(_prefix(kvb, **bad)), None) == kvb.KVP_EINVAL and kvb.last_error()
+
+
+def test_prefix_workspace(kvb):
+    L = kvb.lib()
+    need = L.kvp_prefix_workspace_size(C.byref(_prefix(kvb)))
+    assert 0 < need < 1 << 30
+    for kw in (dict(workspace_bytes=need - 1), dict(workspace=0)):
+        assert L.kvp_prefix_attention(C.byref(_prefix(kvb, **kw)), None) == kvb.KVP_ENOSPACE
+    assert L.kvp_prefix_workspace_size(C.byref(_prefix(kvb, head_dim=48))) == 0 and kvb.last_error()
+    empty = _prefix(kvb, num_seqs=0, num_groups=0, q=0, out=0, workspace=0, workspace_bytes=0)
+    assert L.kvp_prefix_workspace_size(C.byref(empty)) == 0 and not kvb.last_error()
+    assert L.kvp_prefix_attention(C.byref(empty), None) == kvb.KVP_OK
+    assert L.kvp_prefix_workspace_size(None) == 0 and L.kvp_prefix_attention(None, None) == kvb.KVP_EINVAL
+
+
+def test_prefix_groups_from_tables(kvb):
+    groups = lambda tables, lens, B=4: tuple(x.tolist() for x in kvb.shared_prefix_groups(np.array(tables), lens, B))
+    assert groups(np.zeros((0, 3), np.int32), []) == ([], [0])
+    assert groups([[5, 6, 7]], [12]) == ([0], [0, 1])  # alone: nothing is shared
+    assert groups([[5, 6, 7], [5, 6, 8]], [12, 9]) == ([2, 2], [0, 2])
+    assert groups([[5, 6, 7], [5, 6, 7]], [12, 12]) == ([3, 3], [0, 2])
+    assert groups([[5, 6, 7], [5, 6, 7]], [12, 11]) == ([2, 2], [0, 2])  # only full blocks
+    assert groups([[5, 6, 7], [5, 6, 7]], [12, 3]) == ([0, 0], [0, 1, 2])  # no full block
+    # neighbours only; the run takes what all of it shares
+    assert groups([[1, 2, 3], [1, 2, 4], [1, 9, 0], [8, 2, 3], [1, 2, 3], [0, 0, 0]], [12, 12, 6, 9, 12, 0]) == (
+        [1, 1, 1, 0, 0, 0], [0, 3, 4, 5, 6])
+    for tables, lens in (([[1, 2]], [12]), ([[1, 2]], [3, 4]), ([1, 2], [4, 4])):
+        with pytest.raises(ValueError):
+            kvb.shared_prefix_groups(np.array(tables), lens, 4)
+
+
 def test_struct_layouts_match_the_header(kvb, tmp_path):
     structs = {"kvp_rope_args": kvb.RopeArgs, "kvp_beam_args": kvb.BeamArgs}
     if hasattr(kvb, "PrefixArgs"):
