@@ -40,6 +40,14 @@ constexpr int kKeys = 128;         // keys per tile
 constexpr int kRows = 128;         // rows per tile: M of the MMA
 constexpr int kPrefixThreads = 352;  // 8 softmax warps, the MMA warp, the warps that load K (and Q) and V
 constexpr int kTmemCols = 512;
+constexpr int kPrefixLimit = 512;  // at most 128 registers a thread: own_kernel's CTAs fit beside it
+
+// What joins a (sequence, kv head): partial rows of query head 0 begin at row0, and 256 further for each CTA before the
+// first of the span at pair_at (-1: nothing is shared); `parts` per CTA, `rows` apart.
+struct OwnMeta {
+    long long row0, pair_at;
+    int parts, rows, fine, unused;
+};
 
 struct PrefixParams {
     const int32_t* tables;
@@ -50,6 +58,9 @@ struct PrefixParams {
     int2* spans;               // first and last CTA of each (group, kv head, pair), at its first row's (member, kv head)
     float2* part_ml;           // partial rows: (maximum in log2 units, sum)
     float* part_o;
+    OwnMeta* own_meta;         // of each (sequence, kv head), where the own parts are joined by a kernel of their own
+    float2* own_ml;            // own parts, a row per (sequence, query head)
+    float* own_o;
     const void* q;
     const void* k_cache;
     const void* v_cache;
@@ -58,7 +69,8 @@ struct PrefixParams {
     long long wait_limit;
     int num_seqs, num_groups, nh, kvh, g, max_blocks, B, Bshift, run, runs, oob_row;
     int mt;                    // members per row tile
-    int bf16, out_dtype;
+    int own_parts;             // warps that share an own part, where the parts are joined by a kernel of their own
+    int bf16, out_dtype, ctas, own_ctas;  // ctas: prefix_kernel's
     float sl2;
 };
 
@@ -372,7 +384,7 @@ struct Cursor {
 };
 
 template <int D, class KV>
-__global__ void __launch_bounds__(kPrefixThreads, 1)
+__global__ void __launch_bounds__(kPrefixLimit, 1)
     prefix_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap, const PrefixParams p) {
     using Tr = F16Traits<KV>;
@@ -387,7 +399,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     extern __shared__ uint8_t dyn[];
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
     // Slots of K and of V beside two query tiles: 160 KB in all.
-    constexpr int kSlotsK = D == 128 ? 2 : 5, kSlotsV = D == 128 ? 3 : 5;
+    constexpr int kSlotsK = D == 128 ? 2 : 4, kSlotsV = D == 128 ? 2 : 3;
     const uint32_t ring_k = base + 2 * kTile, ring_v = ring_k + kSlotsK * kTile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -772,18 +784,54 @@ struct Fold {
     }
 };
 
-// NT: groups of 8 query heads per kv head.
-template <int D, class KV, int NT>
-__global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 3) own_kernel(const PrefixParams p) {
+__device__ __forceinline__ void store_out(const PrefixParams& p, size_t at, const float4& o, float inv) {
+    const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    if (p.out_dtype == KVP_DTYPE_F32)
+        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
+    else
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+            p.out_dtype == KVP_DTYPE_F16 ? make_uint2(F16Traits<__half>::pack(y[0], y[1]), F16Traits<__half>::pack(y[2], y[3]))
+                                         : make_uint2(F16Traits<__nv_bfloat16>::pack(y[0], y[1]), F16Traits<__nv_bfloat16>::pack(y[2], y[3]));
+}
+
+// Partial rows k0 .. k0 + 3 of the `count` that the shared part left of a query head.
+struct SharedParts {
+    long long row0 = 0;
+    int count = 0, parts = 1, rows = 0;
+    __device__ __forceinline__ void load(const PrefixParams& p, int j, int D, int col, int k0, float2 (&ml)[4], float4 (&x)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = k0 + i;
+            const long long r = row0 + j + (parts == 2 ? static_cast<long long>(k >> 1) * 2 * kRows + (k & 1) * rows
+                                                       : static_cast<long long>(k) * 2 * kRows);
+            ml[i] = k < count ? __ldcg(&p.part_ml[r]) : make_float2(-INFINITY, 0.f);
+            x[i] = k < count ? __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    }
+};
+
+__device__ __forceinline__ SharedParts shared_parts(const PrefixParams& p, const OwnMeta& m) {
+    SharedParts s;
+    if (m.pair_at < 0) return s;
+    const int2 span = __ldcg(p.spans + m.pair_at);
+    const int first = min(max(span.x, 0), p.ctas - 1);  // (a wait that ran out may have left them unwritten)
+    s.row0 = m.row0 + static_cast<long long>(first) * 2 * kRows;
+    s.count = (min(max(span.y, first), p.ctas - 1) - first + 1) * m.parts;
+    s.parts = m.parts;
+    s.rows = m.rows;
+    return s;
+}
+
+// NT: groups of 8 query heads per kv head.  Apart: the own part is left for join_kernel.
+template <int D, class KV, int NT, bool Apart>
+__global__ void __launch_bounds__(Apart ? 32 : kOwnWarps * 32, Apart ? (NT == 1 ? 16 : 12) : NT == 1 ? 4 : 3) own_kernel(const PrefixParams p) {
     using Tr = F16Traits<KV>;
     constexpr int NI = D / 32;   // 16-byte pieces of a row that a lane of four holds
     constexpr int NH = D / 64;   // and that a lane of eight holds
     constexpr int ROWS = 8 * NT;
-    __shared__ float2 sm_ml[kOwnWarps][ROWS];
-    __shared__ __align__(16) float sm_o[kOwnWarps][ROWS][D];
     griddep_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c4 = lane & 3;
-    const int ctas = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
+    const int ctas = Apart ? p.own_parts : static_cast<int>(cluster_size()), rank = Apart ? static_cast<int>(blockIdx.x) % ctas : static_cast<int>(cluster_rank());
     const int item = static_cast<int>(blockIdx.x) / ctas;
     const int seq = item / p.kvh, h = item - seq * p.kvh;
     const int len = __ldg(p.lens + seq), pb = __ldg(p.prefix_blocks + seq);
@@ -791,7 +839,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 3) own_kernel(co
     bool fine = len >= 1 && nblk <= p.max_blocks && pb >= 0 && static_cast<long long>(pb) * p.B <= len;
     const int own = fine ? len - pb * p.B : 0;
     const int32_t* trow = p.tables + static_cast<long long>(seq) * p.max_blocks + (fine ? pb : 0);
-    const int tiles = (own + 15) >> 4, stride = ctas * kOwnWarps;
+    const int tiles = (own + 15) >> 4, stride = Apart ? ctas : ctas * kOwnWarps;
 
     // queries of head 8 nt + gid
     uint4 qr[NT][NI];
@@ -844,7 +892,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 3) own_kernel(co
         }
     };
     // The next tile's K is on its way as soon as this one's scores are there, its V as soon as this one's is used.
-    const int first_tile = rank * kOwnWarps + warp;
+    const int first_tile = Apart ? rank : rank * kOwnWarps + warp;
     {
         const int row = row_of(first_tile);
         load_k(row);
@@ -862,21 +910,20 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 3) own_kernel(co
     }
     const Group grp = load_group(p, lo);
     fine = fine && grp.start <= seq && seq < grp.start + grp.members && grp.blocks == pb;
-    // and the shared part's partial rows of head 0: `parts` for each CTA from the first on, `rows` apart within a CTA, 256
-    // between CTAs
-    griddep_wait();
-    int count = 0, parts = 1, rows = 0;
-    long long row0 = 0;
+    OwnMeta meta = {0, -1, 1, 0, fine, 0};
     if (fine && grp.ktiles > 0) {
         const int member = seq - grp.start, member0 = member / (2 * p.mt) * 2 * p.mt, left = grp.members - member0;
-        const long long pair_at = static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(h) * grp.members + member0;
-        const int2 span = __ldcg(p.spans + pair_at);
-        row0 = 2LL * p.g * pair_at + static_cast<long long>(span.x) * 2 * kRows + (member - member0) * p.g;  // two row tiles: one after the other
+        meta.pair_at = static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(h) * grp.members + member0;
+        meta.row0 = 2LL * p.g * meta.pair_at + (member - member0) * p.g;  // two row tiles: one after the other
         if (left <= p.mt) {  // one: the even and the odd key tiles'
-            parts = 2;
-            rows = left * p.g;
+            meta.parts = 2;
+            meta.rows = left * p.g;
         }
-        count = (span.y - span.x + 1) * parts;
+    }
+    SharedParts shared;
+    if (!Apart) {
+        griddep_wait();
+        shared = shared_parts(p, meta);
     }
     for (int tile = first_tile; tile < tiles; tile += stride) {
         const bool in0 = tile * 16 + gid < own, in1 = tile * 16 + gid + 8 < own;
@@ -940,23 +987,42 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 3) own_kernel(co
         load_v(row);
         row = row_of(tile + 2 * stride);
     }
+    if constexpr (Apart) {  // a lane holds dims 64 i + 8 gid .. + 7 of heads 2 c4, 2 c4 + 1
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float sum = l[nt][e];
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                const int j = 8 * nt + 2 * c4 + e;
+                if (j >= p.g) continue;
+                const long long row = (static_cast<long long>(seq) * p.nh + h * p.g + j) * ctas + rank;
+                if (gid == 0) p.own_ml[row] = make_float2(m[nt][e], sum);
+                if (first_tile >= tiles) continue;  // nothing: never read
+#pragma unroll
+                for (int i = 0; i < NH; ++i)
+#pragma unroll
+                    for (int t = 0; t < 4; t += 2)
+                        *reinterpret_cast<float4*>(p.own_o + row * D + 64 * i + 8 * gid + 2 * t) =
+                            make_float4(o[nt][i * 4 + t][e], o[nt][i * 4 + t][2 + e], o[nt][i * 4 + t + 1][e], o[nt][i * 4 + t + 1][2 + e]);
+            }
+        if (rank == 0 && lane == 0) {
+            p.own_meta[item] = meta;
+            if (!fine && h == 0) report(p.status, KVP_STATUS_BAD_LEN);
+        }
+        // join_kernel waits for this kernel, and through its last CTA for the shared part
+        if (blockIdx.x == gridDim.x - 1) griddep_wait();
+        return;
+    }
+    __shared__ float2 sm_ml[kOwnWarps][ROWS];
+    __shared__ __align__(16) float sm_o[kOwnWarps][ROWS][D];
     // Each thread's outputs, four columns of a query head, are known by now: its first partial rows start on their way before
     // the warps meet.
     const int outs = p.g * (D / 4), at0 = rank * kOwnWarps * 32 + static_cast<int>(threadIdx.x);
     float2 pml[4];
     float4 px[4];
-    auto part = [&](int at, int k0) {
-        const int j = at / (D / 4), col = (at - j * (D / 4)) * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k = k0 + i;
-            const long long r = row0 + j + (parts == 2 ? static_cast<long long>(k >> 1) * 2 * kRows + (k & 1) * rows
-                                                       : static_cast<long long>(k) * 2 * kRows);
-            pml[i] = k < count ? __ldcg(&p.part_ml[r]) : make_float2(-INFINITY, 0.f);
-            px[i] = k < count ? __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-    };
-    if (at0 < outs) part(at0, 0);
+    if (at0 < outs) shared.load(p, at0 / (D / 4), D, at0 % (D / 4) * 4, 0, pml, px);
     // this warp's heads into shared memory: a lane holds dims 64 i + 8 gid .. + 7 of heads 2 c4, 2 c4 + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -978,7 +1044,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 3) own_kernel(co
     else __syncthreads();
     for (int at = at0; at < outs; at += ctas * kOwnWarps * 32) {
         const int j = at / (D / 4), col = (at - j * (D / 4)) * 4;
-        if (at != at0) part(at, 0);
+        if (at != at0) shared.load(p, j, D, col, 0, pml, px);
         Fold all;
         for (int c = 0; c < ctas; ++c) {
             float2 ml[4];
@@ -995,23 +1061,54 @@ __global__ void __launch_bounds__(kOwnWarps * 32, NT == 1 ? 4 : 3) own_kernel(co
             }
             all.add(ml, x);
         }
+        const size_t row = static_cast<size_t>(seq) * p.nh + h * p.g + j;
         all.add(pml, px);
-        for (int k0 = 4; k0 < count; k0 += 4) {
-            part(at, k0);
+        for (int k0 = 4; k0 < shared.count; k0 += 4) {
+            shared.load(p, j, D, col, k0, pml, px);
             all.add(pml, px);
         }
-        if (!fine && at == 0 && h == 0) report(p.status, KVP_STATUS_BAD_LEN);
-        const float inv = fine ? 1.f / all.l : 0.f;
-        const float y[4] = {fine ? all.o.x * inv : 0.f, fine ? all.o.y * inv : 0.f, fine ? all.o.z * inv : 0.f, fine ? all.o.w * inv : 0.f};
-        const size_t out = (static_cast<size_t>(seq) * p.nh + h * p.g + j) * D + col;
-        if (p.out_dtype == KVP_DTYPE_F32)
-            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + out) = make_float4(y[0], y[1], y[2], y[3]);
-        else
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + out) =
-                p.out_dtype == KVP_DTYPE_F16 ? make_uint2(F16Traits<__half>::pack(y[0], y[1]), F16Traits<__half>::pack(y[2], y[3]))
-                                             : make_uint2(F16Traits<__nv_bfloat16>::pack(y[0], y[1]), F16Traits<__nv_bfloat16>::pack(y[2], y[3]));
+        store_out(p, row * D + col, fine ? all.o : make_float4(0.f, 0.f, 0.f, 0.f), fine ? 1.f / all.l : 0.f);
     }
+    if (!fine && h == 0 && rank == 0 && threadIdx.x == 0) report(p.status, KVP_STATUS_BAD_LEN);
     if (ctas > 1) cluster_sync();  // others may still read this CTA's shared memory
+}
+
+// The own part and the shared part's partial rows: a thread folds four columns of a (sequence, query head).
+template <int D>
+__global__ void __launch_bounds__(256) join_kernel(const PrefixParams p) {
+    griddep_launch_dependents();
+    const long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    const long long row = at / (D / 4);
+    const int col = static_cast<int>(at % (D / 4)) * 4;
+    if (row >= static_cast<long long>(p.num_seqs) * p.nh) return;
+    const unsigned item = static_cast<unsigned>(row) / static_cast<unsigned>(p.g);
+    const int j = static_cast<int>(static_cast<unsigned>(row) - item * static_cast<unsigned>(p.g));
+    griddep_wait();
+    const OwnMeta meta = p.own_meta[item];
+    float2 ml[4];
+    float4 x[4];
+    auto own_part = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool some = k0 + i < p.own_parts;
+            const long long r = row * p.own_parts + k0 + i;
+            ml[i] = some ? __ldcg(&p.own_ml[r]) : make_float2(-INFINITY, 0.f);
+            x[i] = some ? __ldcg(reinterpret_cast<const float4*>(p.own_o + r * D + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    own_part(0);
+    const SharedParts shared = shared_parts(p, meta);
+    Fold all;
+    all.add(ml, x);
+    if (p.own_parts > 4) {
+        own_part(4);
+        all.add(ml, x);
+    }
+    for (int k0 = 0; k0 < shared.count; k0 += 4) {
+        shared.load(p, j, D, col, k0, ml, x);
+        all.add(ml, x);
+    }
+    store_out(p, static_cast<size_t>(row) * D + col, meta.fine ? all.o : make_float4(0.f, 0.f, 0.f, 0.f), meta.fine ? 1.f / all.l : 0.f);
 }
 
 }  // namespace kvpd
@@ -1048,10 +1145,13 @@ kvp_attn_args whole_contexts(const kvp_prefix_args& a) {
     return w;
 }
 
+constexpr long long kOwnWaves = 16;
+
 struct PrefixPlan {
     bool shared = false;  // else the plain decode attention over every sequence's whole context
-    size_t ml = 0, o = 0, bytes = 0;
+    size_t ml = 0, o = 0, meta = 0, own_ml = 0, own_o = 0, bytes = 0;
     int mt = 1, run = 8;
+    int own_parts = 0, own_ctas = 1;  // own parts joined apart: warps per (sequence, kv head), else CTAs
 };
 
 int gcd_of(int a, int b) { return b ? gcd_of(b, a % b) : a; }
@@ -1082,7 +1182,15 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
     pl->ml = up256(static_cast<size_t>(a->num_seqs) * a->kv_heads * 8);
     pl->o = pl->ml + up256(parts * 8);
     // (the larger of both: where q or out are not aligned the other path runs in the same workspace)
-    pl->bytes = std::max(pl->bytes, pl->o + parts * a->head_dim * 4);
+    pl->meta = pl->o + up256(parts * a->head_dim * 4);
+    // Few (sequence, kv head) pairs: clusters share one, so that a long own part does not hang on four warps.
+    const long long items = static_cast<long long>(a->num_seqs) * a->kv_heads, sms = sm_count();
+    while (pl->own_ctas < 8 && items * pl->own_ctas * 2 <= sms * 3) pl->own_ctas *= 2;
+    if (pl->own_ctas == 1)
+        for (pl->own_parts = 1; pl->own_parts < 8 && items * pl->own_parts < sms * kOwnWaves;) pl->own_parts *= 2;
+    pl->own_ml = pl->meta + up256(static_cast<size_t>(a->num_seqs) * a->kv_heads * sizeof(kvpd::OwnMeta));
+    pl->own_o = pl->own_ml + up256(rows * pl->own_parts * 8);
+    pl->bytes = std::max(pl->bytes, pl->own_o + rows * pl->own_parts * a->head_dim * 4);
     return KVP_OK;
 }
 
@@ -1106,9 +1214,9 @@ int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMa
     constexpr size_t tile = static_cast<size_t>(kvpd::kKeys) * D * 2;
     // Its start -- barriers, tensor memory -- may overlap the kernel before it.
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(sm_count()));
+    cfg.gridDim = dim3(static_cast<unsigned>(p.ctas));
     cfg.blockDim = dim3(kvpd::kPrefixThreads);
-    cfg.dynamicSmemBytes = 1024 + (2 + (D == 128 ? 5 : 10)) * tile;
+    cfg.dynamicSmemBytes = 1024 + (2 + (D == 128 ? 4 : 7)) * tile;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1120,14 +1228,13 @@ int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMa
 
 template <int D, class KV>
 int launch_own(const kvpd::PrefixParams& p, cudaStream_t s) {
-    auto fn = p.g > 8 ? &kvpd::own_kernel<D, KV, 2> : &kvpd::own_kernel<D, KV, 1>;
-    // Few (sequence, kv head) pairs: clusters share one, so that a long own part does not hang on four warps.
-    const long long items = static_cast<long long>(p.num_seqs) * p.kvh, room = static_cast<long long>(sm_count()) * 3;
-    unsigned ctas = 1;
-    while (ctas < 8 && items * ctas * 2 <= room) ctas *= 2;
+    const bool apart = p.own_parts > 0;
+    const unsigned items = static_cast<unsigned>(p.num_seqs) * static_cast<unsigned>(p.kvh), ctas = static_cast<unsigned>(p.own_ctas);
+    auto fn = p.g > 8 ? (apart ? &kvpd::own_kernel<D, KV, 2, true> : &kvpd::own_kernel<D, KV, 2, false>)
+                      : (apart ? &kvpd::own_kernel<D, KV, 1, true> : &kvpd::own_kernel<D, KV, 1, false>);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(items) * ctas);
-    cfg.blockDim = dim3(kvpd::kOwnWarps * 32);
+    cfg.gridDim = dim3(items * (apart ? static_cast<unsigned>(p.own_parts) : ctas));
+    cfg.blockDim = dim3(apart ? 32 : kvpd::kOwnWarps * 32);
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1137,8 +1244,12 @@ int launch_own(const kvpd::PrefixParams& p, cudaStream_t s) {
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return cuda_status(cudaLaunchKernelEx(&cfg, fn, p), "own part launch");
+    cfg.numAttrs = apart ? 1 : 2;
+    const int rc = cuda_status(cudaLaunchKernelEx(&cfg, fn, p), "own part launch");
+    if (rc != KVP_OK || !apart) return rc;
+    cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(p.num_seqs) * p.nh * (D / 4) + 255) / 256));
+    cfg.blockDim = dim3(256);
+    return cuda_status(cudaLaunchKernelEx(&cfg, &kvpd::join_kernel<D>, p), "join launch");
 }
 
 template <int D, class KV>
@@ -1204,6 +1315,9 @@ extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stre
     p.spans = reinterpret_cast<int2*>(ws);
     p.part_ml = reinterpret_cast<float2*>(ws + pl.ml);
     p.part_o = reinterpret_cast<float*>(ws + pl.o);
+    p.own_meta = reinterpret_cast<kvpd::OwnMeta*>(ws + pl.meta);
+    p.own_ml = reinterpret_cast<float2*>(ws + pl.own_ml);
+    p.own_o = reinterpret_cast<float*>(ws + pl.own_o);
     p.q = a->q;
     p.k_cache = a->k_cache;
     p.v_cache = a->v_cache;
@@ -1224,8 +1338,11 @@ extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stre
     p.runs = kvpd::kKeys / pl.run;
     p.oob_row = static_cast<int>(rows);
     p.mt = pl.mt;
+    p.own_parts = pl.own_parts;
+    p.own_ctas = pl.own_ctas;
     p.bf16 = a->kv_dtype == KVP_DTYPE_BF16;
     p.out_dtype = a->out_dtype;
+    p.ctas = sm_count();
     p.sl2 = (a->scale > 0.f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim))) * 1.4426950408889634f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->head_dim == 64)
