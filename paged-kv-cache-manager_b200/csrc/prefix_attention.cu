@@ -252,7 +252,10 @@ __device__ __forceinline__ long long floor_div(long long a, long long b, long lo
     return q;
 }
 // CTA c of G owns units [c T / G, (c + 1) T / G).
-__device__ __forceinline__ long long first_unit(int c, long long T, int G) { return floor_div(c, T, G); }
+__device__ __forceinline__ long long first_unit(int c, long long T, int G) {
+    if (T < (1 << 22)) return static_cast<unsigned>(c) * static_cast<unsigned>(T) / static_cast<unsigned>(G);  // c <= 1023
+    return floor_div(c, T, G);
+}
 
 // One stretch of a CTA's units: key tiles [k0, k0 + n) of (group, kv head, pair).
 struct Work {
@@ -273,7 +276,7 @@ struct WorkList {
             grp = load_group(p, ++gi);
         }
         const long long rel = t - first;
-        const int triple = static_cast<int>(rel / grp.ktiles);
+        const int triple = static_cast<int>(rel < (1LL << 32) ? static_cast<unsigned>(rel) / static_cast<unsigned>(grp.ktiles) : rel / grp.ktiles);
         w.k0 = static_cast<int>(rel - static_cast<long long>(triple) * grp.ktiles);
         w.n = static_cast<int>(min(static_cast<long long>(grp.ktiles - w.k0), end - t));
         t += w.n;
@@ -292,12 +295,37 @@ struct WorkList {
     }
 };
 
-// Where a CTA's units begin: the total, the group that holds the CTA's first unit and that group's first unit.  One pass over the groups while there is a thread for each, else a second one.
+// Where a CTA's units begin: the total, the group that holds the CTA's first unit and that group's first unit.
 struct Start {
     long long total, first;
     int group;
 };
-__device__ __forceinline__ Start find_start(const PrefixParams& p, long long* warp_sum, Start* found) {
+// Up to 32 groups: every warp by itself, a lane per group.
+__device__ __forceinline__ Start find_start_few(const PrefixParams& p, Group* grp) {
+    const int lane = threadIdx.x & 31;
+    const Group mine = lane < p.num_groups ? load_group(p, lane) : Group{0, 0, 0, 0, 0};
+    const long long u = mine.units(p.kvh);
+    long long x = u;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += y;
+    }
+    Start s{__shfl_sync(0xffffffffu, x, 31), 0, 0};
+    const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), s.total));
+    if (static_cast<int>(blockIdx.x) >= G) return s;
+    const long long at = first_unit(blockIdx.x, s.total, G);
+    s.group = __ffs(__ballot_sync(0xffffffffu, x - u <= at && at < x)) - 1;
+    s.first = __shfl_sync(0xffffffffu, x - u, s.group);
+    grp->start = __shfl_sync(0xffffffffu, mine.start, s.group);
+    grp->members = __shfl_sync(0xffffffffu, mine.members, s.group);
+    grp->blocks = __shfl_sync(0xffffffffu, mine.blocks, s.group);
+    grp->pairs = __shfl_sync(0xffffffffu, mine.pairs, s.group);
+    grp->ktiles = __shfl_sync(0xffffffffu, mine.ktiles, s.group);
+    return s;
+}
+// More: the CTA together, a thread per group and kPrefixThreads groups at a time.
+__device__ __forceinline__ Start find_start(const PrefixParams& p, long long* warp_sum, Start* found, Group* grp) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto scan = [&](long long u, long long carry, long long* mine) {  // all of a chunk; *mine: what lies before this thread
         long long x = u;
@@ -309,7 +337,6 @@ __device__ __forceinline__ Start find_start(const PrefixParams& p, long long* wa
         if (lane == 31) warp_sum[warp] = x;
         __syncthreads();
         long long before = carry, all = 0;
-#pragma unroll
         for (int w = 0; w < kPrefixThreads / 32; ++w) {
             const long long s = warp_sum[w];
             if (w < warp) before += s;
@@ -320,25 +347,20 @@ __device__ __forceinline__ Start find_start(const PrefixParams& p, long long* wa
         return all;
     };
     auto units_of = [&](int gi) { return gi < p.num_groups ? load_group(p, gi).units(p.kvh) : 0ll; };
-    long long total = 0, u = 0, mine = 0;
-    for (int g0 = 0; g0 < p.num_groups; g0 += kPrefixThreads) {
-        const int gi = g0 + static_cast<int>(threadIdx.x);
-        u = units_of(gi);
-        total += scan(u, total, &mine);
-    }
+    long long total = 0, mine = 0;
+    for (int g0 = 0; g0 < p.num_groups; g0 += kPrefixThreads) total += scan(units_of(g0 + static_cast<int>(threadIdx.x)), total, &mine);
     const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
     if (static_cast<int>(blockIdx.x) >= G) return Start{total, 0, 0};
     const long long at = first_unit(blockIdx.x, total, G);
     long long carry = 0;
     for (int g0 = 0; g0 < p.num_groups; g0 += kPrefixThreads) {
         const int gi = g0 + static_cast<int>(threadIdx.x);
-        if (p.num_groups > kPrefixThreads) {
-            u = units_of(gi);
-            carry += scan(u, carry, &mine);
-        }
+        const long long u = units_of(gi);
+        carry += scan(u, carry, &mine);
         if (u > 0 && mine <= at && at < mine + u) *found = Start{total, mine, gi};
     }
     __syncthreads();
+    *grp = load_group(p, found->group);
     return *found;
 }
 
@@ -435,7 +457,8 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
         tmem_alloc(smem_u32(&sh.tmem));
         griddep_launch_dependents();
     }
-    const Start from = find_start(p, sh.warp_sum, &sh.found);
+    WorkList list;
+    const Start from = p.num_groups <= 32 ? find_start_few(p, &list.grp) : find_start(p, sh.warp_sum, &sh.found, &list.grp);
     const int cta = blockIdx.x, G = static_cast<int>(min(static_cast<long long>(gridDim.x), from.total));
     tc_fence_before();
     __syncthreads();
@@ -444,13 +467,11 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
         if (warp == 8) tmem_free(sh.tmem);
         return;
     }
-    WorkList list;
     list.cta = cta;
     list.t = first_unit(cta, from.total, G);
     list.end = first_unit(cta + 1, from.total, G);
     list.gi = from.group;
     list.first = from.first;
-    list.grp = load_group(p, list.gi);
     const uint32_t tmem = sh.tmem;
     Work w;
 
@@ -1020,6 +1041,7 @@ __global__ void __launch_bounds__(Apart ? 32 : kOwnWarps * 32, Apart ? (NT == 1 
     // Each thread's outputs, four columns of a query head, are known by now: its first partial rows start on their way before
     // the warps meet.
     const int outs = p.g * (D / 4), at0 = rank * kOwnWarps * 32 + static_cast<int>(threadIdx.x);
+    const int with_tiles = min(ctas, (tiles + kOwnWarps - 1) / kOwnWarps);  // the first CTAs of the cluster
     float2 pml[4];
     float4 px[4];
     if (at0 < outs) shared.load(p, at0 / (D / 4), D, at0 % (D / 4) * 4, 0, pml, px);
@@ -1040,24 +1062,18 @@ __global__ void __launch_bounds__(Apart ? 32 : kOwnWarps * 32, Apart ? (NT == 1 
                     *reinterpret_cast<float4*>(&sm_o[warp][j][64 * i + 8 * gid + 2 * t]) =
                         make_float4(o[nt][i * 4 + t][e], o[nt][i * 4 + t][2 + e], o[nt][i * 4 + t + 1][e], o[nt][i * 4 + t + 1][2 + e]);
         }
-    if (ctas > 1) cluster_sync();
-    else __syncthreads();
+    cluster_sync();
     for (int at = at0; at < outs; at += ctas * kOwnWarps * 32) {
         const int j = at / (D / 4), col = (at - j * (D / 4)) * 4;
         if (at != at0) shared.load(p, j, D, col, 0, pml, px);
         Fold all;
-        for (int c = 0; c < ctas; ++c) {
+        for (int c = 0; c < with_tiles; ++c) {
             float2 ml[4];
             float4 x[4];
 #pragma unroll
             for (int w = 0; w < kOwnWarps; ++w) {
-                if (ctas == 1) {
-                    ml[w] = sm_ml[w][j];
-                    x[w] = *reinterpret_cast<const float4*>(&sm_o[w][j][col]);
-                } else {
-                    ml[w] = ld_cluster2(map_rank(smem_u32(&sm_ml[w][j]), c));
-                    x[w] = ld_cluster4(map_rank(smem_u32(&sm_o[w][j][col]), c));
-                }
+                ml[w] = ld_cluster2(map_rank(smem_u32(&sm_ml[w][j]), c));
+                x[w] = ld_cluster4(map_rank(smem_u32(&sm_o[w][j][col]), c));
             }
             all.add(ml, x);
         }
@@ -1070,7 +1086,7 @@ __global__ void __launch_bounds__(Apart ? 32 : kOwnWarps * 32, Apart ? (NT == 1 
         store_out(p, row * D + col, fine ? all.o : make_float4(0.f, 0.f, 0.f, 0.f), fine ? 1.f / all.l : 0.f);
     }
     if (!fine && h == 0 && rank == 0 && threadIdx.x == 0) report(p.status, KVP_STATUS_BAD_LEN);
-    if (ctas > 1) cluster_sync();  // others may still read this CTA's shared memory
+    cluster_sync();  // others may still read this CTA's shared memory
 }
 
 // The own part and the shared part's partial rows: a thread folds four columns of a (sequence, query head).

@@ -36,7 +36,7 @@ struct RopeParams {
     const void* k_norm;
     int32_t* status;
     long long q_stride, k_stride, v_stride, q_out_stride, k_out_stride;  // elements between tokens
-    long long num_slots;                                                // 0: unchecked
+    long long num_slots;                                                // of the cache
     float eps, inv_dim;
     int tokens, nh, kvh, rows;  // rows: head rows per token (nh + kvh, + kvh with a cache)
     int dim, units, rot, interleaved, max_positions, out_dtype, kv_dtype;
@@ -99,7 +99,7 @@ __device__ __forceinline__ void store8(void* base, long long at, int dtype, cons
 
 // LPH: lanes per head, the power of two at or above dim / 16.  U: heads per lane group in flight.
 template <class T, int LPH, int U>
-__global__ void __launch_bounds__(128) rope_append_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(128, sizeof(T) == 4 ? 4 : 6) rope_append_kernel(const RopeParams p) {
     constexpr int HPW = 32 / LPH;  // heads a warp takes at once
     const int lane = threadIdx.x & 31;
     const int u = lane & (LPH - 1);
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(128) rope_append_kernel(const RopeParams p) {
             if (lane == 0 && chunk == 0) report(p.status, KVP_STATUS_BAD_POSITION);
             continue;
         }
-        const bool cached = slot >= 0 && (p.num_slots == 0 || slot < p.num_slots);
+        const bool cached = slot >= 0 && slot < p.num_slots;
         if (slot >= 0 && !cached && lane == 0 && chunk == 0) report(p.status, KVP_STATUS_BAD_BLOCK);
         Vec8 c, s;
         if (on && ca >= 0) {
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(128) rope_append_kernel(const RopeParams p) {
 #pragma unroll
                     for (int off = 1; off < LPH; off <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
                     if (w && live) {
-                        const float r = 1.0f / sqrtf(ss * p.inv_dim + p.eps);
+                        const float r = rsqrtf(ss * p.inv_dim + p.eps);
                         Raw8<T> wa, wb;
                         wa.load_kept(static_cast<const T*>(w) + ea);
                         wb.load_kept(static_cast<const T*>(w) + eb);
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(128) rope_append_kernel(const RopeParams p) {
 template <class T, int LPH>
 int launch_rope(const RopeParams& p0, cudaStream_t s) {
     RopeParams p = p0;
-    constexpr int U = sizeof(T) == 4 ? 2 : 4;
+    constexpr int U = 2;
     constexpr int kWarps = 4;
     const int iters = (p.rows + 32 / LPH - 1) / (32 / LPH);  // warp iterations of a token
     // Few tokens: a token's heads are spread over several warps, so that the launch's latency is that of one head;
@@ -273,7 +273,7 @@ extern "C" KVP_API int kvp_rope_append(const kvp_rope_args* a, void* stream) {
             return fail(KVP_EINVAL, "v, k_cache, v_cache and slots go together");
         if (!(a->kv_dtype == KVP_DTYPE_F16 || a->kv_dtype == KVP_DTYPE_BF16))
             return fail(KVP_EINVAL, "pool dtype must be fp16 or bf16");
-        if (a->block_size < 1 || a->num_blocks < 1) return fail(KVP_EINVAL, "block_size and num_blocks bound the slots");
+        if (a->block_size < 1 || a->num_blocks < 1 || a->num_blocks > INT64_MAX / a->block_size) return fail(KVP_EINVAL, "block_size and num_blocks bound the slots");
         if (!aligned16(a->k_cache) || !aligned16(a->v_cache)) return fail(KVP_EINVAL, "pools must be 16-byte aligned");
     } else if (!a->k_out) {
         return fail(KVP_EINVAL, "the keys need k_out or a cache");
