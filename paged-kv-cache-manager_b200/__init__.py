@@ -614,6 +614,15 @@ def _call_on(idx, stream, fn, a):
         _check(fn(C.byref(a), ptr))
 
 
+def _size_on(idx, fn, a):
+    """A workspace size, which depends on the device."""
+    import torch
+    if torch._C._cuda_getDevice() == idx:
+        return fn(C.byref(a))
+    with torch.cuda.device(idx):
+        return fn(C.byref(a))
+
+
 def _new_on(stream, like, shape, dtype):
     """A tensor for an operator's results on the stream that fills it (the caching allocator's blocks belong to the
     stream they were taken on)."""
@@ -739,8 +748,7 @@ def shared_prefix_workspace_bytes(q, k_cache, block_tables, group_starts, num_he
     import torch
     a = PrefixArgs()
     _prefix_shape(a, q, k_cache, block_tables, group_starts, num_heads, kv_heads)
-    with torch.cuda.device(q.device):
-        need = int(lib().kvp_prefix_workspace_size(C.byref(a)))
+    need = _size_on(q.get_device(), _fn("kvp_prefix_workspace_size"), a)
     if need == 0 and last_error():
         raise ValueError(last_error())
     return need
@@ -777,8 +785,7 @@ def shared_prefix_attention(q, k_cache, v_cache, block_tables, seq_lens, prefix_
         raise ValueError("out must have the shape of q")
     a.out, a.out_dtype = _dev(out, "out"), _dtype_code(out)
     if workspace is None:
-        with torch.cuda.device(idx):
-            need = int(lib().kvp_prefix_workspace_size(C.byref(a)))
+        need = _size_on(idx, _fn("kvp_prefix_workspace_size"), a)
         if need:
             workspace = _new_on(stream, q, (need,), torch.uint8)
     if workspace is not None:
@@ -820,7 +827,8 @@ def beam_select(logits, scores, select: int, *, workspace=None, status=None, str
     uint8, allocated here unless given."""
     import torch
     idx = _gpu_of(logits, "logits")
-    _elsewhere(idx, scores=scores, workspace=workspace, status=status)
+    if scores.get_device() != idx or workspace is not None or status is not None:
+        _elsewhere(idx, scores=scores, workspace=workspace, status=status)
     ls, ss, st = logits.shape, scores.shape, logits.stride()
     if len(ss) != 2 or len(ls) != 2 or ls[0] != ss[0] * ss[1]:
         raise ValueError("logits must be [batch * beams][vocab] and scores [batch][beams]")
@@ -838,8 +846,7 @@ def beam_select(logits, scores, select: int, *, workspace=None, status=None, str
     if status is not None:
         a.status = _dev(status, "status")
     if workspace is None:
-        with torch.cuda.device(idx):
-            need = int(lib().kvp_beam_workspace_size(C.byref(a)))
+        need = _size_on(idx, _fn("kvp_beam_workspace_size"), a)
         if need == 0 and batch:
             raise ValueError(last_error())
         workspace = _new_on(stream, logits, (need,), torch.uint8)

@@ -7,8 +7,8 @@
 //   compute 4 * m * g * P * head_dim flops.
 // Up to about 128 rows the bytes take longer than the flops; beyond, the tensor cores and the exponentials bound it.
 //
-// Two launches.  prefix_kernel attends over the shared blocks and leaves partial results; own_kernel attends over each
-// sequence's own blocks, combines both and writes the output.
+// Three launches.  prefix_kernel attends over the shared blocks, own_kernel over each sequence's own blocks, beside it on
+// what it leaves of an SM; both leave partial results, which join_kernel joins.
 //
 // prefix_kernel: one CTA per SM takes an even share of the step's units -- a unit is one tile of 128 keys for one (group,
 // kv head, pair of row tiles) -- regardless of where groups and heads begin and end.  A row tile is as many whole members
@@ -23,6 +23,13 @@
 // than 2^14 (fp16) or 2^40 (bf16) since its last rescaling: P, O and the sum have one scale, so nothing is lost.
 // P is rounded to the pools' 16-bit type: the products' rounding errors (half a step each, independent) average out over
 // the keys and stay below the rounding of a 16-bit output; the sum is taken over the unrounded values in fp32.
+//
+// Measured, 32 query and 8 kv heads of 128, bf16: a pair of row tiles takes 3750 clocks per key tile, of which the matrix
+// products are 2050 and the exponentials the rest; starting (groups, table, first tiles) takes 12000 clocks, writing the
+// partial results 5000.  512 sequences over 2048 shared tokens and up to 100 own ones: 72 us (prefix_kernel alone 33, the
+// own parts alone 20, joining 10); 256 over 16384, up to 512 own: 150 us (80, 44, 9); 4 beams over 2048, 24 own: 16 us.
+// prefix_kernel leaves shared memory unused on purpose: with 224 KB instead of 192 the L1, which the own parts' loads go
+// through, shrinks to 28 KB, and the first two calls took 85 and 174 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -40,7 +47,7 @@ constexpr int kKeys = 128;         // keys per tile
 constexpr int kRows = 128;         // rows per tile: M of the MMA
 constexpr int kPrefixThreads = 352;  // 8 softmax warps, the MMA warp, the warps that load K (and Q) and V
 constexpr int kTmemCols = 512;
-constexpr int kPrefixLimit = 512;  // at most 128 registers a thread: own_kernel's CTAs fit beside it
+constexpr int kPrefixLimit = 512;  // at most 128 registers a thread: five of own_kernel's single warps fit beside a CTA
 
 // What joins a (sequence, kv head): partial rows of query head 0 begin at row0, and 256 further for each CTA before the
 // first of the span at pair_at (-1: nothing is shared); `parts` per CTA, `rows` apart.
@@ -58,8 +65,8 @@ struct PrefixParams {
     int2* spans;               // first and last CTA of each (group, kv head, pair), at its first row's (member, kv head)
     float2* part_ml;           // partial rows: (maximum in log2 units, sum)
     float* part_o;
-    OwnMeta* own_meta;         // of each (sequence, kv head), where the own parts are joined by a kernel of their own
-    float2* own_ml;            // own parts, a row per (sequence, query head)
+    OwnMeta* own_meta;         // of each (sequence, kv head)
+    float2* own_ml;            // own parts, own_parts rows per (sequence, query head)
     float* own_o;
     const void* q;
     const void* k_cache;
@@ -69,8 +76,8 @@ struct PrefixParams {
     long long wait_limit;
     int num_seqs, num_groups, nh, kvh, g, max_blocks, B, Bshift, run, runs, oob_row;
     int mt;                    // members per row tile
-    int own_parts;             // warps that share an own part, where the parts are joined by a kernel of their own
-    int bf16, out_dtype, ctas, own_ctas;  // ctas: prefix_kernel's
+    int own_parts;             // warps that share a (sequence, kv head)'s own tokens
+    int bf16, out_dtype, ctas;  // ctas: prefix_kernel's
     float sl2;
 };
 
@@ -420,7 +427,7 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
     __shared__ PrefixShared sh;
     extern __shared__ uint8_t dyn[];
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
-    // Slots of K and of V beside two query tiles: 160 KB in all.
+    // Slots of K and of V, beside two query tiles: 192 KB in all at head_dim 128, 176 KB at 64.
     constexpr int kSlotsK = D == 128 ? 2 : 4, kSlotsV = D == 128 ? 2 : 3;
     const uint32_t ring_k = base + 2 * kTile, ring_v = ring_k + kSlotsK * kTile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -732,51 +739,18 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
 }
 
 // ---------------------------------------------------------------- own parts
-// One CTA of four warps per (sequence, kv head) -- or, where those are few, a cluster of up to eight CTAs -- attends over
-// the sequence's own blocks, 16 tokens a warp at a time, combines the warps' results with the shared part's partial rows
-// and writes the output.  Bound by HBM, and by latency where the own parts are short, which most of them are: a warp takes K
-// and V from global memory straight into the registers of its matrix instructions, without a pipeline to fill and drain.
+// 1 to 8 single warps, which wait for nothing from each other, share the own tokens of a (sequence, kv head), 16 at a time.
+// Bound by HBM, and by latency where the own parts are short, which most of them are: a warp takes K and V from global memory
+// straight into the registers of its matrix instructions, without a pipeline to fill and drain.  Alone it takes 20 us at 512
+// sequences with up to 100 own tokens, 44 us at 256 with up to 512 (6.5 TB/s).  CTAs of four warps that also joined their
+// results with the shared part's took 42 and 71 us; clusters of eight such CTAs, where pairs are few, 19.2 us for the whole
+// call at 4 beams instead of 16.2.
 //   S^T[tokens x heads] = K Q^T:  a lane holds 8 neighbouring dims of a token's K (one 16-byte load); the sum over dims does
 //                                 not care for their order, so these are the dims of two steps, for K and Q alike.
 //   O^T[dims x heads] += V^T P^T: a lane holds 8 neighbouring dims of four tokens' V and pairs up two tokens' halves; the
 //                                 rows of the instruction are dims in an order of their own.  P^T by an 8 x 8 transposition.
 // The heads are the 8 columns of the instruction (NT times, for more than 8): as its 16 rows they took twice the
 // instructions and accumulators, and twice the time at head_dim 128.
-constexpr int kOwnWarps = 4;  // as many as a Fold takes at once
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// This CTA's shared address as seen in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
-}
-__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-
 // Four partial results (maximum, sum; four columns of the output) at a time, folded into what there is.  One with the maximum
 // -inf is nothing, and its columns may never have been written.
 struct Fold {
@@ -843,24 +817,24 @@ __device__ __forceinline__ SharedParts shared_parts(const PrefixParams& p, const
     return s;
 }
 
-// NT: groups of 8 query heads per kv head.  Apart: the own part is left for join_kernel.
-template <int D, class KV, int NT, bool Apart>
-__global__ void __launch_bounds__(Apart ? 32 : kOwnWarps * 32, Apart ? (NT == 1 ? 16 : 12) : NT == 1 ? 4 : 3) own_kernel(const PrefixParams p) {
+// NT: groups of 8 query heads per kv head.  Its inputs were written before prefix_kernel, which lets this kernel start once it
+// has waited for the kernels ahead; so nothing is waited for, but for the last CTA, through which join_kernel waits for the
+// shared part.
+template <int D, class KV, int NT>
+__global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const PrefixParams p) {
     using Tr = F16Traits<KV>;
     constexpr int NI = D / 32;   // 16-byte pieces of a row that a lane of four holds
     constexpr int NH = D / 64;   // and that a lane of eight holds
-    constexpr int ROWS = 8 * NT;
     griddep_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c4 = lane & 3;
-    const int ctas = Apart ? p.own_parts : static_cast<int>(cluster_size()), rank = Apart ? static_cast<int>(blockIdx.x) % ctas : static_cast<int>(cluster_rank());
-    const int item = static_cast<int>(blockIdx.x) / ctas;
+    const int lane = threadIdx.x, gid = lane >> 2, c4 = lane & 3;
+    const int item = static_cast<int>(blockIdx.x) / p.own_parts, rank = static_cast<int>(blockIdx.x) - item * p.own_parts;
     const int seq = item / p.kvh, h = item - seq * p.kvh;
     const int len = __ldg(p.lens + seq), pb = __ldg(p.prefix_blocks + seq);
     const long long nblk = (static_cast<long long>(len) + p.B - 1) / p.B;
     bool fine = len >= 1 && nblk <= p.max_blocks && pb >= 0 && static_cast<long long>(pb) * p.B <= len;
     const int own = fine ? len - pb * p.B : 0;
     const int32_t* trow = p.tables + static_cast<long long>(seq) * p.max_blocks + (fine ? pb : 0);
-    const int tiles = (own + 15) >> 4, stride = Apart ? ctas : ctas * kOwnWarps;
+    const int tiles = (own + 15) >> 4, stride = p.own_parts;
 
     // queries of head 8 nt + gid
     uint4 qr[NT][NI];
@@ -913,40 +887,39 @@ __global__ void __launch_bounds__(Apart ? 32 : kOwnWarps * 32, Apart ? (NT == 1 
         }
     };
     // The next tile's K is on its way as soon as this one's scores are there, its V as soon as this one's is used.
-    const int first_tile = Apart ? rank : rank * kOwnWarps + warp;
     {
-        const int row = row_of(first_tile);
+        const int row = row_of(rank);
         load_k(row);
         load_v(row);
     }
-    int row = row_of(first_tile + stride);
-    // meanwhile: the sequence's group, the last one that starts at or before it, 32 candidates a step
-    int lo = 0;
-    for (int n = p.num_groups; n > 1;) {
-        const int step = (n + 31) >> 5;
-        const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && __ldg(p.group_starts + lo + lane * step) <= seq);
-        const int k = below ? 31 - __clz(below) : 0;
-        lo += k * step;
-        n = min(step, n - k * step);
-    }
-    const Group grp = load_group(p, lo);
-    fine = fine && grp.start <= seq && seq < grp.start + grp.members && grp.blocks == pb;
-    OwnMeta meta = {0, -1, 1, 0, fine, 0};
-    if (fine && grp.ktiles > 0) {
-        const int member = seq - grp.start, member0 = member / (2 * p.mt) * 2 * p.mt, left = grp.members - member0;
-        meta.pair_at = static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(h) * grp.members + member0;
-        meta.row0 = 2LL * p.g * meta.pair_at + (member - member0) * p.g;  // two row tiles: one after the other
-        if (left <= p.mt) {  // one: the even and the odd key tiles'
-            meta.parts = 2;
-            meta.rows = left * p.g;
+    int row = row_of(rank + stride);
+    if (rank == 0) {  // meanwhile: the sequence's group, the last one that starts at or before it, 32 candidates a step
+        int lo = 0;
+        for (int n = p.num_groups; n > 1;) {
+            const int step = (n + 31) >> 5;
+            const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && __ldg(p.group_starts + lo + lane * step) <= seq);
+            const int k = below ? 31 - __clz(below) : 0;
+            lo += k * step;
+            n = min(step, n - k * step);
+        }
+        const Group grp = load_group(p, lo);
+        fine = fine && grp.start <= seq && seq < grp.start + grp.members && grp.blocks == pb;
+        OwnMeta meta = {0, -1, 1, 0, fine, 0};
+        if (fine && grp.ktiles > 0) {
+            const int member = seq - grp.start, member0 = member / (2 * p.mt) * 2 * p.mt, left = grp.members - member0;
+            meta.pair_at = static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(h) * grp.members + member0;
+            meta.row0 = 2LL * p.g * meta.pair_at + (member - member0) * p.g;  // two row tiles: one after the other
+            if (left <= p.mt) {  // one: the even and the odd key tiles'
+                meta.parts = 2;
+                meta.rows = left * p.g;
+            }
+        }
+        if (lane == 0) {
+            p.own_meta[item] = meta;
+            if (!fine && h == 0) report(p.status, KVP_STATUS_BAD_LEN);
         }
     }
-    SharedParts shared;
-    if (!Apart) {
-        griddep_wait();
-        shared = shared_parts(p, meta);
-    }
-    for (int tile = first_tile; tile < tiles; tile += stride) {
+    for (int tile = rank; tile < tiles; tile += stride) {
         const bool in0 = tile * 16 + gid < own, in1 = tile * 16 + gid + 8 < own;
         uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
@@ -1008,7 +981,7 @@ __global__ void __launch_bounds__(Apart ? 32 : kOwnWarps * 32, Apart ? (NT == 1 
         load_v(row);
         row = row_of(tile + 2 * stride);
     }
-    if constexpr (Apart) {  // a lane holds dims 64 i + 8 gid .. + 7 of heads 2 c4, 2 c4 + 1
+    {  // a lane holds dims 64 i + 8 gid .. + 7 of heads 2 c4, 2 c4 + 1
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -1018,9 +991,9 @@ __global__ void __launch_bounds__(Apart ? 32 : kOwnWarps * 32, Apart ? (NT == 1 
                 for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
                 const int j = 8 * nt + 2 * c4 + e;
                 if (j >= p.g) continue;
-                const long long row = (static_cast<long long>(seq) * p.nh + h * p.g + j) * ctas + rank;
+                const long long row = (static_cast<long long>(seq) * p.nh + h * p.g + j) * p.own_parts + rank;
                 if (gid == 0) p.own_ml[row] = make_float2(m[nt][e], sum);
-                if (first_tile >= tiles) continue;  // nothing: never read
+                if (rank >= tiles) continue;  // nothing, and its columns are not used
 #pragma unroll
                 for (int i = 0; i < NH; ++i)
 #pragma unroll
@@ -1028,68 +1001,12 @@ __global__ void __launch_bounds__(Apart ? 32 : kOwnWarps * 32, Apart ? (NT == 1 
                         *reinterpret_cast<float4*>(p.own_o + row * D + 64 * i + 8 * gid + 2 * t) =
                             make_float4(o[nt][i * 4 + t][e], o[nt][i * 4 + t][2 + e], o[nt][i * 4 + t + 1][e], o[nt][i * 4 + t + 1][2 + e]);
             }
-        if (rank == 0 && lane == 0) {
-            p.own_meta[item] = meta;
-            if (!fine && h == 0) report(p.status, KVP_STATUS_BAD_LEN);
-        }
-        // join_kernel waits for this kernel, and through its last CTA for the shared part
-        if (blockIdx.x == gridDim.x - 1) griddep_wait();
-        return;
     }
-    __shared__ float2 sm_ml[kOwnWarps][ROWS];
-    __shared__ __align__(16) float sm_o[kOwnWarps][ROWS][D];
-    // Each thread's outputs, four columns of a query head, are known by now: its first partial rows start on their way before
-    // the warps meet.
-    const int outs = p.g * (D / 4), at0 = rank * kOwnWarps * 32 + static_cast<int>(threadIdx.x);
-    const int with_tiles = min(ctas, (tiles + kOwnWarps - 1) / kOwnWarps);  // the first CTAs of the cluster
-    float2 pml[4];
-    float4 px[4];
-    if (at0 < outs) shared.load(p, at0 / (D / 4), D, at0 % (D / 4) * 4, 0, pml, px);
-    // this warp's heads into shared memory: a lane holds dims 64 i + 8 gid .. + 7 of heads 2 c4, 2 c4 + 1
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float sum = l[nt][e];
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            const int j = 8 * nt + 2 * c4 + e;
-            if (gid == 0) sm_ml[warp][j] = make_float2(m[nt][e], sum);
-#pragma unroll
-            for (int i = 0; i < NH; ++i)
-#pragma unroll
-                for (int t = 0; t < 4; t += 2)
-                    *reinterpret_cast<float4*>(&sm_o[warp][j][64 * i + 8 * gid + 2 * t]) =
-                        make_float4(o[nt][i * 4 + t][e], o[nt][i * 4 + t][2 + e], o[nt][i * 4 + t + 1][e], o[nt][i * 4 + t + 1][2 + e]);
-        }
-    cluster_sync();
-    for (int at = at0; at < outs; at += ctas * kOwnWarps * 32) {
-        const int j = at / (D / 4), col = (at - j * (D / 4)) * 4;
-        if (at != at0) shared.load(p, j, D, col, 0, pml, px);
-        Fold all;
-        for (int c = 0; c < with_tiles; ++c) {
-            float2 ml[4];
-            float4 x[4];
-#pragma unroll
-            for (int w = 0; w < kOwnWarps; ++w) {
-                ml[w] = ld_cluster2(map_rank(smem_u32(&sm_ml[w][j]), c));
-                x[w] = ld_cluster4(map_rank(smem_u32(&sm_o[w][j][col]), c));
-            }
-            all.add(ml, x);
-        }
-        const size_t row = static_cast<size_t>(seq) * p.nh + h * p.g + j;
-        all.add(pml, px);
-        for (int k0 = 4; k0 < shared.count; k0 += 4) {
-            shared.load(p, j, D, col, k0, pml, px);
-            all.add(pml, px);
-        }
-        store_out(p, row * D + col, fine ? all.o : make_float4(0.f, 0.f, 0.f, 0.f), fine ? 1.f / all.l : 0.f);
-    }
-    if (!fine && h == 0 && rank == 0 && threadIdx.x == 0) report(p.status, KVP_STATUS_BAD_LEN);
-    cluster_sync();  // others may still read this CTA's shared memory
+    if (blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
-// The own part and the shared part's partial rows: a thread folds four columns of a (sequence, query head).
+// The own parts and the shared part's partial rows: a thread folds four columns of a (sequence, query head).  Bound by the
+// partial rows' way through L2, and three latencies.
 template <int D>
 __global__ void __launch_bounds__(256) join_kernel(const PrefixParams p) {
     griddep_launch_dependents();
@@ -1112,7 +1029,7 @@ __global__ void __launch_bounds__(256) join_kernel(const PrefixParams p) {
             x[i] = some ? __ldcg(reinterpret_cast<const float4*>(p.own_o + r * D + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
     };
-    own_part(0);
+    own_part(0);  // on their way while the place of the others is looked up
     const SharedParts shared = shared_parts(p, meta);
     Fold all;
     all.add(ml, x);
@@ -1161,13 +1078,16 @@ kvp_attn_args whole_contexts(const kvp_prefix_args& a) {
     return w;
 }
 
-constexpr long long kOwnWaves = 16;
+// Warps an SM that own parts are split into at least: 16 is what its registers hold.  Half as many took 162 us at 256
+// sequences with up to 512 own tokens instead of 149 (twice as many 146); twice as many 74 us at 512 with up to 100 instead
+// of 72, four times 81, for the parts that join_kernel has to read.
+constexpr long long kOwnWarps = 16;
 
 struct PrefixPlan {
     bool shared = false;  // else the plain decode attention over every sequence's whole context
     size_t ml = 0, o = 0, meta = 0, own_ml = 0, own_o = 0, bytes = 0;
     int mt = 1, run = 8;
-    int own_parts = 0, own_ctas = 1;  // own parts joined apart: warps per (sequence, kv head), else CTAs
+    int own_parts = 1;
 };
 
 int gcd_of(int a, int b) { return b ? gcd_of(b, a % b) : a; }
@@ -1199,11 +1119,8 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
     pl->o = pl->ml + up256(parts * 8);
     // (the larger of both: where q or out are not aligned the other path runs in the same workspace)
     pl->meta = pl->o + up256(parts * a->head_dim * 4);
-    // Few (sequence, kv head) pairs: clusters share one, so that a long own part does not hang on four warps.
-    const long long items = static_cast<long long>(a->num_seqs) * a->kv_heads, sms = sm_count();
-    while (pl->own_ctas < 8 && items * pl->own_ctas * 2 <= sms * 3) pl->own_ctas *= 2;
-    if (pl->own_ctas == 1)
-        for (pl->own_parts = 1; pl->own_parts < 8 && items * pl->own_parts < sms * kOwnWaves;) pl->own_parts *= 2;
+    const long long items = static_cast<long long>(a->num_seqs) * a->kv_heads;
+    while (pl->own_parts < 8 && items * pl->own_parts < sm_count() * kOwnWarps) pl->own_parts *= 2;
     pl->own_ml = pl->meta + up256(static_cast<size_t>(a->num_seqs) * a->kv_heads * sizeof(kvpd::OwnMeta));
     pl->own_o = pl->own_ml + up256(rows * pl->own_parts * 8);
     pl->bytes = std::max(pl->bytes, pl->own_o + rows * pl->own_parts * a->head_dim * 4);
@@ -1222,50 +1139,40 @@ int encode_3d(CUtensorMap* map, int dtype, const void* base, const cuuint64_t (&
     return KVP_OK;
 }
 
-template <int D, class KV>
-int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, kvpd::PrefixParams p, cudaStream_t s) {
-    auto fn = &kvpd::prefix_kernel<D, KV>;
-    const int rc = allow_smem(reinterpret_cast<const void*>(fn));
-    if (rc != KVP_OK) return rc;
-    constexpr size_t tile = static_cast<size_t>(kvpd::kKeys) * D * 2;
-    // Its start -- barriers, tensor memory -- may overlap the kernel before it.
+// A launch that may start before the one ahead has ended.
+template <class... P>
+int launch_early(void (*fn)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const char* what, const P&... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(p.ctas));
-    cfg.blockDim = dim3(kvpd::kPrefixThreads);
-    cfg.dynamicSmemBytes = 1024 + (2 + (D == 128 ? 4 : 7)) * tile;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, fn, qm, km, vm, p), "shared prefix launch");
+    return cuda_status(cudaLaunchKernelEx(&cfg, fn, args...), what);
+}
+
+template <int D, class KV>
+int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, kvpd::PrefixParams p, cudaStream_t s) {
+    auto fn = &kvpd::prefix_kernel<D, KV>;
+    const int rc = allow_smem(reinterpret_cast<const void*>(fn));
+    if (rc != KVP_OK) return rc;
+    constexpr size_t tile = static_cast<size_t>(kvpd::kKeys) * D * 2;
+    return launch_early(fn, static_cast<unsigned>(p.ctas), kvpd::kPrefixThreads, 1024 + (2 + (D == 128 ? 4 : 7)) * tile, s, "shared prefix launch",
+                        qm, km, vm, p);
 }
 
 template <int D, class KV>
 int launch_own(const kvpd::PrefixParams& p, cudaStream_t s) {
-    const bool apart = p.own_parts > 0;
-    const unsigned items = static_cast<unsigned>(p.num_seqs) * static_cast<unsigned>(p.kvh), ctas = static_cast<unsigned>(p.own_ctas);
-    auto fn = p.g > 8 ? (apart ? &kvpd::own_kernel<D, KV, 2, true> : &kvpd::own_kernel<D, KV, 2, false>)
-                      : (apart ? &kvpd::own_kernel<D, KV, 1, true> : &kvpd::own_kernel<D, KV, 1, false>);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(items * (apart ? static_cast<unsigned>(p.own_parts) : ctas));
-    cfg.blockDim = dim3(apart ? 32 : kvpd::kOwnWarps * 32);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ctas;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = apart ? 1 : 2;
-    const int rc = cuda_status(cudaLaunchKernelEx(&cfg, fn, p), "own part launch");
-    if (rc != KVP_OK || !apart) return rc;
-    cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(p.num_seqs) * p.nh * (D / 4) + 255) / 256));
-    cfg.blockDim = dim3(256);
-    return cuda_status(cudaLaunchKernelEx(&cfg, &kvpd::join_kernel<D>, p), "join launch");
+    auto fn = p.g > 8 ? &kvpd::own_kernel<D, KV, 2> : &kvpd::own_kernel<D, KV, 1>;
+    const unsigned warps = static_cast<unsigned>(p.num_seqs) * static_cast<unsigned>(p.kvh) * static_cast<unsigned>(p.own_parts);
+    const int rc = launch_early(fn, warps, 32, 0, s, "own part launch", p);
+    if (rc != KVP_OK) return rc;
+    const long long threads = static_cast<long long>(p.num_seqs) * p.nh * (D / 4);
+    return launch_early(&kvpd::join_kernel<D>, static_cast<unsigned>((threads + 255) / 256), 256, 0, s, "join launch", p);
 }
 
 template <int D, class KV>
@@ -1355,7 +1262,6 @@ extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stre
     p.oob_row = static_cast<int>(rows);
     p.mt = pl.mt;
     p.own_parts = pl.own_parts;
-    p.own_ctas = pl.own_ctas;
     p.bf16 = a->kv_dtype == KVP_DTYPE_BF16;
     p.out_dtype = a->out_dtype;
     p.ctas = sm_count();
