@@ -70,6 +70,8 @@ class PagedEngine:
             kind = getattr(rot, "rope_type", "default")
             if "dynamic" in kind or kind == "longrope":  # frequencies that change with the length
                 raise ValueError(f"fused_rope needs fixed rotary frequencies; this model's are {kind}")
+            if self.hd % 16 or self.hd > 256 or rot.inv_freq.numel() % 8:
+                raise ValueError("fused_rope needs head_dim and the rotated part of it to be multiples of 16, at most 256")
 
     # ------------------------------------------------------------------ internals
     def _rope_table(self, positions: int) -> torch.Tensor:
@@ -237,6 +239,8 @@ class PagedEngine:
             raise ValueError("beam_search takes 1 to 32 beams (16 with eos), fewer than the vocabulary, and new_tokens >= 1")
         if len(set(rids)) != beams or any(self.kv.contains(r) for r in rids):
             raise ValueError("rids must be distinct and not in use")
+        if len(prompt) < 1:
+            raise ValueError("beam_search needs a prompt")
         logits = self.prefill(rids[0], prompt)
         if logits is None:
             return None

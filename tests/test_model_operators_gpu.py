@@ -215,6 +215,8 @@ def test_refusals(kvb):
     for rids, new, eos in (([], 1, None), (list(range(33)), 1, None), (list(range(17)), 1, 5), ([1, 1], 3, None), ([1], 0, None)):
         with pytest.raises(ValueError):
             eng.beam_search(rids, [1, 2, 3], new, eos)
+    with pytest.raises(ValueError):
+        eng.beam_search([1], [], 2)
     assert eng.kv.admit(4, 3)
     with pytest.raises(ValueError):
         eng.beam_search([3, 4], [1, 2, 3], 2)

@@ -302,3 +302,57 @@ def test_empty_batch_and_refusals(kvb, cuda):
         b.run(kvb, workspace=torch.empty(256, dtype=torch.uint8, device="cuda"))
     none = kvb.shared_prefix_attention(b.q[:0], b.k, b.v, b.tables[:0], b.lens[:0], b.prefix[:0], b.starts[:1], 8, 2)
     assert none.shape == (0, 8, 64)
+
+
+@pytest.mark.parametrize("groups,own,nh,kvh,D,t", [([(290, 3), (15, 0)], mixed, 16, 8, 128, "bf16"),  # a warp per (sequence, kv head)
+                                                   ([(310, 2)], few, 32, 8, 64, "fp16"),
+                                                   ([(80, 4)], mixed, 8, 8, 128, "fp16"),              # four warps
+                                                   ([(9, 1), (30, 6)], lambda r: r.integers(500, 900), 16, 1, 64, "bf16"),
+                                                   ([(2, 3)] * 32, few, 8, 2, 64, "fp16"),            # found by a warp alone
+                                                   ([(2, 3)] * 33, few, 8, 2, 64, "fp16"),            # and by the CTA
+                                                   ([(1, 0)] * 40, mixed, 8, 2, 128, "bf16")])         # nothing is shared
+def test_splits_of_the_own_parts(kvb, cuda, groups, own, nh, kvh, D, t):
+    b = Batch(groups, own, nh, kvh, D, 16, t, t, seed=len(groups) + nh)
+    b.check(b.run(kvb))
+
+
+def test_calls_behind_each_other(kvb, cuda):
+    """Every kernel may start before the one ahead has ended: calls on one workspace, whose queries, lengths and pools are
+    overwritten by kernels in between and whose output is read by the next, give what they give one at a time."""
+    import torch
+    b = Batch([(40, 6), (3, 9)], lambda r: r.integers(20, 200), 16, 4, 128, 16, seed=31)
+    ws = torch.empty(kvb.shared_prefix_workspace_bytes(b.q, b.k, b.tables, b.starts, 16, 4), dtype=torch.uint8, device="cuda")
+    qs = [torch.randn_like(b.q, dtype=torch.float32).to(b.q.dtype) for _ in range(6)]
+    lens, k = b.lens.clone(), b.k.clone()
+
+    def step(i):
+        b.lens.copy_(lens - i)
+        b.k.copy_(k).mul_(1.0 + i / 8)
+        b.q.copy_(qs[i])
+        x = b.run(kvb, workspace=ws)
+        return kvb.shared_prefix_attention(x, *b.args()[1:], workspace=ws, status=b.status)
+
+    alone = []
+    for i in range(6):
+        alone.append(step(i))
+        torch.cuda.synchronize()
+    for _ in range(5):
+        behind = [step(i) for i in range(6)]
+        torch.cuda.synchronize()
+        for x, y in zip(alone, behind):
+            assert torch.equal(x, y)
+    assert int(b.status.item()) == 0
+
+
+def test_pool_behind_32_bit_offsets(kvb, cuda):
+    """The same blocks at the end of pools of more than 2^32 elements: the same bits."""
+    import torch
+    b = Batch([(20, 12), (4, 3)], mixed, 32, 8, 128, 16, seed=12)
+    want = b.run(kvb)
+    nb = b.k.shape[0]
+    many = (1 << 32) // (16 * 8 * 128) + 1000
+    big = [torch.empty((many, 16, 8, 128), dtype=b.k.dtype, device="cuda") for _ in range(2)]
+    for x, y in zip(big, (b.k, b.v)):
+        x[-nb:].copy_(y)
+    got = kvb.shared_prefix_attention(b.q, *big, b.tables + (many - nb), b.lens, b.prefix, b.starts, 32, 8, status=b.status)
+    assert torch.equal(got, want) and int(b.status.item()) == 0

@@ -235,3 +235,24 @@ def test_refusals(kvb, cuda):
             call(**bad)
     with pytest.raises(ValueError):
         kvb.qk_norm_rope(q, k, pos, table, k_out=torch.empty(4, 2, 64, device="cuda"))
+
+
+def test_slots_behind_32_bit_offsets(kvb, cuda):
+    """Slots at the end of pools of more than 2^32 elements hold what the same call stores in a small pool."""
+    import torch
+    n, B, kvh, D = 40, 16, 8, 128
+    q, k, v = (torch.randn(n, h, D, device="cuda", dtype=torch.bfloat16) for h in (32, kvh, kvh))
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    table = kvb.rope_table(n, D)
+    slots = torch.randperm(3 * B, device="cuda")[:n].int()
+    many = (1 << 32) // (B * kvh * D) + 100
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    small = [torch.zeros(3, B, kvh, D, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    big = [torch.empty(many, B, kvh, D, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    for x in big:
+        x[-3:].zero_()
+    a = kvb.rope_append(q, k, v, pos, table, *small, slots, status=status)
+    b = kvb.rope_append(q, k, v, pos, table, *big, slots + (many - 3) * B, status=status)
+    assert torch.equal(a, b) and int(status.item()) == 0
+    for x, y in zip(small, big):
+        assert torch.equal(x, y[-3:])
