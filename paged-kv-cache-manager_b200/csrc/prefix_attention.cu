@@ -13,7 +13,9 @@
 // prefix_kernel: one CTA per SM takes an even share of the step's units -- a unit is one tile of 128 keys for one (group,
 // kv head, pair of row tiles) -- regardless of where groups and heads begin and end.  A row tile is as many whole members
 // as fit 128 rows (tcgen05's M).  Two warpgroups of softmax, one per accumulator pair in TMEM, take turns with the tensor
-// cores: while one exponentiates its scores, the MMAs of the other run.
+// cores: while one exponentiates its scores, the MMAs of the other run.  Exponentiating at the same time gains nothing: with
+// two score buffers of 64 keys each, which keep both at it, 256 sequences over 16384 tokens took 176 us instead of 148; with
+// a quarter of the exponentials as a polynomial on the FMA pipe 150.
 //   two row tiles:  the warpgroups take one tile each and every key tile; K and V are read once for 256 rows.
 //   one row tile:   both warpgroups take the same rows, one the even, the other the odd key tiles, so that the wait for a
 //                   tile's exponentials is covered by the other tile; they leave two partial results.
@@ -26,8 +28,8 @@
 //
 // Measured, 32 query and 8 kv heads of 128, bf16: a pair of row tiles takes 3750 clocks per key tile, of which the matrix
 // products are 2050 and the exponentials the rest; starting (groups, table, first tiles) takes 12000 clocks, writing the
-// partial results 5000.  512 sequences over 2048 shared tokens and up to 100 own ones: 72 us (prefix_kernel alone 33, the
-// own parts alone 20, joining 10); 256 over 16384, up to 512 own: 150 us (80, 44, 9); 4 beams over 2048, 24 own: 16 us.
+// partial results 5000.  512 sequences over 2048 shared tokens and up to 100 own ones: 71 us (prefix_kernel alone 33, the
+// own parts alone 20, joining 10); 256 over 16384, up to 512 own: 148 us (80, 44, 9); 4 beams over 2048, 24 own: 16 us.
 // prefix_kernel leaves shared memory unused on purpose: with 224 KB instead of 192 the L1, which the own parts' loads go
 // through, shrinks to 28 KB, and the first two calls took 85 and 174 us.
 #include <cuda.h>
@@ -209,26 +211,6 @@ __device__ __forceinline__ float exp2_unit(float x) {  // free to be moved, unli
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 2^x of a pair on the FMA pipe: x = n + f with n the nearest whole number (added as the exponent) and f in
-// [-1/2, 1/2], 2^f by the polynomial of degree 4 with the smallest largest relative error there (2.7e-6, found by the
-// Remez exchange), far below the rounding of P.  One pair in four goes this way: the special-function unit, at 16 results
-// a clock, would otherwise take as long as both matrix products of a tile.  What lies below 2^-126 stays there (the
-// exponent must not wrap), which no sum of this kernel notices.
-__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
-    const float2 v = unpack2(x);
-    const uint64_t y = pack2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
-    const uint64_t t = add2(y, pack2(12582912.f, 12582912.f));  // 1.5 * 2^23: n in the low bits
-    const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), y);
-    uint64_t q = pack2(0.00957010221f, 0.00957010221f);
-    q = fma2(q, f, pack2(0.0559178591f, 0.0559178591f));
-    q = fma2(q, f, pack2(0.240247443f, 0.240247443f));
-    q = fma2(q, f, pack2(0.693121791f, 0.693121791f));
-    q = fma2(q, f, pack2(0.999999285f, 0.999999285f));
-    const float2 qv = unpack2(q), tv = unpack2(t);
-    return pack2(__uint_as_float(__float_as_uint(qv.x) + (__float_as_uint(tv.x) << 23)),
-                 __uint_as_float(__float_as_uint(qv.y) + (__float_as_uint(tv.y) << 23)));
-}
-
 // ---------------------------------------------------------------- units
 // Units of a group: kv heads x pairs of row tiles x key tiles.  A group with a bad range or a bad block count has none.
 struct Group {
@@ -675,17 +657,10 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                             uint32_t pk[16];
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
-                                const uint64_t x = fma2(pack2(__uint_as_float(s[b][2 * i]), __uint_as_float(s[b][2 * i + 1])), scale2, ref2);
-                                uint64_t e;
-                                if (i % 4 == 3) {
-                                    e = exp2_poly2(x);
-                                } else {
-                                    const float2 v = unpack2(x);
-                                    e = pack2(exp2_unit(v.x), exp2_unit(v.y));
-                                }
-                                sum[i & 1] = add2(sum[i & 1], e);
-                                const float2 v = unpack2(e);
-                                pk[i] = Tr::pack(v.x, v.y);
+                                const float2 x = unpack2(fma2(pack2(__uint_as_float(s[b][2 * i]), __uint_as_float(s[b][2 * i + 1])), scale2, ref2));
+                                const float2 e = make_float2(exp2_unit(x.x), exp2_unit(x.y));
+                                sum[i & 1] = add2(sum[i & 1], pack2(e.x, e.y));
+                                pk[i] = Tr::pack(e.x, e.y);
                             }
                             tmem_st16(s_addr + h * 16, pk);
                         }
