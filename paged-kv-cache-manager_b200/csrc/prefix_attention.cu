@@ -11,8 +11,9 @@
 // what it leaves of an SM; both leave partial results, which join_kernel joins.
 //
 // prefix_kernel: one CTA per SM takes an even share of the step's units -- a unit is one tile of 128 keys for one (group,
-// kv head, pair of row tiles) -- regardless of where groups and heads begin and end.  A row tile is as many whole members
-// as fit 128 rows (tcgen05's M).  Two warpgroups of softmax, one per accumulator pair in TMEM, take turns with the tensor
+// kv head, pair of row tiles), of fewer where the blocks' size shares no factor of 8 with it: as many whole blocks as fit,
+// copied one by one (16 groups with blocks of 5 tokens: 50 us, of 16 tokens 47; by whole contexts 916) -- regardless of where
+// groups and heads begin and end.  A row tile is as many whole members as fit 128 rows (tcgen05's M).  Two warpgroups of softmax, one per accumulator pair in TMEM, take turns with the tensor
 // cores: while one exponentiates its scores, the MMAs of the other run.  Exponentiating at the same time gains nothing: with
 // two score buffers of 64 keys each, which keep both at it, 256 sequences over 16384 tokens took 176 us instead of 148; with
 // a quarter of the exponentials as a polynomial on the FMA pipe 150.
@@ -78,6 +79,7 @@ struct PrefixParams {
     long long wait_limit;
     int num_seqs, num_groups, nh, kvh, g, max_blocks, B, Bshift, run, runs, oob_row;
     int mt;                    // members per row tile
+    int keys;                  // keys that a tile holds: 128, or as many whole blocks as fit
     int own_parts;             // warps that share a (sequence, kv head)'s own tokens
     int bf16, out_dtype, ctas;  // ctas: prefix_kernel's
     float sl2;
@@ -229,7 +231,8 @@ __device__ __forceinline__ Group load_group(const PrefixParams& p, int gi) {
         if (b > 0 && b <= p.max_blocks) r.blocks = b;
     }
     r.pairs = (r.members + 2 * p.mt - 1) / (2 * p.mt);
-    r.ktiles = static_cast<int>((static_cast<long long>(r.blocks) * p.B + kKeys - 1) / kKeys);
+    const long long last = static_cast<long long>(r.blocks) * p.B + p.keys - 1;
+    r.ktiles = static_cast<int>(p.keys == kKeys ? last / kKeys : last / p.keys);
     return r;
 }
 
@@ -442,6 +445,14 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
     // The kernels behind start only once every CTA here has its own: one of them that takes tensor memory while it waits
     // for this kernel could otherwise keep it from ever getting any.
     griddep_wait();
+    if (p.keys < kKeys) {  // rows of V that no copy fills: their weights are zero, and so have they to be
+        const int words = (kKeys - p.keys) * 8;  // of 16 bytes
+        for (int i = threadIdx.x; i < words * NCH * kSlotsV; i += kPrefixThreads) {
+            const uint32_t to = ring_v + (i / words) * kCol + p.keys * 128 + (i % words) * 16;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
     if (warp == 8) {
         tmem_alloc(smem_u32(&sh.tmem));
         griddep_launch_dependents();
@@ -476,11 +487,11 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
         int loaded = 0, queries = 0;  // tiles and query loads issued
         while (ok && list.next(p, w)) {
             const int32_t* trow = p.tables + static_cast<long long>(w.start) * p.max_blocks;
+            // The pool row of a run of a tile; for the runs of a lane's own, looked up a tile ahead, so that the table's latency is
+            // past when it is needed.
             const int run = lane / NCH, c = lane - run * NCH;
-            // The pool row of this lane's run of a tile, looked up a tile ahead, so that the table's latency is past when it is
-            // needed.
-            auto row_of = [&](int kt) {
-                const int tok = kt * kKeys + run * p.run;
+            auto row_at = [&](int kt, int run) {
+                const int tok = kt * p.keys + run * p.run;
                 if (run >= p.runs || tok >= w.tokens || kt >= w.k0 + w.n) return p.oob_row;  // zeros behind the shared tokens
                 const int bi = p.Bshift >= 0 ? tok >> p.Bshift : tok / p.B;
                 const int blk = __ldg(trow + bi);
@@ -488,6 +499,7 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                 report(p.status, KVP_STATUS_BAD_BLOCK);
                 return p.oob_row;
             };
+            auto row_of = [&](int kt) { return row_at(kt, run); };
             int row = row_of(w.k0);
             if (v == 0) {  // queries, once the previous stretch's products have read theirs
                 if (queries > 0) ok = warp_wait(&sh.q_free, (queries - 1) & 1, p, sh);
@@ -507,11 +519,14 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                 const int next_row = row_of(w.k0 + j + 1);
                 if (loaded >= slots && !(ok = warp_wait(&sh.empty[v][at.slot], at.parity ^ 1u, p, sh))) break;
                 const uint32_t bar = smem_u32(&sh.full[v][at.slot]);
-                if (lane == 0) mbar_arrive_expect_tx(bar, kTile);
+                if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(p.keys) * NCH * 128u);
                 __syncwarp();
                 if (run < p.runs)
                     tma_load_3d(ring + at.slot * kTile + c * kCol + static_cast<uint32_t>(run * p.run) * 128u, map, bar, c * 64,
                                 w.head, row);
+                for (int i = 32 + lane; i < p.runs * NCH; i += 32)  // small blocks: more runs than lanes
+                    tma_load_3d(ring + at.slot * kTile + (i % NCH) * kCol + static_cast<uint32_t>(i / NCH * p.run) * 128u, map, bar,
+                                i % NCH * 64, w.head, row_at(w.k0 + j, i / NCH));
                 row = next_row;
                 at = at.next(slots);
                 ++loaded;
@@ -622,7 +637,7 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                 ++uses;
                 if (busy) {
                     tc_fence_after();
-                    const int valid = w.tokens - (w.k0 + j) * kKeys;
+                    const int valid = min(w.tokens - (w.k0 + j) * p.keys, p.keys);
                     // The row's maximum, then the exponentials, the scores read twice and 32 at a time: loops, not one long
                     // stretch of code, whose way through the instruction caches cost a launch 10 us.
                     uint32_t s[2][32];
@@ -1061,7 +1076,7 @@ constexpr long long kOwnWarps = 16;
 struct PrefixPlan {
     bool shared = false;  // else the plain decode attention over every sequence's whole context
     size_t ml = 0, o = 0, meta = 0, own_ml = 0, own_o = 0, bytes = 0;
-    int mt = 1, run = 8;
+    int mt = 1, run = 8, keys = 0;
     int own_parts = 1;
 };
 
@@ -1077,12 +1092,18 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
     kvp_attn_args w = whole_contexts(*a);
     if (a->num_seqs == 0) return KVP_OK;
     if (a->kv_dtype == KVP_DTYPE_F32) return KVP_OK;
-    // The shared kernel's tiles are 8-row atoms of 64 elements of one 16-bit type.
+    // The shared kernel's tiles hold 128 keys, copied in runs of at least 8 within a block; of blocks that have no such runs, as
+    // many whole ones as fit.
     pl->run = gcd_of(a->block_size, kvpd::kKeys);
+    pl->keys = kvpd::kKeys;
+    if (pl->run < 8) {
+        pl->run = a->block_size;
+        pl->keys = kvpd::kKeys / a->block_size * a->block_size;  // 0: none fits
+    }
     AttnPlan whole;
     const int rc = plan_attention(w, true, &whole);
     if (rc != KVP_OK) return rc;
-    pl->shared = (a->head_dim == 64 || a->head_dim == 128) && a->q_dtype == a->kv_dtype && pl->run >= 8 && aligned16(a->q) &&
+    pl->shared = (a->head_dim == 64 || a->head_dim == 128) && a->q_dtype == a->kv_dtype && pl->keys > 0 && aligned16(a->q) &&
                  aligned16(a->out) && static_cast<long long>(a->num_seqs) * a->kv_heads <= (1LL << 27) &&
                  static_cast<long long>(a->max_blocks) * a->block_size <= 0x7fffffffLL;  // tokens of a table row, 32 bits below
     pl->bytes = whole.ws_bytes;
@@ -1233,7 +1254,8 @@ extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stre
     if ((a->block_size & (a->block_size - 1)) == 0)
         for (p.Bshift = 0; (1 << p.Bshift) < a->block_size;) ++p.Bshift;
     p.run = pl.run;
-    p.runs = kvpd::kKeys / pl.run;
+    p.keys = pl.keys;
+    p.runs = pl.keys / pl.run;
     p.oob_row = static_cast<int>(rows);
     p.mt = pl.mt;
     p.own_parts = pl.own_parts;

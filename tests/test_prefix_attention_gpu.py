@@ -356,3 +356,13 @@ def test_pool_behind_32_bit_offsets(kvb, cuda):
         x[-nb:].copy_(y)
     got = kvb.shared_prefix_attention(b.q, *big, b.tables + (many - nb), b.lens, b.prefix, b.starts, 32, 8, status=b.status)
     assert torch.equal(got, want) and int(b.status.item()) == 0
+
+
+@pytest.mark.parametrize("groups,nh,kvh,D,B,t", [([(70, 60), (3, 9)], 8, 2, 128, 5, "bf16"), ([(9, 200)], 32, 8, 64, 1, "fp16"),
+                                                 ([(40, 7)], 16, 4, 128, 33, "fp16"), ([(6, 3), (2, 0), (80, 2)], 32, 4, 64, 100, "bf16"),
+                                                 ([(5, 40)], 8, 2, 128, 12, "bf16"), ([(7, 30)], 14, 2, 64, 7, "fp16"),
+                                                 ([(20, 2)], 8, 2, 64, 127, "bf16"), ([(20, 2)], 8, 2, 64, 130, "bf16")])
+def test_blocks_of_odd_sizes(kvb, cuda, groups, nh, kvh, D, B, t):
+    """Tiles of as many whole blocks as fit 128 keys (none of 130 tokens)."""
+    b = Batch(groups, mixed, nh, kvh, D, B, t, t, seed=B)
+    b.check(b.run(kvb))
