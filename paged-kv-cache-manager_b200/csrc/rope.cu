@@ -99,7 +99,7 @@ __device__ __forceinline__ void store8(void* base, long long at, int dtype, cons
 
 // LPH: lanes per head, the power of two at or above dim / 16.  U: heads per lane group in flight.
 // A long prompt (16384 tokens, 32 + 8 + 8 heads of 128, norms): 411 MB in 82 us, 5.0 TB/s, 77% of a copy's rate, with the
-// instructions (290 a warp for 4 heads of 128) taking 60% of the issue slots.  Two heads in flight and six CTAs an SM: four
+// instructions (270 a warp for 4 heads of 128) taking 64% of the issue slots.  Two heads in flight and six CTAs an SM: four
 // heads and five CTAs took 88 us; a coefficient form of norm and rotation in paired operations took fewer instructions,
 // but 150 registers and 114 us; a token's rows spread over three warps 104 us, for its position and table read thrice.
 // A decode step (1 to 256 tokens) takes 2.5 to 3.4 us on the GPU, the latencies of position, table row and heads in turn.
