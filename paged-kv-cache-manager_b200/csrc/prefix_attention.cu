@@ -27,9 +27,9 @@
 // P is rounded to the pools' 16-bit type: the products' rounding errors (half a step each, independent) average out over
 // the keys and stay below the rounding of a 16-bit output; the sum is taken over the unrounded values in fp32.
 //
-// Measured, 32 query and 8 kv heads of 128, bf16: a pair of row tiles takes 3750 clocks per key tile, of which the matrix
-// products are 2050 and the exponentials the rest; starting (groups, table, first tiles) takes 12000 clocks, writing the
-// partial results 5000.  512 sequences over 2048 shared tokens and up to 100 own ones: 71 us (prefix_kernel alone 33, the
+// Measured, 32 query and 8 kv heads of 128, bf16: a pair of row tiles takes 3750 clocks per key tile (4000 beside the own
+// parts), of which the matrix products are 2050 and the exponentials the rest; starting (groups, table, first tiles) takes
+// 12000 clocks, writing the partial results 5000 to 8000.  512 sequences over 2048 shared tokens and up to 100 own ones: 71 us (prefix_kernel alone 33, the
 // own parts alone 20, joining 10); 256 over 16384, up to 512 own: 148 us (80, 44, 9); 4 beams over 2048, 24 own: 16 us.
 // prefix_kernel leaves shared memory unused on purpose: with 224 KB instead of 192 the L1, which the own parts' loads go
 // through, shrinks to 28 KB, and the first two calls took 85 and 174 us.
