@@ -607,8 +607,10 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                     if (more) done_k();
                 }
                 if (ok) {
+                    // Only to a warpgroup that has a tile here: its own P gates the next stretch's products, so this barrier
+                    // never completes twice before it has looked.  One without a tile would be gated by nothing.
                     tc_commit(smem_u32(&sh.o_full[0]));
-                    tc_commit(smem_u32(&sh.o_full[1]));
+                    if (two || w.n > 1) tc_commit(smem_u32(&sh.o_full[1]));
                     tc_commit(smem_u32(&sh.q_free));
                 }
                 ++seg;
@@ -625,7 +627,7 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes per warp, in bits 16 and up
         const uint32_t s_addr = tmem + lanes + t * kKeys, o_addr = tmem + lanes + kO + t * D;
         bool ok = true;
-        int uses = 0, seg = 0;
+        int uses = 0, seg = 0;  // tiles, and stretches in which this warpgroup has some
         while (ok && list.next(p, w)) {
             const bool two = w.rows1 > 0;
             const int rows = two && t ? w.rows1 : w.rows0;
@@ -693,8 +695,11 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                 __syncwarp();
             }
             if (!ok) break;
-            if (!(ok = warp_wait(&sh.o_full[t], seg & 1, p, sh))) break;
-            ++seg;
+            const bool some = two || t < w.n;
+            if (some) {
+                if (!(ok = warp_wait(&sh.o_full[t], seg & 1, p, sh))) break;
+                ++seg;
+            }
             if (threadIdx.x == 0) {
                 if (w.k0 == 0) p.spans[w.pair_at].x = cta;
                 if (w.k0 + w.n == w.ktiles) p.spans[w.pair_at].y = cta;
@@ -703,7 +708,7 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                 tc_fence_after();
                 const long long r0 = w.part_row + (t ? w.rows0 : 0) + row;
                 if (row < rows) p.part_ml[r0] = make_float2(m, l);
-                if (two || t < w.n) {
+                if (some) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];

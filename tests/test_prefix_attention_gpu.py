@@ -366,3 +366,17 @@ def test_blocks_of_odd_sizes(kvb, cuda, groups, nh, kvh, D, B, t):
     """Tiles of as many whole blocks as fit 128 keys (none of 130 tokens)."""
     b = Batch(groups, mixed, nh, kvh, D, B, t, t, seed=B)
     b.check(b.run(kvb))
+
+
+@pytest.mark.parametrize("groups,nh,kvh,D", [([(100, 500)] + [(2, 1)] * 40, 32, 8, 128), ([(2, 1)] * 300, 8, 8, 64),
+                                             ([(3, 8), (2, 9), (2, 1), (2, 1), (4, 17), (2, 2)] * 30, 16, 8, 64)])
+def test_groups_of_one_key_tile(kvb, cuda, groups, nh, kvh, D):
+    """CTAs with stretch after stretch of a single key tile (and of one, two and three in turn), behind a long one: one
+    warpgroup has nothing to do in most of them and falls behind the other by as much as it likes."""
+    import torch
+    b = Batch(groups, few, nh, kvh, D, 16, seed=len(groups))
+    first = b.run(kvb)
+    b.check(first)
+    for _ in range(20):
+        assert torch.equal(b.run(kvb), first)
+    assert int(b.status.item()) == 0
