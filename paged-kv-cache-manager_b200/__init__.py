@@ -642,6 +642,8 @@ def _token_stride(t, name, shape):
     st = t.stride()
     if (st[2] != 1 and shape[2] > 1) or (st[1] != shape[2] and shape[1] > 1):
         raise ValueError(f"{name}: a token's heads must be contiguous")
+    if shape[0] > 1 and st[0] < shape[1] * shape[2]:  # one row for several tokens; a stride of 0 means contiguous below
+        raise ValueError(f"{name}: the rows of different tokens must not overlap")
     return st[0] if shape[0] > 1 else shape[1] * shape[2]
 
 

@@ -214,3 +214,20 @@ def test_reorder_refuses_and_changes_nothing(kvb):
     assert before == ([mgr.block_table(r) for r in (0, 1)], mgr.stats()) and mgr.validate() == ""
     assert kvb.lib().kvp_mgr_reorder(None, None, None, 0) == kvb.KVP_EINVAL
     assert kvb.lib().kvp_mgr_reorder(mgr.handle, None, None, -1) == kvb.KVP_EINVAL
+
+
+@pytest.mark.parametrize("shape,strides", [((4, 8, 64), (0, 64, 1)), ((2, 8, 64), (0, 64, 1)), ((4, 8, 64), (256, 64, 1)),
+                                           ((4, 1, 64), (0, 64, 1)), ((4, 1, 64), (32, 64, 1))])
+def test_rows_that_several_tokens_share_are_refused(kvb, shape, strides):
+    """One row expanded over the tokens, or rows that run into each other: below, a stride of 0 stands for contiguous rows,
+    which the storage does not hold."""
+    import torch
+    with pytest.raises(ValueError):
+        kvb._token_stride(torch.zeros(4096).as_strided(shape, strides), "q", torch.Size(shape))
+
+
+def test_strides_that_are_fine(kvb):
+    import torch
+    stride = lambda t: kvb._token_stride(t, "q", t.shape)  # noqa: E731
+    assert stride(torch.zeros(4, 8, 64)) == 512 and stride(torch.zeros(4, 1024)[:, 256:768].view(4, 8, 64)) == 1024
+    assert stride(torch.zeros(8, 64).expand(1, 8, 64)) == 512 and stride(torch.zeros(0, 8, 64)) == 512

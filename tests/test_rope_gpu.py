@@ -256,3 +256,20 @@ def test_slots_behind_32_bit_offsets(kvb, cuda):
     assert torch.equal(a, b) and int(status.item()) == 0
     for x, y in zip(small, big):
         assert torch.equal(x, y[-3:])
+
+
+def test_rows_that_several_tokens_share_are_refused(kvb, cuda):
+    """Inputs and outputs that are expanded over the tokens hold one row, not as many as there are tokens."""
+    import torch
+    q, k, v, pos, _, _ = _inputs(4, 8, 2, 64, torch.bfloat16, 4, False, False)
+    table = kvb.rope_table(300, 64)
+    pools = [torch.zeros((4, 1, 2, 64), device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    slots = torch.arange(4, dtype=torch.int32, device="cuda")
+    one = lambda t: t[:1].clone().expand(4, -1, -1)  # noqa: E731
+    for bad in (dict(q=one(q)), dict(k=one(k)), dict(v=one(v)), dict(q_out=one(q)), dict(k_out=one(k))):
+        with pytest.raises(ValueError, match="overlap"):
+            kvb.rope_append(**{**dict(q=q, k=k, v=v, positions=pos, table=table, k_cache=pools[0], v_cache=pools[1],
+                                      slots=slots), **bad})
+    for bad in (dict(q=one(q)), dict(k=one(k)), dict(q_out=one(q)), dict(k_out=one(k))):
+        with pytest.raises(ValueError, match="overlap"):
+            kvb.qk_norm_rope(**{**dict(q=q, k=k, positions=pos, table=table), **bad})
