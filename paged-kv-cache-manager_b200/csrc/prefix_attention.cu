@@ -50,6 +50,9 @@ constexpr int kKeys = 128;         // keys per tile
 constexpr int kRows = 128;         // rows per tile: M of the MMA
 constexpr int kPrefixThreads = 352;  // 8 softmax warps, the MMA warp, the warps that load K (and Q) and V
 constexpr int kTmemCols = 512;
+// Most tokens of a table row: places are 32-bit numbers, and those of the tiles that are looked up ahead lie up to 300
+// behind the row's end.
+constexpr long long kPrefixTokens = (1LL << 31) - 1024;
 constexpr int kPrefixLimit = 512;  // at most 128 registers a thread: five of own_kernel's single warps fit beside a CTA
 
 // What joins a (sequence, kv head): partial rows of query head 0 begin at row0, and 256 further for each CTA before the
@@ -1110,7 +1113,7 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
     if (rc != KVP_OK) return rc;
     pl->shared = (a->head_dim == 64 || a->head_dim == 128) && a->q_dtype == a->kv_dtype && pl->keys > 0 && aligned16(a->q) &&
                  aligned16(a->out) && static_cast<long long>(a->num_seqs) * a->kv_heads <= (1LL << 27) &&
-                 static_cast<long long>(a->max_blocks) * a->block_size <= 0x7fffffffLL;  // tokens of a table row, 32 bits below
+                 static_cast<long long>(a->max_blocks) * a->block_size <= kvpd::kPrefixTokens;
     pl->bytes = whole.ws_bytes;
     if (!pl->shared) return KVP_OK;
     const size_t rows = static_cast<size_t>(a->num_seqs) * a->num_heads;

@@ -231,3 +231,13 @@ def test_strides_that_are_fine(kvb):
     stride = lambda t: kvb._token_stride(t, "q", t.shape)  # noqa: E731
     assert stride(torch.zeros(4, 8, 64)) == 512 and stride(torch.zeros(4, 1024)[:, 256:768].view(4, 8, 64)) == 1024
     assert stride(torch.zeros(8, 64).expand(1, 8, 64)) == 512 and stride(torch.zeros(0, 8, 64)) == 512
+
+
+def test_prefix_table_rows_near_32_bits(kvb):
+    """A table row of nearly 2^31 tokens, whose last tiles' places would pass 32 bits, goes the way of longer ones: it needs
+    the same workspace."""
+    size = lambda blocks: kvb.lib().kvp_prefix_workspace_size(C.byref(_prefix(kvb, num_seqs=2000, max_blocks=blocks)))  # noqa: E731
+    longer = size(1 << 27)
+    assert 0 < longer < size((1 << 27) - 64) == size(10)
+    for blocks in ((1 << 27) - 1, (1 << 27) - 20, (1 << 27) - 63):
+        assert size(blocks) == longer
