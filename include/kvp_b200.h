@@ -197,10 +197,10 @@ KVP_API int kvp_paged_attention_noalloc(const kvp_attn_args* a, void* stream);
  * A sequence that breaks these rules, or whose length is invalid, gets zeros and sets KVP_STATUS_BAD_LEN.
  * Types, head shapes and layouts as in kvp_paged_attention.  Sharing takes head_dim 64 and 128, queries of the pools'
  * 16-bit dtype, block sizes up to 128 or multiples of 8, q and out on 16-byte boundaries, num_seqs * kv_heads <= 2^27 and
- * max_blocks * block_size <= 2^31 - 1024; over the shared keys it rounds the probabilities to the pools' dtype before the
- * product with V (sums in fp32).  Every other call attends over each sequence's whole context, as
- * kvp_paged_attention does.  The workspace (256-byte aligned) needs no initial value and keeps none; calls that overlap
- * on the GPU need one each. */
+ * max_blocks * block_size <= 2^31 - 1024; every other call attends over each sequence's whole context, as
+ * kvp_paged_attention does.  The probabilities go into the product with V as a part and a rest of the pools' dtype, sums
+ * are fp32, as there.  The workspace (256-byte aligned) needs no initial value and keeps none; calls that overlap on the
+ * GPU need one each. */
 typedef struct kvp_prefix_args {
     const void* q;
     const void* k_cache; /* this layer's pools */

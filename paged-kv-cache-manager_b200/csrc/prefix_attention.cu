@@ -21,11 +21,14 @@
 //   one row tile:   both warpgroups take the same rows, one the even, the other the odd key tiles, so that the wait for a
 //                   tile's exponentials is covered by the other tile; they leave two partial results.
 // Scores S and accumulators O live in TMEM (S0, S1 at columns 0 and 128, O0, O1 at 256 and 256 + head_dim); the
-// probabilities P overwrite S as 16-bit pairs and are the A operand of the second product straight from TMEM.  A thread
+// probabilities P overwrite S as 16-bit numbers and are the A operand of the second product straight from TMEM.  A thread
 // owns one row: the running maximum and sum need no exchange.  O is rescaled only when a row's maximum has grown by more
 // than 2^14 (fp16) or 2^40 (bf16) since its last rescaling: P, O and the sum have one scale, so nothing is lost.
-// P is rounded to the pools' 16-bit type: the products' rounding errors (half a step each, independent) average out over
-// the keys and stay below the rounding of a 16-bit output; the sum is taken over the unrounded values in fp32.
+// P is kept as a part and a rest of the pools' 16-bit type each, as the own parts and the decode attention keep it: the two
+// products with V hold 16 (bf16) or 22 (fp16) bits of each weight, and the output's only rounding that counts is its own.
+// With one 16-bit number each the weights' roundings were as large as a bf16 output's (1.66e-3 against 64 bits became
+// 2.3e-3, relative to all outputs' size 1e-4 became 2.5e-3), and an fp32 output held no more.  It costs half of the tensor
+// cores' work on top: 16 groups 46.9 -> 51.9 us, 512 samples 71.2 -> 78.7, 256 over 16384 154.9 -> 186.4, 4 beams the same.
 //
 // Measured, 32 query and 8 kv heads of 128, bf16: a pair of row tiles takes 3750 clocks per key tile (4000 beside the own
 // parts), of which the matrix products are 2050 and the exponentials the rest; starting (groups, table, first tiles) takes
@@ -595,8 +598,11 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                             if (!ok) break;
                             tc_fence_after();
 #pragma unroll
-                            for (int s = half * 4; s < half * 4 + 4; ++s)
-                                mma_ts(tmem + kO + t * D, tmem + t * kKeys + s * 8, v + s * (2048 >> 4), kDescHi, pv_desc, add || s > 0);
+                            for (int s = half * 4; s < half * 4 + 4; ++s) {
+                                const uint32_t at = tmem + t * kKeys + s * 16;
+                                mma_ts(tmem + kO + t * D, at, v + s * (2048 >> 4), kDescHi, pv_desc, add || s > 0);
+                                mma_ts(tmem + kO + t * D, at + 8, v + s * (2048 >> 4), kDescHi, pv_desc, true);
+                            }
                         }
                         if (!ok) break;
                         if (more) {
@@ -669,20 +675,26 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                     for (int half = 0; half < 2; ++half) {
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
-                            // P's columns 16 h .. lie in score columns that are in registers
+                            // P takes the place of scores that are in registers: of each 16 keys 8 columns of 16-bit
+                            // parts, then 8 of the rests
                             const int h = half * 2 + b;
                             tmem_wait_ld(s[b]);
                             if (h < 3) tmem_ld32(s_addr + (h + 1) * 32, s[b ^ 1]);
                             mask_keys(s[b], valid - h * 32);
-                            uint32_t pk[16];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const float2 x = unpack2(fma2(pack2(__uint_as_float(s[b][2 * i]), __uint_as_float(s[b][2 * i + 1])), scale2, ref2));
-                                const float2 e = make_float2(exp2_unit(x.x), exp2_unit(x.y));
-                                sum[i & 1] = add2(sum[i & 1], pack2(e.x, e.y));
-                                pk[i] = Tr::pack(e.x, e.y);
+                            for (int k = 0; k < 32; k += 16) {
+                                uint32_t pk[16];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const float2 x = unpack2(fma2(
+                                        pack2(__uint_as_float(s[b][k + 2 * i]), __uint_as_float(s[b][k + 2 * i + 1])), scale2, ref2));
+                                    const float2 e = make_float2(exp2_unit(x.x), exp2_unit(x.y));
+                                    sum[i & 1] = add2(sum[i & 1], pack2(e.x, e.y));
+                                    pk[i] = Tr::pack(e.x, e.y);
+                                    pk[8 + i] = Tr::pack(e.x - Tr::unpack_lo(pk[i]), e.y - Tr::unpack_hi(pk[i]));
+                                }
+                                tmem_st16(s_addr + h * 32 + k, pk);
                             }
-                            tmem_st16(s_addr + h * 16, pk);
                         }
                         tmem_wait_st();
                         tc_fence_before();

@@ -380,3 +380,31 @@ def test_groups_of_one_key_tile(kvb, cuda, groups, nh, kvh, D):
     for _ in range(20):
         assert torch.equal(b.run(kvb), first)
     assert int(b.status.item()) == 0
+
+
+def _check_close(b, got, scale=None, lift=0):
+    """The module's account with weights kept as two 16-bit numbers, a part and the rest: off by at most u^2, and in fp16 by
+    2^-25 of the largest where the rest lies below the type's smallest steps (2^-25 - lift, where the largest weight is
+    represented by 2^lift)."""
+    import torch
+    want, mag, err, top = b.reference(scale)
+    n = b.lens.double()[:, None, None]
+    u = torch.finfo(b.k.dtype).eps / 2
+    tol = want.abs() * (torch.finfo(got.dtype).eps / 2) + (u * u + 4 * err + 2.0 ** -15 + 2 * n * 2.0 ** -24) * mag
+    if b.k.dtype == torch.float16:
+        tol = tol + n * 2.0 ** (-25 - lift) * top
+    if got.dtype == torch.float16:
+        tol = tol + 2.0 ** -25  # the output's smallest step
+    assert bool(torch.isfinite(got).all()) and int(b.status.item()) == 0
+    assert float(((got.double() - want).abs() - tol).max()) <= 0
+
+
+@pytest.mark.parametrize("groups,nh,kvh,D,t", [([(4, 8)], 32, 8, 128, "bf16"), ([(40, 30), (3, 1)], 32, 8, 128, "bf16"),
+                                               ([(70, 20)], 8, 2, 64, "bf16"), ([(40, 30)], 16, 4, 64, "fp16"),
+                                               ([(9, 12), (65, 9)], 32, 8, 128, "fp16")])
+@pytest.mark.parametrize("out", ["same", "fp32"])
+@pytest.mark.parametrize("spread", [1.0, 4.0])
+def test_weights_of_shared_keys_keep_their_bits(kvb, cuda, groups, nh, kvh, D, t, out, spread):
+    """Shared keys' weights are as exact as those of own ones and of the decode attention: an fp32 output shows it."""
+    b = Batch(groups, lambda r: r.integers(0, 3), nh, kvh, D, 16, t, t, seed=nh + D, spread=spread)
+    _check_close(b, b.run(kvb, out_dtype=_dt(t if out == "same" else out)))
