@@ -23,7 +23,7 @@
 // Scores S and accumulators O live in TMEM (S0, S1 at columns 0 and 128, O0, O1 at 256 and 256 + head_dim); the
 // probabilities P overwrite S as 16-bit numbers and are the A operand of the second product straight from TMEM.  A thread
 // owns one row: the running maximum and sum need no exchange.  O is rescaled only when a row's maximum has grown by more
-// than 2^14 (fp16) or 2^40 (bf16) since its last rescaling: P, O and the sum have one scale, so nothing is lost.
+// than 2^3 (fp16) or 2^40 (bf16) since its last rescaling: P, O and the sum have one scale, so nothing is lost.
 // P is kept as a part and a rest of the pools' 16-bit type each, as the own parts and the decode attention keep it: the two
 // products with V hold 16 (bf16) or 22 (fp16) bits of each weight, and the output's only rounding that counts is its own.
 // With one 16-bit number each the weights' roundings were as large as a bf16 output's (1.66e-3 against 64 bits became
@@ -56,6 +56,10 @@ constexpr int kTmemCols = 512;
 // Most tokens of a table row: places are 32-bit numbers, and those of the tiles that are looked up ahead lie up to 300
 // behind the row's end.
 constexpr long long kPrefixTokens = (1LL << 31) - 1024;
+// The weight of a row's reference score is represented by 2^kLift: fp16 numbers, a part and its rest, end at 2^-25, and
+// of many keys far below the largest one the numerator would lose what the sum of the weights holds.
+template <class KV>
+constexpr float kLift = std::is_same<KV, __half>::value ? 12.f : 0.f;
 constexpr int kPrefixLimit = 512;  // at most 128 registers a thread: five of own_kernel's single warps fit beside a CTA
 
 // What joins a (sequence, kv head): partial rows of query head 0 begin at row0, and 256 further for each CTA before the
@@ -412,9 +416,9 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
     constexpr uint32_t kCol = kKeys * 128;           // bytes of one such column of a tile
     constexpr uint32_t kTile = NCH * kCol;           // one tile of Q, K or V
     constexpr uint32_t kO = 256;                     // TMEM column of the first accumulator
-    // How far (log2) a score may exceed the maximum that P, O and the sum refer to: P has to stay below the type's
-    // largest value, O and the sum below fp32's; nothing is lost up to there.
-    constexpr float kFar = std::is_same<KV, __half>::value ? 14.f : 40.f;
+    // How far (log2) a score may exceed the maximum that P, O and the sum refer to: P, which starts at 2^kLift, has to stay
+    // below the type's largest value, O and the sum below fp32's; nothing is lost up to there.
+    constexpr float kFar = std::is_same<KV, __half>::value ? 3.f : 40.f;
     __shared__ PrefixShared sh;
     extern __shared__ uint8_t dyn[];
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
@@ -668,7 +672,7 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                             tmem_st32(o_addr + c, s[1]);
                         }
                     }
-                    const float ref = m == -INFINITY ? 0.f : m;
+                    const float ref = (m == -INFINITY ? 0.f : m) - kLift<KV>;
                     const uint64_t scale2 = pack2(p.sl2, p.sl2), ref2 = pack2(-ref, -ref);
                     uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll 1
@@ -722,7 +726,7 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
             if (busy) {
                 tc_fence_after();
                 const long long r0 = w.part_row + (t ? w.rows0 : 0) + row;
-                if (row < rows) p.part_ml[r0] = make_float2(m, l);
+                if (row < rows) p.part_ml[r0] = make_float2(m - kLift<KV>, l);
                 if (some) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
@@ -954,8 +958,8 @@ __global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const Prefix
                 for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
                 const float mn = fmaxf(m[nt][e], mx), ref = mn == -INFINITY ? 0.f : mn, f = fast_exp2(m[nt][e] - ref);
                 m[nt][e] = mn;
-                s[e] = fast_exp2(s[e] - ref);
-                s[2 + e] = fast_exp2(s[2 + e] - ref);
+                s[e] = fast_exp2(s[e] - (ref - kLift<KV>));
+                s[2 + e] = fast_exp2(s[2 + e] - (ref - kLift<KV>));
                 l[nt][e] = l[nt][e] * f + (s[e] + s[2 + e]);
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
@@ -1002,7 +1006,7 @@ __global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const Prefix
                 const int j = 8 * nt + 2 * c4 + e;
                 if (j >= p.g) continue;
                 const long long row = (static_cast<long long>(seq) * p.nh + h * p.g + j) * p.own_parts + rank;
-                if (gid == 0) p.own_ml[row] = make_float2(m[nt][e], sum);
+                if (gid == 0) p.own_ml[row] = make_float2(m[nt][e] - kLift<KV>, sum);
                 if (rank >= tiles) continue;  // nothing, and its columns are not used
 #pragma unroll
                 for (int i = 0; i < NH; ++i)

@@ -408,3 +408,21 @@ def test_weights_of_shared_keys_keep_their_bits(kvb, cuda, groups, nh, kvh, D, t
     """Shared keys' weights are as exact as those of own ones and of the decode attention: an fp32 output shows it."""
     b = Batch(groups, lambda r: r.integers(0, 3), nh, kvh, D, 16, t, t, seed=nh + D, spread=spread)
     _check_close(b, b.run(kvb, out_dtype=_dt(t if out == "same" else out)))
+
+
+@pytest.mark.parametrize("t", ["fp16", "bf16"])
+@pytest.mark.parametrize("shared,n,nh,kvh", [(True, 1 << 17, 4, 1), (False, 1 << 17, 4, 1), (True, 1 << 15, 148, 148)])
+@pytest.mark.parametrize("first", [True, False])
+def test_long_flat_tail_below_one_key(kvb, cuda, t, shared, n, nh, kvh, first):
+    """One key (the first, or a late one) and n - 1 others of 2^-25.5 of its weight: in fp16 numbers of the weights
+    themselves all of these are zero, though they make up to 0.3% of the output.  148 heads: a head per CTA."""
+    import torch
+    b = Batch([(2, n // 16)] if shared else [(2, 0)], (lambda r: 0) if shared else (lambda r: n), nh, kvh, 64, 16, t, t)
+    b.q.zero_()[..., 0] = 1
+    slot = b.tables[:, :n // 16].long()[..., None] * 16 + torch.arange(16, device="cuda")
+    at = slot.flatten(1)[:, 0 if first else n - 1000]
+    k, v = b.k.view(-1, kvh, 64), b.v.view(-1, kvh, 64)
+    k.zero_()[..., 0] = -17.67
+    v.fill_(1)
+    k[at, :, 0], v[at] = 0, 0
+    _check_close(b, b.run(kvb, out_dtype=torch.float32, scale=1.0), scale=1.0, lift=12)
