@@ -23,7 +23,7 @@
 // Scores S and accumulators O live in TMEM (S0, S1 at columns 0 and 128, O0, O1 at 256 and 256 + head_dim); the
 // probabilities P overwrite S as 16-bit numbers and are the A operand of the second product straight from TMEM.  A thread
 // owns one row: the running maximum and sum need no exchange.  O is rescaled only when a row's maximum has grown by more
-// than 2^3 (fp16) or 2^40 (bf16) since its last rescaling: P, O and the sum have one scale, so nothing is lost.
+// than 2^3 (fp16) or 2^8 (bf16) since its last rescaling: P, O and the sum have one scale, so nothing is lost.
 // P is kept as a part and a rest of the pools' 16-bit type each, as the own parts and the decode attention keep it: the two
 // products with V hold 16 (bf16) or 22 (fp16) bits of each weight, and the output's only rounding that counts is its own.
 // With one 16-bit number each the weights' roundings were as large as a bf16 output's (1.66e-3 against 64 bits became
@@ -417,8 +417,9 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
     constexpr uint32_t kTile = NCH * kCol;           // one tile of Q, K or V
     constexpr uint32_t kO = 256;                     // TMEM column of the first accumulator
     // How far (log2) a score may exceed the maximum that P, O and the sum refer to: P, which starts at 2^kLift, has to stay
-    // below the type's largest value, O and the sum below fp32's; nothing is lost up to there.
-    constexpr float kFar = std::is_same<KV, __half>::value ? 3.f : 40.f;
+    // below the type's largest value, and O below fp32's, which a bf16 V may come near to by itself (with 2^40 values of
+    // 2^88 became infinite).
+    constexpr float kFar = std::is_same<KV, __half>::value ? 3.f : 8.f;
     __shared__ PrefixShared sh;
     extern __shared__ uint8_t dyn[];
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;

@@ -426,3 +426,16 @@ def test_long_flat_tail_below_one_key(kvb, cuda, t, shared, n, nh, kvh, first):
     v.fill_(1)
     k[at, :, 0], v[at] = 0, 0
     _check_close(b, b.run(kvb, out_dtype=torch.float32, scale=1.0), scale=1.0, lift=12)
+
+
+def test_large_values_behind_rising_scores(kvb, cuda):
+    """Scores that rise by 2^39 behind the first key tiles, over values near 2^100: the weights' reference has to follow, or
+    weight times value passes fp32's range.  148 heads: a head's eight key tiles for each CTA."""
+    import torch
+    b = Batch([(2, 64)], few, 148, 148, 64, 16, seed=4)
+    b.v.mul_(2.0 ** 100)
+    b.q.mul_(0.01)
+    b.q[..., 0] = 1
+    slot = (b.tables[0, :64].long()[:, None] * 16 + torch.arange(16, device="cuda")).flatten()
+    b.k.view(-1, 148, 64)[slot, :, 0] = torch.where(torch.arange(1024, device="cuda") < 256, 0.0, 27.0).to(b.k.dtype)[:, None]
+    b.check(b.run(kvb, scale=1.0), scale=1.0)
