@@ -223,6 +223,12 @@ __device__ __forceinline__ float exp2_unit(float x) {  // free to be moved, unli
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// A partial row's maximum and sum as they are left for joining.  Where every score was NaN the maximum, which passes over
+// them, is still -inf, the mark of a part without keys: the row has to become NaN, not to go without these keys.
+template <class KV>
+__device__ __forceinline__ float2 partial(float m, float l) {
+    return make_float2(m == -INFINITY && l != l ? 0.f : m - kLift<KV>, l);
+}
 // ---------------------------------------------------------------- units
 // Units of a group: kv heads x pairs of row tiles x key tiles.  A group with a bad range or a bad block count has none.
 struct Group {
@@ -727,7 +733,7 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
             if (busy) {
                 tc_fence_after();
                 const long long r0 = w.part_row + (t ? w.rows0 : 0) + row;
-                if (row < rows) p.part_ml[r0] = make_float2(m - kLift<KV>, l);
+                if (row < rows) p.part_ml[r0] = partial<KV>(m, l);
                 if (some) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
@@ -1007,7 +1013,7 @@ __global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const Prefix
                 const int j = 8 * nt + 2 * c4 + e;
                 if (j >= p.g) continue;
                 const long long row = (static_cast<long long>(seq) * p.nh + h * p.g + j) * p.own_parts + rank;
-                if (gid == 0) p.own_ml[row] = make_float2(m[nt][e] - kLift<KV>, sum);
+                if (gid == 0) p.own_ml[row] = partial<KV>(m[nt][e], sum);
                 if (rank >= tiles) continue;  // nothing, and its columns are not used
 #pragma unroll
                 for (int i = 0; i < NH; ++i)

@@ -439,3 +439,42 @@ def test_large_values_behind_rising_scores(kvb, cuda):
     slot = (b.tables[0, :64].long()[:, None] * 16 + torch.arange(16, device="cuda")).flatten()
     b.k.view(-1, 148, 64)[slot, :, 0] = torch.where(torch.arange(1024, device="cuda") < 256, 0.0, 27.0).to(b.k.dtype)[:, None]
     b.check(b.run(kvb, scale=1.0), scale=1.0)
+
+
+@pytest.mark.parametrize("D,t", [(64, "fp16"), (128, "bf16")])
+@pytest.mark.parametrize("where", ["one", "tile", "prefix", "own"])
+def test_nan_keys_show(kvb, cuda, where, D, t):
+    """NaN keys inside the context -- one, a tile's, all shared ones, all own ones of a sequence -- make the outputs of their kv
+    head NaN, as softmax does and the decode attention does; the other head, and other sequences, keep their answers."""
+    import torch
+    base = lambda: Batch([(5, 30), (3, 9)], lambda r: r.integers(1, 60), 8, 2, D, 16, t, t, seed=21)  # noqa: E731
+    good, b = base().run(kvb), base()
+    blocks = {"one": b.tables[0, 7:8], "tile": b.tables[0, 8:16], "prefix": b.tables[0, :30], "own": b.tables[2, 30:]}[where].long()
+    rows = [2] if where == "own" else list(range(5))
+    if where == "own":
+        blocks = blocks[:-(-(int(b.lens[2]) - 480) // 16)]
+    b.k[blocks[:, None], torch.arange(1 if where == "one" else 16, device="cuda")[None], 1] = math.nan
+    got, whole = b.run(kvb), kvb.paged_attention(b.q, b.k, b.v, b.tables, b.lens, 8, 2)
+    hit = torch.zeros((8, 8), dtype=torch.bool, device="cuda")
+    hit[rows, 4:] = True
+    for x in (got, whole):
+        assert bool(x[hit].isnan().all()) and bool(torch.isfinite(x[~hit]).all())
+    assert torch.equal(got[~hit], good[~hit])
+
+
+def test_infinite_scores_of_some_keys(kvb, cuda):
+    """Scores of -inf weigh nothing, in part or all of what is shared."""
+    import torch
+    for blocks in (slice(3, 4), slice(0, 30)):
+        b = Batch([(5, 30)], lambda r: r.integers(1, 60), 8, 2, 64, 16, seed=22)
+        b.q[..., 0] = 1
+        b.k[b.tables[0, blocks].long(), :, :, 0] = -math.inf
+        got = b.run(kvb)
+        keep = [i for i in range(30) if not blocks.start <= i < blocks.stop]
+        c = Batch([(5, 30)], lambda r: r.integers(1, 60), 8, 2, 64, 16, seed=22)
+        c.q[..., 0] = 1
+        n = 16 * (blocks.stop - blocks.start)
+        c.tables = torch.cat([c.tables[:, keep], c.tables[:, 30:]], 1).contiguous()
+        c.lens, c.prefix = c.lens - n, c.prefix - n // 16
+        c.check(got)
+        assert int(b.status.item()) == 0
