@@ -1131,20 +1131,24 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
         pl->run = a->block_size;
         pl->keys = kvpd::kKeys / a->block_size * a->block_size;  // 0: none fits
     }
-    AttnPlan whole;
-    const int rc = plan_attention(w, true, &whole);
-    if (rc != KVP_OK) return rc;
+    // The decode attention's workspace depends on whether q is aligned, which a size query does not know: both.
+    for (uintptr_t q : {uintptr_t{16}, uintptr_t{2}}) {
+        AttnPlan whole;
+        w.q = reinterpret_cast<const void*>(q);
+        const int rc = plan_attention(w, true, &whole);
+        if (rc != KVP_OK) return rc;
+        pl->bytes = std::max(pl->bytes, whole.ws_bytes);
+    }
     pl->shared = (a->head_dim == 64 || a->head_dim == 128) && a->q_dtype == a->kv_dtype && pl->keys > 0 && aligned16(a->q) &&
                  aligned16(a->out) && static_cast<long long>(a->num_seqs) * a->kv_heads <= (1LL << 27) &&
                  static_cast<long long>(a->max_blocks) * a->block_size <= kvpd::kPrefixTokens;
-    pl->bytes = whole.ws_bytes;
     if (!pl->shared) return KVP_OK;
     const size_t rows = static_cast<size_t>(a->num_seqs) * a->num_heads;
     const size_t parts = 2 * rows + static_cast<size_t>(sm_count()) * 2 * kvpd::kRows;
     pl->mt = kvpd::kRows / (a->num_heads / a->kv_heads);
     pl->ml = up256(static_cast<size_t>(a->num_seqs) * a->kv_heads * 8);
     pl->o = pl->ml + up256(parts * 8);
-    // (the larger of both: where q or out are not aligned the other path runs in the same workspace)
+    // (the largest of all: where q or out are not aligned the other path runs in the same workspace)
     pl->meta = pl->o + up256(parts * a->head_dim * 4);
     const long long items = static_cast<long long>(a->num_seqs) * a->kv_heads;
     while (pl->own_parts < 8 && items * pl->own_parts < sm_count() * kOwnWarps) pl->own_parts *= 2;

@@ -241,3 +241,17 @@ def test_prefix_table_rows_near_32_bits(kvb):
     assert 0 < longer < size((1 << 27) - 64) == size(10)
     for blocks in ((1 << 27) - 1, (1 << 27) - 20, (1 << 27) - 63):
         assert size(blocks) == longer
+
+
+@pytest.mark.parametrize("D,g", [(32, 16), (64, 16), (128, 8), (256, 8), (96, 4)])
+@pytest.mark.parametrize("B", [5, 16, 130])
+@pytest.mark.parametrize("kv", ["BF16", "F16"])
+def test_prefix_workspace_covers_any_alignment(kvb, D, g, B, kv):
+    """A size asked for without buffers serves any of them: queries or outputs off a 16-byte boundary go another way."""
+    for q in ("BF16", "F32"):
+        for kvh in (1, 2, 8):
+            size = lambda **kw: kvb.lib().kvp_prefix_workspace_size(C.byref(_prefix(  # noqa: E731
+                kvb, head_dim=D, kv_heads=kvh, num_heads=kvh * g, block_size=B, kv_dtype=getattr(kvb, kv),
+                q_dtype=getattr(kvb, q), **kw)))
+            # (a call off the boundary shares nothing and may need less)
+            assert size(q=0, out=0) == size() >= max(size(q=PTR + 2), size(out=PTR + 4), size(q=PTR + 2, out=PTR + 4)) > 0

@@ -478,3 +478,28 @@ def test_infinite_scores_of_some_keys(kvb, cuda):
         c.lens, c.prefix = c.lens - n, c.prefix - n // 16
         c.check(got)
         assert int(b.status.item()) == 0
+
+
+@pytest.mark.parametrize("nh,kvh,D,B,t", [(8, 2, 64, 130, "bf16"), (8, 2, 128, 250, "fp16"), (32, 2, 64, 129, "fp16"),
+                                          (8, 2, 32, 130, "bf16")])
+def test_blocks_that_do_not_fit_a_tile(kvb, cuda, nh, kvh, D, B, t):
+    """Block sizes above 128 without runs of 8: whole contexts, the same answers."""
+    b = Batch([(4, 3), (3, 0), (5, 2)], mixed, nh, kvh, D, B, t, t, seed=D + B)
+    b.check(b.run(kvb))
+
+
+@pytest.mark.parametrize("nh,kvh,D,t", [(16, 1, 64, "bf16"), (32, 8, 128, "fp16"), (16, 2, 128, "bf16")])
+@pytest.mark.parametrize("off", ["q", "out", "both"])
+def test_queries_and_outputs_off_16_bytes(kvb, cuda, nh, kvh, D, t, off):
+    """They go the way of the decode attention, in a workspace of the size that was asked for without them."""
+    import torch
+    b = Batch([(6, 9), (2, 0)], mixed, nh, kvh, D, 16, t, t, seed=nh)
+    ws = torch.empty(kvb.shared_prefix_workspace_bytes(b.q, b.k, b.tables, b.starts, nh, kvh), dtype=torch.uint8, device="cuda")
+    moved = lambda x: torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")[1:].view(x.shape).copy_(x)  # noqa: E731
+    out = torch.zeros_like(b.q)
+    if off != "out":
+        b.q = moved(b.q)
+    if off != "q":
+        out = moved(out)
+    assert kvb.shared_prefix_attention(*b.args(), out=out, workspace=ws, status=b.status) is out
+    b.check(out)
