@@ -1131,13 +1131,14 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
         pl->run = a->block_size;
         pl->keys = kvpd::kKeys / a->block_size * a->block_size;  // 0: none fits
     }
-    // The decode attention's workspace depends on whether q is aligned, which a size query does not know: both.
-    for (uintptr_t q : {uintptr_t{16}, uintptr_t{2}}) {
-        AttnPlan whole;
-        w.q = reinterpret_cast<const void*>(q);
-        const int rc = plan_attention(w, true, &whole);
-        if (rc != KVP_OK) return rc;
-        pl->bytes = std::max(pl->bytes, whole.ws_bytes);
+    AttnPlan whole;
+    const int rc = plan_attention(w, true, &whole);
+    if (rc != KVP_OK) return rc;
+    pl->bytes = whole.ws_bytes;
+    if (aligned16(a->q)) {  // unaligned queries may need more, which a size asked for without buffers has to cover
+        w.q = reinterpret_cast<const void*>(uintptr_t{2});
+        if (plan_attention(w, true, &whole) == KVP_OK) pl->bytes = std::max(pl->bytes, whole.ws_bytes);
+        else clear_error();
     }
     pl->shared = (a->head_dim == 64 || a->head_dim == 128) && a->q_dtype == a->kv_dtype && pl->keys > 0 && aligned16(a->q) &&
                  aligned16(a->out) && static_cast<long long>(a->num_seqs) * a->kv_heads <= (1LL << 27) &&

@@ -253,5 +253,10 @@ def test_prefix_workspace_covers_any_alignment(kvb, D, g, B, kv):
             size = lambda **kw: kvb.lib().kvp_prefix_workspace_size(C.byref(_prefix(  # noqa: E731
                 kvb, head_dim=D, kv_heads=kvh, num_heads=kvh * g, block_size=B, kv_dtype=getattr(kvb, kv),
                 q_dtype=getattr(kvb, q), **kw)))
+            need = size()
+            assert need == size(q=0, out=0)
+            if need == 0:  # a shape that the decode attention does not take
+                assert "shared memory" in kvb.last_error()
+                continue
             # (a call off the boundary shares nothing and may need less)
-            assert size(q=0, out=0) == size() >= max(size(q=PTR + 2), size(out=PTR + 4), size(q=PTR + 2, out=PTR + 4)) > 0
+            assert need >= max(size(q=PTR + 2), size(out=PTR + 4), size(q=PTR + 2, out=PTR + 4)) > 0
