@@ -353,9 +353,10 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
             sum = sum * exp_of(m - mn) + add;
             m = mn;
         }
-        const unsigned long long known = *reinterpret_cast<volatile unsigned long long*>(&floor_key);
+        unsigned long long known = *reinterpret_cast<volatile unsigned long long*>(&floor_key);
         if (__any_sync(0xffffffffu, known > least)) {
-            least = known;
+            known = __shfl_sync(0xffffffffu, known, 0);  // written at any time: the lanes take the same one
+            least = known > least ? known : least;
             refresh();
         }
         const bool ties = at < ltok;
