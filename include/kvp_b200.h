@@ -351,9 +351,12 @@ KVP_API int kvp_swap_in(const kvp_swap_args* a, void* stream);
  * rows, 0: vocab; rows need no alignment beyond their type's), scores fp32 [batch][beams] (the running sums of
  * log-probabilities; -inf: a beam not in use, as all but one are in a search's first step).  A logit of -inf is a banned
  * token.  Continuations of value -inf are chosen only when the others run out, and are ordered like the rest.  NaN and
- * +inf, in logits and scores, count as -inf and set KVP_STATUS_BAD_VALUE.  out_scores / out_parents / out_tokens:
- * [batch][select].  beams and select at most 32, vocab at most 2^26.  The states follow their beams by
- * kvp_mgr_reorder(), which moves no bytes.  The workspace (16-byte aligned) needs no initial value and keeps none. */
+ * +inf, in logits and scores, count as -inf and set KVP_STATUS_BAD_VALUE.  The sums of exponentials are taken in fp32:
+ * a value's error from them is some 1e-7, at most (16 + 34 s) 2^-24 where a warp takes s steps of 512 logits of a row, and
+ * continuations of different beams that lie nearer than twice that may change places (those of one beam never do).
+ * out_scores / out_parents / out_tokens: [batch][select].  beams and select at most 32, vocab at most 2^26.  The states
+ * follow their beams by kvp_mgr_reorder(), which moves no bytes.  The workspace (16-byte aligned) needs no initial value
+ * and keeps none. */
 typedef struct kvp_beam_args {
     const void* logits;
     int64_t row_stride;

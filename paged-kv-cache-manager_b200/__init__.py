@@ -823,8 +823,8 @@ def shared_prefix_groups(tables, lens, block_size: int):
 
 def beam_select(logits, scores, select: int, *, workspace=None, status=None, stream=None):
     """kvp_beam_select: for each request the `select` best continuations over its beams and the vocabulary by running
-    score + log-probability, ties to the lower beam, then the lower token.  logits [batch * beams][vocab] (rows may be
-    strided), scores fp32 [batch][beams] (-inf: a beam not in use).  Returns (scores fp32, parents int32, tokens int32),
+    score + log-probability, ties to the lower beam, then the lower token (values of different beams carry the fp32 error of
+    their log-sums, some 1e-7, and are ordered up to that).  logits [batch * beams][vocab] (rows may be strided), scores fp32 [batch][beams] (-inf: a beam not in use).  Returns (scores fp32, parents int32, tokens int32),
     each [batch][select]; KVManager.reorder then moves the states.  workspace: kvp_beam_workspace_size() bytes of
     uint8, allocated here unless given."""
     import torch

@@ -13,9 +13,11 @@
 // passes into the lists.
 //
 // beam_pick_kernel (bound by latency): one CTA per request joins each beam's segments -- their sums in 64 bits, their lists
-// by bitonic merges -- and takes the best head of the beams' lists `select` times, comparing values in 64 bits:
-// continuations of different beams are ordered by their values, not by a 32-bit rounding.  About 8 us, most of it the way
-// from the partial sums to the first choice.
+// by bitonic merges -- and takes the best head of the beams' lists `select` times, comparing values in 64 bits, so that no
+// 32-bit rounding of a value decides.  A beam's own continuations are in the exact order of their logits.  Between beams the
+// log-sums' errors remain, whose terms lanes and warps add in fp32: at most (16 + 34 s) 2^-24 with s steps a warp, 1.7e-5 at
+// 8 steps; values that lie nearer to each other than twice that may change places.  About 8 us, most of it the way from the
+// partial sums to the first choice.
 #include <cuda_runtime.h>
 
 #include <algorithm>
