@@ -647,6 +647,13 @@ def _token_stride(t, name, shape):
     return st[0] if shape[0] > 1 else shape[1] * shape[2]
 
 
+def _i32(x, name):
+    """A size of the C structures (ctypes would cut it to 32 bits without a word)."""
+    if not -0x80000000 <= x <= 0x7fffffff:
+        raise ValueError(f"{name} must stay below 2^31")
+    return x
+
+
 def _vector(t, name, dtype, shape):
     if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
@@ -674,14 +681,14 @@ def _rope(q, k, v, positions, table, k_cache, v_cache, slots, q_out, k_out, q_no
     if table.dim() != 2:
         raise ValueError("table must be [max_positions][rot_dim]")
     tshape = table.shape
-    a.table, a.max_positions, a.rot_dim = _vector(table, "table", torch.float32, tshape), tshape[0], tshape[1]
+    a.table, a.max_positions, a.rot_dim = _vector(table, "table", torch.float32, tshape), _i32(tshape[0], "max_positions"), tshape[1]
     a.positions = _vector(positions, "positions", torch.int32, (n,))
     if q_norm is not None:
         a.q_norm = _vector(q_norm, "q_norm", dtype, (D,))
     if k_norm is not None:
         a.k_norm = _vector(k_norm, "k_norm", dtype, (D,))
     a.eps, a.interleaved = eps, 1 if interleaved else 0
-    a.num_tokens, a.num_heads, a.kv_heads, a.head_dim = n, nh, kvh, D
+    a.num_tokens, a.num_heads, a.kv_heads, a.head_dim = _i32(n, "the number of tokens"), nh, kvh, D
     if k_cache is not None:
         if v.dtype is not dtype:
             raise ValueError("q, k and v must share a dtype")
@@ -741,8 +748,8 @@ def _prefix_shape(a, q, k_cache, block_tables, group_starts, num_heads, kv_heads
     if len(ts) != 2 or ts[0] != qs[0] or len(gs) != 1 or gs[0] < 1:
         raise ValueError("block_tables must be [num_seqs][max_blocks] and group_starts [num_groups + 1]")
     a.q_dtype, a.kv_dtype = _dtype_code(q), _dtype_code(k_cache)
-    a.num_seqs, a.num_groups, a.num_heads, a.kv_heads, a.head_dim = qs[0], gs[0] - 1, num_heads, kv_heads, qs[2]
-    a.max_blocks, a.num_blocks, a.block_size = ts[1], ks[0], ks[1]
+    a.num_seqs, a.num_groups, a.num_heads, a.kv_heads, a.head_dim = _i32(qs[0], "num_seqs"), _i32(gs[0] - 1, "num_groups"), num_heads, kv_heads, qs[2]
+    a.max_blocks, a.num_blocks, a.block_size = _i32(ts[1], "max_blocks"), ks[0], _i32(ks[1], "block_size")
 
 
 def shared_prefix_workspace_bytes(q, k_cache, block_tables, group_starts, num_heads: int, kv_heads: int) -> int:
@@ -838,13 +845,13 @@ def beam_select(logits, scores, select: int, *, workspace=None, status=None, str
     if ls[1] > 1 and st[1] != 1:
         raise ValueError("the logits of a row must be contiguous")
     a = BeamArgs()
-    a.logits, a.logits_dtype, a.vocab = logits.data_ptr(), _dtype_code(logits), ls[1]
+    a.logits, a.logits_dtype, a.vocab = logits.data_ptr(), _dtype_code(logits), _i32(ls[1], "vocab")
     if ls[0] > 1:
         a.row_stride = st[0]
         if st[0] < ls[1]:
             raise ValueError("the rows of logits must not overlap")
     a.scores = _vector(scores, "scores", torch.float32, ss)
-    a.batch, a.beams, a.select = batch, beams, select
+    a.batch, a.beams, a.select = _i32(batch, "batch"), beams, _i32(select, "select")
     if status is not None:
         a.status = _dev(status, "status")
     if workspace is None:

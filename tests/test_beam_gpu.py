@@ -242,3 +242,13 @@ def test_refusals_and_empty(kvb, cuda):
         kvb.beam_select(x, s, 4, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
     out = kvb.beam_select(x[:0], s[:0], 4)
     assert [tuple(t.shape) for t in out] == [(0, 4)] * 3
+
+
+def test_numbers_that_pass_32_bits(kvb, cuda):
+    import torch
+    x, s = torch.zeros(2, 8, device="cuda"), torch.zeros(1, 2, device="cuda")
+    for select in (2 ** 32 + 3, 2 ** 31, -2 ** 40):
+        with pytest.raises(ValueError):
+            kvb.beam_select(x, s, select)
+    with pytest.raises(ValueError):  # 2^32 + 8 tokens are not 8
+        kvb.beam_select(torch.zeros(1, 2 ** 32 + 8, dtype=torch.half, device="cuda"), s[:, :1], 3)

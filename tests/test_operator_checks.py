@@ -260,3 +260,11 @@ def test_prefix_workspace_covers_any_alignment(kvb, D, g, B, kv):
                 continue
             # (a call off the boundary shares nothing and may need less)
             assert need >= max(size(q=PTR + 2), size(out=PTR + 4), size(q=PTR + 2, out=PTR + 4)) > 0
+
+
+def test_sizes_beyond_32_bits_are_refused(kvb):
+    """ctypes cuts a number to a field's 32 bits: select = 2^32 + 3 would have become 3."""
+    assert kvb._i32(2 ** 31 - 1, "x") == 2 ** 31 - 1 and kvb._i32(-1, "x") == -1
+    for x in (2 ** 31, 2 ** 32 + 3, -2 ** 31 - 1):
+        with pytest.raises(ValueError):
+            kvb._i32(x, "x")
