@@ -654,6 +654,13 @@ def _i32(x, name):
     return x
 
 
+def _status_word(t):
+    import torch
+    if t.dtype is not torch.int32 or t.numel() < 1:
+        raise ValueError("status must be an int32 tensor of one element")
+    return _dev(t, "status")
+
+
 def _vector(t, name, dtype, shape):
     if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
@@ -701,7 +708,7 @@ def _rope(q, k, v, positions, table, k_cache, v_cache, slots, q_out, k_out, q_no
         a.slots = _vector(slots, "slots", torch.int32, (n,))
         a.num_blocks, a.block_size = pool[0], pool[1]
     if status is not None:
-        a.status = _dev(status, "status")
+        a.status = _status_word(status)
     if q_out is None:
         q_out = _new_on(stream, q, shape, dtype)
         a.q_out, a.out_dtype = q_out.data_ptr(), a.in_dtype
@@ -787,7 +794,7 @@ def shared_prefix_attention(q, k_cache, v_cache, block_tables, seq_lens, prefix_
     a.group_starts = _vector(group_starts, "group_starts", i32, group_starts.shape)
     a.scale = scale
     if status is not None:
-        a.status = _dev(status, "status")
+        a.status = _status_word(status)
     if out is None:
         out = _new_on(stream, q, q.shape, out_dtype or q.dtype)
     elif out.shape != q.shape:
@@ -853,7 +860,7 @@ def beam_select(logits, scores, select: int, *, workspace=None, status=None, str
     a.scores = _vector(scores, "scores", torch.float32, ss)
     a.batch, a.beams, a.select = _i32(batch, "batch"), beams, _i32(select, "select")
     if status is not None:
-        a.status = _dev(status, "status")
+        a.status = _status_word(status)
     if workspace is None:
         need = _size_on(idx, _fn("kvp_beam_workspace_size"), a)
         if need == 0 and batch:

@@ -252,3 +252,14 @@ def test_numbers_that_pass_32_bits(kvb, cuda):
             kvb.beam_select(x, s, select)
     with pytest.raises(ValueError):  # 2^32 + 8 tokens are not 8
         kvb.beam_select(torch.zeros(1, 2 ** 32 + 8, dtype=torch.half, device="cuda"), s[:, :1], 3)
+
+
+def test_status_words_of_other_types(kvb, cuda):
+    import torch
+    x, s = torch.zeros(2, 8, device="cuda"), torch.zeros(1, 2, device="cuda")
+    for bad in (torch.zeros(4, dtype=torch.uint8, device="cuda")[1:], torch.zeros(0, dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError):
+            kvb.beam_select(x, s, 3, status=bad)
+        with pytest.raises(ValueError):
+            kvb.qk_norm_rope(torch.zeros(1, 1, 16, device="cuda"), torch.zeros(1, 1, 16, device="cuda"),
+                             torch.zeros(1, dtype=torch.int32, device="cuda"), kvb.rope_table(1, 16), status=bad)

@@ -268,3 +268,10 @@ def test_sizes_beyond_32_bits_are_refused(kvb):
     for x in (2 ** 31, 2 ** 32 + 3, -2 ** 31 - 1):
         with pytest.raises(ValueError):
             kvb._i32(x, "x")
+
+
+def test_status_words_of_other_types_are_refused(kvb):
+    import torch
+    for bad in (torch.zeros(1, dtype=torch.uint8), torch.zeros(1), torch.zeros(0, dtype=torch.int32), torch.zeros(1, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="status"):
+            kvb._status_word(bad)
