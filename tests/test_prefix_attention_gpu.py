@@ -503,3 +503,14 @@ def test_queries_and_outputs_off_16_bytes(kvb, cuda, nh, kvh, D, t, off):
         out = moved(out)
     assert kvb.shared_prefix_attention(*b.args(), out=out, workspace=ws, status=b.status) is out
     b.check(out)
+
+
+@pytest.mark.parametrize("groups,own,nh,kvh,D,t", [([(2, 1)], lambda r: 30000 + int(r.integers(0, 9)), 32, 8, 128, "bf16"),
+                                                   ([(64, 5)], lambda r: 7001 if r.random() < 0.1 else int(r.integers(0, 100)),
+                                                    8, 2, 64, "fp16"),
+                                                   ([(3, 40), (1, 0)], lambda r: int(10 ** r.uniform(0, 4)), 16, 1, 128, "bf16")])
+def test_long_and_uneven_own_parts(kvb, cuda, groups, own, nh, kvh, D, t):
+    """Own contexts of thousands of tokens, and of lengths that are orders of magnitude apart."""
+    b = Batch(groups, own, nh, kvh, D, 16, t, t, seed=51)
+    assert int(b.lens.max()) > 5000
+    _check_close(b, b.run(kvb), lift=12)
