@@ -224,3 +224,22 @@ def test_refusals(kvb):
     with pytest.raises(ValueError):
         _engine()(model, 8, 16, fused_rope=True)
     _engine()(model, 8, 16)
+
+
+@pytest.mark.gpu
+def test_a_long_context_among_those_that_share(models, counted):
+    """One request whose own context would hold up the shared-prefix attention: the step runs as without the option, with the
+    same bits; without that request it goes by groups."""
+    import torch
+    model, _ = models[False]
+    r = np.random.default_rng(4)
+    base = r.integers(0, VOCAB, 4000).tolist()
+    logits = {}
+    for shared in (False, True):
+        eng = _engine()(model, 300, 16, shared_prefix=shared)
+        assert eng.prefill(1, base[:70]) is not None and eng.prefill(2, base[:64] + base[100:110], 1, 64) is not None
+        assert eng.prefill(3, base[:64] + base[200:], 1, 64) is not None
+        counted.clear()
+        logits[shared] = [eng.decode_batch([3, 2, 1], [5, 6, 7]), eng.decode_batch([2, 1], [8, 9])]
+        assert counted.get("shared_prefix_attention", 0) == (4 if shared else 0) and int(eng.status.item()) == 0
+    assert torch.equal(logits[True][0], logits[False][0]) and _rel(logits[True][1], logits[False][1]) < TOL

@@ -275,3 +275,24 @@ def test_status_words_of_other_types_are_refused(kvb):
     for bad in (torch.zeros(1, dtype=torch.uint8), torch.zeros(1), torch.zeros(0, dtype=torch.int32), torch.zeros(1, dtype=torch.int64)):
         with pytest.raises(ValueError, match="status"):
             kvb._status_word(bad)
+
+
+def test_when_a_step_goes_by_groups(kvb):
+    """The engine's rule between the shared-prefix attention and the decode attention, on both sides of it."""
+    import importlib
+    pays = importlib.import_module("paged-kv-cache-manager_b200.model")._sharing_pays
+
+    def step(groups, block=16, kv_heads=8, dim=128):  # (shared blocks, own tokens of each member)
+        prefix, starts, lens = [], [0], []
+        for blocks, own in groups:
+            prefix += [blocks] * len(own)
+            lens += [blocks * block + x for x in own]
+            starts.append(len(lens))
+        return pays(np.array(prefix, np.int32), np.array(starts, np.int32), lens, block, kv_heads, dim, 148)
+
+    for yes in ([(128, [100] * 256)], [(1024, [8192] * 16)], [(1, [100] * 16)], [(128, [1000] * 2)], [(5, [1, 2, 3])],
+                [(0, [50]), (9, [3, 4])], [(128, [100] * 255 + [3000])], [(256, [4000] * 64)]):
+        assert step(yes), yes
+    for no in ([(1, [100] * 255 + [30000])], [(1, [30000, 30000])], [(1024, [8192] * 4)], [(16, [100] * 128 + [4000])],
+               [(0, [30000]), (9, [3, 4])], [(1, [8192] * 64)]):
+        assert not step(no), no
