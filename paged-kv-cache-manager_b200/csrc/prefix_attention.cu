@@ -4,19 +4,20 @@
 // For one kv head, a group of m sequences with g query heads each has m * g query rows over the same keys, so what is a
 // matrix-vector product per sequence becomes a matrix product, S = Q K^T and O = P V, for the tensor cores:
 //   read  2 * P * head_dim * 2 bytes of K and V per kv head (P shared tokens),
-//   compute 4 * m * g * P * head_dim flops.
-// Up to about 128 rows the bytes take longer than the flops; beyond, the tensor cores and the exponentials bound it.
+//   compute 4 * m * g * P * head_dim flops (half as many again for the rests of P, below).
+// Up to about 170 rows the bytes take longer than these products at the rates of a copy and of a large matrix product (256
+// without the rests); beyond, the tensor cores and the exponentials bound it.
 //
 // Three launches.  prefix_kernel attends over the shared blocks, own_kernel over each sequence's own blocks, beside it on
 // what it leaves of an SM; both leave partial results, which join_kernel joins.
 //
 // prefix_kernel: one CTA per SM takes an even share of the step's units -- a unit is one tile of 128 keys for one (group,
 // kv head, pair of row tiles), of fewer where the blocks' size shares no factor of 8 with it: as many whole blocks as fit,
-// copied one by one (16 groups with blocks of 5 tokens: 50 us, of 16 tokens 47; by whole contexts 916) -- regardless of where
+// copied one by one (16 groups with blocks of 5 tokens: 55 us, of 16 tokens 51; by whole contexts 916) -- regardless of where
 // groups and heads begin and end.  A row tile is as many whole members as fit 128 rows (tcgen05's M).  Two warpgroups of softmax, one per accumulator pair in TMEM, take turns with the tensor
 // cores: while one exponentiates its scores, the MMAs of the other run.  Exponentiating at the same time gains nothing: with
 // two score buffers of 64 keys each, which keep both at it, 256 sequences over 16384 tokens took 176 us instead of 148; with
-// a quarter of the exponentials as a polynomial on the FMA pipe 150.
+// a quarter of the exponentials as a polynomial on the FMA pipe 150 (all three with P in one 16-bit number).
 //   two row tiles:  the warpgroups take one tile each and every key tile; K and V are read once for 256 rows.
 //   one row tile:   both warpgroups take the same rows, one the even, the other the odd key tiles, so that the wait for a
 //                   tile's exponentials is covered by the other tile; they leave two partial results.
@@ -30,12 +31,16 @@
 // 2.3e-3, relative to all outputs' size 1e-4 became 2.5e-3), and an fp32 output held no more.  It costs half of the tensor
 // cores' work on top: 16 groups 46.9 -> 51.9 us, 512 samples 71.2 -> 78.7, 256 over 16384 154.9 -> 186.4, 4 beams the same.
 //
-// Measured, 32 query and 8 kv heads of 128, bf16: a pair of row tiles takes 3750 clocks per key tile (4000 beside the own
-// parts), of which the matrix products are 2050 and the exponentials the rest; starting (groups, table, first tiles) takes
-// 12000 clocks, writing the partial results 5000 to 8000.  512 sequences over 2048 shared tokens and up to 100 own ones: 71 us (prefix_kernel alone 33, the
-// own parts alone 20, joining 10); 256 over 16384, up to 512 own: 148 us (80, 44, 9); 4 beams over 2048, 24 own: 16 us.
+// Measured, 32 query and 8 kv heads of 128, bf16: a pair of row tiles takes 5260 clocks per key tile, of which the matrix
+// products are 3070 (3750 and 2050 with P in one 16-bit number); starting (groups, table, first tiles) takes 12000 clocks,
+// writing the partial results 5000 to 8000.  512 sequences over 2048 shared tokens and up to 100 own ones: 79 us (prefix_kernel
+// alone 49, the own parts alone 31, joining 13, each with cold caches); 256 over 16384, up to 512 own: 171 us (119, 63, 12);
+// 4 beams over 2048, 24 own: 17 us.
 // prefix_kernel leaves shared memory unused on purpose: with 224 KB instead of 192 the L1, which the own parts' loads go
-// through, shrinks to 28 KB, and the first two calls took 85 and 174 us.
+// through, shrinks to 28 KB, and the first two calls took 85 and 174 us where they took 72 and 149.
+// The own parts are cut alike, into at most 8 each: a long one beside many short ones, or few long ones, are slower than by
+// kvp_paged_attention, whose partition follows the lengths (2 sequences of 30000 own tokens: 320 us against 105; 255 of 100
+// beside one of 30000: 1227 against 96; 64 of 8192 over 2048 shared ones: 400 against 363).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -429,7 +434,7 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
     __shared__ PrefixShared sh;
     extern __shared__ uint8_t dyn[];
     const uint32_t base = (smem_u32(dyn) + 1023u) & ~1023u;
-    // Slots of K and of V, beside two query tiles: 192 KB in all at head_dim 128, 176 KB at 64.
+    // Slots of K and of V, beside two query tiles: 192 KB in all at head_dim 128, 144 KB at 64.
     constexpr int kSlotsK = D == 128 ? 2 : 4, kSlotsV = D == 128 ? 2 : 3;
     const uint32_t ring_k = base + 2 * kTile, ring_v = ring_k + kSlotsK * kTile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -763,7 +768,7 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
 // 1 to 8 single warps, which wait for nothing from each other, share the own tokens of a (sequence, kv head), 16 at a time.
 // Bound by HBM, and by latency where the own parts are short, which most of them are: a warp takes K and V from global memory
 // straight into the registers of its matrix instructions, without a pipeline to fill and drain.  Alone it takes 20 us at 512
-// sequences with up to 100 own tokens, 44 us at 256 with up to 512 (6.5 TB/s).  CTAs of four warps that also joined their
+// sequences with up to 100 own tokens, 44 us at 256 with up to 512 (6.5 TB/s), 31 and 63 with cold caches.  CTAs of four warps that also joined their
 // results with the shared part's took 42 and 71 us; clusters of eight such CTAs, where pairs are few, 19.2 us for the whole
 // call at 4 beams instead of 16.2.
 //   S^T[tokens x heads] = K Q^T:  a lane holds 8 neighbouring dims of a token's K (one 16-byte load); the sum over dims does
@@ -771,7 +776,10 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
 //   O^T[dims x heads] += V^T P^T: a lane holds 8 neighbouring dims of four tokens' V and pairs up two tokens' halves; the
 //                                 rows of the instruction are dims in an order of their own.  P^T by an 8 x 8 transposition.
 // The heads are the 8 columns of the instruction (NT times, for more than 8): as its 16 rows they took twice the
-// instructions and accumulators, and twice the time at head_dim 128.
+// instructions and accumulators, and twice the time at head_dim 128.  With more than 8 heads per kv head and head_dim 128 the
+// kernel spills 140 bytes of registers, else at most 16; ten warps an SM, which need no spills, took 116 us instead of 113 (256 sequences, 64
+// query and 4 kv heads, 256 shared and 512 own tokens).
+
 // Four partial results (maximum, sum; four columns of the output) at a time, folded into what there is.  One with the maximum
 // -inf is nothing, and its columns may never have been written.
 struct Fold {
@@ -1099,9 +1107,9 @@ kvp_attn_args whole_contexts(const kvp_prefix_args& a) {
     return w;
 }
 
-// Warps an SM that own parts are split into at least: 16 is what its registers hold.  Half as many took 162 us at 256
-// sequences with up to 512 own tokens instead of 149 (twice as many 146); twice as many 74 us at 512 with up to 100 instead
-// of 72, four times 81, for the parts that join_kernel has to read.
+// Warps an SM that own parts are split into at least: 16 is what its registers hold.  Half as many took 186 us at 256
+// sequences with up to 512 own tokens instead of 171 (twice as many 170); twice as many 82 us at 512 with up to 100 instead
+// of 79, four times 90, for the parts that join_kernel has to read.
 constexpr long long kOwnWarps = 16;
 
 struct PrefixPlan {
