@@ -81,7 +81,6 @@ class PagedEngine:
         self.prefill_tokens_computed = 0
         self.cow_data_copies = 0
         self.fused_rope, self.shared_prefix = fused_rope, shared_prefix
-        self._sms = torch.cuda.get_device_properties(self.dev).multi_processor_count
         self._table = None
         if fused_rope:
             rot = model.model.rotary_emb
@@ -227,7 +226,8 @@ class PagedEngine:
             by_table = sorted(range(len(rows)), key=lambda i: rows[i])  # requests that share blocks side by side
             side_by_side = [rows[i] for i in by_table], [before[i] + 1 for i in by_table]
             prefix, starts = kvb.shared_prefix_groups(self._dense(side_by_side[0]), side_by_side[1], self.B)
-            if prefix.any() and _sharing_pays(prefix, starts, side_by_side[1], self.B, self.kvh, self.hd, self._sms):
+            if prefix.any() and _sharing_pays(prefix, starts, side_by_side[1], self.B, self.kvh, self.hd,
+                                               torch.cuda.get_device_properties(self.dev).multi_processor_count):
                 order, groups = by_table, (torch.from_numpy(prefix).to(self.dev), torch.from_numpy(starts).to(self.dev))
                 rows, before, slots = [rows[i] for i in order], [before[i] for i in order], [slots[i] for i in order]
                 last_tokens = [last_tokens[i] for i in order]
