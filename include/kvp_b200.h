@@ -196,11 +196,12 @@ KVP_API int kvp_paged_attention_noalloc(const kvp_attn_args* a, void* stream);
  *     table row gives the blocks.
  * A sequence that breaks these rules, or whose length is invalid, gets zeros and sets KVP_STATUS_BAD_LEN.
  * Types, head shapes and layouts as in kvp_paged_attention.  Sharing takes head_dim 64 and 128, queries of the pools'
- * 16-bit dtype, block sizes up to 128 or multiples of 8, q and out on 16-byte boundaries, num_seqs * kv_heads <= 2^27 and
- * max_blocks * block_size <= 2^31 - 1024; every other call attends over each sequence's whole context, as
- * kvp_paged_attention does.  The probabilities go into the product with V as a part and a rest of the pools' dtype, sums
- * are fp32, as there.  The workspace (256-byte aligned) needs no initial value and keeps none; calls that overlap on the
- * GPU need one each. */
+ * 16-bit dtype, block sizes up to 128 or multiples of 8, q and out on 16-byte boundaries, num_seqs * kv_heads <= 2^27
+ * and max_blocks * block_size <= 2^31 - 1024; every other call attends over each sequence's whole context, as
+ * kvp_paged_attention does, and does not look at the groups.  The probabilities go into the product with V as a part and
+ * a rest of the pools' dtype, sums are fp32, as there.  Own contexts are cut into equally many parts each, 8 at most: a
+ * long one among short ones is better off in kvp_paged_attention.  The workspace (256-byte aligned) needs no initial
+ * value and keeps none; calls that overlap on the GPU need one each. */
 typedef struct kvp_prefix_args {
     const void* q;
     const void* k_cache; /* this layer's pools */
@@ -347,16 +348,16 @@ KVP_API int kvp_swap_in(const kvp_swap_args* a, void* stream);
 /* ======================================================================== beam selection
  * For each request: the `select` best continuations (beam, token) by
  *   value = scores[beam] + logits[beam][token] - log(sum over tokens of exp(logits[beam][.])),
- * best first, ties to the lower beam, then the lower token.  logits [batch * beams][vocab] (row_stride elements between
- * rows, 0: vocab; rows need no alignment beyond their type's), scores fp32 [batch][beams] (the running sums of
- * log-probabilities; -inf: a beam not in use, as all but one are in a search's first step).  A logit of -inf is a banned
- * token.  Continuations of value -inf are chosen only when the others run out, and are ordered like the rest.  NaN and
- * +inf, in logits and scores, count as -inf and set KVP_STATUS_BAD_VALUE.  The sums of exponentials are taken in fp32:
- * a value's error from them is some 1e-7, at most (16 + 34 s) 2^-24 where a warp takes s steps of 512 logits of a row, and
- * continuations of different beams that lie nearer than twice that may change places (those of one beam never do).
- * out_scores / out_parents / out_tokens: [batch][select].  beams and select at most 32, vocab at most 2^26.  The states
- * follow their beams by kvp_mgr_reorder(), which moves no bytes.  The workspace (16-byte aligned) needs no initial value
- * and keeps none. */
+ * best first, ties to the lower beam, then the lower token.  logits [batch * beams][vocab] (row_stride elements
+ * between rows, 0: vocab; rows need no alignment beyond their type's), scores fp32 [batch][beams] (the running sums of
+ * log-probabilities; -inf: a beam not in use, as all but one are in a search's first step).  A logit of -inf is a
+ * banned token.  Continuations of value -inf are chosen only when the others run out, and are ordered like the rest.
+ * NaN and +inf, in logits and scores, count as -inf and set KVP_STATUS_BAD_VALUE.  The sums of exponentials are taken
+ * in fp32: a value's error from them is some 1e-7, at most (16 + 34 s) 2^-24 where a warp takes s steps of 512 logits
+ * of a row, and continuations of different beams that lie nearer than twice that may change places (those of one beam
+ * never do).  out_scores / out_parents / out_tokens: [batch][select].  beams and select at most 32, vocab at most
+ * 2^26.  The states follow their beams by kvp_mgr_reorder(), which moves no bytes.  The workspace (16-byte aligned)
+ * needs no initial value and keeps none. */
 typedef struct kvp_beam_args {
     const void* logits;
     int64_t row_stride;

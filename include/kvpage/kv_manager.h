@@ -83,8 +83,8 @@ public:
     // When on, every mutating call validates and throws std::logic_error on a violation.  Default: on in
     // builds without NDEBUG.
     void set_check_each_op(bool on) { check_each_op_ = on; }
-    // Calls so far that created, changed or removed a block table (admissions, forks, appends, frees, reorders): a caller
-    // mirroring tables elsewhere (the decode-step runtime's staged rows) can tell whether any table changed since
+    // Calls so far that created, changed or removed a block table (admissions, forks, appends, frees, reorders): a
+    // caller mirroring tables elsewhere (the decode-step runtime's staged rows) can tell whether any table changed since
     // it last looked.  Not part of the reference's interface.
     uint64_t table_changes() const { return table_changes_; }
 

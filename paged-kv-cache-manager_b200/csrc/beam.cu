@@ -2,22 +2,21 @@
 //     value = score[beam] + logit[beam][token] - log(sum over tokens of exp(logit[beam][.])),
 // ties to the lower beam, then the lower token.  One read of the logits, two launches.
 //
-// beam_scan_kernel (bound by HBM): a warp takes its share of one row, 512 logits a step, three steps in
-// flight.  It keeps a running maximum and sum of exponentials per lane, and its best
-// `select` logits as a list sorted over its 32 lanes; within a row the order of the values is the order of the logits, so
-// no logarithm is needed here.  The list starts from the lanes' own maxima of the first step (one sort); of the rest only
-// what passes the list's last entry -- or that of another warp of the CTA, which works on the same row -- costs more than
-// one vote per step, and is inserted with a ballot and a shift.  Entries are 64-bit keys (ordered logit, ~token): all
-// different, so ties fall to the lower token however the row is cut.  512 rows of 128000 fp32 logits, select 16: 262 MB in
-// 61 us (4.3 TB/s), the issue slots 63% busy: about 100 instructions a step of 512 logits, and as many again for what
-// passes into the lists.
+// beam_scan_kernel (bound by HBM): a warp takes its share of one row, 512 logits a step, three steps in flight.  It
+// keeps a running maximum and sum of exponentials per lane, and its best `select` logits as a list sorted over its 32
+// lanes; within a row the order of the values is the order of the logits, so no logarithm is needed here.  The list
+// starts from the lanes' own maxima of the first step (one sort); of the rest only what passes the list's last entry --
+// or that of another warp of the CTA, which works on the same row -- costs more than one vote per step, and is inserted
+// with a ballot and a shift.  Entries are 64-bit keys (ordered logit, ~token): all different, so ties fall to the lower
+// token however the row is cut.  512 rows of 128000 fp32 logits, select 16: 262 MB in 61 us (4.3 TB/s), the issue slots
+// 63% busy: about 100 instructions a step of 512 logits, and as many again for what passes into the lists.
 //
-// beam_pick_kernel (bound by latency): one CTA per request joins each beam's segments -- their sums in 64 bits, their lists
-// by bitonic merges -- and takes the best head of the beams' lists `select` times, comparing values in 64 bits, so that no
-// 32-bit rounding of a value decides.  A beam's own continuations are in the exact order of their logits.  Between beams the
-// log-sums' errors remain, whose terms lanes and warps add in fp32: at most (16 + 34 s) 2^-24 with s steps a warp, 1.7e-5 at
-// 8 steps; values that lie nearer to each other than twice that may change places.  About 8 us, most of it the way from the
-// partial sums to the first choice.
+// beam_pick_kernel (bound by latency): one CTA per request joins each beam's segments -- their sums in 64 bits, their
+// lists by bitonic merges -- and takes the best head of the beams' lists `select` times, comparing values in 64 bits,
+// so that no 32-bit rounding of a value decides.  A beam's own continuations are in the exact order of their logits.
+// Between beams the log-sums' errors remain, whose terms lanes and warps add in fp32: at most (16 + 34 s) 2^-24 with s
+// steps a warp, 1.7e-5 at 8 steps; values that lie nearer to each other than twice that may change places.  About 8 us,
+// most of it the way from the partial sums to the first choice.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -92,8 +91,8 @@ __device__ __forceinline__ unsigned long long warp_merge_desc(unsigned long long
 
 // One step of a row, 16 logits per lane: element e of a lane is token at + ((e / N) * 32 + lane) * N + e % N - shift.
 // Vec: 16-byte loads, where all rows of a request lie alike against 16-byte boundaries.  Else single loads of
-// neighbouring tokens by neighbouring lanes: with an odd vocabulary the rows start at different offsets, and vectors would
-// group the sums of two equal rows differently, so that their tie fell to a rounding.
+// neighbouring tokens by neighbouring lanes: with an odd vocabulary the rows start at different offsets, and vectors
+// would group the sums of two equal rows differently, so that their tie fell to a rounding.
 template <class T, bool Vec>
 struct BeamStep {
     static constexpr int N = 1;
@@ -117,8 +116,8 @@ struct BeamStep<T, true> {
     static constexpr int kVecs = kBeamLane / N;    // vectors of a lane
     static __device__ __forceinline__ float one(const T* p) { return BeamStep<T, false>::one(p); }
 };
-// A warp's steps on their way, each lane's vectors in places of its own: copied asynchronously, so that three steps are in
-// flight without registers, and read back by the lane that asked for them.
+// A warp's steps on their way, each lane's vectors in places of its own: copied asynchronously, so that three steps are
+// in flight without registers, and read back by the lane that asked for them.
 template <class T>
 struct BeamRing {
     using Step = BeamStep<T, true>;
@@ -126,12 +125,16 @@ struct BeamRing {
     __device__ __forceinline__ void load(int slot, const T* p, int lane) const {
 #pragma unroll
         for (int j = 0; j < Step::kVecs; ++j)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + static_cast<uint32_t>(slot * Step::kVecs + j) * 512u),
-                         "l"(p + (j * 32 + lane) * Step::N)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                         :
+                         : "r"(at + static_cast<uint32_t>(slot * Step::kVecs + j) * 512u),
+                           "l"(p + (j * 32 + lane) * Step::N)
                          : "memory");
     }
     static __device__ __forceinline__ void close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-    static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kBeamRing - 1) : "memory"); }
+    static __device__ __forceinline__ void wait() {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kBeamRing - 1) : "memory");
+    }
     __device__ __forceinline__ void get(int slot, float (&x)[kBeamLane]) const {
 #pragma unroll
         for (int j = 0; j < Step::kVecs; ++j) {
@@ -161,14 +164,15 @@ __device__ __forceinline__ float max_of(const float (&x)[kBeamLane], float (&gro
     float top = -INFINITY;
 #pragma unroll
     for (int g = 0; g < kBeamLane / 8; ++g) {
-        const float a = fmaxf(fmaxf(x[8 * g], x[8 * g + 1]), x[8 * g + 2]), b = fmaxf(fmaxf(x[8 * g + 3], x[8 * g + 4]), x[8 * g + 5]);
+        const float a = fmaxf(fmaxf(x[8 * g], x[8 * g + 1]), x[8 * g + 2]);
+        const float b = fmaxf(fmaxf(x[8 * g + 3], x[8 * g + 4]), x[8 * g + 5]);
         group[g] = fmaxf(fmaxf(a, b), fmaxf(x[8 * g + 6], x[8 * g + 7]));
         top = fmaxf(top, group[g]);
     }
     return top;
 }
-// Sum of exp(x - ref), two at a time: the difference is taken first, so that the large terms, whose difference is small,
-// are exact to the exponential's own error.
+// Sum of exp(x - ref), two at a time: the difference is taken first, so that the large terms, whose difference is
+// small, are exact to the exponential's own error.
 __device__ __forceinline__ float expsum(const float (&x)[kBeamLane], float ref) {
     const uint64_t back = pack2(-ref, -ref), log2e = pack2(1.4426950408889634f, 1.4426950408889634f);
     uint64_t t[2] = {0ull, 0ull};
@@ -231,8 +235,8 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
         return;
     }
     const T* base = static_cast<const T*>(p.logits) + row * p.row_stride;
-    // Steps start at 16-byte boundaries: token = place - shift.  A row's warps take its steps in turn, so that at any time
-    // they read one stretch of memory.
+    // Steps start at 16-byte boundaries: token = place - shift.  A row's warps take its steps in turn, so that at any
+    // time they read one stretch of memory.
     const int shift = Vec ? static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15u) / sizeof(T)) : 0;
     const int end = p.vocab + shift, first = seg * kBeamStep, ahead = p.segs * kBeamStep;
     const int n = first < end ? (end - first - 1) / ahead + 1 : 0;  // steps of this warp
@@ -275,8 +279,8 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
     for (int k = 0; k < (Vec ? kBeamRing : 1); ++k) ask(k);
     float m = -INFINITY, sum = 0.f;
     unsigned long long best = 0ull, least = 0ull;  // the list (one entry per lane); what an entry has to exceed
-    // The same as a value and a token.  An equal value counts only before that token, which lies ahead only where another
-    // warp set the floor.
+    // The same as a value and a token.  An equal value counts only before that token, which lies ahead only where
+    // another warp set the floor.
     float lv = -INFINITY;
     int ltok = 0x7fffffff;
     auto refresh = [&] {
@@ -285,9 +289,9 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
             ltok = static_cast<int>(~static_cast<uint32_t>(least));
         }
     };
-    // After steps 1, 2, 4, ... the warps show their lists; the first one joins them and raises the floor for all.  Each such
-    // moment has its own barrier and its own place, so the other warps only arrive and go on.  Every warp of the CTA that has
-    // a share takes part in all of them.
+    // After steps 1, 2, 4, ... the warps show their lists; the first one joins them and raises the floor for all.  Each
+    // such moment has its own barrier and its own place, so the other warps only arrive and go on.  Every warp of the
+    // CTA that has a share takes part in all of them.
     int show = 0, shows = 0;
     if (partners > 1)
         while (shows < kBeamShows && (1 << shows) < p.seg_steps) ++shows;
@@ -343,8 +347,8 @@ __global__ void __launch_bounds__(kBeamWarps * 32, 7) beam_scan_kernel(const Bea
         float top = max_of(x, group);
         float mn = fmaxf(m, top);
         float add = expsum(x, mn > -INFINITY ? mn : 0.f);
-        // A NaN or a +inf among them shows here: each term is at most 1 else.  (Asked of the whole warp, so that what is rare
-        // is branched over and not predicated.)
+        // A NaN or a +inf among them shows here: each term is at most 1 else.  (Asked of the whole warp, so that what
+        // is rare is branched over and not predicated.)
         if (__any_sync(0xffffffffu, !(add <= static_cast<float>(kBeamLane)))) {
             ban(x);
             top = max_of(x, group);
@@ -424,7 +428,8 @@ __global__ void __launch_bounds__(kPickWarps * 32) beam_pick_kernel(const BeamPa
     const long long row0 = static_cast<long long>(blockIdx.x) * p.beams;
     const int per = max(1, kPickWarps / p.beams);  // warps that share a beam's lists
     auto fold = [&](unsigned long long best, unsigned long long k) {  // only a list whose head gets in
-        return __shfl_sync(0xffffffffu, k, 0) > __shfl_sync(0xffffffffu, best, p.select - 1) ? warp_merge_desc(best, k, lane) : best;
+        const bool in = __shfl_sync(0xffffffffu, k, 0) > __shfl_sync(0xffffffffu, best, p.select - 1);
+        return in ? warp_merge_desc(best, k, lane) : best;
     };
     griddep_wait();
     for (int b0 = 0; b0 < p.beams; b0 += kPickWarps) {
@@ -460,7 +465,8 @@ __global__ void __launch_bounds__(kPickWarps * 32) beam_pick_kernel(const BeamPa
                 double total = 0.0;
 #pragma unroll
                 for (int i = 0; i < kBeamSegs / 32; ++i)
-                    if (ml[i].x > -INFINITY) total += static_cast<double>(ml[i].y) * exp(static_cast<double>(ml[i].x) - top);
+                    if (ml[i].x > -INFINITY)
+                        total += static_cast<double>(ml[i].y) * exp(static_cast<double>(ml[i].x) - top);
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
                 lse = top > -INFINITY ? top + log(total) : -static_cast<double>(INFINITY);
@@ -510,8 +516,8 @@ __global__ void __launch_bounds__(kPickWarps * 32) beam_pick_kernel(const BeamPa
 namespace kvpi {
 namespace {
 
-// Segments of a row: about 28 warps for each processor -- what the scan's registers let reside -- in fours, since a CTA's
-// warps share what they have found; none shorter than one step.
+// Segments of a row: about 28 warps for each processor -- what the scan's registers let reside -- in fours, since a
+// CTA's warps share what they have found; none shorter than one step.
 void plan_beam(const kvp_beam_args& a, int* segs, int* steps) {
     const long long rows = static_cast<long long>(a.batch) * a.beams;
     const long long total = (static_cast<long long>(a.vocab) + 7 + kvpd::kBeamStep - 1) / kvpd::kBeamStep;
@@ -553,15 +559,18 @@ extern "C" KVP_API int kvp_beam_select(const kvp_beam_args* a, void* stream) {
     clear_error();
     int rc = check_beam(a);
     if (rc != KVP_OK || a->batch == 0) return rc;
-    if (!a->logits || !a->scores || !a->out_scores || !a->out_parents || !a->out_tokens) return fail(KVP_EINVAL, "null buffer");
-    if (reinterpret_cast<uintptr_t>(a->logits) % dtype_bytes(a->logits_dtype)) return fail(KVP_EINVAL, "misaligned logits");
+    if (!a->logits || !a->scores || !a->out_scores || !a->out_parents || !a->out_tokens)
+        return fail(KVP_EINVAL, "null buffer");
+    if (reinterpret_cast<uintptr_t>(a->logits) % dtype_bytes(a->logits_dtype))
+        return fail(KVP_EINVAL, "misaligned logits");
     kvpd::BeamParams p;
     plan_beam(*a, &p.segs, &p.seg_steps);
     const size_t items = static_cast<size_t>(a->batch) * a->beams * p.segs;
     const size_t keys_off = (items * 8 + 255) / 256 * 256;
     if (!a->workspace || a->workspace_bytes < keys_off + items * a->select * 8)
         return fail(KVP_ENOSPACE, "workspace smaller than kvp_beam_workspace_size()");
-    if ((reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0) return fail(KVP_EINVAL, "workspace must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0)
+        return fail(KVP_EINVAL, "workspace must be 16-byte aligned");
     p.logits = a->logits;
     p.scores = a->scores;
     p.out_scores = a->out_scores;
@@ -579,10 +588,11 @@ extern "C" KVP_API int kvp_beam_select(const kvp_beam_args* a, void* stream) {
     const unsigned grid = static_cast<unsigned>(static_cast<size_t>(a->batch) * a->beams *
                                                 ((p.segs + kvpd::kBeamWarps - 1) / kvpd::kBeamWarps));
     const bool vec = a->beams == 1 || (p.row_stride * dtype_bytes(a->logits_dtype)) % 16 == 0;
-    auto scan = a->logits_dtype == KVP_DTYPE_F32   ? (vec ? kvpd::beam_scan_kernel<float, true> : kvpd::beam_scan_kernel<float, false>)
-                : a->logits_dtype == KVP_DTYPE_F16 ? (vec ? kvpd::beam_scan_kernel<__half, true> : kvpd::beam_scan_kernel<__half, false>)
-                                                   : (vec ? kvpd::beam_scan_kernel<__nv_bfloat16, true>
-                                                          : kvpd::beam_scan_kernel<__nv_bfloat16, false>);
+    auto scan = vec ? kvpd::beam_scan_kernel<__nv_bfloat16, true> : kvpd::beam_scan_kernel<__nv_bfloat16, false>;
+    if (a->logits_dtype == KVP_DTYPE_F32)
+        scan = vec ? kvpd::beam_scan_kernel<float, true> : kvpd::beam_scan_kernel<float, false>;
+    else if (a->logits_dtype == KVP_DTYPE_F16)
+        scan = vec ? kvpd::beam_scan_kernel<__half, true> : kvpd::beam_scan_kernel<__half, false>;
     scan<<<grid, kvpd::kBeamWarps * 32, 0, s>>>(p);
     rc = cuda_status(cudaGetLastError(), "beam scan launch");
     if (rc != KVP_OK) return rc;

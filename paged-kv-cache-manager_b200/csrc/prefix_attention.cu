@@ -5,42 +5,44 @@
 // matrix-vector product per sequence becomes a matrix product, S = Q K^T and O = P V, for the tensor cores:
 //   read  2 * P * head_dim * 2 bytes of K and V per kv head (P shared tokens),
 //   compute 4 * m * g * P * head_dim flops (half as many again for the rests of P, below).
-// Up to about 170 rows the bytes take longer than these products at the rates of a copy and of a large matrix product (256
-// without the rests); beyond, the tensor cores and the exponentials bound it.
+// Up to about 170 rows the bytes take longer than these products at the rates of a copy and of a large matrix product
+// (256 without the rests); beyond, the tensor cores and the exponentials bound it.
 //
-// Three launches.  prefix_kernel attends over the shared blocks, own_kernel over each sequence's own blocks, beside it on
-// what it leaves of an SM; both leave partial results, which join_kernel joins.
+// Three launches.  prefix_kernel attends over the shared blocks, own_kernel over each sequence's own blocks, beside it
+// on what it leaves of an SM; both leave partial results, which join_kernel joins.
 //
-// prefix_kernel: one CTA per SM takes an even share of the step's units -- a unit is one tile of 128 keys for one (group,
-// kv head, pair of row tiles), of fewer where the blocks' size shares no factor of 8 with it: as many whole blocks as fit,
-// copied one by one (16 groups with blocks of 5 tokens: 55 us, of 16 tokens 51; by whole contexts 916) -- regardless of where
-// groups and heads begin and end.  A row tile is as many whole members as fit 128 rows (tcgen05's M).  Two warpgroups of softmax, one per accumulator pair in TMEM, take turns with the tensor
-// cores: while one exponentiates its scores, the MMAs of the other run.  Exponentiating at the same time gains nothing: with
-// two score buffers of 64 keys each, which keep both at it, 256 sequences over 16384 tokens took 176 us instead of 148; with
-// a quarter of the exponentials as a polynomial on the FMA pipe 150 (all three with P in one 16-bit number).
+// prefix_kernel: one CTA per SM takes an even share of the step's units -- a unit is one tile of 128 keys for one
+// (group, kv head, pair of row tiles), of fewer where the blocks' size shares no factor of 8 with it: as many whole
+// blocks as fit, copied one by one (16 groups with blocks of 5 tokens: 55 us, of 16 tokens 51; by whole contexts 916)
+// -- regardless of where groups and heads begin and end.  A row tile is as many whole members as fit 128 rows
+// (tcgen05's M).  Two warpgroups of softmax, one per accumulator pair in TMEM, take turns with the tensor cores: while
+// one exponentiates its scores, the MMAs of the other run.  Exponentiating at the same time gains nothing: with two
+// score buffers of 64 keys each, which keep both at it, 256 sequences over 16384 tokens took 176 us instead of 148;
+// with a quarter of the exponentials as a polynomial on the FMA pipe 150 (all three with P in one 16-bit number).
 //   two row tiles:  the warpgroups take one tile each and every key tile; K and V are read once for 256 rows.
-//   one row tile:   both warpgroups take the same rows, one the even, the other the odd key tiles, so that the wait for a
-//                   tile's exponentials is covered by the other tile; they leave two partial results.
+//   one row tile:   both warpgroups take the same rows, one the even, the other the odd key tiles, so that the wait for
+//                   a tile's exponentials is covered by the other tile; they leave two partial results.
 // Scores S and accumulators O live in TMEM (S0, S1 at columns 0 and 128, O0, O1 at 256 and 256 + head_dim); the
-// probabilities P overwrite S as 16-bit numbers and are the A operand of the second product straight from TMEM.  A thread
-// owns one row: the running maximum and sum need no exchange.  O is rescaled only when a row's maximum has grown by more
-// than 2^3 (fp16) or 2^8 (bf16) since its last rescaling: P, O and the sum have one scale, so nothing is lost.
-// P is kept as a part and a rest of the pools' 16-bit type each, as the own parts and the decode attention keep it: the two
-// products with V hold 16 (bf16) or 22 (fp16) bits of each weight, and the output's only rounding that counts is its own.
-// With one 16-bit number each the weights' roundings were as large as a bf16 output's (1.66e-3 against 64 bits became
-// 2.3e-3, relative to all outputs' size 1e-4 became 2.5e-3), and an fp32 output held no more.  It costs half of the tensor
-// cores' work on top: 16 groups 46.9 -> 51.9 us, 512 samples 71.2 -> 78.7, 256 over 16384 154.9 -> 186.4, 4 beams the same.
+// probabilities P overwrite S as 16-bit numbers and are the A operand of the second product straight from TMEM.  A
+// thread owns one row: the running maximum and sum need no exchange.  O is rescaled only when a row's maximum has grown
+// by more than 2^3 (fp16) or 2^8 (bf16) since its last rescaling: P, O and the sum have one scale, so nothing is lost.
+// P is kept as a part and a rest of the pools' 16-bit type each, as the own parts and the decode attention keep it: the
+// two products with V hold 16 (bf16) or 22 (fp16) bits of each weight, and the output's only rounding that counts is
+// its own.  With one 16-bit number each the weights' roundings were as large as a bf16 output's (1.66e-3 against 64
+// bits became 2.3e-3, relative to all outputs' size 1e-4 became 2.5e-3), and an fp32 output held no more.  It costs half of
+// the tensor cores' work on top: 16 groups 46.9 -> 51.9 us, 512 samples 71.2 -> 78.7, 256 over 16384 154.9 -> 186.4, 4
+// beams the same.
 //
-// Measured, 32 query and 8 kv heads of 128, bf16: a pair of row tiles takes 5260 clocks per key tile, of which the matrix
-// products are 3070 (3750 and 2050 with P in one 16-bit number); starting (groups, table, first tiles) takes 12000 clocks,
-// writing the partial results 5000 to 8000.  512 sequences over 2048 shared tokens and up to 100 own ones: 79 us (prefix_kernel
-// alone 49, the own parts alone 31, joining 13, each with cold caches); 256 over 16384, up to 512 own: 171 us (119, 63, 12);
-// 4 beams over 2048, 24 own: 17 us.
-// prefix_kernel leaves shared memory unused on purpose: with 224 KB instead of 192 the L1, which the own parts' loads go
-// through, shrinks to 28 KB, and the first two calls took 85 and 174 us where they took 72 and 149.
-// The own parts are cut alike, into at most 8 each: a long one beside many short ones, or few long ones, are slower than by
-// kvp_paged_attention, whose partition follows the lengths (2 sequences of 30000 own tokens: 320 us against 105; 255 of 100
-// beside one of 30000: 1227 against 96; 64 of 8192 over 2048 shared ones: 400 against 363).
+// Measured, 32 query and 8 kv heads of 128, bf16: a pair of row tiles takes 5260 clocks per key tile, of which the
+// matrix products are 3070 (3750 and 2050 with P in one 16-bit number); starting (groups, table, first tiles) takes
+// 12000 clocks, writing the partial results 5000 to 8000.  512 sequences over 2048 shared tokens and up to 100 own
+// ones: 79 us (prefix_kernel alone 49, the own parts alone 31, joining 13, each with cold caches); 256 over 16384, up
+// to 512 own: 171 us (119, 63, 12); 4 beams over 2048, 24 own: 17 us.
+// prefix_kernel leaves shared memory unused on purpose: with 224 KB instead of 192 the L1, which the own parts' loads
+// go through, shrinks to 28 KB, and the first two calls took 85 and 174 us where they took 72 and 149.
+// The own parts are cut alike, into at most 8 each: a long one beside many short ones, or few long ones, are slower
+// than by kvp_paged_attention, whose partition follows the lengths (2 sequences of 30000 own tokens: 320 us against
+// 105; 255 of 100 beside one of 30000: 1227 against 96; 64 of 8192 over 2048 shared ones: 400 against 363).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -80,7 +82,8 @@ struct PrefixParams {
     const int32_t* prefix_blocks;
     const int32_t* group_starts;
     int32_t* status;
-    int2* spans;               // first and last CTA of each (group, kv head, pair), at its first row's (member, kv head)
+    // first and last CTA of each (group, kv head, pair), at its first row's (member, kv head)
+    int2* spans;
     float2* part_ml;           // partial rows: (maximum in log2 units, sum)
     float* part_o;
     OwnMeta* own_meta;         // of each (sequence, kv head)
@@ -166,18 +169,20 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
 // Waits for the loads so far; r: what the last one fills, so that no use of it is moved before the wait.
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15])::"memory");
     asm volatile(""
-                 : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+                 : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])::"memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // One 32-byte sector of global memory.
 __device__ __forceinline__ void store_sector(float* p, const uint32_t* v) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
 
@@ -218,7 +223,8 @@ __device__ __forceinline__ float row_max(uint32_t addr, uint32_t (&s)[2][32], in
             mask_keys(s[b], valid - (h + b) * 32);
 #pragma unroll
             for (int e = 0; e < 32; e += 2)
-                top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[b][e])), __uint_as_float(s[b][e + 1]));
+                top[(e >> 1) & 3] = fmaxf(fmaxf(top[(e >> 1) & 3], __uint_as_float(s[b][e])),
+                                          __uint_as_float(s[b][e + 1]));
         }
     }
     return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
@@ -228,8 +234,8 @@ __device__ __forceinline__ float exp2_unit(float x) {  // free to be moved, unli
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// A partial row's maximum and sum as they are left for joining.  Where every score was NaN the maximum, which passes over
-// them, is still -inf, the mark of a part without keys: the row has to become NaN, not to go without these keys.
+// A partial row's maximum and sum as they are left for joining.  Where every score was NaN the maximum, which passes
+// over them, is still -inf, the mark of a part without keys: the row has to become NaN, not to go without these keys.
 template <class KV>
 __device__ __forceinline__ float2 partial(float m, float l) {
     return make_float2(m == -INFINITY && l != l ? 0.f : m - kLift<KV>, l);
@@ -266,7 +272,8 @@ __device__ __forceinline__ long long floor_div(long long a, long long b, long lo
 }
 // CTA c of G owns units [c T / G, (c + 1) T / G).
 __device__ __forceinline__ long long first_unit(int c, long long T, int G) {
-    if (T < (1 << 22)) return static_cast<unsigned>(c) * static_cast<unsigned>(T) / static_cast<unsigned>(G);  // c <= 1023
+    // c <= 1023
+    if (T < (1 << 22)) return static_cast<unsigned>(c) * static_cast<unsigned>(T) / static_cast<unsigned>(G);
     return floor_div(c, T, G);
 }
 
@@ -289,7 +296,8 @@ struct WorkList {
             grp = load_group(p, ++gi);
         }
         const long long rel = t - first;
-        const int triple = static_cast<int>(rel < (1LL << 32) ? static_cast<unsigned>(rel) / static_cast<unsigned>(grp.ktiles) : rel / grp.ktiles);
+        const int triple = static_cast<int>(
+            rel < (1LL << 32) ? static_cast<unsigned>(rel) / static_cast<unsigned>(grp.ktiles) : rel / grp.ktiles);
         w.k0 = static_cast<int>(rel - static_cast<long long>(triple) * grp.ktiles);
         w.n = static_cast<int>(min(static_cast<long long>(grp.ktiles - w.k0), end - t));
         t += w.n;
@@ -302,7 +310,8 @@ struct WorkList {
         w.rows0 = min(left, p.mt) * p.g;
         w.rows1 = min(max(left - p.mt, 0), p.mt) * p.g;
         // two partial rows per (member, head) row of the batch, 256 more per CTA: a stretch's rows are its own
-        w.pair_at = static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(w.head) * grp.members + w.member0;
+        w.pair_at = static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(w.head) * grp.members +
+            w.member0;
         w.part_row = 2LL * p.g * w.pair_at + static_cast<long long>(cta) * 2 * kRows;
         return true;
     }
@@ -340,7 +349,8 @@ __device__ __forceinline__ Start find_start_few(const PrefixParams& p, Group* gr
 // More: the CTA together, a thread per group and kPrefixThreads groups at a time.
 __device__ __forceinline__ Start find_start(const PrefixParams& p, long long* warp_sum, Start* found, Group* grp) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto scan = [&](long long u, long long carry, long long* mine) {  // all of a chunk; *mine: what lies before this thread
+    // all of a chunk; *mine: what lies before this thread
+    auto scan = [&](long long u, long long carry, long long* mine) {
         long long x = u;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -361,7 +371,8 @@ __device__ __forceinline__ Start find_start(const PrefixParams& p, long long* wa
     };
     auto units_of = [&](int gi) { return gi < p.num_groups ? load_group(p, gi).units(p.kvh) : 0ll; };
     long long total = 0, mine = 0;
-    for (int g0 = 0; g0 < p.num_groups; g0 += kPrefixThreads) total += scan(units_of(g0 + static_cast<int>(threadIdx.x)), total, &mine);
+    for (int g0 = 0; g0 < p.num_groups; g0 += kPrefixThreads)
+        total += scan(units_of(g0 + static_cast<int>(threadIdx.x)), total, &mine);
     const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
     if (static_cast<int>(blockIdx.x) >= G) return Start{total, 0, 0};
     const long long at = first_unit(blockIdx.x, total, G);
@@ -427,9 +438,9 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
     constexpr uint32_t kCol = kKeys * 128;           // bytes of one such column of a tile
     constexpr uint32_t kTile = NCH * kCol;           // one tile of Q, K or V
     constexpr uint32_t kO = 256;                     // TMEM column of the first accumulator
-    // How far (log2) a score may exceed the maximum that P, O and the sum refer to: P, which starts at 2^kLift, has to stay
-    // below the type's largest value, and O below fp32's, which a bf16 V may come near to by itself (with 2^40 values of
-    // 2^88 became infinite).
+    // How far (log2) a score may exceed the maximum that P, O and the sum refer to: P, which starts at 2^kLift, has to
+    // stay below the type's largest value, and O below fp32's, which a bf16 V may come near to by itself (with 2^40
+    // values of 2^88 became infinite).
     constexpr float kFar = std::is_same<KV, __half>::value ? 3.f : 8.f;
     __shared__ PrefixShared sh;
     extern __shared__ uint8_t dyn[];
@@ -463,9 +474,9 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
         prefetch_tensormap(&kmap);
         prefetch_tensormap(&vmap);
     }
-    // Nothing is read or written before the kernels ahead are done, and no tensor memory is held while waiting for them.
-    // The kernels behind start only once every CTA here has its own: one of them that takes tensor memory while it waits
-    // for this kernel could otherwise keep it from ever getting any.
+    // Nothing is read or written before the kernels ahead are done, and no tensor memory is held while waiting for
+    // them.  The kernels behind start only once every CTA here has its own: one of them that takes tensor memory while
+    // it waits for this kernel could otherwise keep it from ever getting any.
     griddep_wait();
     if (p.keys < kKeys) {  // rows of V that no copy fills: their weights are zero, and so have they to be
         const int words = (kKeys - p.keys) * 8;  // of 16 bytes
@@ -480,7 +491,8 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
         griddep_launch_dependents();
     }
     WorkList list;
-    const Start from = p.num_groups <= 32 ? find_start_few(p, &list.grp) : find_start(p, sh.warp_sum, &sh.found, &list.grp);
+    const Start from =
+        p.num_groups <= 32 ? find_start_few(p, &list.grp) : find_start(p, sh.warp_sum, &sh.found, &list.grp);
     const int cta = blockIdx.x, G = static_cast<int>(min(static_cast<long long>(gridDim.x), from.total));
     tc_fence_before();
     __syncthreads();
@@ -499,8 +511,8 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
 
     if (warp >= 9) {
         // ------------------------------------------------------------ loads: K and the queries, and V
-        // Each lane issues one copy (a run of tokens within a block, 64 dims); the copies of a warp's lanes are issued one
-        // after the other, at about 60 clocks each, which is why K and V have a warp each.
+        // Each lane issues one copy (a run of tokens within a block, 64 dims); the copies of a warp's lanes are issued
+        // one after the other, at about 60 clocks each, which is why K and V have a warp each.
         const int v = warp - 9, slots = v ? kSlotsV : kSlotsK;
         const uint32_t ring = v ? ring_v : ring_k;
         const CUtensorMap* map = v ? &vmap : &kmap;
@@ -509,12 +521,13 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
         int loaded = 0, queries = 0;  // tiles and query loads issued
         while (ok && list.next(p, w)) {
             const int32_t* trow = p.tables + static_cast<long long>(w.start) * p.max_blocks;
-            // The pool row of a run of a tile; for the runs of a lane's own, looked up a tile ahead, so that the table's latency is
-            // past when it is needed.
+            // The pool row of a run of a tile; for the runs of a lane's own, looked up a tile ahead, so that the
+            // table's latency is past when it is needed.
             const int run = lane / NCH, c = lane - run * NCH;
             auto row_at = [&](int kt, int run) {
                 const int tok = kt * p.keys + run * p.run;
-                if (run >= p.runs || tok >= w.tokens || kt >= w.k0 + w.n) return p.oob_row;  // zeros behind the shared tokens
+                // zeros behind the shared tokens
+                if (run >= p.runs || tok >= w.tokens || kt >= w.k0 + w.n) return p.oob_row;
                 const int bi = p.Bshift >= 0 ? tok >> p.Bshift : tok / p.B;
                 const int blk = __ldg(trow + bi);
                 if (blk >= 0 && blk < p.num_blocks) return blk * p.B + (tok - bi * p.B);
@@ -533,7 +546,8 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                     mbar_arrive_expect_tx(bar, static_cast<uint32_t>(tiles * NCH * p.mt * p.g) * 128u);
                     for (int t = 0; t < tiles; ++t)
                         for (int k = 0; k < NCH; ++k)
-                            tma_load_3d(base + t * kTile + k * kCol, &qmap, bar, k * 64, w.head * p.g, w.start + w.member0 + t * p.mt);
+                            tma_load_3d(base + t * kTile + k * kCol, &qmap, bar, k * 64, w.head * p.g,
+                                        w.start + w.member0 + t * p.mt);
                 }
                 __syncwarp();
             }
@@ -544,10 +558,11 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                 if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(p.keys) * NCH * 128u);
                 __syncwarp();
                 if (run < p.runs)
-                    tma_load_3d(ring + at.slot * kTile + c * kCol + static_cast<uint32_t>(run * p.run) * 128u, map, bar, c * 64,
-                                w.head, row);
+                    tma_load_3d(ring + at.slot * kTile + c * kCol + static_cast<uint32_t>(run * p.run) * 128u, map, bar,
+                                c * 64, w.head, row);
                 for (int i = 32 + lane; i < p.runs * NCH; i += 32)  // small blocks: more runs than lanes
-                    tma_load_3d(ring + at.slot * kTile + (i % NCH) * kCol + static_cast<uint32_t>(i / NCH * p.run) * 128u, map, bar,
+                    tma_load_3d(ring + at.slot * kTile + (i % NCH) * kCol +
+                                static_cast<uint32_t>(i / NCH * p.run) * 128u, map, bar,
                                 i % NCH * 64, w.head, row_at(w.k0 + j, i / NCH));
                 row = next_row;
                 at = at.next(slots);
@@ -566,14 +581,15 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
     } else if (warp == 8) {
         // ------------------------------------------------------------ MMAs, one thread
         // One thread for both warpgroups keeps their products one after the other, and with them the turns of the
-        // warpgroups: issued by two threads the products of both ran side by side, both softmaxes waited for them and then
-        // ran at the same time, 4950 clocks for a pair of tiles.
+        // warpgroups: issued by two threads the products of both ran side by side, both softmaxes waited for them and
+        // then ran at the same time, 4950 clocks for a pair of tiles.
         if (lane == 0) {
             const uint32_t qk_desc = mma_desc(p.bf16, kKeys, false);
             const uint32_t pv_desc = mma_desc(p.bf16, D, true);
             bool ok = true;
             Cursor kat{0, 0u}, vat{0, 0u};
-            uint32_t seg = 0, turn0 = 0, turn1 = 0;  // parities of the next queries and of the next P tile of each warpgroup
+            // parities of the next queries and of the next P tile of each warpgroup
+            uint32_t seg = 0, turn0 = 0, turn1 = 0;
             const uint32_t q_lo = desc_lo(base, 16), k_lo = desc_lo(ring_k, 16), v_lo = desc_lo(ring_v, kCol);
             auto qk = [&](int t, int qt, int slot) {
                 const uint32_t q = q_lo + qt * (kTile >> 4), k = k_lo + static_cast<uint32_t>(slot) * (kTile >> 4);
@@ -581,7 +597,8 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                 for (int c = 0; c < NCH; ++c)
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
-                        mma_ss(tmem + t * kKeys, q + ((c * kCol + s * 32) >> 4), kDescHi, k + ((c * kCol + s * 32) >> 4), kDescHi,
+                        mma_ss(tmem + t * kKeys, q + ((c * kCol + s * 32) >> 4), kDescHi,
+                               k + ((c * kCol + s * 32) >> 4), kDescHi,
                                qk_desc, c + s > 0);
                 tc_commit(smem_u32(&sh.s_full[t]));
             };
@@ -632,8 +649,9 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                     if (more) done_k();
                 }
                 if (ok) {
-                    // Only to a warpgroup that has a tile here: its own P gates the next stretch's products, so this barrier
-                    // never completes twice before it has looked.  One without a tile would be gated by nothing.
+                    // Only to a warpgroup that has a tile here: its own P gates the next stretch's products, so this
+                    // barrier never completes twice before it has looked.  One without a tile would be gated by
+                    // nothing.
                     tc_commit(smem_u32(&sh.o_full[0]));
                     if (two || w.n > 1) tc_commit(smem_u32(&sh.o_full[1]));
                     tc_commit(smem_u32(&sh.q_free));
@@ -665,8 +683,8 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
                 if (busy) {
                     tc_fence_after();
                     const int valid = min(w.tokens - (w.k0 + j) * p.keys, p.keys);
-                    // The row's maximum, then the exponentials, the scores read twice and 32 at a time: loops, not one long
-                    // stretch of code, whose way through the instruction caches cost a launch 10 us.
+                    // The row's maximum, then the exponentials, the scores read twice and 32 at a time: loops, not one
+                    // long stretch of code, whose way through the instruction caches cost a launch 10 us.
                     uint32_t s[2][32];
                     const float mx = row_max(s_addr, s, valid) * p.sl2;
                     if (j == j0) {
@@ -703,7 +721,8 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
 #pragma unroll
                                 for (int i = 0; i < 8; ++i) {
                                     const float2 x = unpack2(fma2(
-                                        pack2(__uint_as_float(s[b][k + 2 * i]), __uint_as_float(s[b][k + 2 * i + 1])), scale2, ref2));
+                                        pack2(__uint_as_float(s[b][k + 2 * i]), __uint_as_float(s[b][k + 2 * i + 1])),
+                                            scale2, ref2));
                                     const float2 e = make_float2(exp2_unit(x.x), exp2_unit(x.y));
                                     sum[i & 1] = add2(sum[i & 1], pack2(e.x, e.y));
                                     pk[i] = Tr::pack(e.x, e.y);
@@ -765,23 +784,24 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
 }
 
 // ---------------------------------------------------------------- own parts
-// 1 to 8 single warps, which wait for nothing from each other, share the own tokens of a (sequence, kv head), 16 at a time.
-// Bound by HBM, and by latency where the own parts are short, which most of them are: a warp takes K and V from global memory
-// straight into the registers of its matrix instructions, without a pipeline to fill and drain.  Alone it takes 20 us at 512
-// sequences with up to 100 own tokens, 44 us at 256 with up to 512 (6.5 TB/s), 31 and 63 with cold caches.  CTAs of four warps that also joined their
-// results with the shared part's took 42 and 71 us; clusters of eight such CTAs, where pairs are few, 19.2 us for the whole
-// call at 4 beams instead of 16.2.
-//   S^T[tokens x heads] = K Q^T:  a lane holds 8 neighbouring dims of a token's K (one 16-byte load); the sum over dims does
-//                                 not care for their order, so these are the dims of two steps, for K and Q alike.
-//   O^T[dims x heads] += V^T P^T: a lane holds 8 neighbouring dims of four tokens' V and pairs up two tokens' halves; the
-//                                 rows of the instruction are dims in an order of their own.  P^T by an 8 x 8 transposition.
+// 1 to 8 single warps, which wait for nothing from each other, share the own tokens of a (sequence, kv head), 16 at a
+// time.  Bound by HBM, and by latency where the own parts are short, which most of them are: a warp takes K and V from
+// global memory straight into the registers of its matrix instructions, without a pipeline to fill and drain.  Alone it
+// takes 20 us at 512 sequences with up to 100 own tokens, 44 us at 256 with up to 512 (6.5 TB/s), 31 and 63 with cold
+// caches.  CTAs of four warps that also joined their results with the shared part's took 42 and 71 us; clusters of
+// eight such CTAs, where pairs are few, 19.2 us for the whole call at 4 beams instead of 16.2.
+//   S^T[tokens x heads] = K Q^T:  a lane holds 8 neighbouring dims of a token's K (one 16-byte load); the sum over dims
+//                                 does not care for their order, so these are the dims of two steps, for K and Q alike.
+//   O^T[dims x heads] += V^T P^T: a lane holds 8 neighbouring dims of four tokens' V and pairs up two tokens' halves;
+//                                 the rows of the instruction are dims in an order of their own.  P^T by an 8 x 8
+//                                 transposition.
 // The heads are the 8 columns of the instruction (NT times, for more than 8): as its 16 rows they took twice the
-// instructions and accumulators, and twice the time at head_dim 128.  With more than 8 heads per kv head and head_dim 128 the
-// kernel spills 140 bytes of registers, else at most 16; ten warps an SM, which need no spills, took 116 us instead of 113 (256 sequences, 64
-// query and 4 kv heads, 256 shared and 512 own tokens).
+// instructions and accumulators, and twice the time at head_dim 128.  With more than 8 heads per kv head and head_dim
+// 128 the kernel spills 140 bytes of registers, else at most 16; ten warps an SM, which need no spills, took 116 us
+// instead of 113 (256 sequences, 64 query and 4 kv heads, 256 shared and 512 own tokens).
 
-// Four partial results (maximum, sum; four columns of the output) at a time, folded into what there is.  One with the maximum
-// -inf is nothing, and its columns may never have been written.
+// Four partial results (maximum, sum; four columns of the output) at a time, folded into what there is.  One with the
+// maximum -inf is nothing, and its columns may never have been written.
 struct Fold {
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -814,22 +834,26 @@ __device__ __forceinline__ void store_out(const PrefixParams& p, size_t at, cons
         *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
     else
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
-            p.out_dtype == KVP_DTYPE_F16 ? make_uint2(F16Traits<__half>::pack(y[0], y[1]), F16Traits<__half>::pack(y[2], y[3]))
-                                         : make_uint2(F16Traits<__nv_bfloat16>::pack(y[0], y[1]), F16Traits<__nv_bfloat16>::pack(y[2], y[3]));
+            p.out_dtype == KVP_DTYPE_F16 ? make_uint2(F16Traits<__half>::pack(y[0], y[1]),
+                                                      F16Traits<__half>::pack(y[2], y[3]))
+                                         : make_uint2(F16Traits<__nv_bfloat16>::pack(y[0], y[1]),
+                                                      F16Traits<__nv_bfloat16>::pack(y[2], y[3]));
 }
 
 // Partial rows k0 .. k0 + 3 of the `count` that the shared part left of a query head.
 struct SharedParts {
     long long row0 = 0;
     int count = 0, parts = 1, rows = 0;
-    __device__ __forceinline__ void load(const PrefixParams& p, int j, int D, int col, int k0, float2 (&ml)[4], float4 (&x)[4]) const {
+    __device__ __forceinline__ void load(const PrefixParams& p, int j, int D, int col, int k0, float2 (&ml)[4],
+                                         float4 (&x)[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int k = k0 + i;
             const long long r = row0 + j + (parts == 2 ? static_cast<long long>(k >> 1) * 2 * kRows + (k & 1) * rows
                                                        : static_cast<long long>(k) * 2 * kRows);
             ml[i] = k < count ? __ldcg(&p.part_ml[r]) : make_float2(-INFINITY, 0.f);
-            x[i] = k < count ? __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[i] = k < count ? __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D + col))
+                : make_float4(0.f, 0.f, 0.f, 0.f);
         }
     }
 };
@@ -846,9 +870,9 @@ __device__ __forceinline__ SharedParts shared_parts(const PrefixParams& p, const
     return s;
 }
 
-// NT: groups of 8 query heads per kv head.  Its inputs were written before prefix_kernel, which lets this kernel start once it
-// has waited for the kernels ahead; so nothing is waited for, but for the last CTA, through which join_kernel waits for the
-// shared part.
+// NT: groups of 8 query heads per kv head.  Its inputs were written before prefix_kernel, which lets this kernel start
+// once it has waited for the kernels ahead; so nothing is waited for, but for the last CTA, through which join_kernel
+// waits for the shared part.
 template <int D, class KV, int NT>
 __global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const PrefixParams p) {
     using Tr = F16Traits<KV>;
@@ -856,7 +880,8 @@ __global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const Prefix
     constexpr int NH = D / 64;   // and that a lane of eight holds
     griddep_launch_dependents();
     const int lane = threadIdx.x, gid = lane >> 2, c4 = lane & 3;
-    const int item = static_cast<int>(blockIdx.x) / p.own_parts, rank = static_cast<int>(blockIdx.x) - item * p.own_parts;
+    const int item = static_cast<int>(blockIdx.x) / p.own_parts,
+        rank = static_cast<int>(blockIdx.x) - item * p.own_parts;
     const int seq = item / p.kvh, h = item - seq * p.kvh;
     const int len = __ldg(p.lens + seq), pb = __ldg(p.prefix_blocks + seq);
     const long long nblk = (static_cast<long long>(len) + p.B - 1) / p.B;
@@ -871,7 +896,8 @@ __global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const Prefix
     for (int nt = 0; nt < NT; ++nt) {
         const int j = 8 * nt + gid;
         const uint4* src = reinterpret_cast<const uint4*>(
-            static_cast<const KV*>(p.q) + (static_cast<long long>(seq) * p.nh + h * p.g + min(j, p.g - 1)) * D + c4 * 8);
+            static_cast<const KV*>(p.q) + (static_cast<long long>(seq) * p.nh + h * p.g + min(j, p.g - 1)) * D +
+                c4 * 8);
 #pragma unroll
         for (int i = 0; i < NI; ++i) qr[nt][i] = j < p.g ? __ldg(src + i * 4) : make_uint4(0u, 0u, 0u, 0u);
     }
@@ -900,7 +926,8 @@ __global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const Prefix
         for (int r = 0; r < 2; ++r) {
             const int x = __shfl_sync(0xffffffffu, row, gid + 8 * r);
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const KV*>(p.k_cache) +
-                                                              (static_cast<long long>(max(x, 0)) * p.kvh + h) * D + c4 * 8);
+                                                              (static_cast<long long>(max(x, 0)) * p.kvh + h) * D +
+                                                                  c4 * 8);
 #pragma unroll
             for (int i = 0; i < NI; ++i) kr[r][i] = x >= 0 ? __ldg(src + i * 4) : make_uint4(0u, 0u, 0u, 0u);
         }
@@ -910,7 +937,8 @@ __global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const Prefix
         for (int r = 0; r < 4; ++r) {
             const int x = __shfl_sync(0xffffffffu, row, 2 * c4 + (r & 1) + (r >> 1) * 8);
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const KV*>(p.v_cache) +
-                                                              (static_cast<long long>(max(x, 0)) * p.kvh + h) * D + gid * 8);
+                                                              (static_cast<long long>(max(x, 0)) * p.kvh + h) * D +
+                                                                  gid * 8);
 #pragma unroll
             for (int i = 0; i < NH; ++i) vr[r][i] = x >= 0 ? __ldg(src + i * 8) : make_uint4(0u, 0u, 0u, 0u);
         }
@@ -926,7 +954,8 @@ __global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const Prefix
         int lo = 0;
         for (int n = p.num_groups; n > 1;) {
             const int step = (n + 31) >> 5;
-            const unsigned below = __ballot_sync(0xffffffffu, lane * step < n && __ldg(p.group_starts + lo + lane * step) <= seq);
+            const unsigned below = __ballot_sync(0xffffffffu, lane * step < n &&
+                                                 __ldg(p.group_starts + lo + lane * step) <= seq);
             const int k = below ? 31 - __clz(below) : 0;
             lo += k * step;
             n = min(step, n - k * step);
@@ -936,7 +965,8 @@ __global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const Prefix
         OwnMeta meta = {0, -1, 1, 0, fine, 0};
         if (fine && grp.ktiles > 0) {
             const int member = seq - grp.start, member0 = member / (2 * p.mt) * 2 * p.mt, left = grp.members - member0;
-            meta.pair_at = static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(h) * grp.members + member0;
+            meta.pair_at = static_cast<long long>(grp.start) * p.kvh + static_cast<long long>(h) * grp.members +
+                member0;
             meta.row0 = 2LL * p.g * meta.pair_at + (member - member0) * p.g;  // two row tiles: one after the other
             if (left <= p.mt) {  // one: the even and the odd key tiles'
                 meta.parts = 2;
@@ -1028,14 +1058,15 @@ __global__ void __launch_bounds__(32, NT == 1 ? 16 : 12) own_kernel(const Prefix
 #pragma unroll
                     for (int t = 0; t < 4; t += 2)
                         *reinterpret_cast<float4*>(p.own_o + row * D + 64 * i + 8 * gid + 2 * t) =
-                            make_float4(o[nt][i * 4 + t][e], o[nt][i * 4 + t][2 + e], o[nt][i * 4 + t + 1][e], o[nt][i * 4 + t + 1][2 + e]);
+                            make_float4(o[nt][i * 4 + t][e], o[nt][i * 4 + t][2 + e], o[nt][i * 4 + t + 1][e],
+                                        o[nt][i * 4 + t + 1][2 + e]);
             }
     }
     if (blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
-// The own parts and the shared part's partial rows: a thread folds four columns of a (sequence, query head).  Bound by the
-// partial rows' way through L2, and three latencies.
+// The own parts and the shared part's partial rows: a thread folds four columns of a (sequence, query head).  Bound by
+// the partial rows' way through L2, and three latencies.
 template <int D>
 __global__ void __launch_bounds__(256) join_kernel(const PrefixParams p) {
     griddep_launch_dependents();
@@ -1055,7 +1086,8 @@ __global__ void __launch_bounds__(256) join_kernel(const PrefixParams p) {
             const bool some = k0 + i < p.own_parts;
             const long long r = row * p.own_parts + k0 + i;
             ml[i] = some ? __ldcg(&p.own_ml[r]) : make_float2(-INFINITY, 0.f);
-            x[i] = some ? __ldcg(reinterpret_cast<const float4*>(p.own_o + r * D + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[i] = some ? __ldcg(reinterpret_cast<const float4*>(p.own_o + r * D + col))
+                : make_float4(0.f, 0.f, 0.f, 0.f);
         }
     };
     own_part(0);  // on their way while the place of the others is looked up
@@ -1070,7 +1102,8 @@ __global__ void __launch_bounds__(256) join_kernel(const PrefixParams p) {
         shared.load(p, j, D, col, k0, ml, x);
         all.add(ml, x);
     }
-    store_out(p, static_cast<size_t>(row) * D + col, meta.fine ? all.o : make_float4(0.f, 0.f, 0.f, 0.f), meta.fine ? 1.f / all.l : 0.f);
+    store_out(p, static_cast<size_t>(row) * D + col, meta.fine ? all.o : make_float4(0.f, 0.f, 0.f, 0.f),
+              meta.fine ? 1.f / all.l : 0.f);
 }
 
 }  // namespace kvpd
@@ -1108,8 +1141,8 @@ kvp_attn_args whole_contexts(const kvp_prefix_args& a) {
 }
 
 // Warps an SM that own parts are split into at least: 16 is what its registers hold.  Half as many took 186 us at 256
-// sequences with up to 512 own tokens instead of 171 (twice as many 170); twice as many 82 us at 512 with up to 100 instead
-// of 79, four times 90, for the parts that join_kernel has to read.
+// sequences with up to 512 own tokens instead of 171 (twice as many 170); twice as many 82 us at 512 with up to 100
+// instead of 79, four times 90, for the parts that join_kernel has to read.
 constexpr long long kOwnWarps = 16;
 
 struct PrefixPlan {
@@ -1127,12 +1160,13 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
         return fail(KVP_EINVAL, "unsupported dtype");
     if (a->num_seqs < 0 || a->num_groups < 0 || (a->num_seqs > 0 && a->num_groups < 1) || a->num_groups > a->num_seqs)
         return fail(KVP_EINVAL, "bad num_seqs / num_groups");
-    if (a->num_blocks < 1 || a->block_size < 1 || a->max_blocks < 1) return fail(KVP_EINVAL, "bad num_blocks / block_size / max_blocks");
+    if (a->num_blocks < 1 || a->block_size < 1 || a->max_blocks < 1)
+        return fail(KVP_EINVAL, "bad num_blocks / block_size / max_blocks");
     kvp_attn_args w = whole_contexts(*a);
     if (a->num_seqs == 0) return KVP_OK;
     if (a->kv_dtype == KVP_DTYPE_F32) return KVP_OK;
-    // The shared kernel's tiles hold 128 keys, copied in runs of at least 8 within a block; of blocks that have no such runs, as
-    // many whole ones as fit.
+    // The shared kernel's tiles hold 128 keys, copied in runs of at least 8 within a block; of blocks that have no such
+    // runs, as many whole ones as fit.
     pl->run = gcd_of(a->block_size, kvpd::kKeys);
     pl->keys = kvpd::kKeys;
     if (pl->run < 8) {
@@ -1148,7 +1182,8 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
         if (plan_attention(w, true, &whole) == KVP_OK) pl->bytes = std::max(pl->bytes, whole.ws_bytes);
         else clear_error();
     }
-    pl->shared = (a->head_dim == 64 || a->head_dim == 128) && a->q_dtype == a->kv_dtype && pl->keys > 0 && aligned16(a->q) &&
+    pl->shared = (a->head_dim == 64 || a->head_dim == 128) && a->q_dtype == a->kv_dtype && pl->keys > 0 &&
+        aligned16(a->q) &&
                  aligned16(a->out) && static_cast<long long>(a->num_seqs) * a->kv_heads <= (1LL << 27) &&
                  static_cast<long long>(a->max_blocks) * a->block_size <= kvpd::kPrefixTokens;
     if (!pl->shared) return KVP_OK;
@@ -1167,21 +1202,24 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
     return KVP_OK;
 }
 
-int encode_3d(CUtensorMap* map, int dtype, const void* base, const cuuint64_t (&dims)[3], const cuuint64_t (&strides)[2],
-              const cuuint32_t (&box)[3]) {
+int encode_3d(CUtensorMap* map, int dtype, const void* base, const cuuint64_t (&dims)[3],
+              const cuuint64_t (&strides)[2], const cuuint32_t (&box)[3]) {
     auto fn = encode_fn();
     if (!fn) return fail(KVP_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
     const cuuint32_t one[3] = {1, 1, 1};
-    const CUresult r = fn(map, dtype == KVP_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-                          const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUtensorMapDataType type =
+        dtype == KVP_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUresult r = fn(map, type, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(KVP_ECUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(r));
     return KVP_OK;
 }
 
 // A launch that may start before the one ahead has ended.
 template <class... P>
-int launch_early(void (*fn)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const char* what, const P&... args) {
+int launch_early(void (*fn)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const char* what,
+                 const P&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(threads);
@@ -1196,27 +1234,32 @@ int launch_early(void (*fn)(P...), unsigned grid, unsigned threads, size_t smem,
 }
 
 template <int D, class KV>
-int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, kvpd::PrefixParams p, cudaStream_t s) {
+int launch_prefix(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, kvpd::PrefixParams p,
+                  cudaStream_t s) {
     auto fn = &kvpd::prefix_kernel<D, KV>;
     const int rc = allow_smem(reinterpret_cast<const void*>(fn));
     if (rc != KVP_OK) return rc;
     constexpr size_t tile = static_cast<size_t>(kvpd::kKeys) * D * 2;
-    return launch_early(fn, static_cast<unsigned>(p.ctas), kvpd::kPrefixThreads, 1024 + (2 + (D == 128 ? 4 : 7)) * tile, s, "shared prefix launch",
+    return launch_early(fn, static_cast<unsigned>(p.ctas), kvpd::kPrefixThreads, 1024 + (2 + (D == 128 ? 4 : 7)) * tile,
+                        s, "shared prefix launch",
                         qm, km, vm, p);
 }
 
 template <int D, class KV>
 int launch_own(const kvpd::PrefixParams& p, cudaStream_t s) {
     auto fn = p.g > 8 ? &kvpd::own_kernel<D, KV, 2> : &kvpd::own_kernel<D, KV, 1>;
-    const unsigned warps = static_cast<unsigned>(p.num_seqs) * static_cast<unsigned>(p.kvh) * static_cast<unsigned>(p.own_parts);
+    const unsigned warps = static_cast<unsigned>(p.num_seqs) * static_cast<unsigned>(p.kvh) *
+        static_cast<unsigned>(p.own_parts);
     const int rc = launch_early(fn, warps, 32, 0, s, "own part launch", p);
     if (rc != KVP_OK) return rc;
     const long long threads = static_cast<long long>(p.num_seqs) * p.nh * (D / 4);
-    return launch_early(&kvpd::join_kernel<D>, static_cast<unsigned>((threads + 255) / 256), 256, 0, s, "join launch", p);
+    return launch_early(&kvpd::join_kernel<D>, static_cast<unsigned>((threads + 255) / 256), 256, 0, s, "join launch",
+                        p);
 }
 
 template <int D, class KV>
-int launch_both(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const kvpd::PrefixParams& p, cudaStream_t s) {
+int launch_both(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const kvpd::PrefixParams& p,
+                cudaStream_t s) {
     const int rc = launch_prefix<D, KV>(qm, km, vm, p, s);
     return rc != KVP_OK ? rc : launch_own<D, KV>(p, s);
 }
@@ -1236,17 +1279,20 @@ extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stre
     PrefixPlan pl;
     int rc = plan_prefix(a, &pl);
     if (rc != KVP_OK || a->num_seqs == 0) return rc;
-    if (!a->q || !a->k_cache || !a->v_cache || !a->block_tables || !a->seq_lens || !a->prefix_blocks || !a->group_starts || !a->out)
+    if (!a->q || !a->k_cache || !a->v_cache || !a->block_tables || !a->seq_lens || !a->prefix_blocks ||
+        !a->group_starts || !a->out)
         return fail(KVP_EINVAL, "null buffer");
     if (pl.bytes > 0 && (!a->workspace || a->workspace_bytes < pl.bytes))
         return fail(KVP_ENOSPACE, "workspace smaller than kvp_prefix_workspace_size()");
-    if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0) return fail(KVP_EINVAL, "workspace must be 256-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(a->workspace) & 255u) != 0)
+        return fail(KVP_EINVAL, "workspace must be 256-byte aligned");
     if (!pl.shared) {
         const kvp_attn_args w = whole_contexts(*a);
         return kvp_paged_attention(&w, stream);
     }
     if (!aligned16(a->k_cache) || !aligned16(a->v_cache)) return fail(KVP_EINVAL, "K/V pools must be 16-byte aligned");
-    if (a->num_blocks > 0x7fffffffLL / a->block_size) return fail(KVP_EINVAL, "num_blocks * block_size must stay below 2^31");
+    if (a->num_blocks > 0x7fffffffLL / a->block_size)
+        return fail(KVP_EINVAL, "num_blocks * block_size must stay below 2^31");
     const long long rows = a->num_blocks * a->block_size;
     const int g = a->num_heads / a->kv_heads;
     const cuuint64_t D = static_cast<cuuint64_t>(a->head_dim);

@@ -98,11 +98,13 @@ __device__ __forceinline__ void store8(void* base, long long at, int dtype, cons
 }
 
 // LPH: lanes per head, the power of two at or above dim / 16.  U: heads per lane group in flight.
-// A long prompt (16384 tokens, 32 + 8 + 8 heads of 128, norms): 411 MB in 82 us, 5.0 TB/s, 77% of a copy's rate, with the
-// instructions (270 a warp for 4 heads of 128) taking 64% of the issue slots.  Two heads in flight and six CTAs an SM: four
-// heads and five CTAs took 88 us; a coefficient form of norm and rotation in paired operations took fewer instructions,
-// but 150 registers and 114 us; a token's rows spread over three warps 104 us, for its position and table read thrice.
-// A decode step (1 to 256 tokens) takes 2.5 to 3.4 us on the GPU, the latencies of position, table row and heads in turn.
+// A long prompt (16384 tokens, 32 + 8 + 8 heads of 128, norms): 411 MB in 82 us, 5.0 TB/s, 77% of a copy's rate, with
+// the instructions (270 a warp for 4 heads of 128) taking 64% of the issue slots.  Two heads in flight and six CTAs an
+// SM: four heads and five CTAs took 88 us; a coefficient form of norm and rotation in paired operations took fewer
+// instructions, but 150 registers and 114 us; a token's rows spread over three warps 104 us, for its position and table
+// read thrice.
+// A decode step (1 to 256 tokens) takes 2.5 to 3.4 us on the GPU, the latencies of position, table row and heads in
+// turn.
 template <class T, int LPH, int U>
 __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 4 : 6) rope_append_kernel(const RopeParams p) {
     constexpr int HPW = 32 / LPH;  // heads a warp takes at once
@@ -122,7 +124,8 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 4 : 6) rope_append_kerne
     }
     const long long items = static_cast<long long>(p.tokens) * p.chunks;
     const long long stride = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
-    for (long long it = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); it < items; it += stride) {
+    const long long it0 = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    for (long long it = it0; it < items; it += stride) {
         const long long tok = p.chunks == 1 ? it : it / p.chunks;
         const int chunk = static_cast<int>(it - tok * p.chunks);
         const int pos = __ldg(p.positions + tok);
@@ -137,7 +140,8 @@ __global__ void __launch_bounds__(128, sizeof(T) == 4 ? 4 : 6) rope_append_kerne
         Vec8 c, s;
         if (on && ca >= 0) {
             const float4* t = reinterpret_cast<const float4*>(p.table + static_cast<long long>(pos) * p.rot + ca);
-            const float4* t2 = reinterpret_cast<const float4*>(p.table + static_cast<long long>(pos) * p.rot + (p.rot >> 1) + ca);
+            const float4* t2 = reinterpret_cast<const float4*>(p.table + static_cast<long long>(pos) * p.rot +
+                                                               (p.rot >> 1) + ca);
             const float4 c0 = __ldg(t), c1 = __ldg(t + 1), s0 = __ldg(t2), s1 = __ldg(t2 + 1);
             c = Vec8{{c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}};
             s = Vec8{{s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w}};
@@ -244,7 +248,8 @@ int launch_rope(const RopeParams& p0, cudaStream_t s) {
     p.per_chunk = (iters + p.chunks - 1) / p.chunks;
     p.chunks = (iters + p.per_chunk - 1) / p.per_chunk;
     const long long items = static_cast<long long>(p.tokens) * p.chunks;
-    const long long grid = std::min<long long>((items + kWarps - 1) / kWarps, static_cast<long long>(kvpi::sm_count()) * 16);
+    const long long grid = std::min<long long>((items + kWarps - 1) / kWarps,
+                                               static_cast<long long>(kvpi::sm_count()) * 16);
     rope_append_kernel<T, LPH, U><<<static_cast<unsigned>(grid), kWarps * 32, 0, s>>>(p);
     return kvpi::cuda_status(cudaGetLastError(), "rope append launch");
 }
@@ -278,7 +283,8 @@ extern "C" KVP_API int kvp_rope_append(const kvp_rope_args* a, void* stream) {
             return fail(KVP_EINVAL, "v, k_cache, v_cache and slots go together");
         if (!(a->kv_dtype == KVP_DTYPE_F16 || a->kv_dtype == KVP_DTYPE_BF16))
             return fail(KVP_EINVAL, "pool dtype must be fp16 or bf16");
-        if (a->block_size < 1 || a->num_blocks < 1 || a->num_blocks > INT64_MAX / a->block_size) return fail(KVP_EINVAL, "block_size and num_blocks bound the slots");
+        if (a->block_size < 1 || a->num_blocks < 1 || a->num_blocks > INT64_MAX / a->block_size)
+            return fail(KVP_EINVAL, "block_size and num_blocks bound the slots");
         if (!aligned16(a->k_cache) || !aligned16(a->v_cache)) return fail(KVP_EINVAL, "pools must be 16-byte aligned");
     } else if (!a->k_out) {
         return fail(KVP_EINVAL, "the keys need k_out or a cache");
@@ -293,7 +299,8 @@ extern "C" KVP_API int kvp_rope_append(const kvp_rope_args* a, void* stream) {
     p.q_out_stride = a->q_out_stride ? a->q_out_stride : qrow;
     p.k_out_stride = a->k_out_stride ? a->k_out_stride : krow;
     const int in_b = dtype_bytes(a->in_dtype), out_b = dtype_bytes(a->out_dtype);
-    if (p.q_stride < qrow || p.k_stride < krow || p.q_out_stride < qrow || p.k_out_stride < krow || (cache && p.v_stride < krow))
+    if (p.q_stride < qrow || p.k_stride < krow || p.q_out_stride < qrow || p.k_out_stride < krow ||
+        (cache && p.v_stride < krow))
         return fail(KVP_EINVAL, "token strides must cover a token's heads");
     if ((p.q_stride * in_b) % 16 || (p.k_stride * in_b) % 16 || (cache && (p.v_stride * in_b) % 16) ||
         (p.q_out_stride * out_b) % 16 || (p.k_out_stride * out_b) % 16)

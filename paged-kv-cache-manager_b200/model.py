@@ -57,7 +57,8 @@ class PagedEngine:
     """Paged-KV inference for one model on one GPU.  K/V pools are [layers][num_blocks][B][kv_heads][head_dim]
     in the model's dtype (fp16 or bf16)."""
 
-    def __init__(self, model, num_blocks: int, block_size: int, *, fused_rope: bool = False, shared_prefix: bool = False):
+    def __init__(self, model, num_blocks: int, block_size: int, *, fused_rope: bool = False,
+                 shared_prefix: bool = False):
         from transformers.models.llama.modeling_llama import apply_rotary_pos_emb  # same for Qwen2 and Llama
 
         kvb = _lib()
@@ -88,7 +89,8 @@ class PagedEngine:
             if "dynamic" in kind or kind == "longrope":  # frequencies that change with the length
                 raise ValueError(f"fused_rope needs fixed rotary frequencies; this model's are {kind}")
             if self.hd % 16 or self.hd > 256 or rot.inv_freq.numel() % 8:
-                raise ValueError("fused_rope needs head_dim and the rotated part of it to be multiples of 16, at most 256")
+                raise ValueError("fused_rope needs head_dim and the rotated part of it to be multiples of 16, at most "
+                                 "256")
 
     # ------------------------------------------------------------------ internals
     def _rope_table(self, positions: int) -> torch.Tensor:
@@ -136,7 +138,8 @@ class PagedEngine:
                 q, k = self._rope(q.transpose(1, 2), k.transpose(1, 2), cos, sin)
                 kn, vn = k[0].transpose(0, 1).contiguous(), v[0].contiguous()
                 if slots is not None:
-                    kvb.append_scatter(kn[None], vn[None], self.K[li:li + 1], self.V[li:li + 1], slots, status=self.status)
+                    kvb.append_scatter(kn[None], vn[None], self.K[li:li + 1], self.V[li:li + 1], slots,
+                                       status=self.status)
                     kn = vn = None
                 q = q[0].transpose(0, 1).contiguous()
             if groups is not None:
@@ -247,14 +250,15 @@ class PagedEngine:
 
     @torch.no_grad()
     def beam_search(self, rids: Sequence[int], prompt: Sequence[int], new_tokens: int, eos: Optional[int] = None):
-        """Beam search with len(rids) beams for the continuation of `prompt` with the largest sum of log-probabilities, of
-        new_tokens tokens or up to and with `eos`.  Returns up to len(rids) pairs (sum, tokens), best first, or None if
-        the prompt finds no room.  `rids`: ids for the beams, freed at the end.  Running out of blocks on the way raises
-        RuntimeError, as in decode_batch."""
+        """Beam search with len(rids) beams for the continuation of `prompt` with the largest sum of log-probabilities,
+        of new_tokens tokens or up to and with `eos`.  Returns up to len(rids) pairs (sum, tokens), best first, or None
+        if the prompt finds no room.  `rids`: ids for the beams, freed at the end.  Running out of blocks on the way
+        raises RuntimeError, as in decode_batch."""
         kvb, beams = _lib(), len(rids)
         select = beams if eos is None else 2 * beams  # at most one continuation of each beam ends
         if not 1 <= select <= 32 or beams >= self.m.config.vocab_size or new_tokens < 1:
-            raise ValueError("beam_search takes 1 to 32 beams (16 with eos), fewer than the vocabulary, and new_tokens >= 1")
+            raise ValueError("beam_search takes 1 to 32 beams (16 with eos), fewer than the vocabulary, and "
+                             "new_tokens >= 1")
         if len(set(rids)) != beams or any(self.kv.contains(r) for r in rids):
             raise ValueError("rids must be distinct and not in use")
         if len(prompt) < 1:
