@@ -194,7 +194,8 @@ KVP_API int kvp_paged_attention_noalloc(const kvp_attn_args* a, void* stream);
  *   prefix_blocks [num_seqs]: leading blocks of each sequence that its group shares (equal within a group; 0 where
  *     nothing is shared); they are completely filled, so prefix_blocks * block_size <= seq_len.  The first member's
  *     table row gives the blocks.
- * A sequence that breaks these rules, or whose length is invalid, gets zeros and sets KVP_STATUS_BAD_LEN.
+ * A sequence that breaks these rules, or whose length is invalid, gets zeros and sets KVP_STATUS_BAD_LEN; where
+ * a group starts before the one ahead of it all sequences do.
  * Types, head shapes and layouts as in kvp_paged_attention.  Sharing takes head_dim 64 and 128, queries of the pools'
  * 16-bit dtype, block sizes up to 128 or multiples of 8, q and out on 16-byte boundaries, num_seqs * kv_heads <= 2^27
  * and max_blocks * block_size <= 2^31 - 1024; every other call attends over each sequence's whole context, as

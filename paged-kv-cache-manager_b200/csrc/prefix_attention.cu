@@ -29,9 +29,9 @@
 // P is kept as a part and a rest of the pools' 16-bit type each, as the own parts and the decode attention keep it: the
 // two products with V hold 16 (bf16) or 22 (fp16) bits of each weight, and the output's only rounding that counts is
 // its own.  With one 16-bit number each the weights' roundings were as large as a bf16 output's (1.66e-3 against 64
-// bits became 2.3e-3, relative to all outputs' size 1e-4 became 2.5e-3), and an fp32 output held no more.  It costs half of
-// the tensor cores' work on top: 16 groups 46.9 -> 51.9 us, 512 samples 71.2 -> 78.7, 256 over 16384 154.9 -> 186.4, 4
-// beams the same.
+// bits became 2.3e-3, relative to all outputs' size 1e-4 became 2.5e-3), and an fp32 output held no more.  It costs
+// half of the tensor cores' work on top: 16 groups 46.9 -> 51.9 us, 512 samples 71.2 -> 78.7, 256 over 16384 154.9 ->
+// 186.4, 4 beams the same.
 //
 // Measured, 32 query and 8 kv heads of 128, bf16: a pair of row tiles takes 5260 clocks per key tile, of which the
 // matrix products are 3070 (3750 and 2050 with P in one 16-bit number); starting (groups, table, first tiles) takes
@@ -82,6 +82,7 @@ struct PrefixParams {
     const int32_t* prefix_blocks;
     const int32_t* group_starts;
     int32_t* status;
+    int32_t* unsorted;  // a group starts before the one ahead: they overlap, and nobody's partial rows are their own
     // first and last CTA of each (group, kv head, pair), at its first row's (member, kv head)
     int2* spans;
     float2* part_ml;           // partial rows: (maximum in log2 units, sum)
@@ -321,6 +322,7 @@ struct WorkList {
 struct Start {
     long long total, first;
     int group;
+    bool unsorted;  // nothing is done then
 };
 // Up to 32 groups: every warp by itself, a lane per group.
 __device__ __forceinline__ Start find_start_few(const PrefixParams& p, Group* grp) {
@@ -333,7 +335,9 @@ __device__ __forceinline__ Start find_start_few(const PrefixParams& p, Group* gr
         const long long y = __shfl_up_sync(0xffffffffu, x, off);
         if (lane >= off) x += y;
     }
-    Start s{__shfl_sync(0xffffffffu, x, 31), 0, 0};
+    Start s{__shfl_sync(0xffffffffu, x, 31), 0, 0, false};
+    const int next = __shfl_down_sync(0xffffffffu, mine.start, 1);
+    if (__any_sync(0xffffffffu, lane + 1 < p.num_groups && next < mine.start)) return Start{0, 0, 0, true};
     const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), s.total));
     if (static_cast<int>(blockIdx.x) >= G) return s;
     const long long at = first_unit(blockIdx.x, s.total, G);
@@ -370,18 +374,22 @@ __device__ __forceinline__ Start find_start(const PrefixParams& p, long long* wa
         return all;
     };
     auto units_of = [&](int gi) { return gi < p.num_groups ? load_group(p, gi).units(p.kvh) : 0ll; };
+    bool back = false;
+    for (int gi = static_cast<int>(threadIdx.x); gi + 1 < p.num_groups; gi += kPrefixThreads)
+        back = back || __ldg(p.group_starts + gi + 1) < __ldg(p.group_starts + gi);
+    if (__syncthreads_or(back)) return Start{0, 0, 0, true};
     long long total = 0, mine = 0;
     for (int g0 = 0; g0 < p.num_groups; g0 += kPrefixThreads)
         total += scan(units_of(g0 + static_cast<int>(threadIdx.x)), total, &mine);
     const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
-    if (static_cast<int>(blockIdx.x) >= G) return Start{total, 0, 0};
+    if (static_cast<int>(blockIdx.x) >= G) return Start{total, 0, 0, false};
     const long long at = first_unit(blockIdx.x, total, G);
     long long carry = 0;
     for (int g0 = 0; g0 < p.num_groups; g0 += kPrefixThreads) {
         const int gi = g0 + static_cast<int>(threadIdx.x);
         const long long u = units_of(gi);
         carry += scan(u, carry, &mine);
-        if (u > 0 && mine <= at && at < mine + u) *found = Start{total, mine, gi};
+        if (u > 0 && mine <= at && at < mine + u) *found = Start{total, mine, gi, false};
     }
     __syncthreads();
     *grp = load_group(p, found->group);
@@ -494,6 +502,10 @@ __global__ void __launch_bounds__(kPrefixLimit, 1)
     const Start from =
         p.num_groups <= 32 ? find_start_few(p, &list.grp) : find_start(p, sh.warp_sum, &sh.found, &list.grp);
     const int cta = blockIdx.x, G = static_cast<int>(min(static_cast<long long>(gridDim.x), from.total));
+    if (cta == 0 && threadIdx.x == 0) {
+        *p.unsorted = from.unsorted;
+        if (from.unsorted) report(p.status, KVP_STATUS_BAD_LEN);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -1077,6 +1089,7 @@ __global__ void __launch_bounds__(256) join_kernel(const PrefixParams p) {
     const unsigned item = static_cast<unsigned>(row) / static_cast<unsigned>(p.g);
     const int j = static_cast<int>(static_cast<unsigned>(row) - item * static_cast<unsigned>(p.g));
     griddep_wait();
+    const int32_t unsorted = __ldcg(p.unsorted);
     const OwnMeta meta = p.own_meta[item];
     float2 ml[4];
     float4 x[4];
@@ -1102,8 +1115,9 @@ __global__ void __launch_bounds__(256) join_kernel(const PrefixParams p) {
         shared.load(p, j, D, col, k0, ml, x);
         all.add(ml, x);
     }
-    store_out(p, static_cast<size_t>(row) * D + col, meta.fine ? all.o : make_float4(0.f, 0.f, 0.f, 0.f),
-              meta.fine ? 1.f / all.l : 0.f);
+    const bool fine = meta.fine && !unsorted;
+    store_out(p, static_cast<size_t>(row) * D + col, fine ? all.o : make_float4(0.f, 0.f, 0.f, 0.f),
+              fine ? 1.f / all.l : 0.f);
 }
 
 }  // namespace kvpd
@@ -1147,7 +1161,7 @@ constexpr long long kOwnWarps = 16;
 
 struct PrefixPlan {
     bool shared = false;  // else the plain decode attention over every sequence's whole context
-    size_t ml = 0, o = 0, meta = 0, own_ml = 0, own_o = 0, bytes = 0;
+    size_t spans = 0, ml = 0, o = 0, meta = 0, own_ml = 0, own_o = 0, bytes = 0;
     int mt = 1, run = 8, keys = 0;
     int own_parts = 1;
 };
@@ -1190,7 +1204,8 @@ int plan_prefix(const kvp_prefix_args* a, PrefixPlan* pl) {
     const size_t rows = static_cast<size_t>(a->num_seqs) * a->num_heads;
     const size_t parts = 2 * rows + static_cast<size_t>(sm_count()) * 2 * kvpd::kRows;
     pl->mt = kvpd::kRows / (a->num_heads / a->kv_heads);
-    pl->ml = up256(static_cast<size_t>(a->num_seqs) * a->kv_heads * 8);
+    pl->spans = 256;  // behind the word that tells of unsorted groups
+    pl->ml = pl->spans + up256(static_cast<size_t>(a->num_seqs) * a->kv_heads * 8);
     pl->o = pl->ml + up256(parts * 8);
     // (the largest of all: where q or out are not aligned the other path runs in the same workspace)
     pl->meta = pl->o + up256(parts * a->head_dim * 4);
@@ -1321,7 +1336,8 @@ extern "C" KVP_API int kvp_prefix_attention(const kvp_prefix_args* a, void* stre
     p.prefix_blocks = a->prefix_blocks;
     p.group_starts = a->group_starts;
     p.status = a->status;
-    p.spans = reinterpret_cast<int2*>(ws);
+    p.unsorted = reinterpret_cast<int32_t*>(ws);
+    p.spans = reinterpret_cast<int2*>(ws + pl.spans);
     p.part_ml = reinterpret_cast<float2*>(ws + pl.ml);
     p.part_o = reinterpret_cast<float*>(ws + pl.o);
     p.own_meta = reinterpret_cast<kvpd::OwnMeta*>(ws + pl.meta);

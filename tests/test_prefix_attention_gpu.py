@@ -514,3 +514,24 @@ def test_long_and_uneven_own_parts(kvb, cuda, groups, own, nh, kvh, D, t):
     b = Batch(groups, own, nh, kvh, D, 16, t, t, seed=51)
     assert int(b.lens.max()) > 5000
     _check_close(b, b.run(kvb), lift=12)
+
+
+@pytest.mark.parametrize("groups,change", [([(4, 6), (3, 2), (5, 9)], {1: 8, 2: 4}), ([(4, 6), (3, 6), (5, 6)], {1: 12, 2: 0}),
+                                           ([(4, 6), (3, 2), (5, 9)], {1: 99}), ([(2, 3)] * 40, {20: 10}),
+                                           ([(2, 3)] * 40, {1: 80, 2: 0, 3: 80, 4: 0}), ([(2, 2)] * 400, {398: 12})])
+def test_groups_that_overlap(kvb, cuda, groups, change):
+    """A group that starts before the one ahead puts sequences into two groups, whose partial results would mix with those
+    of others: all get zeros and the status bit; the next call in the same workspace is as ever."""
+    import torch
+    b = Batch(groups, few, 8, 2, 64, 16, seed=61)
+    ws = torch.empty(kvb.shared_prefix_workspace_bytes(b.q, b.k, b.tables, b.starts, 8, 2), dtype=torch.uint8, device="cuda")
+    good, starts = b.run(kvb, workspace=ws), b.starts.clone()
+    for i, v in change.items():
+        b.starts[i] = v
+    got = b.run(kvb, workspace=ws)
+    torch.cuda.synchronize()
+    assert int(b.status.item()) == kvb.KVP_STATUS_BAD_LEN and bool((got == 0).all())
+    b.starts.copy_(starts)
+    b.status.zero_()
+    assert torch.equal(b.run(kvb, workspace=ws), good)
+    b.check(good)
