@@ -224,18 +224,17 @@ class PagedEngine:
             raise RuntimeError("out of blocks in decode_batch")
         self._cow(pairs)
         rows = [self.kv.block_table(r)[: (p + self.B) // self.B] for r, p in zip(rids, before)]
+        tables, lens = self._dense(rows), torch.tensor([p + 1 for p in before], dtype=torch.int32)
         order, groups = None, None
         if self.shared_prefix and len(rows) > 1:
             by_table = sorted(range(len(rows)), key=lambda i: rows[i])  # requests that share blocks side by side
-            side_by_side = [rows[i] for i in by_table], [before[i] + 1 for i in by_table]
-            prefix, starts = kvb.shared_prefix_groups(self._dense(side_by_side[0]), side_by_side[1], self.B)
-            if prefix.any() and _sharing_pays(prefix, starts, side_by_side[1], self.B, self.kvh, self.hd,
+            prefix, starts = kvb.shared_prefix_groups(tables[by_table], lens[by_table], self.B)
+            if prefix.any() and _sharing_pays(prefix, starts, lens[by_table].tolist(), self.B, self.kvh, self.hd,
                                                torch.cuda.get_device_properties(self.dev).multi_processor_count):
                 order, groups = by_table, (torch.from_numpy(prefix).to(self.dev), torch.from_numpy(starts).to(self.dev))
-                rows, before, slots = [rows[i] for i in order], [before[i] for i in order], [slots[i] for i in order]
+                tables, lens = tables[order], lens[order]
+                before, slots = [before[i] for i in order], [slots[i] for i in order]
                 last_tokens = [last_tokens[i] for i in order]
-        tables = self._dense(rows)
-        lens = torch.tensor([p + 1 for p in before], dtype=torch.int32)
         if not (self.fused_rope or groups):
             slots = None  # fused append
         else:
