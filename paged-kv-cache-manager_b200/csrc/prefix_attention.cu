@@ -37,7 +37,7 @@
 // matrix products are 3070 (3750 and 2050 with P in one 16-bit number); starting (groups, table, first tiles) takes
 // 12000 clocks, writing the partial results 5000 to 8000.  512 sequences over 2048 shared tokens and up to 100 own
 // ones: 79 us (prefix_kernel alone 49, the own parts alone 31, joining 13, each with cold caches); 256 over 16384, up
-// to 512 own: 171 us (119, 63, 12); 4 beams over 2048, 24 own: 17 us.
+// to 512 own: 172 us (119, 63, 12); 4 beams over 2048, 24 own: 18 us.
 // prefix_kernel leaves shared memory unused on purpose: with 224 KB instead of 192 the L1, which the own parts' loads
 // go through, shrinks to 28 KB, and the first two calls took 85 and 174 us where they took 72 and 149.
 // The own parts are cut alike, into at most 8 each: a long one beside many short ones, or few long ones, are slower
